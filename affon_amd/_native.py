@@ -72,6 +72,74 @@ class FloorGeometry(ctypes.Structure):
     ]
 
 
+class KvCache(ctypes.Structure):
+    """affon_rocm_kv_cache."""
+    _fields_ = [
+        ("keys", c_void_p),
+        ("values", c_void_p),
+        ("bytes", c_size_t),
+        ("layers", c_int64),
+        ("pages", c_int64),
+        ("kv_heads", c_int64),
+        ("page_size", c_int64),
+        ("head_dim", c_int64),
+        ("dtype", c_int32),
+    ]
+
+
+class DraftBatch(ctypes.Structure):
+    """affon_rocm_draft_batch."""
+    _fields_ = [
+        ("page_table", View),
+        ("lengths", c_void_p),
+        ("counts", c_void_p),
+        ("rows", c_int64),
+    ]
+
+
+class AppendDesc(ctypes.Structure):
+    """affon_rocm_append_desc."""
+    _fields_ = [
+        ("query", View),
+        ("key", View),
+        ("value", View),
+        ("positions", c_void_p),
+        ("rotary", c_void_p),
+        ("rotary_rows", c_int64),
+        ("rotary_dim", c_int64),
+        ("interleaved", c_int32),
+        ("layer", c_int64),
+        ("output", c_void_p),
+        ("output_bytes", c_size_t),
+    ]
+
+
+class AttentionDesc(ctypes.Structure):
+    """affon_rocm_attention_desc."""
+    _fields_ = [
+        ("query", View),
+        ("mask", View),
+        ("scale", ctypes.c_float),
+        ("layer", c_int64),
+        ("output", c_void_p),
+        ("output_bytes", c_size_t),
+    ]
+
+
+class ResidualNormDesc(ctypes.Structure):
+    """affon_rocm_residual_norm_desc."""
+    _fields_ = [
+        *((name, c_void_p) for name in ("stream", "update", "gate", "post_weight", "weight", "stream_out",
+                                        "normalized")),
+        *((name, c_int64) for name in ("rows", "cols", "stream_stride", "update_stride", "gate_stride",
+                                       "stream_out_stride", "normalized_stride")),
+        *((name, c_int32) for name in ("stream_dtype", "update_dtype", "gate_dtype", "weight_dtype",
+                                       "normalized_dtype", "post_norm")),
+        ("scale", ctypes.c_float),
+        ("epsilon", ctypes.c_float),
+    ]
+
+
 SIGNATURES = {
     "affon_rocm_device_count": (c_int, [ctypes.POINTER(c_int)]),
     "affon_rocm_session_create": (c_int, [c_int, ctypes.POINTER(c_void_p)]),
@@ -112,6 +180,13 @@ SIGNATURES = {
     "affon_rocm_softmax": (c_int, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_void_p]),
     "affon_rocm_index_select": (c_int, [c_void_p, c_void_p, c_int32, c_int64, c_int64, c_int32, c_void_p, c_int64,
                                         c_void_p]),
+    "affon_rocm_cache_append": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                        ctypes.POINTER(AppendDesc)]),
+    "affon_rocm_tree_attention": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                          ctypes.POINTER(AttentionDesc)]),
+    "affon_rocm_cache_commit": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                        ctypes.POINTER(View), c_void_p]),
+    "affon_rocm_residual_norm": (c_int, [c_void_p, ctypes.POINTER(ResidualNormDesc)]),
 }
 
 _LIB: ctypes.CDLL | None = None

@@ -12,6 +12,7 @@
 #include <cstdio>
 #include <cstring>
 #include <exception>
+#include <initializer_list>
 #include <limits>
 #include <memory>
 #include <mutex>
@@ -105,24 +106,24 @@ int element_size(int dtype) {
 bool is_float_dtype(int dtype) { return dtype == AFFON_ROCM_F32 || dtype == AFFON_ROCM_BF16; }
 
 // Checks that every element a view names lies inside its allocation.
-int check_view(const affon_rocm_view& v, const char* name) {
+int check_view(const affon_rocm_view& v, const char* name, const char* op = "quantized_matmul") {
   const int esize = element_size(v.dtype);
-  if (v.data == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s has no data", name);
+  if (v.data == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s has no data", op, name);
   if (v.shape[0] <= 0 || v.shape[1] <= 0)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s has an empty dimension", name);
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s has an empty dimension", op, name);
   if (v.stride[0] < 0 || v.stride[1] < 0)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s has a negative stride", name);
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s has a negative stride", op, name);
   if (v.byte_offset % static_cast<size_t>(esize) != 0)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s byte offset is not element aligned", name);
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s byte offset is not element aligned", op, name);
   uint64_t last0 = 0, last1 = 0, last = 0, bytes = 0, end = 0;
   if (!mul_ok(static_cast<uint64_t>(v.shape[0] - 1), static_cast<uint64_t>(v.stride[0]), &last0) ||
       !mul_ok(static_cast<uint64_t>(v.shape[1] - 1), static_cast<uint64_t>(v.stride[1]), &last1) ||
       !add_ok(last0, last1, &last) || !add_ok(last, 1, &last) ||
       !mul_ok(last, static_cast<uint64_t>(esize), &bytes) ||
       !add_ok(bytes, static_cast<uint64_t>(v.byte_offset), &end))
-    return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s extent overflows", name);
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s extent overflows", op, name);
   if (end > v.buffer_bytes)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "quantized_matmul %s view exceeds its buffer (%llu > %llu bytes)", name,
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s view exceeds its buffer (%llu > %llu bytes)", op, name,
                 static_cast<unsigned long long>(end), static_cast<unsigned long long>(v.buffer_bytes));
   return AFFON_ROCM_OK;
 }
@@ -895,6 +896,252 @@ int affon_rocm_index_select(affon_rocm_session* session, const void* x, int32_t 
   if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
   hipError_t e = affon::index_select_launch(x, dtype, rows, cols, axis, index, count, out, session->stream);
   if (e != hipSuccess) return hip_fail(e, "index_select");
+  return AFFON_ROCM_OK;
+}
+
+// ---- drafted tokens over a paged cache, and the norms between blocks ----
+
+namespace {
+
+bool aligned(const void* p, size_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+// A view of a rank-two operand [rows, cols] with unit inner stride.
+int check_matrix(const affon_rocm_view& v, int64_t rows, int64_t cols, const char* name, const char* op) {
+  if (v.shape[0] != rows || v.shape[1] != cols)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s must be [%lld, %lld]", op, name, static_cast<long long>(rows),
+                static_cast<long long>(cols));
+  if (cols > 1 && v.stride[1] != 1)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s must have a unit inner stride", op, name);
+  if (!aligned(v.data, element_size(v.dtype)))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s %s is not element aligned", op, name);
+  return check_view(v, name, op);
+}
+
+const uint8_t* origin(const affon_rocm_view& v) { return static_cast<const uint8_t*>(v.data) + v.byte_offset; }
+
+constexpr int64_t kMaxInt = std::numeric_limits<int32_t>::max();
+
+// The product of positive factors, or false where one is not positive or it passes 2^40.
+bool extent(std::initializer_list<int64_t> factors, uint64_t* out) {
+  *out = 1;
+  for (int64_t f : factors)
+    if (f <= 0 || !mul_ok(*out, static_cast<uint64_t>(f), out) || *out > (uint64_t(1) << 40)) return false;
+  return true;
+}
+
+// `layer`: the one that is used, or -1 for all.
+int check_cache(const affon_rocm_kv_cache* c, int64_t layer, const char* op, affon::PagedCache* out) {
+  if (c == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s cache is null", op);
+  if (!is_float_dtype(c->dtype)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires an f32 or bf16 cache", op);
+  uint64_t count = 0;
+  if (!extent({c->layers, c->pages, c->kv_heads, c->page_size, c->head_dim}, &count))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s cache has an empty dimension or its size overflows", op);
+  if (c->page_size % 16 != 0 || c->page_size > 65536)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s page_size must be a multiple of 16, at most 65536", op);
+  if (c->head_dim % 8 != 0 || c->head_dim > 256)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s head_dim must be a multiple of 8, at most 256", op);
+  if (c->layers > kMaxInt || c->pages > kMaxInt || c->kv_heads > 65535)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s cache size overflows", op);
+  const uint64_t bytes = count * static_cast<uint64_t>(element_size(c->dtype));
+  if (c->keys == nullptr || c->values == nullptr || c->bytes < bytes)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s cache memory is smaller than its shape", op);
+  if (!aligned(c->keys, 16) || !aligned(c->values, 16))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s cache must be 16-byte aligned", op);
+  if (layer < -1 || layer >= c->layers) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
+  out->layer_bytes = static_cast<int64_t>(bytes / static_cast<uint64_t>(c->layers));
+  const int64_t at = layer > 0 ? layer * out->layer_bytes : 0;
+  out->keys = static_cast<uint8_t*>(c->keys) + at;
+  out->values = static_cast<uint8_t*>(c->values) + at;
+  out->dtype = c->dtype;
+  out->layers = layer < 0 ? static_cast<int>(c->layers) : 1;
+  out->pages = static_cast<int>(c->pages);
+  out->kv_heads = static_cast<int>(c->kv_heads);
+  out->page_size = static_cast<int>(c->page_size);
+  out->head_dim = static_cast<int>(c->head_dim);
+  return AFFON_ROCM_OK;
+}
+
+int check_batch(const affon_rocm_draft_batch* b, const affon::PagedCache& cache, const char* op,
+                affon::DraftBatch* out) {
+  if (b == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s batch is null", op);
+  const affon_rocm_view& t = b->page_table;
+  if (t.dtype != AFFON_ROCM_U32) return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 page table", op);
+  int status = check_matrix(t, t.shape[0], t.shape[1], "page table", op);
+  if (status != AFFON_ROCM_OK) return status;
+  uint64_t rows = 0, tokens = 0;
+  if (!extent({t.shape[0], b->rows}, &rows) || rows > static_cast<uint64_t>(kMaxInt / 2))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires at least one row per sequence, and their number to fit 30 bits", op);
+  if (!extent({t.shape[1], cache.page_size}, &tokens) || tokens + static_cast<uint64_t>(b->rows) > static_cast<uint64_t>(kMaxInt))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s page table covers too many tokens", op);
+  if (b->lengths == nullptr || !aligned(b->lengths, 4) || !aligned(b->counts, 4))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 lengths", op);
+  out->sequences = static_cast<int>(t.shape[0]);
+  out->rows = static_cast<int>(b->rows);
+  out->table = reinterpret_cast<const uint32_t*>(origin(t));
+  out->table_stride = t.stride[0];
+  out->capacity = static_cast<uint32_t>(tokens);
+  out->lengths = b->lengths;
+  out->counts = b->counts;
+  return AFFON_ROCM_OK;
+}
+
+// The queries of a batch: [B*T, heads*head_dim], heads a multiple of kv_heads; and an output of their shape.
+int check_query(const affon_rocm_view& q, const affon::PagedCache& cache, const affon::DraftBatch& batch,
+                const void* output, size_t output_bytes, const char* op, int* heads) {
+  const int64_t rows = static_cast<int64_t>(batch.sequences) * batch.rows;
+  const int64_t unit = static_cast<int64_t>(cache.kv_heads) * cache.head_dim;
+  if (q.shape[1] <= 0 || q.shape[1] % unit != 0 || q.shape[1] / cache.head_dim > 65535)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s query width must be a multiple of kv_heads * head_dim", op);
+  const int status = check_matrix(q, rows, q.shape[1], "query", op);
+  if (status != AFFON_ROCM_OK) return status;
+  uint64_t count = 0;
+  if (!extent({rows, q.shape[1]}, &count)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s query size overflows", op);
+  if (output == nullptr || output_bytes < count * static_cast<uint64_t>(element_size(cache.dtype)) ||
+      !aligned(output, element_size(cache.dtype)))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s output buffer is smaller than the query", op);
+  *heads = static_cast<int>(q.shape[1] / cache.head_dim);
+  return AFFON_ROCM_OK;
+}
+
+}  // namespace
+
+int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                            const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* d) {
+  clear_error();
+  const char* op = "cache_append";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AppendProblem p{};
+  if (d->layer < 0) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
+  int status = check_cache(cache, d->layer, op, &p.cache);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, p.cache, op, &p.batch)) != AFFON_ROCM_OK) return status;
+  if (!is_float_dtype(d->query.dtype) || d->key.dtype != d->query.dtype || d->value.dtype != d->query.dtype)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires query, key and value of one type, f32 or bf16", op);
+  if ((status = check_query(d->query, p.cache, p.batch, d->output, d->output_bytes, op, &p.heads)) != AFFON_ROCM_OK)
+    return status;
+  const int64_t rows = d->query.shape[0], width = static_cast<int64_t>(p.cache.kv_heads) * p.cache.head_dim;
+  if ((status = check_matrix(d->key, rows, width, "key", op)) != AFFON_ROCM_OK ||
+      (status = check_matrix(d->value, rows, width, "value", op)) != AFFON_ROCM_OK)
+    return status;
+  if (d->rotary_dim < 2 || d->rotary_dim % 2 != 0 || d->rotary_dim > p.cache.head_dim)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s rotary_dim must be even, and at most head_dim", op);
+  if (d->rotary == nullptr || !aligned(d->rotary, 4) || !aligned(d->positions, 4) || d->rotary_rows <= 0 ||
+      d->rotary_rows > kMaxInt)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires an f32 rotary table", op);
+  p.query = origin(d->query);
+  p.key = origin(d->key);
+  p.value = origin(d->value);
+  p.query_stride = d->query.stride[0];
+  p.key_stride = d->key.stride[0];
+  p.value_stride = d->value.stride[0];
+  p.x_dtype = d->query.dtype;
+  p.positions = d->positions;
+  p.rotary = d->rotary;
+  p.rotary_rows = static_cast<uint32_t>(d->rotary_rows);
+  p.rotary_dim = static_cast<int>(d->rotary_dim);
+  p.interleaved = d->interleaved != 0;
+  p.out = static_cast<uint8_t*>(d->output);
+  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  const hipError_t e = affon::append_launch(p, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                              const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* d) {
+  clear_error();
+  const char* op = "tree_attention";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AttentionProblem p{};
+  if (d->layer < 0) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
+  int status = check_cache(cache, d->layer, op, &p.cache);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, p.cache, op, &p.batch)) != AFFON_ROCM_OK) return status;
+  if (d->query.dtype != p.cache.dtype)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires query and cache of one type", op);
+  if ((status = check_query(d->query, p.cache, p.batch, d->output, d->output_bytes, op, &p.heads)) != AFFON_ROCM_OK)
+    return status;
+  if (d->mask.data != nullptr) {
+    if (d->mask.dtype != AFFON_ROCM_U32 || d->mask.shape[1] < (p.batch.rows + 31) / 32)
+      return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 mask with a bit for every row of a sequence", op);
+    if ((status = check_matrix(d->mask, d->query.shape[0], d->mask.shape[1], "mask", op)) != AFFON_ROCM_OK) return status;
+    p.mask = reinterpret_cast<const uint32_t*>(origin(d->mask));
+    p.mask_stride = d->mask.stride[0];
+  }
+  if (!(d->scale - d->scale == 0.0f)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s scale must be finite", op);
+  p.query = origin(d->query);
+  p.query_stride = d->query.stride[0];
+  p.scale = d->scale;
+  p.out = static_cast<uint8_t*>(d->output);
+  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  affon::Launch launch;
+  launch.stream = session->stream;
+  launch.workspace = session->workspace;
+  const hipError_t e = affon::attention_launch(p, launch);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                            const affon_rocm_draft_batch* batch, const affon_rocm_view* path,
+                            const uint32_t* accepted) {
+  clear_error();
+  const char* op = "cache_commit";
+  affon::PagedCache c{};
+  affon::DraftBatch b{};
+  int status = check_cache(cache, -1, op, &c);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, c, op, &b)) != AFFON_ROCM_OK) return status;
+  if (path == nullptr || path->dtype != AFFON_ROCM_U32 || path->shape[1] > b.rows)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 path of at most the batch's rows", op);
+  if ((status = check_matrix(*path, b.sequences, path->shape[1], "path", op)) != AFFON_ROCM_OK) return status;
+  if (accepted == nullptr || !aligned(accepted, 4))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 counts of accepted tokens", op);
+  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  const hipError_t e = affon::commit_launch(c, b, reinterpret_cast<const uint32_t*>(origin(*path)), path->stride[0],
+                                            static_cast<int>(path->shape[1]), accepted, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_residual_norm(affon_rocm_session* session, const affon_rocm_residual_norm_desc* d) {
+  clear_error();
+  const char* op = "residual_norm";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  for (int dtype : {d->stream_dtype, d->update_dtype, d->gate_dtype, d->weight_dtype, d->normalized_dtype})
+    if (!is_float_dtype(dtype)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires f32 or bf16 tensors", op);
+  uint64_t count = 0;
+  if (!extent({d->rows, d->cols}, &count) || d->rows > kMaxInt || d->cols > (int64_t(1) << 28))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a non-empty rank-two tensor of at most 2^40 values", op);
+  if (d->stream == nullptr || d->normalized == nullptr || (d->update != nullptr && d->stream_out == nullptr))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s buffer is null", op);
+  if (d->update == nullptr && (d->gate != nullptr || d->post_norm != 0))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s without an update takes no gate and no post_norm", op);
+  if (d->post_norm == 0 && d->post_weight != nullptr)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s post_weight needs post_norm", op);
+  const struct {
+    const void* data;
+    int dtype;
+    int64_t stride, least;
+  } operands[] = {{d->stream, d->stream_dtype, d->stream_stride, 0},
+                  {d->update, d->update_dtype, d->update_stride, 0},
+                  {d->gate, d->gate_dtype, d->gate_stride, 0},
+                  {d->post_weight, d->weight_dtype, 0, 0},
+                  {d->weight, d->weight_dtype, 0, 0},
+                  {d->stream_out, d->stream_dtype, d->stream_out_stride, d->cols},
+                  {d->normalized, d->normalized_dtype, d->normalized_stride, d->cols}};
+  for (const auto& o : operands) {
+    if (o.data == nullptr) continue;
+    if (!aligned(o.data, element_size(o.dtype)))
+      return fail(AFFON_ROCM_INVALID_SHAPE, "%s buffer is not element aligned", op);
+    // Rows of an output do not overlap.
+    if (o.stride < 0 || (d->rows > 1 && o.stride < o.least) || o.stride > (int64_t(1) << 40) / d->rows)
+      return fail(AFFON_ROCM_INVALID_SHAPE, "%s has an invalid row stride", op);
+  }
+  if (!(d->epsilon > 0.0f) || d->epsilon == std::numeric_limits<float>::infinity())
+    return fail(AFFON_ROCM_INVALID_SHAPE, "invalid residual_norm options: epsilon must be finite and positive");
+  if (!(d->scale - d->scale == 0.0f)) return fail(AFFON_ROCM_INVALID_SHAPE, "invalid residual_norm options: scale must be finite");
+  int status = check_session(session);
+  if (status != AFFON_ROCM_OK) return status;
+  const hipError_t e = affon::residual_norm_launch(*d, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
   return AFFON_ROCM_OK;
 }
 

@@ -101,6 +101,56 @@ hipError_t rms_norm_launch(const void* x, int dtype, int64_t rows, int64_t cols,
 hipError_t softmax_launch(const void* x, int dtype, int64_t rows, int64_t cols, void* out, const Launch& l);
 hipError_t index_select_launch(const void* x, int dtype, int64_t rows, int64_t cols, int axis, const int64_t* index,
                                int64_t count, void* out, hipStream_t stream);
+// A validated paged cache of one layer (commit: of all), a batch of drafted
+// tokens over it, and the calls on them (affon_rocm.h says what they compute).
+struct PagedCache {
+  uint8_t* keys;
+  uint8_t* values;
+  int dtype;
+  int layers, pages, kv_heads, page_size, head_dim;
+  int64_t layer_bytes;
+};
+struct DraftBatch {
+  int sequences, rows;
+  const uint32_t* table;
+  int64_t table_stride;
+  uint32_t capacity;  // tokens that a row of the table holds
+  const uint32_t* lengths;
+  const uint32_t* counts;  // or null
+};
+struct AppendProblem {
+  PagedCache cache;
+  DraftBatch batch;
+  const uint8_t *query, *key, *value;
+  int64_t query_stride, key_stride, value_stride;
+  int x_dtype, heads;
+  const uint32_t* positions;
+  const float* rotary;
+  uint32_t rotary_rows;
+  int rotary_dim;
+  bool interleaved;
+  uint8_t* out;
+};
+hipError_t append_launch(const AppendProblem& p, hipStream_t stream);
+
+struct AttentionProblem {
+  PagedCache cache;
+  DraftBatch batch;
+  const uint8_t* query;
+  int64_t query_stride;
+  int heads;
+  const uint32_t* mask;  // or null: a chain
+  int64_t mask_stride;
+  float scale;
+  uint8_t* out;
+};
+hipError_t attention_launch(const AttentionProblem& p, const Launch& l);
+
+hipError_t commit_launch(const PagedCache& cache, const DraftBatch& batch, const uint32_t* path, int64_t path_stride,
+                         int path_columns, const uint32_t* accepted, hipStream_t stream);
+
+hipError_t residual_norm_launch(const affon_rocm_residual_norm_desc& d, hipStream_t stream);
+
 // One launch that reads every whole 16-byte chunk of up to four buffers once
 // (diag.hip); sink receives at most one word.
 hipError_t read_floor_launch(const void* const* buffers, const uint64_t* bytes, int count, uint32_t* sink,

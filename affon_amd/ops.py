@@ -607,3 +607,93 @@ def _run_index_select(x: Tensor, axis: int, indices: Tensor) -> Tensor:
                                                          axis, indices.data_ptr, count, out.data_ptr),
                   "Program execution failed")
     return out
+
+
+# ---- the norms between blocks (no counterpart op in the reference) ----
+
+def _rows_operand(name: str, t: Any, like: Tensor, rank_one: bool = False) -> Tensor:
+    """An f32/bf16 operand of residual_norm shaped like the stream (rank_one:
+    or of its columns), of its Session and with consecutive columns."""
+    if not isinstance(t, Tensor) or t.dtype not in ("f32", "bf16") or \
+            t.shape != like.shape and not (rank_one and t.shape == like.shape[1:]):
+        raise TypeError(f"residual_norm {name} must be an f32/bf16 tensor of the stream's shape"
+                        + (" or of its columns" if rank_one else ""))
+    if t.shape[-1] > 1 and t.strides[-1] != 1:
+        raise TypeError(f"residual_norm {name} must have consecutive columns")
+    if t.session is not like.session:
+        raise TypeError("residual_norm operands must belong to the same Session")
+    return t
+
+
+def _weight_operand(name: str, t: Any, like: Tensor) -> Tensor:
+    if not isinstance(t, Tensor) or t.dtype not in ("f32", "bf16") or t.shape != like.shape[1:] or \
+            not t.is_contiguous():
+        raise TypeError(f"residual_norm {name} must be a contiguous f32/bf16 [{like.shape[1]}] tensor")
+    if t.session is not like.session:
+        raise TypeError("residual_norm operands must belong to the same Session")
+    return t
+
+
+def residual_norm(stream: Tensor, update: Tensor | None = None, *, gate: Tensor | None = None, scale: float = 1.0,
+                  post_norm: bool = False, post_weight: Tensor | None = None, weight: Tensor | None = None,
+                  epsilon: float = 1e-5, dtype: str | None = None,
+                  out: tuple[Tensor, Tensor] | None = None) -> tuple[Tensor, Tensor]:
+    """The norms between two blocks with the residual add, in one launch:
+
+        u = update, or with post_norm rms_norm(update) * post_weight
+        stream' = stream + scale * gate * u
+        normalized = rms_norm(stream') * weight
+
+    computed in f32 and rounded once each; returns (stream', normalized).
+    ``stream`` and ``update`` [M, N], each f32 or bf16, columns consecutive and
+    rows at any stride; ``gate`` [M, N] or [N]; weights [N], both of one type.
+    Without an update the stream is only normalized, and returned as it is.
+    ``dtype`` of normalized: by default the stream's. ``out``: tensors for
+    both results; the first may be the stream itself."""
+    if not isinstance(stream, Tensor) or len(stream.shape) != 2:
+        raise TypeError("residual_norm requires an evaluated rank-two stream")
+    _rows_operand("stream", stream, stream)
+    epsilon, scale = float(epsilon), float(scale)
+    if not np.isfinite(epsilon) or epsilon <= 0:
+        raise TypeError("invalid residual_norm options: epsilon must be finite and positive")
+    if not np.isfinite(scale):
+        raise TypeError("invalid residual_norm options: scale must be finite")
+    if update is None and (gate is not None or post_norm):
+        raise TypeError("residual_norm without an update takes no gate and no post_norm")
+    if post_weight is not None and not post_norm:
+        raise TypeError("residual_norm post_weight needs post_norm")
+    if post_weight is not None and weight is not None and post_weight.dtype != weight.dtype:
+        raise TypeError("residual_norm weights must have one type")
+    if dtype not in (None, "f32", "bf16"):
+        raise TypeError("residual_norm result must be f32 or bf16")
+    code = {"f32": _native.F32, "bf16": _native.BF16}
+    desc = _native.ResidualNormDesc(rows=stream.shape[0], cols=stream.shape[1], scale=scale, epsilon=epsilon,
+                                    post_norm=1 if post_norm else 0, stream=stream.data_ptr,
+                                    stream_stride=stream.strides[0], stream_dtype=code[stream.dtype])
+    if update is not None:
+        _rows_operand("update", update, stream)
+        desc.update, desc.update_stride, desc.update_dtype = update.data_ptr, update.strides[0], code[update.dtype]
+    if gate is not None:
+        _rows_operand("gate", gate, stream, rank_one=True)
+        desc.gate, desc.gate_dtype = gate.data_ptr, code[gate.dtype]
+        desc.gate_stride = gate.strides[0] if len(gate.shape) == 2 else 0
+    if post_weight is not None:
+        _weight_operand("post_weight", post_weight, stream)
+        desc.post_weight, desc.weight_dtype = post_weight.data_ptr, code[post_weight.dtype]
+    if weight is not None:
+        _weight_operand("weight", weight, stream)
+        desc.weight, desc.weight_dtype = weight.data_ptr, code[weight.dtype]
+    if out is None:
+        out = (stream if update is None else stream.session.empty(stream.dtype, stream.shape),
+               stream.session.empty(dtype or stream.dtype, stream.shape))
+    first, normalized = out
+    _rows_operand("output", first, stream)
+    _rows_operand("output", normalized, stream)
+    if first.dtype != stream.dtype or dtype not in (None, normalized.dtype):
+        raise TypeError("residual_norm outputs must have the stream's type and that of the result")
+    desc.stream_out, desc.stream_out_stride = first.data_ptr, first.strides[0]
+    desc.normalized, desc.normalized_stride = normalized.data_ptr, normalized.strides[0]
+    desc.normalized_dtype = code[normalized.dtype]
+    _native.check(_native.load().affon_rocm_residual_norm(stream.session._handle, ctypes.byref(desc)),
+                  "Program execution failed")
+    return first, normalized

@@ -322,6 +322,119 @@ int affon_rocm_softmax(affon_rocm_session* session, const void* x, int32_t dtype
 int affon_rocm_index_select(affon_rocm_session* session, const void* x, int32_t dtype, int64_t rows, int64_t cols,
                             int32_t axis, const int64_t* index, int64_t count, void* out);
 
+/* ---- drafted tokens over a paged cache (no reference counterpart: the
+ *      reference's models keep a fixed-capacity cache and decode token by
+ *      token, packages/@affon/models/src/llama/model.ts:93-202) ----
+ *
+ * What a decoder block needs between its projections while T drafted tokens
+ * of each of B sequences are checked at once: T = 1 is ordinary decoding, a
+ * chain of T tokens a piece of a prompt, and a tree of them speculative
+ * decoding. All calls enqueue on the session's stream, allocate nothing but
+ * workspace and can be captured (warm a shape up once first). Lengths, counts, page
+ * tables, masks and paths are read on the device when the call runs, so a
+ * captured step is replayed with new ones. */
+
+/* Keys and values of `layers` layers: [layers, pages, kv_heads, page_size,
+ * head_dim] each, contiguous, 16-byte aligned, f32 or bf16. page_size: a
+ * multiple of 16. head_dim: a multiple of 8, at most 256. Nothing is read from a slot that
+ * was not appended to, so new memory needs no clearing. */
+typedef struct {
+  void* keys;
+  void* values;
+  size_t bytes; /* of the memory behind keys, and of that behind values */
+  int64_t layers, pages, kv_heads, page_size, head_dim;
+  int32_t dtype;
+} affon_rocm_kv_cache;
+
+/* `rows` (T) drafted tokens of each sequence: row b*T + i of the operands is
+ * token i of sequence b. Sequence b holds lengths[b] tokens; its token n lies
+ * in line n % page_size of page page_table[b, n / page_size], and drafted token i is
+ * its token lengths[b] + i. A table entry that names no page (>= pages) and
+ * tokens past the table hold nothing: appends to them are dropped, attention
+ * does not see them. Only the first counts[b] rows are in use (null: all);
+ * the others append nothing, and their outputs are zeros. */
+typedef struct {
+  affon_rocm_view page_table; /* [B, columns] u32, unit inner stride */
+  const uint32_t* lengths;    /* [B] device words */
+  const uint32_t* counts;     /* [B] device words, or null */
+  int64_t rows;
+} affon_rocm_draft_batch;
+
+/* Rotates the queries and keys of drafted tokens by their positions, and
+ * appends keys and values to one layer of the cache. For a pair (x1, x2),
+ * dims j and j + h of a head with h = rotary_dim / 2 (interleaved: dims 2j and
+ * 2j + 1), c = rotary[p, j] and s = rotary[p, h + j] of its row's position p:
+ *   y1 = x1 c - x2 s,  y2 = x2 c + x1 s,
+ * in f32, rounded once to the cache's type; dims from rotary_dim on are kept.
+ * A position outside the table turns with zeros. */
+typedef struct {
+  affon_rocm_view query; /* [B*T, heads*head_dim], heads a multiple of kv_heads */
+  affon_rocm_view key;   /* [B*T, kv_heads*head_dim] */
+  affon_rocm_view value; /* [B*T, kv_heads*head_dim]; all three f32 or all bf16, unit inner stride */
+  const uint32_t* positions; /* [B*T] device words, or null: lengths[b] + i */
+  const float* rotary;       /* [rotary_rows, rotary_dim]: cosines, then sines */
+  int64_t rotary_rows, rotary_dim; /* rotary_dim: even, at most head_dim */
+  int32_t interleaved;
+  int64_t layer;
+  void* output; /* rotated queries [B*T, heads*head_dim], contiguous, the cache's type */
+  size_t output_bytes;
+} affon_rocm_append_desc;
+int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                            const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* desc);
+
+/* Attention of drafted tokens over one layer of the cache, which already
+ * holds their own keys and values. Row (b, i) sees the lengths[b] tokens
+ * before and drafted token j < counts[b] where bit j % 32 of mask[b*T + i,
+ * j / 32] is set (no mask: j <= i). For each of its heads, with key head
+ * head / (heads / kv_heads):
+ *   out = sum_n e^(scale q.k_n - m) v_n / sum_n e^(scale q.k_n - m),
+ * m the largest score seen; a row that sees nothing gives zeros, whatever
+ * unseen slots hold, infinities and NaN included, does not reach its output. Scores, the
+ * softmax and sums in f32; for bf16 the probabilities are rounded to bf16
+ * for the product with v. */
+typedef struct {
+  affon_rocm_view query; /* [B*T, heads*head_dim] of the cache's type, unit inner stride */
+  affon_rocm_view mask;  /* [B*T, >= T/32 rounded up] u32, unit inner stride; data null: a chain */
+  float scale;
+  int64_t layer;
+  void* output; /* [B*T, heads*head_dim], contiguous, the cache's type */
+  size_t output_bytes;
+} affon_rocm_attention_desc;
+int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                              const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* desc);
+
+/* Keeps the accepted tokens: in every layer, drafted token i < accepted[b] of
+ * sequence b becomes what drafted token path[b, i] was. path[b, :accepted[b]]
+ * ascends strictly (a walk down a tree whose tokens follow their parents), which
+ * a call relies on to move keys and values in place. The
+ * caller then adds accepted[b] to lengths[b]. */
+int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                            const affon_rocm_draft_batch* batch, const affon_rocm_view* path /* [B, n] u32 */,
+                            const uint32_t* accepted /* [B] device words */);
+
+/* The norms before and after a block, with its gate and residual scale:
+ *   u = update, or update / sqrt(mean(update^2) + epsilon) * post_weight (post_norm),
+ *   stream' = stream + scale * gate * u,
+ *   normalized = stream' / sqrt(mean(stream'^2) + epsilon) * weight
+ * of each row, in f32 (normalized from stream' before it is rounded). A null
+ * update leaves the stream as it is (stream_out may then be null); null weights and gates are ones. Every
+ * operand is f32 or bf16 by itself; row strides are in elements. stream_out may be the stream itself. */
+typedef struct {
+  const void* stream;
+  const void* update;
+  const void* gate;        /* [rows, cols], or with gate_stride 0 [cols] */
+  const void* post_weight; /* [cols] */
+  const void* weight;      /* [cols] */
+  void* stream_out;
+  void* normalized;
+  int64_t rows, cols;
+  int64_t stream_stride, update_stride, gate_stride, stream_out_stride, normalized_stride;
+  int32_t stream_dtype /* of stream_out too */, update_dtype, gate_dtype, weight_dtype /* of both weights */, normalized_dtype;
+  int32_t post_norm;
+  float scale, epsilon;
+} affon_rocm_residual_norm_desc;
+int affon_rocm_residual_norm(affon_rocm_session* session, const affon_rocm_residual_norm_desc* desc);
+
 #ifdef __cplusplus
 }
 #endif
