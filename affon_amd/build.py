@@ -38,10 +38,12 @@ EXACT_FLAGS = {"quantize.hip": ["-ffp-contract=off"], "generic.hip": ["-ffp-cont
 # Decode-batch kernels whose MFMA results feed VALU scaling every step: the
 # MFMAs write ordinary VGPRs, so no accumulator-register read
 # (v_accvgpr_read) sits between each MFMA and its scaling. No kernel in
-# these files needs scratch memory with it.
+# these files needs scratch memory with it. The attention kernels' softmax
+# reads every product's result the same way.
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 UNIT_FLAGS = {**EXACT_FLAGS, **{f: VGPR_MFMA for f in ("gemv_mfma.hip", "vrow_b2.hip", "vrow_b4.hip", "vrow_b8.hip",
-                                                     "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip")}}
+                                                     "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip", "attention_bf16.hip",
+                                                     "attention_f32.hip")}}
 
 
 def _sources() -> list[pathlib.Path]:

@@ -1,0 +1,582 @@
+// Attention of drafted tokens over a paged cache on the matrix cores.
+//
+// The query heads that share a key head, G of them, and the T drafted tokens
+// of a sequence make T*G rows over the same keys and values. A wave holds 16
+// to 64 of these rows and walks over keys 32 (bf16) or 16 (f32) at a time:
+//   S^T = K Q^T      (MFMA, rows of the queries as columns of the result),
+//   P = e^(S - m)    (one running reference m per row),
+//   O^T += V^T P^T   (MFMA).
+// Both products leave a query row in the column lane % 16 of a result, so a
+// row's m and sum are plain per-lane values, and P^T leaves the first product
+// in the lanes in which the second one takes it: lane group lane / 16 holds
+// keys 4 (lane / 16) .. + 3 of each 16, and the order of the keys inside a
+// product is free as long as V^T is read in the same one.
+//
+// m follows the largest score only where a score passes it by more than
+// kSlack: e^(S - m) then stays below 2^kSlack, the sums and O are in f32 and
+// a later m only scales them, so that most steps neither reduce across lanes
+// nor touch O.
+//
+// Keys and values reach LDS by direct transfers, several steps ahead; 16
+// keys of one head and page are consecutive in memory, and every transfer
+// moves whole 1 KiB pieces of them. LDS keeps their order, its 16-byte pieces
+// permuted inside each row where the row is a power of two long (the banks
+// would otherwise meet): the permutation is made by the source addresses.
+// bf16 values are read transposed (ds_read_b64_tr_b16).
+#pragma once
+
+#include "lds_pipeline.h"
+#include "paged.h"
+
+namespace affon {
+namespace attention {
+
+using pipeline::bf16x8_t;
+using pipeline::dma16;
+using pipeline::f32x4_t;
+using pipeline::lds_address;
+using pipeline::pack_bf16;
+using pipeline::u32x4_t;
+using pipeline::wait_lds_reads;
+using pipeline::wait_vmcnt;
+typedef short s16x4_t __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) s16x4_t* lds_s16x4;
+
+struct Args {
+  AttentionProblem p;
+  int group;        // query heads per key head
+  int rows;         // T * group
+  int row_groups;   // workgroups that share a sequence's rows
+  uint32_t chunk;   // keys of a workgroup, a multiple of kKeysAhead
+  int splits;       // workgroups along the keys
+  float log2_scale; // |scale| * log2(e)
+  float sign;       // of the scale: a factor of the queries
+  // splits > 1: sums [unit][split][row][head_dim] and (m, l) [unit][split][row],
+  // unit = sequence * kv_heads + key head, row_slots rows each.
+  float* sums;
+  float2* stats;
+  int row_slots;
+};
+
+constexpr float kSlack = 8.0f;
+constexpr float kLowest = -3.0e38f;  // m before the first score
+constexpr int kPageList = 256;       // pages of 16-key tiles that a workgroup holds
+
+// A bf16 word holds an infinity or a NaN in its low or high half.
+__device__ __forceinline__ bool not_finite(uint32_t w, bool half) {
+  if (half) return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
+  return (w & 0x7f800000u) == 0x7f800000u;
+}
+
+// Bits of a row's mask for keys base .. base + 31 of the drafted tokens (base
+// may be negative: committed ones, all seen); none from count on.
+__device__ __forceinline__ uint32_t seen_bits(const AttentionProblem& p, int64_t row, int t, int base, int count) {
+  uint32_t bits;
+  if (p.mask == nullptr) {
+    const int ones = t + 1 - base;
+    bits = ones >= 32 ? ~0u : ones <= 0 ? 0u : (1u << ones) - 1;
+  } else {
+    const uint32_t* words = p.mask + row * p.mask_stride;
+    const int last = (p.batch.rows - 1) / 32;
+    if (base >= 0) {
+      const int w = base / 32, shift = base % 32;
+      const uint32_t low = w <= last ? words[w] : 0u, high = w + 1 <= last ? words[w + 1] : 0u;
+      bits = __funnelshift_r(low, high, shift);
+    } else {
+      bits = base <= -32 ? ~0u : words[0] << -base | ((1u << -base) - 1);
+    }
+  }
+  const int left = count - base;
+  if (left < 32) bits &= left <= 0 ? 0u : (1u << left) - 1;
+  return bits;
+}
+
+// T: element type; DT: 16-wide tiles of the head (an even number); EXACT: the
+// head is 16 * DT wide, 64, 128 or 256, else at most that; RT: 16-row tiles
+// of a wave; WR: waves side by side over the rows, sharing the keys in LDS;
+// WK: waves side by side over the keys, each with its own; STAGES: steps in LDS.
+template <typename T, int DT, bool EXACT, int RT, int WR, int WK, int STAGES>
+struct Kernel {
+  static constexpr bool kHalf = T::bytes == 2;
+  static constexpr int kKT = kHalf ? 2 : 1;  // 16-key tiles of a step
+  static constexpr int kKeys = 16 * kKT;
+  static constexpr int kThreads = 64 * WR * WK;
+  static constexpr int kMaxRow = 16 * DT * T::bytes;             // bytes of a head
+  static constexpr int kTile = (16 * kMaxRow + 1023) / 1024 * 1024;  // LDS bytes of 16 keys
+  static constexpr int kPieces = kTile / 1024;
+  static constexpr int kStage = 2 * kKT * kTile;
+  static constexpr int kQSteps = kHalf ? DT / 2 : DT;  // 64-byte pieces of a head
+  // Transfers of a wave and step: pieces p = wave, wave + WR, .. of the keys'
+  // and the values' 2 * kPieces, each for every tile of the step.
+  static constexpr int kPer = (2 * kPieces + WR - 1) / WR;
+  static constexpr int kTransfers = kPer * kKT;
+  static_assert(WR == 1 || WK == 1, "waves share keys or rows");
+  static_assert(STAGES >= 2 && kTransfers * (STAGES - 1) < 64, "transfers in flight");
+  static constexpr int kRing = WK * STAGES * kStage;
+  // The waves' sums, where they share rows: rows padded by 16 bytes.
+  static constexpr int kJoinRow = 16 * DT + 4;
+  static constexpr int kJoin = WK > 1 ? WK * RT * 16 * kJoinRow * 4 : 0;
+  static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+
+  // Place of 16-byte piece c of key k's row, before the row's own offset.
+  static __device__ __forceinline__ int key_swizzle(int k) { return !EXACT ? 0 : kMaxRow >= 256 ? (k & 15) : (k >> 1) & 7; }
+  static __device__ __forceinline__ int value_swizzle(int k) {
+    if (!EXACT) return 0;
+    if (kHalf) return kMaxRow >= 256 ? 2 * (k & 7) : 2 * ((k >> 1) & 3);
+    return (k >> 2 & 1) << 2;
+  }
+
+  static __device__ void run(const Args& a) {
+    const AttentionProblem& p = a.p;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
+    __shared__ uint32_t page_list[kPageList], line_list[kPageList];
+    __shared__ float2 join_stats[WK > 1 ? WK * RT * 16 : 1];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 15, quad = lane >> 4;
+    const int D = EXACT ? 16 * DT : p.cache.head_dim;
+    const int row_bytes = D * T::bytes;
+
+    // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow
+    // each other there, to find them in its L2.
+    int id = blockIdx.x >> 3;
+    const int rg = id % a.row_groups;
+    id = id / a.row_groups * 8 + (blockIdx.x & 7);
+    const int kv = id % p.cache.kv_heads;
+    id /= p.cache.kv_heads;
+    const int b = id % p.batch.sequences, split = id / p.batch.sequences;
+    if (split >= a.splits) return;
+
+    const uint32_t length = committed(p.batch, b);
+    const uint32_t count = drafted(p.batch, b);
+    const uint32_t n = min(length + count, p.batch.capacity);
+    const uint32_t begin = min(static_cast<uint32_t>(split) * a.chunk, n);
+    const uint32_t end = split == a.splits - 1 ? n : min(begin + a.chunk, n);
+    if (begin >= end && a.splits > 1) return;
+
+    // This wave's rows, as columns of its results.
+    const int row0 = (rg * WR + (WR > 1 ? wave : 0)) * RT * 16;
+    const uint8_t* queries = p.query + static_cast<int64_t>(b) * p.batch.rows * p.query_stride * T::bytes;
+    const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * T::bytes)) % 16 == 0;
+    u32x4_t q[RT][kQSteps];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      const int r = row0 + rt * 16 + col, t = r / a.group;
+      const uint8_t* from = queries + (t * p.query_stride + static_cast<int64_t>(kv * a.group + r - t * a.group) * D) * T::bytes;
+#pragma unroll
+      for (int s = 0; s < kQSteps; ++s) {
+        const int at = s * 64 + quad * 16;
+        u32x4_t v{0, 0, 0, 0};
+        if (r < a.rows && at < row_bytes) {
+          if (aligned) {
+            v = *reinterpret_cast<const u32x4_t*>(from + at);
+          } else {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              if constexpr (kHalf) {
+                const auto* h = reinterpret_cast<const uint16_t*>(from + at + 4 * e);
+                v[e] = h[0] | static_cast<uint32_t>(h[1]) << 16;
+              } else {
+                v[e] = *reinterpret_cast<const uint32_t*>(from + at + 4 * e);
+              }
+            }
+          }
+        }
+        // The scale's sign (0: every score is 0).
+        if (a.sign != 1.0f) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) v[e] = a.sign == 0.0f ? 0u : v[e] ^ (kHalf ? 0x80008000u : 0x80000000u);
+        }
+        q[rt][s] = v;
+      }
+    }
+
+    f32x4_t o[RT][DT];
+    float m[RT], l[RT];
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kLowest;
+      l[rt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0, 0, 0, 0};
+    }
+
+    // Transfers: where this lane's 16 bytes of every piece come from.
+    uint32_t from[kPer];
+    const int first_piece = WR > 1 ? wave : 0;
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int piece = min(first_piece + i * WR, 2 * kPieces - 1);
+      const int at = (piece % kPieces) * 1024 + lane * 16;
+      if constexpr (EXACT) {
+        const int k = at / kMaxRow, c = at % kMaxRow / 16;
+        from[i] = k * kMaxRow + (c ^ (piece >= kPieces ? value_swizzle(k) : key_swizzle(k))) * 16;
+      } else {
+        from[i] = min(at, 16 * row_bytes - 16);  // rows that are shorter end before the tile does
+      }
+    }
+    const uint32_t ring = lds_address(lds) + (WK > 1 ? wave * STAGES * kStage : 0);
+    const uint8_t* ring_data = lds + (WK > 1 ? wave * STAGES * kStage : 0);
+    const int64_t head_bytes = static_cast<int64_t>(p.cache.page_size) * row_bytes;
+
+    for (uint32_t segment = begin; segment < end; segment += kPageList * 16) {
+      const uint32_t segment_end = min(end, segment + kPageList * 16);
+      __syncthreads();
+      for (uint32_t i = threadIdx.x; i < kPageList && segment + i * 16 < segment_end; i += kThreads) {
+        const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
+        page_list[i] = page_of(p.cache, p.batch, b, index);
+        line_list[i] = at - index * p.cache.page_size;
+      }
+      __syncthreads();
+      const int all = static_cast<int>((segment_end - segment + kKeys - 1) / kKeys);
+      // Steps of this wave: first, first + stride, .. below all.
+      const int first = WK > 1 ? wave : 0;
+      const int steps = all > first ? (all - first + WK - 1) / WK : 0;
+
+      auto issue = [&](int step) {
+        const int s = (first + step * WK) * kKT;
+        const uint32_t to = ring + (step % STAGES) * kStage;
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt) {
+          // A tile past the last one repeats it: the keys there are not seen.
+          const int tile = min(s + kt, static_cast<int>((segment_end - segment - 1) / 16));
+          const uint32_t page = __builtin_amdgcn_readfirstlane(page_list[tile]);
+          const uint32_t line = __builtin_amdgcn_readfirstlane(line_list[tile]);
+          const int64_t at = (static_cast<int64_t>(page == kNoPage ? 0 : page) * p.cache.kv_heads + kv) * head_bytes +
+                             static_cast<int64_t>(line) * row_bytes;
+#pragma unroll
+          for (int i = 0; i < kPer; ++i) {
+            const int piece = min(first_piece + i * WR, 2 * kPieces - 1);
+            const bool value = piece >= kPieces;
+            dma16((value ? p.cache.values : p.cache.keys) + at, from[i],
+                  to + (value ? kKT * kTile : 0) + kt * kTile + (value ? piece - kPieces : piece) * 1024);
+          }
+        }
+      };
+#pragma unroll
+      for (int s = 0; s < STAGES - 1; ++s)
+        if (s < steps) issue(s);
+
+      for (int step = 0; step < steps; ++step) {
+        if (step + STAGES - 1 <= steps)
+          wait_vmcnt<(STAGES - 2) * kTransfers>();
+        else
+          wait_vmcnt<0>();
+        if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (step + STAGES - 1 < steps) issue(step + STAGES - 1);
+
+        const uint8_t* keys = ring_data + (step % STAGES) * kStage;
+        const uint8_t* values = keys + kKT * kTile;
+        const uint32_t key0 = segment + static_cast<uint32_t>(first + step * WK) * kKeys;
+
+        // ---- scores ----
+        f32x4_t s[RT][kKT];
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4_t{0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < kQSteps; ++i) {
+            const int c = i * 4 + quad;
+            u32x4_t k;
+            if constexpr (EXACT) {
+              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + col * kMaxRow + (c ^ key_swizzle(col)) * 16);
+            } else {
+              // Past the head: zeros, as the queries hold there.
+              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + col * row_bytes + min(c * 16, row_bytes - 16));
+              if (c * 16 >= row_bytes) k = u32x4_t{0, 0, 0, 0};
+            }
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              if constexpr (kHalf) {
+                s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k),
+                                                                    __builtin_bit_cast(bf16x8_t, q[rt][i]), s[rt][kt], 0, 0, 0);
+              } else {
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                  const uint32_t ke = k[e], qe = q[rt][i][e];
+                  s[rt][kt] = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ke), __uint_as_float(qe), s[rt][kt], 0, 0, 0);
+                }
+              }
+            }
+          }
+        }
+
+        // ---- steps with keys that not every row sees ----
+        bool edge = key0 + kKeys > length;
+        uint32_t there = 0;  // bits of the step's keys that lie anywhere
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt) {
+          const int tile = static_cast<int>((key0 - segment) / 16) + kt;
+          const bool lies = segment + tile * 16 < segment_end &&
+                            __builtin_amdgcn_readfirstlane(page_list[tile]) != kNoPage;
+          if (lies) there |= 0xffffu << (16 * kt);
+          edge |= !lies;
+        }
+        uint32_t flagged = 0;
+        uint32_t seen[RT];
+        if (edge) {
+          const int base = static_cast<int>(key0) - static_cast<int>(length);
+          const int left = static_cast<int>(n) - static_cast<int>(length);  // drafted tokens that have a place
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) {
+            const int t = min(row0 + rt * 16 + col, a.rows - 1) / a.group;
+            seen[rt] = there & seen_bits(p, static_cast<int64_t>(b) * p.batch.rows + t, t, base, left);
+#pragma unroll
+            for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+              for (int i = 0; i < 4; ++i)
+                if (!(seen[rt] >> (16 * kt + 4 * quad + i) & 1)) s[rt][kt][i] = -INFINITY;
+          }
+          // Values that some row does not see must not reach its sums as 0 *
+          // infinity: those of no token are cleared, and those of drafted
+          // tokens that are not finite are cleared and added by themselves.
+          const int past = static_cast<int>(n) - static_cast<int>(key0);
+          const uint32_t exists = there & (past >= 32 ? ~0u : past <= 0 ? 0u : (1u << past) - 1);
+          const uint32_t all_see = base >= 0 ? 0u : base <= -32 ? ~0u : (1u << -base) - 1;
+          uint32_t bad = 0;
+          auto for_pieces = [&](auto&& f) {
+#pragma unroll
+            for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+              for (int i = 0; i < kPieces; ++i) {
+                const int at = i * 1024 + lane * 16;
+                if (at < 16 * row_bytes) f(kt * 16 + at / row_bytes, const_cast<uint8_t*>(values) + kt * kTile + at);
+              }
+          };
+          for_pieces([&](int k, uint8_t* piece) {
+            const u32x4_t v = *reinterpret_cast<const u32x4_t*>(piece);
+            if (not_finite(v[0], kHalf) || not_finite(v[1], kHalf) || not_finite(v[2], kHalf) || not_finite(v[3], kHalf))
+              bad |= 1u << k;
+          });
+#pragma unroll
+          for (int offset = 32; offset > 0; offset >>= 1) bad |= __shfl_xor(bad, offset);
+          flagged = __builtin_amdgcn_readfirstlane(bad) & exists & ~all_see;
+          const uint32_t clear = flagged | (~exists & (kKeys == 32 ? ~0u : 0xffffu));
+          if constexpr (WR > 1) __syncthreads();  // every wave has looked
+          if (clear != 0)
+            for_pieces([&](int k, uint8_t* piece) {
+              if (clear >> k & 1) *reinterpret_cast<u32x4_t*>(piece) = u32x4_t{0, 0, 0, 0};
+            });
+          if constexpr (WR > 1)
+            __syncthreads();
+          else
+            wait_lds_reads();
+        }
+
+        // ---- softmax ----
+        u32x4_t packed[RT];
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          float top = fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3]));
+          if constexpr (kKT == 2)
+            top = fmaxf(top, fmaxf(fmaxf(s[rt][kKT - 1][0], s[rt][kKT - 1][1]), fmaxf(s[rt][kKT - 1][2], s[rt][kKT - 1][3])));
+          top *= a.log2_scale;
+          if (__any(top > m[rt] + kSlack)) {
+            top = fmaxf(top, __shfl_xor(top, 16));
+            top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m[rt]);
+            const float keep = __builtin_amdgcn_exp2f(m[rt] - top);
+            m[rt] = top;
+            l[rt] *= keep;
+#pragma unroll
+            for (int dt = 0; dt < DT; ++dt) o[rt][dt] *= keep;
+          }
+#pragma unroll
+          for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              s[rt][kt][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kt][i], a.log2_scale, -m[rt]));
+              l[rt] += s[rt][kt][i];
+            }
+          if constexpr (kHalf)
+            packed[rt] = u32x4_t{pack_bf16(s[rt][0][0], s[rt][0][1]), pack_bf16(s[rt][0][2], s[rt][0][3]),
+                                 pack_bf16(s[rt][kKT - 1][0], s[rt][kKT - 1][1]),
+                                 pack_bf16(s[rt][kKT - 1][2], s[rt][kKT - 1][3])};
+        }
+
+        // ---- sums of values ----
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          if constexpr (kHalf) {
+            // Lanes 4e .. 4e + 3 of 16 address key 4 * quad + e; lane j gets column j of the four.
+            const int k = 4 * quad + (col >> 2), at = 2 * dt + ((col & 3) >> 1);
+            const int row = EXACT ? k * kMaxRow : k * row_bytes;
+            const int off = row + (at ^ value_swizzle(k)) * 16 + (col & 1) * 8;
+            u32x2_t v[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+              const uint32_t address = lds_address(values + kt * kTile + (EXACT ? off : min(off, 16 * row_bytes - 8)));
+              v[kt] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                      reinterpret_cast<lds_s16x4>(static_cast<uintptr_t>(address))));
+            }
+            const u32x4_t v8{v[0][0], v[0][1], v[1][0], v[1][1]};
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt)
+              o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v8),
+                                                                  __builtin_bit_cast(bf16x8_t, packed[rt]), o[rt][dt], 0, 0, 0);
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int k = 4 * quad + i, c = 4 * dt + (col >> 2);
+              const int off = (EXACT ? k * kMaxRow : k * row_bytes) + (c ^ value_swizzle(k)) * 16 + (col & 3) * 4;
+              const float v = *reinterpret_cast<const float*>(values + (EXACT ? off : min(off, 16 * row_bytes - 4)));
+#pragma unroll
+              for (int rt = 0; rt < RT; ++rt)
+                o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[rt][0][i], o[rt][dt], 0, 0, 0);
+            }
+          }
+        }
+
+        if (flagged != 0) {  // rare: a drafted token's value that is not finite, for the rows that see it
+          for (int k = 0; k < kKeys; ++k) {
+            if (!(flagged >> k & 1)) continue;
+            const int64_t line = line_of(p.cache, p.batch, b, key0 + k) + static_cast<int64_t>(kv) * p.cache.page_size;
+#pragma unroll
+            for (int rt = 0; rt < RT; ++rt) {
+              float e = 0.0f;
+#pragma unroll
+              for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i)
+                  if (k / 16 == kt && k % 4 == i) e = s[rt][kt][i];
+              e = __shfl(e, (k % 16) / 4 * 16 + col);
+              if (!(seen[rt] >> k & 1)) continue;
+#pragma unroll
+              for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                  const int d = 16 * dt + 4 * quad + i;
+                  if (d < D) o[rt][dt][i] = fmaf(e, T::load(p.cache.values, line * D + d), o[rt][dt][i]);
+                }
+            }
+          }
+        }
+        wait_lds_reads();
+      }
+    }
+
+    // ---- results ----
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      l[rt] += __shfl_xor(l[rt], 16);
+      l[rt] += __shfl_xor(l[rt], 32);
+    }
+    const int64_t unit = static_cast<int64_t>(b) * p.cache.kv_heads + kv;
+    const int64_t part = (unit * a.splits + split) * a.row_slots;
+    // Four values of a row, d .. d + 3: of the result, or of this split's sums.
+    auto write = [&](int r, int d, f32x4_t v, float row_m, float row_l) {
+      if (r >= a.rows || d >= D) return;
+      if (a.splits > 1) {
+        *reinterpret_cast<f32x4_t*>(a.sums + (part + r) * D + d) = v;
+        if (d == 0) a.stats[part + r] = float2{row_m, row_l};
+        return;
+      }
+      const int t = r / a.group;
+      const float scale = row_l == 0.0f || t >= static_cast<int>(count) ? 0.0f : 1.0f / row_l;
+      v = scale == 0.0f ? f32x4_t{0, 0, 0, 0} : v * scale;
+      const int64_t to = ((static_cast<int64_t>(b) * p.batch.rows + t) * p.heads + kv * a.group + r - t * a.group) * D + d;
+      if constexpr (kHalf) {
+        const u32x2_t h{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+        if (reinterpret_cast<uintptr_t>(p.out) % 8 == 0) {
+          *reinterpret_cast<u32x2_t*>(p.out + to * 2) = h;
+        } else {
+          auto* out = reinterpret_cast<uint16_t*>(p.out) + to;
+#pragma unroll
+          for (int e = 0; e < 4; ++e) out[e] = static_cast<uint16_t>(h[e / 2] >> (16 * (e % 2)));
+        }
+      } else if (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) {
+        *reinterpret_cast<f32x4_t*>(p.out + to * 4) = v;
+      } else {
+        auto* out = reinterpret_cast<float*>(p.out) + to;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) out[e] = v[e];
+      }
+    };
+    if constexpr (WK == 1) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) write(row0 + rt * 16 + col, 16 * dt + 4 * quad, o[rt][dt], m[rt], l[rt]);
+    } else {
+      auto* joined = reinterpret_cast<float*>(lds);
+      __syncthreads();  // the ring is free
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        const int r = wave * RT * 16 + rt * 16 + col;
+        if (quad == 0) join_stats[r] = float2{m[rt], l[rt]};
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) *reinterpret_cast<f32x4_t*>(joined + r * kJoinRow + 16 * dt + 4 * quad) = o[rt][dt];
+      }
+      __syncthreads();
+      const int pieces = D / 4;
+      for (int i = threadIdx.x; i < RT * 16 * pieces; i += kThreads) {
+        const int r = i / pieces, d = (i - r * pieces) * 4;
+        if (row0 + r >= a.rows) break;
+        float top = kLowest, sum = 0.0f;
+#pragma unroll
+        for (int w = 0; w < WK; ++w) top = fmaxf(top, join_stats[w * RT * 16 + r].x);
+        f32x4_t v{0, 0, 0, 0};
+#pragma unroll
+        for (int w = 0; w < WK; ++w) {
+          const float2 st = join_stats[w * RT * 16 + r];
+          const float keep = __builtin_amdgcn_exp2f(st.x - top);
+          sum = fmaf(st.y, keep, sum);
+          v += *reinterpret_cast<const f32x4_t*>(joined + (w * RT * 16 + r) * kJoinRow + d) * keep;
+        }
+        write(row0 + r, d, v, top, sum);
+      }
+    }
+  }
+};
+
+template <typename K>
+__global__ __launch_bounds__(K::kThreads) void kernel(Args a) {
+  K::run(a);
+}
+
+// Shape of the kernel that takes `rows` rows: 16-row tiles of a wave, waves
+// over the rows (1: waves over the keys).
+struct Shape {
+  int tiles, waves;
+  int rows() const { return 16 * tiles * waves; }
+};
+
+void launch_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+
+template <typename T, int DT, bool EXACT, int RT, int WR>
+void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
+  using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
+  // Waves over the keys: as many as two stages each leave room for.
+  constexpr int WK = WR > 1 ? 1 : Probe::kStage > 16384 ? 2 : 4;
+  constexpr int STAGES = WR == 1 ? 2 : 3;
+  using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
+  hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
+}
+
+template <typename T, int DT, bool EXACT>
+void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
+  if (shape.waves == 1) {
+    if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1>(a, grid, stream);
+    return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
+  }
+  if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
+  return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
+}
+
+template <typename T>
+void launch_head(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
+  const int D = a.p.cache.head_dim;
+  if (D == 64) return launch_width<T, 4, true>(a, shape, grid, stream);
+  if (D == 128) return launch_width<T, 8, true>(a, shape, grid, stream);
+  if (D == 256) return launch_width<T, 16, true>(a, shape, grid, stream);
+  if (D < 64) return launch_width<T, 4, false>(a, shape, grid, stream);
+  if (D <= 96) return launch_width<T, 6, false>(a, shape, grid, stream);
+  if (D < 128) return launch_width<T, 8, false>(a, shape, grid, stream);
+  launch_width<T, 16, false>(a, shape, grid, stream);
+}
+
+}  // namespace attention
+}  // namespace affon
