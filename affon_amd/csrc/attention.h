@@ -55,13 +55,22 @@ struct Args {
   // splits > 1: sums [unit][split][row][head_dim] and (m, l) [unit][split][row],
   // unit = sequence * kv_heads + key head, row_slots rows each.
   float* sums;
-  float2* stats;
+  float* stats;
   int row_slots;
+  // One per unit and row group, 0 between calls: the workgroup that raises it
+  // to the number of splits in use joins their results. Null: a second launch does.
+  uint32_t* tickets;
 };
 
 constexpr float kSlack = 8.0f;
 constexpr float kLowest = -3.0e38f;  // m before the first score
 constexpr int kPageList = 256;       // pages of 16-key tiles that a workgroup holds
+
+// A value the compiler keeps in a register instead of computing it again.
+__device__ __forceinline__ int pinned(int v) {
+  asm volatile("" : "+v"(v));
+  return v;
+}
 
 // A bf16 word holds an infinity or a NaN in its low or high half.
 __device__ __forceinline__ bool not_finite(uint32_t w, bool half) {
@@ -92,6 +101,87 @@ __device__ __forceinline__ uint32_t seen_bits(const AttentionProblem& p, int64_t
   return bits;
 }
 
+// Results of one split, which a workgroup on another XCD may join: stored past
+// this XCD's L2 and loaded past the reader's (relaxed accesses of agent scope),
+// so that neither side has to write back or drop a whole cache: with fences
+// instead, 32 sequences of one token each over up to 4160 tokens took 197 us
+// in five splits, against 76 in two launches.
+__device__ __forceinline__ void store_shared(float* to, float a, float b) {
+  const uint64_t v = __float_as_uint(a) | static_cast<uint64_t>(__float_as_uint(b)) << 32;
+  __hip_atomic_store(reinterpret_cast<uint64_t*>(to), v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+}
+__device__ __forceinline__ float2 load_shared(const float* from) {
+  const uint64_t v = __hip_atomic_load(reinterpret_cast<const uint64_t*>(from), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+  return float2{__uint_as_float(static_cast<uint32_t>(v)), __uint_as_float(static_cast<uint32_t>(v >> 32))};
+}
+
+// Values at .. at + 3 of the result: sums over their probabilities' sum (0: nothing was seen).
+template <typename T>
+__device__ __forceinline__ void store_result(uint8_t* out, int64_t at, f32x4_t v, float sum) {
+  v = sum == 0.0f ? f32x4_t{0, 0, 0, 0} : v * (1.0f / sum);
+  if constexpr (T::bytes == 2) {
+    const u32x2_t h{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
+    if (reinterpret_cast<uintptr_t>(out) % 8 == 0) {
+      *reinterpret_cast<u32x2_t*>(out + at * 2) = h;
+    } else {
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        reinterpret_cast<uint16_t*>(out)[at + e] = static_cast<uint16_t>(e % 2 ? h[e / 2] >> 16 : h[e / 2]);
+    }
+  } else if (reinterpret_cast<uintptr_t>(out) % 16 == 0) {
+    *reinterpret_cast<f32x4_t*>(out + at * 4) = v;
+  } else {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) reinterpret_cast<float*>(out)[at + e] = v[e];
+  }
+}
+
+// sum_s 2^(m_s - m) sums_s, d .. d + 3, over the splits s = first, first + step,
+// .. below `used` of the row whose slot in split 0 is `slot`, with *max = m the
+// largest m_s and *sum = sum_s 2^(m_s - m) l_s. kAtOnce
+// splits are loaded together: their time is the memory's latency (one by one,
+// the 63 splits of one sequence of 32000 tokens took 40 us).
+template <bool SHARED>
+__device__ __forceinline__ f32x4_t joined_sums(const Args& a, int64_t slot, int d, int D, uint32_t first, uint32_t used,
+                                               uint32_t step, float* max, float* sum) {
+  constexpr int kAtOnce = 8;
+  float top = kLowest, l = 0.0f;
+  f32x4_t v{0, 0, 0, 0};
+  for (uint32_t s0 = first; s0 < used; s0 += kAtOnce * step) {
+    float2 st[kAtOnce];
+    f32x4_t part[kAtOnce];
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      const int64_t at = slot + static_cast<int64_t>(min(s0 + i * step, used - 1)) * a.row_slots;
+      if constexpr (SHARED) {
+        st[i] = load_shared(a.stats + 2 * at);
+        const float2 low = load_shared(a.sums + at * D + d), high = load_shared(a.sums + at * D + d + 2);
+        part[i] = f32x4_t{low.x, low.y, high.x, high.y};
+      } else {
+        st[i] = *reinterpret_cast<const float2*>(a.stats + 2 * at);
+        part[i] = *reinterpret_cast<const f32x4_t*>(a.sums + at * D + d);
+      }
+    }
+    float peak = top;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) peak = fmaxf(peak, st[i].x);
+    const float keep = __builtin_amdgcn_exp2f(top - peak);
+    top = peak;
+    l *= keep;
+    v *= keep;
+#pragma unroll
+    for (int i = 0; i < kAtOnce; ++i) {
+      if (s0 + i * step >= used) break;
+      const float w = __builtin_amdgcn_exp2f(st[i].x - top);
+      l = fmaf(st[i].y, w, l);
+      v += part[i] * w;
+    }
+  }
+  *max = top;
+  *sum = l;
+  return v;
+}
+
 // T: element type; DT: 16-wide tiles of the head (an even number); EXACT: the
 // head is 16 * DT wide, 64, 128 or 256, else at most that; RT: 16-row tiles
 // of a wave; WR: waves side by side over the rows, sharing the keys in LDS;
@@ -111,6 +201,10 @@ struct Kernel {
   // and the values' 2 * kPieces, each for every tile of the step.
   static constexpr int kPer = (2 * kPieces + WR - 1) / WR;
   static constexpr int kTransfers = kPer * kKT;
+#ifndef MINW
+#define MINW 1
+#endif
+  static constexpr int kMinWaves = WR > 1 && RT == 2 && DT == 8 ? MINW : 1;
   static_assert(WR == 1 || WK == 1, "waves share keys or rows");
   static_assert(STAGES >= 2 && kTransfers * (STAGES - 1) < 64, "transfers in flight");
   static constexpr int kRing = WK * STAGES * kStage;
@@ -118,6 +212,11 @@ struct Kernel {
   static constexpr int kJoinRow = 16 * DT + 4;
   static constexpr int kJoin = WK > 1 ? WK * RT * 16 * kJoinRow * 4 : 0;
   static constexpr int kLds = kRing > kJoin ? kRing : kJoin;
+
+  // Offsets of a lane's reads that its permutation sets: the later ones follow
+  // at whole multiples.
+  static constexpr int kKeySpots = !EXACT ? 1 : kQSteps < 4 ? kQSteps : 4;
+  static constexpr int kValueSpots = !EXACT ? 1 : kHalf ? (DT < 8 ? DT : 8) : 2;
 
   // Place of 16-byte piece c of key k's row, before the row's own offset.
   static __device__ __forceinline__ int key_swizzle(int k) { return !EXACT ? 0 : kMaxRow >= 256 ? (k & 15) : (k >> 1) & 7; }
@@ -130,7 +229,8 @@ struct Kernel {
   static __device__ void run(const Args& a) {
     const AttentionProblem& p = a.p;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-    __shared__ uint32_t page_list[kPageList], line_list[kPageList];
+    __shared__ int64_t tile_list[kPageList];  // byte offsets of 16-key tiles in keys and values, or -1
+    __shared__ int missing;
     __shared__ float2 join_stats[WK > 1 ? WK * RT * 16 : 1];
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -148,12 +248,20 @@ struct Kernel {
     const int b = id % p.batch.sequences, split = id / p.batch.sequences;
     if (split >= a.splits) return;
 
+    // The page list's first part, whose loads need not wait for the lengths.
+    const uint32_t start = static_cast<uint32_t>(split) * a.chunk;
+    const uint32_t early_at = start + threadIdx.x * 16;
+    uint32_t early = kNoPage;
+    if (early_at < p.batch.capacity) early = p.batch.table[b * p.batch.table_stride + early_at / p.cache.page_size];
+
     const uint32_t length = committed(p.batch, b);
     const uint32_t count = drafted(p.batch, b);
     const uint32_t n = min(length + count, p.batch.capacity);
-    const uint32_t begin = min(static_cast<uint32_t>(split) * a.chunk, n);
+    const uint32_t begin = min(start, n);
     const uint32_t end = split == a.splits - 1 ? n : min(begin + a.chunk, n);
-    if (begin >= end && a.splits > 1) return;
+    if (begin >= end && split > 0) return;
+    const uint32_t used = max(1u, (n + a.chunk - 1) / a.chunk);  // splits that hold keys
+    const bool whole = a.splits == 1 || used == 1;               // the result is this workgroup's
 
     // This wave's rows, as columns of its results.
     const int row0 = (rg * WR + (WR > 1 ? wave : 0)) * RT * 16;
@@ -162,36 +270,27 @@ struct Kernel {
     u32x4_t q[RT][kQSteps];
 #pragma unroll
     for (int rt = 0; rt < RT; ++rt) {
-      const int r = row0 + rt * 16 + col, t = r / a.group;
+      // Rows past the last one and dims past the head load what lies before them.
+      const int r = min(row0 + rt * 16 + col, a.rows - 1), t = r / a.group;
       const uint8_t* from = queries + (t * p.query_stride + static_cast<int64_t>(kv * a.group + r - t * a.group) * D) * T::bytes;
 #pragma unroll
       for (int s = 0; s < kQSteps; ++s) {
-        const int at = s * 64 + quad * 16;
-        u32x4_t v{0, 0, 0, 0};
-        if (r < a.rows && at < row_bytes) {
-          if (aligned) {
-            v = *reinterpret_cast<const u32x4_t*>(from + at);
-          } else {
+        const uint8_t* piece = from + min(s * 64 + quad * 16, row_bytes - 16);
+        if (aligned) {
+          q[rt][s] = *reinterpret_cast<const u32x4_t*>(piece);
+        } else {
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              if constexpr (kHalf) {
-                const auto* h = reinterpret_cast<const uint16_t*>(from + at + 4 * e);
-                v[e] = h[0] | static_cast<uint32_t>(h[1]) << 16;
-              } else {
-                v[e] = *reinterpret_cast<const uint32_t*>(from + at + 4 * e);
-              }
+          for (int e = 0; e < 4; ++e) {
+            if constexpr (kHalf) {
+              const auto* h = reinterpret_cast<const uint16_t*>(piece) + 2 * e;
+              q[rt][s][e] = h[0] | static_cast<uint32_t>(h[1]) << 16;
+            } else {
+              q[rt][s][e] = reinterpret_cast<const uint32_t*>(piece)[e];
             }
           }
         }
-        // The scale's sign (0: every score is 0).
-        if (a.sign != 1.0f) {
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = a.sign == 0.0f ? 0u : v[e] ^ (kHalf ? 0x80008000u : 0x80000000u);
-        }
-        q[rt][s] = v;
       }
     }
-
     f32x4_t o[RT][DT];
     float m[RT], l[RT];
 #pragma unroll
@@ -201,6 +300,17 @@ struct Kernel {
 #pragma unroll
       for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0, 0, 0, 0};
     }
+
+    auto place_queries = [&] {  // dims past the head are 0, and the scale's sign is theirs
+      const uint32_t keep = a.sign == 0.0f ? 0u : ~0u, flip = a.sign < 0.0f ? (kHalf ? 0x80008000u : 0x80000000u) : 0u;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int s = 0; s < kQSteps; ++s)
+#pragma unroll
+          for (int e = 0; e < 4; ++e)
+            q[rt][s][e] = !EXACT && s * 64 + quad * 16 >= row_bytes ? 0u : (q[rt][s][e] & keep) ^ flip;
+    };
 
     // Transfers: where this lane's 16 bytes of every piece come from.
     uint32_t from[kPer];
@@ -216,6 +326,22 @@ struct Kernel {
         from[i] = min(at, 16 * row_bytes - 16);  // rows that are shorter end before the tile does
       }
     }
+    // Where this lane reads the step's keys and values, from the step's place
+    // in LDS on; pinned, so that the loop adds one base to them.
+    int key_at[kKeySpots], value_at[kValueSpots];
+#pragma unroll
+    for (int i = 0; i < kKeySpots; ++i) key_at[i] = pinned(col * row_bytes + ((i * 4 + quad) ^ key_swizzle(col)) * 16);
+#pragma unroll
+    for (int i = 0; i < kValueSpots; ++i) {
+      if constexpr (kHalf) {
+        // Lanes 4e .. 4e + 3 of 16 address key 4 * quad + e; lane j gets column j of the four.
+        const int k = 4 * quad + (col >> 2);
+        value_at[i] = pinned(k * row_bytes + ((2 * i + ((col & 3) >> 1)) ^ value_swizzle(k)) * 16 + (col & 1) * 8);
+      } else {
+        const int k = 4 * quad;
+        value_at[i] = pinned(k * row_bytes + ((4 * i + (col >> 2)) ^ value_swizzle(k)) * 16 + (col & 3) * 4);
+      }
+    }
     const uint32_t ring = lds_address(lds) + (WK > 1 ? wave * STAGES * kStage : 0);
     const uint8_t* ring_data = lds + (WK > 1 ? wave * STAGES * kStage : 0);
     const int64_t head_bytes = static_cast<int64_t>(p.cache.page_size) * row_bytes;
@@ -223,12 +349,21 @@ struct Kernel {
     for (uint32_t segment = begin; segment < end; segment += kPageList * 16) {
       const uint32_t segment_end = min(end, segment + kPageList * 16);
       __syncthreads();
+      if (threadIdx.x == 0) missing = 0;
+      __syncthreads();
       for (uint32_t i = threadIdx.x; i < kPageList && segment + i * 16 < segment_end; i += kThreads) {
         const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
-        page_list[i] = page_of(p.cache, p.batch, b, index);
-        line_list[i] = at - index * p.cache.page_size;
+        const uint32_t page = segment == begin && i < kThreads
+                                  ? (early < static_cast<uint32_t>(p.cache.pages) ? early : kNoPage)
+                                  : page_of(p.cache, p.batch, b, index);
+        tile_list[i] = page == kNoPage ? -1
+                                       : (static_cast<int64_t>(page) * p.cache.kv_heads + kv) * head_bytes +
+                                             static_cast<int64_t>(at - index * p.cache.page_size) * row_bytes;
+        if (page == kNoPage) missing = 1;
       }
       __syncthreads();
+      if (segment == begin) place_queries();
+      const bool gaps = __builtin_amdgcn_readfirstlane(missing) != 0;
       const int all = static_cast<int>((segment_end - segment + kKeys - 1) / kKeys);
       // Steps of this wave: first, first + stride, .. below all.
       const int first = WK > 1 ? wave : 0;
@@ -241,15 +376,16 @@ struct Kernel {
         for (int kt = 0; kt < kKT; ++kt) {
           // A tile past the last one repeats it: the keys there are not seen.
           const int tile = min(s + kt, static_cast<int>((segment_end - segment - 1) / 16));
-          const uint32_t page = __builtin_amdgcn_readfirstlane(page_list[tile]);
-          const uint32_t line = __builtin_amdgcn_readfirstlane(line_list[tile]);
-          const int64_t at = (static_cast<int64_t>(page == kNoPage ? 0 : page) * p.cache.kv_heads + kv) * head_bytes +
-                             static_cast<int64_t>(line) * row_bytes;
+          const int64_t listed = tile_list[tile];
+          const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(listed >> 32))) << 32 |
+                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(listed)));
+          const uint8_t* key_tile = p.cache.keys + max(at, static_cast<int64_t>(0));
+          const uint8_t* value_tile = p.cache.values + max(at, static_cast<int64_t>(0));
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int piece = min(first_piece + i * WR, 2 * kPieces - 1);
             const bool value = piece >= kPieces;
-            dma16((value ? p.cache.values : p.cache.keys) + at, from[i],
+            dma16(value ? value_tile : key_tile, from[i],
                   to + (value ? kKT * kTile : 0) + kt * kTile + (value ? piece - kPieces : piece) * 1024);
           }
         }
@@ -257,7 +393,6 @@ struct Kernel {
 #pragma unroll
       for (int s = 0; s < STAGES - 1; ++s)
         if (s < steps) issue(s);
-
       for (int step = 0; step < steps; ++step) {
         if (step + STAGES - 1 <= steps)
           wait_vmcnt<(STAGES - 2) * kTransfers>();
@@ -282,7 +417,7 @@ struct Kernel {
             const int c = i * 4 + quad;
             u32x4_t k;
             if constexpr (EXACT) {
-              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + col * kMaxRow + (c ^ key_swizzle(col)) * 16);
+              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + key_at[i % kKeySpots] + i / kKeySpots * kKeySpots * 64);
             } else {
               // Past the head: zeros, as the queries hold there.
               k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + col * row_bytes + min(c * 16, row_bytes - 16));
@@ -305,21 +440,19 @@ struct Kernel {
         }
 
         // ---- steps with keys that not every row sees ----
-        bool edge = key0 + kKeys > length;
-        uint32_t there = 0;  // bits of the step's keys that lie anywhere
-#pragma unroll
-        for (int kt = 0; kt < kKT; ++kt) {
-          const int tile = static_cast<int>((key0 - segment) / 16) + kt;
-          const bool lies = segment + tile * 16 < segment_end &&
-                            __builtin_amdgcn_readfirstlane(page_list[tile]) != kNoPage;
-          if (lies) there |= 0xffffu << (16 * kt);
-          edge |= !lies;
-        }
+        const bool edge = gaps || key0 + kKeys > length;
         uint32_t flagged = 0;
         uint32_t seen[RT];
         if (edge) {
           const int base = static_cast<int>(key0) - static_cast<int>(length);
           const int left = static_cast<int>(n) - static_cast<int>(length);  // drafted tokens that have a place
+          uint32_t there = 0;  // bits of the step's keys that lie anywhere
+#pragma unroll
+          for (int kt = 0; kt < kKT; ++kt) {
+            const int tile = static_cast<int>((key0 - segment) / 16) + kt;
+            if (segment + tile * 16 < segment_end && __builtin_amdgcn_readfirstlane(static_cast<int>(tile_list[tile] >> 32)) >= 0)
+              there |= 0xffffu << (16 * kt);
+          }
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) {
             const int t = min(row0 + rt * 16 + col, a.rows - 1) / a.group;
@@ -400,10 +533,7 @@ struct Kernel {
 #pragma unroll
         for (int dt = 0; dt < DT; ++dt) {
           if constexpr (kHalf) {
-            // Lanes 4e .. 4e + 3 of 16 address key 4 * quad + e; lane j gets column j of the four.
-            const int k = 4 * quad + (col >> 2), at = 2 * dt + ((col & 3) >> 1);
-            const int row = EXACT ? k * kMaxRow : k * row_bytes;
-            const int off = row + (at ^ value_swizzle(k)) * 16 + (col & 1) * 8;
+            const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 32;
             u32x2_t v[2];
 #pragma unroll
             for (int kt = 0; kt < 2; ++kt) {
@@ -419,8 +549,7 @@ struct Kernel {
           } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-              const int k = 4 * quad + i, c = 4 * dt + (col >> 2);
-              const int off = (EXACT ? k * kMaxRow : k * row_bytes) + (c ^ value_swizzle(k)) * 16 + (col & 3) * 4;
+              const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 64 + i * row_bytes;
               const float v = *reinterpret_cast<const float*>(values + (EXACT ? off : min(off, 16 * row_bytes - 4)));
 #pragma unroll
               for (int rt = 0; rt < RT; ++rt)
@@ -465,33 +594,24 @@ struct Kernel {
     }
     const int64_t unit = static_cast<int64_t>(b) * p.cache.kv_heads + kv;
     const int64_t part = (unit * a.splits + split) * a.row_slots;
+    auto write_result = [&](int r, int d, f32x4_t v, float row_l) {
+      const int t = r / a.group;
+      const int64_t slot = (static_cast<int64_t>(b) * p.batch.rows + t) * p.heads + kv * a.group + r - t * a.group;
+      store_result<T>(p.out, slot * D + d, v, t < static_cast<int>(count) ? row_l : 0.0f);
+    };
     // Four values of a row, d .. d + 3: of the result, or of this split's sums.
     auto write = [&](int r, int d, f32x4_t v, float row_m, float row_l) {
       if (r >= a.rows || d >= D) return;
-      if (a.splits > 1) {
-        *reinterpret_cast<f32x4_t*>(a.sums + (part + r) * D + d) = v;
-        if (d == 0) a.stats[part + r] = float2{row_m, row_l};
-        return;
-      }
-      const int t = r / a.group;
-      const float scale = row_l == 0.0f || t >= static_cast<int>(count) ? 0.0f : 1.0f / row_l;
-      v = scale == 0.0f ? f32x4_t{0, 0, 0, 0} : v * scale;
-      const int64_t to = ((static_cast<int64_t>(b) * p.batch.rows + t) * p.heads + kv * a.group + r - t * a.group) * D + d;
-      if constexpr (kHalf) {
-        const u32x2_t h{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-        if (reinterpret_cast<uintptr_t>(p.out) % 8 == 0) {
-          *reinterpret_cast<u32x2_t*>(p.out + to * 2) = h;
-        } else {
-          auto* out = reinterpret_cast<uint16_t*>(p.out) + to;
-#pragma unroll
-          for (int e = 0; e < 4; ++e) out[e] = static_cast<uint16_t>(h[e / 2] >> (16 * (e % 2)));
-        }
-      } else if (reinterpret_cast<uintptr_t>(p.out) % 16 == 0) {
-        *reinterpret_cast<f32x4_t*>(p.out + to * 4) = v;
+      if (whole) return write_result(r, d, v, row_l);
+      float* to = a.sums + (part + r) * D + d;
+      float* stats = a.stats + 2 * (part + r);
+      if (a.tickets != nullptr) {
+        store_shared(to, v[0], v[1]);
+        store_shared(to + 2, v[2], v[3]);
+        if (d == 0) store_shared(stats, row_m, row_l);
       } else {
-        auto* out = reinterpret_cast<float*>(p.out) + to;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) out[e] = v[e];
+        *reinterpret_cast<f32x4_t*>(to) = v;
+        if (d == 0) *reinterpret_cast<float2*>(stats) = float2{row_m, row_l};
       }
     };
     if constexpr (WK == 1) {
@@ -528,11 +648,30 @@ struct Kernel {
         write(row0 + r, d, v, top, sum);
       }
     }
+    if (whole || a.tickets == nullptr) return;
+
+    // The last of the splits joins them, in their order whichever it is.
+    __shared__ uint32_t arrived;
+    wait_vmcnt<0>();  // this wave's results are past its L2
+    __syncthreads();
+    uint32_t* ticket = a.tickets + unit * a.row_groups + rg;
+    if (threadIdx.x == 0) arrived = __hip_atomic_fetch_add(ticket, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    if (arrived + 1 != used) return;
+    if (threadIdx.x == 0) __hip_atomic_store(ticket, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    const int first_row = rg * WR * RT * 16, pieces = D / 4;
+    const int own_rows = min(WR * RT * 16, a.rows - first_row);
+    for (int i = threadIdx.x; i < own_rows * pieces; i += kThreads) {
+      const int r = i / pieces, d = (i - r * pieces) * 4;
+      float top, sum;
+      const f32x4_t v = joined_sums<true>(a, unit * a.splits * a.row_slots + first_row + r, d, D, 0, used, 1, &top, &sum);
+      write_result(first_row + r, d, v, sum);
+    }
   }
 };
 
 template <typename K>
-__global__ __launch_bounds__(K::kThreads) void kernel(Args a) {
+__global__ __launch_bounds__(K::kThreads, K::kMinWaves) void kernel(Args a) {
   K::run(a);
 }
 
@@ -550,7 +689,7 @@ template <typename T, int DT, bool EXACT, int RT, int WR>
 void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
   // Waves over the keys: as many as two stages each leave room for.
-  constexpr int WK = WR > 1 ? 1 : Probe::kStage > 16384 ? 2 : 4;
+    constexpr int WK = WR > 1 ? 1 : Probe::kStage > 16384 ? 1 : Probe::kStage > 8192 ? 2 : 4;
   constexpr int STAGES = WR == 1 ? 2 : 3;
   using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
   hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);

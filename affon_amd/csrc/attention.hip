@@ -11,52 +11,54 @@ namespace affon {
 namespace attention {
 namespace {
 
-// out = sum_s 2^(m_s - m) sums_s / sum_s 2^(m_s - m) l_s over the splits that
-// hold keys of the row's sequence; four values per thread.
+// Joins the splits, where the kernel's own workgroups do not: head_dim / 4
+// threads for each of `shares` shares of the splits of a row and head, which
+// then meet in LDS; several rows and heads to a workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(Args a) {
+__global__ __launch_bounds__(256) void join_kernel(Args a, int shares) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[256];
+  __shared__ float2 stats[256];
   const AttentionProblem& p = a.p;
-  const int D = p.cache.head_dim, pieces = D / 4;
-  const int64_t item = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  const int64_t slot = item / pieces;  // of [row][head]
-  const int d = static_cast<int>(item - slot * pieces) * 4;
+  const int D = p.cache.head_dim, pieces = D / 4, own = pieces * shares, per = 256 / own;
+  const int local = threadIdx.x / own, share = (threadIdx.x - local * own) / pieces;
+  const int piece = threadIdx.x % pieces, d = 4 * piece;
+  const int64_t slot = static_cast<int64_t>(blockIdx.x) * per + local;  // of [row][head]
   const int64_t row = slot / p.heads;
-  if (row >= static_cast<int64_t>(p.batch.sequences) * p.batch.rows) return;
+  const bool there = local < per && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   const int head = static_cast<int>(slot - row * p.heads), kv = head / a.group;
-  const int b = static_cast<int>(row / p.batch.rows), t = static_cast<int>(row - static_cast<int64_t>(b) * p.batch.rows);
+  const int b = there ? static_cast<int>(row / p.batch.rows) : 0;
+  const int t = static_cast<int>(row - static_cast<int64_t>(b) * p.batch.rows);
   const uint32_t count = drafted(p.batch, b);
   const uint32_t n = min(committed(p.batch, b) + count, p.batch.capacity);
+  const uint32_t used = (n + a.chunk - 1) / a.chunk;
+  const bool works = there && used > 1;  // else the result is there
   f32x4_t v{0, 0, 0, 0};
-  if (t < static_cast<int>(count)) {
-    const int used = min(static_cast<uint32_t>(a.splits), (n + a.chunk - 1) / a.chunk);
+  float top = kLowest, sum = 0.0f;
+  if (works && share < static_cast<int>(used)) {
     const int64_t first = (static_cast<int64_t>(b) * p.cache.kv_heads + kv) * a.splits * a.row_slots + t * a.group +
                           head - kv * a.group;
-    float top = kLowest, sum = 0.0f;
-    for (int s = 0; s < used; ++s) top = fmaxf(top, a.stats[first + static_cast<int64_t>(s) * a.row_slots].x);
-    for (int s = 0; s < used; ++s) {
-      const int64_t at = first + static_cast<int64_t>(s) * a.row_slots;
-      const float2 st = a.stats[at];
+    v = joined_sums<false>(a, first, d, D, share, used, shares, &top, &sum);
+  }
+  if (shares > 1) {
+    part[threadIdx.x] = v;
+    stats[threadIdx.x] = float2{top, sum};
+    __syncthreads();
+    if (share != 0 || local >= per) return;
+    for (int s = 1; s < shares; ++s) top = fmaxf(top, stats[threadIdx.x + s * pieces].x);
+    v = f32x4_t{0, 0, 0, 0};
+    sum = 0.0f;
+    for (int s = 0; s < shares; ++s) {
+      const float2 st = stats[threadIdx.x + s * pieces];
       const float keep = __builtin_amdgcn_exp2f(st.x - top);
       sum = fmaf(st.y, keep, sum);
-      v += *reinterpret_cast<const f32x4_t*>(a.sums + at * D + d) * keep;
+      v += part[threadIdx.x + s * pieces] * keep;
     }
-    v = sum == 0.0f ? f32x4_t{0, 0, 0, 0} : v * (1.0f / sum);
   }
-  const int64_t to = slot * D + d;
-  if constexpr (T::bytes == 2) {
-    auto* out = reinterpret_cast<uint16_t*>(p.out) + to;
-    const u32x2_t h{pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3])};
-    if (reinterpret_cast<uintptr_t>(p.out) % 8 == 0) {
-      *reinterpret_cast<u32x2_t*>(out) = h;
-    } else {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) out[e] = static_cast<uint16_t>(h[e / 2] >> (16 * (e % 2)));
-    }
-  } else {
-    auto* out = reinterpret_cast<float*>(p.out) + to;
-#pragma unroll
-    for (int e = 0; e < 4; ++e) out[e] = v[e];
-  }
+  if (works) store_result<T>(p.out, slot * D + d, v, t < static_cast<int>(count) ? sum : 0.0f);
+}
+
+__global__ __launch_bounds__(256) void clear_kernel(uint32_t* words, int count) {
+  for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) words[i] = 0;
 }
 
 // Few rows: waves side by side over the keys; more: over the rows.
@@ -87,11 +89,20 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // Pieces of the context: enough workgroups for the GPU, none so short that
   // its results weigh against the keys it reads.
   const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
-  constexpr int64_t kWanted = 1024;
   const int64_t capacity = p.batch.capacity;
-  int64_t splits = std::max<int64_t>(1, kWanted / (units * a.row_groups));
-  const int64_t least = std::max<int64_t>(128, 8 * std::min(a.rows, shape.rows()));
-  splits = std::min(splits, (capacity + least - 1) / least);
+  const bool half = p.cache.dtype == AFFON_ROCM_BF16;
+  const int64_t own_rows = std::min(a.rows, shape.rows());
+  // One round of workgroups, two to a CU: a second round of shorter ones costs
+  // more in starts and joins than it evens out (32 sequences of one token over
+  // up to 4096 tokens: 68.0 us in 512 workgroups, 76.8 in 768; trees of 24 of
+  // 8 sequences 57.8 and 69.6). Longer pieces than kEven leave the GPU uneven
+  // where lengths differ (trees of 64 over up to 16384: 541 us in 512
+  // workgroups, 450 in 2048), and pieces of fewer keys than rows cost more to
+  // join than they read.
+  constexpr int64_t kRound = 512, kEven = 2048;
+  int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 16 * own_rows));
+  splits = std::min(splits, capacity / std::max<int64_t>(128, (half ? 2 : 1) * own_rows));
+  splits = std::max<int64_t>(splits, 1);
   a.chunk = static_cast<uint32_t>((capacity + splits - 1) / splits + 127) / 128 * 128;
   a.splits = static_cast<int>((capacity + a.chunk - 1) / a.chunk);
   if (a.splits > 1) {
@@ -100,7 +111,17 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
     auto* scratch = static_cast<uint8_t*>(l.scratch(sums + slots * sizeof(float2)));
     if (scratch != nullptr) {
       a.sums = reinterpret_cast<float*>(scratch);
-      a.stats = reinterpret_cast<float2*>(scratch + sums);
+      a.stats = reinterpret_cast<float*>(scratch + sums);
+      bool fresh = false;
+      // Few results are joined by the workgroup that is last to end (one token
+      // over 777: 9.4 us against 11.8 with a second launch; 32 sequences 67.7
+      // and 70.2), more by a launch of their own (one token over 32000, 129 KB
+      // a head: 36.6 and 34.6; trees of 24 94 and 62).
+      constexpr int64_t kJoined = 32768;
+      if (own_rows * p.cache.head_dim * 4 * a.splits <= kJoined && units * a.row_groups <= Workspace::kTickets &&
+          l.workspace != nullptr)
+        a.tickets = l.workspace->tickets(&fresh);
+      if (fresh) hipLaunchKernelGGL(clear_kernel, dim3(64), dim3(256), 0, l.stream, a.tickets, Workspace::kTickets);
     } else {  // a captured stream whose workspace cannot grow
       a.splits = 1;
     }
@@ -109,17 +130,20 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   const int64_t blocks = (groups + 7) / 8 * 8 * a.row_groups;
   if (blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
-  const bool half = p.cache.dtype == AFFON_ROCM_BF16;
   (half ? launch_bf16 : launch_f32)(a, shape, grid, l.stream);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || a.splits == 1) return e;
-  const int64_t items = static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads * (p.cache.head_dim / 4);
-  const int64_t join_blocks = (items + 255) / 256;
+  if (e != hipSuccess || a.splits == 1 || a.tickets != nullptr) return e;
+  // A share takes the eight splits that a thread has in flight.
+  const int pieces = p.cache.head_dim / 4;
+  const int shares = std::min((a.splits + 7) / 8, 256 / pieces);
+  const int64_t per = 256 / (pieces * shares);
+  const int64_t join_blocks = (static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads + per - 1) / per;
   if (join_blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  const dim3 join_grid(static_cast<unsigned>(join_blocks));
   if (half)
-    hipLaunchKernelGGL(join_kernel<BF16>, dim3(static_cast<unsigned>(join_blocks)), dim3(256), 0, l.stream, a);
+    hipLaunchKernelGGL(join_kernel<BF16>, join_grid, dim3(256), 0, l.stream, a, shares);
   else
-    hipLaunchKernelGGL(join_kernel<F32>, dim3(static_cast<unsigned>(join_blocks)), dim3(256), 0, l.stream, a);
+    hipLaunchKernelGGL(join_kernel<F32>, join_grid, dim3(256), 0, l.stream, a, shares);
   return hipGetLastError();
 }
 

@@ -6,13 +6,31 @@ namespace affon {
 Workspace::~Workspace() {
   if (hipSetDevice(device_) != hipSuccess) return;
   if (ptr_ != nullptr) (void)hipFree(ptr_);
+  if (tickets_ != nullptr) (void)hipFree(tickets_);
   for (void* p : retired_) (void)hipFree(p);
+}
+
+bool Workspace::capturing() const {
+  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+  return hipStreamIsCapturing(stream_, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone;
+}
+
+uint32_t* Workspace::tickets(bool* fresh) {
+  *fresh = false;
+  if (tickets_ == nullptr && !capturing()) {
+    if (hipMalloc(&tickets_, kTickets * sizeof(uint32_t)) == hipSuccess) {
+      *fresh = true;
+    } else {
+      tickets_ = nullptr;
+      (void)hipGetLastError();
+    }
+  }
+  return static_cast<uint32_t*>(tickets_);
 }
 
 void* Workspace::get(size_t bytes) {
   if (bytes <= bytes_) return ptr_;
-  hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-  if (hipStreamIsCapturing(stream_, &capture) != hipSuccess || capture != hipStreamCaptureStatusNone) return nullptr;
+  if (capturing()) return nullptr;
   // The old buffer stays allocated (retired) until the session ends: work
   // already enqueued, and graphs captured with its address, may still use it.
   if (ptr_ != nullptr) {

@@ -3,6 +3,7 @@
 
 #include <hip/hip_runtime.h>
 #include <cstddef>
+#include <cstdint>
 #include <map>
 #include <mutex>
 #include <unordered_map>
@@ -23,15 +24,22 @@ class Workspace {
   // At least `bytes` of device memory, or nullptr when it cannot grow now
   // (the stream is being captured into a graph, or the allocation failed).
   void* get(size_t bytes);
+  // kTickets words for workgroups of one launch to count each other, which
+  // every launch leaves at 0; *fresh: they were allocated now, and the caller
+  // clears them on the stream. Null when they cannot be allocated now.
+  static constexpr int kTickets = 65536;
+  uint32_t* tickets(bool* fresh);
   size_t retired() const { return retired_.size(); }
   std::mutex& mutex() { return mutex_; }
 
  private:
+  bool capturing() const;
   std::mutex mutex_;
   int device_;
   hipStream_t stream_;
   void* ptr_ = nullptr;
   size_t bytes_ = 0;
+  void* tickets_ = nullptr;
   std::vector<void*> retired_;
   size_t retired_bytes_ = 0;  // size of the last retired buffer
 };
