@@ -201,12 +201,8 @@ struct Kernel {
   // and the values' 2 * kPieces, each for every tile of the step.
   static constexpr int kPer = (2 * kPieces + WR - 1) / WR;
   static constexpr int kTransfers = kPer * kKT;
-#ifndef MINW
-#define MINW 1
-#endif
-  static constexpr int kMinWaves = WR > 1 && RT == 2 && DT == 8 ? MINW : 1;
   static_assert(WR == 1 || WK == 1, "waves share keys or rows");
-  static_assert(STAGES >= 2 && kTransfers * (STAGES - 1) < 64, "transfers in flight");
+  static_assert(STAGES >= 2 && kTransfers * STAGES < 64, "transfers in flight");
   static constexpr int kRing = WK * STAGES * kStage;
   // The waves' sums, where they share rows: rows padded by 16 bytes.
   static constexpr int kJoinRow = 16 * DT + 4;
@@ -293,13 +289,6 @@ struct Kernel {
     }
     f32x4_t o[RT][DT];
     float m[RT], l[RT];
-#pragma unroll
-    for (int rt = 0; rt < RT; ++rt) {
-      m[rt] = kLowest;
-      l[rt] = 0.0f;
-#pragma unroll
-      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0, 0, 0, 0};
-    }
 
     auto place_queries = [&] {  // dims past the head are 0, and the scale's sign is theirs
       const uint32_t keep = a.sign == 0.0f ? 0u : ~0u, flip = a.sign < 0.0f ? (kHalf ? 0x80008000u : 0x80000000u) : 0u;
@@ -346,6 +335,19 @@ struct Kernel {
     const uint8_t* ring_data = lds + (WK > 1 ? wave * STAGES * kStage : 0);
     const int64_t head_bytes = static_cast<int64_t>(p.cache.page_size) * row_bytes;
 
+    // A value that is not finite in a drafted token that some row does not see
+    // would reach that row as 0 * infinity. Such values are rare, and leave
+    // sums that are not finite: then, and only then, everything is done again
+    // with a look at every drafted token's values (`careful`).
+    bool careful = false;
+  again:
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      m[rt] = kLowest;
+      l[rt] = 0.0f;
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) o[rt][dt] = f32x4_t{0, 0, 0, 0};
+    }
     for (uint32_t segment = begin; segment < end; segment += kPageList * 16) {
       const uint32_t segment_end = min(end, segment + kPageList * 16);
       __syncthreads();
@@ -362,67 +364,65 @@ struct Kernel {
         if (page == kNoPage) missing = 1;
       }
       __syncthreads();
-      if (segment == begin) place_queries();
+      if (segment == begin && !careful) place_queries();
       const bool gaps = __builtin_amdgcn_readfirstlane(missing) != 0;
       const int all = static_cast<int>((segment_end - segment + kKeys - 1) / kKeys);
       // Steps of this wave: first, first + stride, .. below all.
       const int first = WK > 1 ? wave : 0;
       const int steps = all > first ? (all - first + WK - 1) / WK : 0;
 
-      auto issue = [&](int step) {
-        const int s = (first + step * WK) * kKT;
+      // Byte offsets of a step's tiles. A tile past the last one repeats it:
+      // the keys there are not seen.
+      auto tile_offset = [&](int step, int kt) {
+        const int tile = (first + step * WK) * kKT + kt, last = static_cast<int>((segment_end - segment - 1) / 16);
+        return tile_list[min(tile, last)];
+      };
+      auto issue = [&](int step, const int64_t (&offsets)[kKT]) {
         const uint32_t to = ring + (step % STAGES) * kStage;
 #pragma unroll
         for (int kt = 0; kt < kKT; ++kt) {
-          // A tile past the last one repeats it: the keys there are not seen.
-          const int tile = min(s + kt, static_cast<int>((segment_end - segment - 1) / 16));
-          const int64_t listed = tile_list[tile];
-          const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(listed >> 32))) << 32 |
-                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(listed)));
+          const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt] >> 32))) << 32 |
+                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt])));
           const uint8_t* key_tile = p.cache.keys + max(at, static_cast<int64_t>(0));
           const uint8_t* value_tile = p.cache.values + max(at, static_cast<int64_t>(0));
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int piece = min(first_piece + i * WR, 2 * kPieces - 1);
-            const bool value = piece >= kPieces;
+            const bool value = kPieces % WR == 0 ? i >= kPieces / WR : piece >= kPieces;
             dma16(value ? value_tile : key_tile, from[i],
                   to + (value ? kKT * kTile : 0) + kt * kTile + (value ? piece - kPieces : piece) * 1024);
           }
         }
       };
+      u32x4_t keys[kKT][kQSteps];
+      auto read_keys = [&](int step) {
+        const uint8_t* from_lds = ring_data + (step % STAGES) * kStage;
 #pragma unroll
-      for (int s = 0; s < STAGES - 1; ++s)
-        if (s < steps) issue(s);
-      for (int step = 0; step < steps; ++step) {
-        if (step + STAGES - 1 <= steps)
-          wait_vmcnt<(STAGES - 2) * kTransfers>();
-        else
-          wait_vmcnt<0>();
-        if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
-        if (step + STAGES - 1 < steps) issue(step + STAGES - 1);
-
-        const uint8_t* keys = ring_data + (step % STAGES) * kStage;
-        const uint8_t* values = keys + kKT * kTile;
-        const uint32_t key0 = segment + static_cast<uint32_t>(first + step * WK) * kKeys;
-
-        // ---- scores ----
-        f32x4_t s[RT][kKT];
+        for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
-        for (int kt = 0; kt < kKT; ++kt) {
+          for (int i = 0; i < kQSteps; ++i) {
+            if constexpr (EXACT) {
+              keys[kt][i] = *reinterpret_cast<const u32x4_t*>(from_lds + kt * kTile + key_at[i % kKeySpots] +
+                                                              i / kKeySpots * kKeySpots * 64);
+            } else {
+              const int at = (i * 4 + quad) * 16;
+              keys[kt][i] = *reinterpret_cast<const u32x4_t*>(from_lds + kt * kTile + col * row_bytes + min(at, row_bytes - 16));
+            }
+          }
+      };
+      f32x4_t s[RT][kKT];
+      auto multiply_keys = [&] {
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
           for (int rt = 0; rt < RT; ++rt) s[rt][kt] = f32x4_t{0, 0, 0, 0};
 #pragma unroll
-          for (int i = 0; i < kQSteps; ++i) {
-            const int c = i * 4 + quad;
-            u32x4_t k;
-            if constexpr (EXACT) {
-              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + key_at[i % kKeySpots] + i / kKeySpots * kKeySpots * 64);
-            } else {
-              // Past the head: zeros, as the queries hold there.
-              k = *reinterpret_cast<const u32x4_t*>(keys + kt * kTile + col * row_bytes + min(c * 16, row_bytes - 16));
-              if (c * 16 >= row_bytes) k = u32x4_t{0, 0, 0, 0};
-            }
+        for (int i = 0; i < kQSteps; ++i) {
+#pragma unroll
+          for (int kt = 0; kt < kKT; ++kt) {
+            u32x4_t k = keys[kt][i];
+            // Past the head: zeros, as the queries hold there.
+            if (!EXACT && (i * 4 + quad) * 16 >= row_bytes) k = u32x4_t{0, 0, 0, 0};
 #pragma unroll
             for (int rt = 0; rt < RT; ++rt) {
               if constexpr (kHalf) {
@@ -438,6 +438,35 @@ struct Kernel {
             }
           }
         }
+      };
+
+      // A step's scores are computed at the end of the one before, so that its
+      // keys come from LDS beside the values' products and both products follow
+      // each other; its values come beside the softmax. A step's place in LDS
+      // is free when its values are in registers.
+#pragma unroll
+      for (int i = 0; i < STAGES; ++i) {
+        if (i >= steps) continue;
+        int64_t offsets[kKT];
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt) offsets[kt] = tile_offset(i, kt);
+        issue(i, offsets);
+      }
+      if (steps >= STAGES)
+        wait_vmcnt<(STAGES - 1) * kTransfers>();
+      else
+        wait_vmcnt<0>();
+      if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      read_keys(0);
+      multiply_keys();
+
+      for (int step = 0; step < steps; ++step) {
+        const uint8_t* values = ring_data + (step % STAGES) * kStage + kKT * kTile;
+        const uint32_t key0 = segment + static_cast<uint32_t>(first + step * WK) * kKeys;
+        int64_t offsets[kKT];
+#pragma unroll
+        for (int kt = 0; kt < kKT; ++kt) offsets[kt] = tile_offset(step + STAGES, kt);
 
         // ---- steps with keys that not every row sees ----
         const bool edge = gaps || key0 + kKeys > length;
@@ -463,13 +492,11 @@ struct Kernel {
               for (int i = 0; i < 4; ++i)
                 if (!(seen[rt] >> (16 * kt + 4 * quad + i) & 1)) s[rt][kt][i] = -INFINITY;
           }
-          // Values that some row does not see must not reach its sums as 0 *
-          // infinity: those of no token are cleared, and those of drafted
-          // tokens that are not finite are cleared and added by themselves.
+          // What lies in the slots of no token is cleared, as it may be
+          // infinite too.
           const int past = static_cast<int>(n) - static_cast<int>(key0);
           const uint32_t exists = there & (past >= 32 ? ~0u : past <= 0 ? 0u : (1u << past) - 1);
-          const uint32_t all_see = base >= 0 ? 0u : base <= -32 ? ~0u : (1u << -base) - 1;
-          uint32_t bad = 0;
+          uint32_t clear = ~exists & (kKeys == 32 ? ~0u : 0xffffu);
           auto for_pieces = [&](auto&& f) {
 #pragma unroll
             for (int kt = 0; kt < kKT; ++kt)
@@ -479,24 +506,53 @@ struct Kernel {
                 if (at < 16 * row_bytes) f(kt * 16 + at / row_bytes, const_cast<uint8_t*>(values) + kt * kTile + at);
               }
           };
-          for_pieces([&](int k, uint8_t* piece) {
-            const u32x4_t v = *reinterpret_cast<const u32x4_t*>(piece);
-            if (not_finite(v[0], kHalf) || not_finite(v[1], kHalf) || not_finite(v[2], kHalf) || not_finite(v[3], kHalf))
-              bad |= 1u << k;
-          });
+          if (careful) {  // and so are values that are not finite, which are added by themselves
+            const uint32_t all_see = base >= 0 ? 0u : base <= -32 ? ~0u : (1u << -base) - 1;
+            uint32_t bad = 0;
+            for_pieces([&](int k, uint8_t* piece) {
+              const u32x4_t v = *reinterpret_cast<const u32x4_t*>(piece);
+              if (not_finite(v[0], kHalf) || not_finite(v[1], kHalf) || not_finite(v[2], kHalf) || not_finite(v[3], kHalf))
+                bad |= 1u << k;
+            });
 #pragma unroll
-          for (int offset = 32; offset > 0; offset >>= 1) bad |= __shfl_xor(bad, offset);
-          flagged = __builtin_amdgcn_readfirstlane(bad) & exists & ~all_see;
-          const uint32_t clear = flagged | (~exists & (kKeys == 32 ? ~0u : 0xffffu));
-          if constexpr (WR > 1) __syncthreads();  // every wave has looked
-          if (clear != 0)
+            for (int offset = 32; offset > 0; offset >>= 1) bad |= __shfl_xor(bad, offset);
+            flagged = __builtin_amdgcn_readfirstlane(bad) & exists & ~all_see;
+            clear |= flagged;
+            if constexpr (WR > 1) __syncthreads();  // every wave has looked
+          }
+          if (clear != 0) {
             for_pieces([&](int k, uint8_t* piece) {
               if (clear >> k & 1) *reinterpret_cast<u32x4_t*>(piece) = u32x4_t{0, 0, 0, 0};
             });
-          if constexpr (WR > 1)
-            __syncthreads();
-          else
-            wait_lds_reads();
+            if constexpr (WR > 1)
+              __syncthreads();
+            else
+              wait_lds_reads();
+          }
+        }
+
+        // ---- values, on the way beside the softmax ----
+        using Value = typename std::conditional<kHalf, u32x4_t, f32x4_t>::type;  // eight keys, or four, of a column
+        Value v[DT];
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt) {
+          if constexpr (kHalf) {
+            const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 32;
+            u32x2_t half[2];
+#pragma unroll
+            for (int kt = 0; kt < 2; ++kt) {
+              const uint32_t address = lds_address(values + kt * kTile + (EXACT ? off : min(off, 16 * row_bytes - 8)));
+              half[kt] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                         reinterpret_cast<lds_s16x4>(static_cast<uintptr_t>(address))));
+            }
+            v[dt] = Value{half[0][0], half[0][1], half[1][0], half[1][1]};
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 64 + i * row_bytes;
+              v[dt][i] = *reinterpret_cast<const float*>(values + (EXACT ? off : min(off, 16 * row_bytes - 4)));
+            }
+          }
         }
 
         // ---- softmax ----
@@ -529,34 +585,31 @@ struct Kernel {
                                  pack_bf16(s[rt][kKT - 1][2], s[rt][kKT - 1][3])};
         }
 
+        // ---- the next step's keys, and the step after whose place is free ----
+        wait_lds_reads();
+        if (step + STAGES <= steps)
+          wait_vmcnt<(STAGES - 2) * kTransfers>();
+        else
+          wait_vmcnt<0>();
+        if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (step + STAGES < steps) issue(step + STAGES, offsets);
+        read_keys(step + 1);  // after the last step: what lies there, for scores that nothing reads
+
         // ---- sums of values ----
 #pragma unroll
-        for (int dt = 0; dt < DT; ++dt) {
-          if constexpr (kHalf) {
-            const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 32;
-            u32x2_t v[2];
+        for (int dt = 0; dt < DT; ++dt)
 #pragma unroll
-            for (int kt = 0; kt < 2; ++kt) {
-              const uint32_t address = lds_address(values + kt * kTile + (EXACT ? off : min(off, 16 * row_bytes - 8)));
-              v[kt] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
-                                                      reinterpret_cast<lds_s16x4>(static_cast<uintptr_t>(address))));
-            }
-            const u32x4_t v8{v[0][0], v[0][1], v[1][0], v[1][1]};
-#pragma unroll
-            for (int rt = 0; rt < RT; ++rt)
-              o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v8),
+          for (int rt = 0; rt < RT; ++rt) {
+            if constexpr (kHalf) {
+              o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, v[dt]),
                                                                   __builtin_bit_cast(bf16x8_t, packed[rt]), o[rt][dt], 0, 0, 0);
-          } else {
+            } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const int off = value_at[dt % kValueSpots] + dt / kValueSpots * kValueSpots * 64 + i * row_bytes;
-              const float v = *reinterpret_cast<const float*>(values + (EXACT ? off : min(off, 16 * row_bytes - 4)));
-#pragma unroll
-              for (int rt = 0; rt < RT; ++rt)
-                o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v, s[rt][0][i], o[rt][dt], 0, 0, 0);
+              for (int i = 0; i < 4; ++i)
+                o[rt][dt] = __builtin_amdgcn_mfma_f32_16x16x4f32(v[dt][i], s[rt][0][i], o[rt][dt], 0, 0, 0);
             }
           }
-        }
 
         if (flagged != 0) {  // rare: a drafted token's value that is not finite, for the rows that see it
           for (int k = 0; k < kKeys; ++k) {
@@ -582,7 +635,22 @@ struct Kernel {
             }
           }
         }
-        wait_lds_reads();
+        multiply_keys();
+      }
+      wait_lds_reads();
+    }
+
+    if (end > length && !careful) {  // the drafted tokens are among the keys
+      float odd = 0.0f;
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) odd = fmaf(o[rt][dt][i], 0.0f, odd);  // 0, or NaN
+      if (__syncthreads_or(odd != 0.0f || odd != odd)) {
+        careful = true;
+        goto again;
       }
     }
 
@@ -671,7 +739,7 @@ struct Kernel {
 };
 
 template <typename K>
-__global__ __launch_bounds__(K::kThreads, K::kMinWaves) void kernel(Args a) {
+__global__ __launch_bounds__(K::kThreads) void kernel(Args a) {
   K::run(a);
 }
 
@@ -689,19 +757,27 @@ template <typename T, int DT, bool EXACT, int RT, int WR>
 void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
   // Waves over the keys: as many as two stages each leave room for.
-    constexpr int WK = WR > 1 ? 1 : Probe::kStage > 16384 ? 1 : Probe::kStage > 8192 ? 2 : 4;
-  constexpr int STAGES = WR == 1 ? 2 : 3;
+    constexpr int WK = WR > 1 ? 1 : Probe::kStage > 8192 ? 2 : 4;
+  #ifndef ST4
+#define ST4 3
+#endif
+  constexpr int STAGES = WR == 1 ? 2 : ST4;
   using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
   hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
 }
 
 template <typename T, int DT, bool EXACT>
 void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
-  if (shape.waves == 1) {
-    if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1>(a, grid, stream);
-    return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
+  if constexpr (DT <= 8) {
+    if (shape.waves == 1) {
+      if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1>(a, grid, stream);
+      return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
+    }
   }
   if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
+  if constexpr (T::bytes == 2 && DT <= 8) {
+    if (shape.tiles == 4) return launch_shape<T, DT, EXACT, 4, 4>(a, grid, stream);
+  }
   return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
 }
 

@@ -4,6 +4,7 @@
 
 #include <algorithm>
 #include <cmath>
+#include <cstdlib>
 
 #include "attention.h"
 
@@ -61,10 +62,11 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* words, int count) 
   for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) words[i] = 0;
 }
 
-// Few rows: waves side by side over the keys; more: over the rows.
-Shape shape_for(int rows) {
-  if (rows <= 16) return {1, 1};
-  if (rows <= 32) return {2, 1};
+// Few rows: waves side by side over the keys; more: over the rows, and where
+// the keys of two waves do not fit in LDS twice to a CU.
+Shape shape_for(int rows, int head_dim, bool half) {
+  if (rows <= 16 && head_dim <= 128) return {1, 1};
+  if (rows <= 32 && head_dim <= 128) return {2, 1};
   if (rows <= 64) return {1, 4};
   return {2, 4};
 }
@@ -80,7 +82,8 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   const int64_t rows = static_cast<int64_t>(p.batch.rows) * a.group;
   if (rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
-  const Shape shape = shape_for(a.rows);
+  const bool half = p.cache.dtype == AFFON_ROCM_BF16;
+  const Shape shape = shape_for(a.rows, p.cache.head_dim, half);
   a.row_groups = (a.rows + shape.rows() - 1) / shape.rows();
   a.row_slots = a.rows;
   a.log2_scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
@@ -90,7 +93,6 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // its results weigh against the keys it reads.
   const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
   const int64_t capacity = p.batch.capacity;
-  const bool half = p.cache.dtype == AFFON_ROCM_BF16;
   const int64_t own_rows = std::min(a.rows, shape.rows());
   // One round of workgroups, two to a CU: a second round of shorter ones costs
   // more in starts and joins than it evens out (32 sequences of one token over
@@ -99,7 +101,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // where lengths differ (trees of 64 over up to 16384: 541 us in 512
   // workgroups, 450 in 2048), and pieces of fewer keys than rows cost more to
   // join than they read.
-  constexpr int64_t kRound = 512, kEven = 2048;
+  const int64_t kRound = 512, kEven = getenv("KE") ? atoi(getenv("KE")) : 2048;
   int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 16 * own_rows));
   splits = std::min(splits, capacity / std::max<int64_t>(128, (half ? 2 : 1) * own_rows));
   splits = std::max<int64_t>(splits, 1);
