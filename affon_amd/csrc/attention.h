@@ -72,6 +72,14 @@ __device__ __forceinline__ int pinned(int v) {
   return v;
 }
 
+// A wave's address in scalar registers, as the transfers take it.
+__device__ __forceinline__ const uint8_t* uniform(const uint8_t* p) {
+  const uint64_t v = reinterpret_cast<uint64_t>(p);
+  const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<int>(v));
+  const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<int>(v >> 32));
+  return reinterpret_cast<const uint8_t*>(static_cast<uint64_t>(high) << 32 | low);
+}
+
 // A bf16 word holds an infinity or a NaN in its low or high half.
 __device__ __forceinline__ bool not_finite(uint32_t w, bool half) {
   if (half) return (w & 0x7f80u) == 0x7f80u || (w & 0x7f800000u) == 0x7f800000u;
@@ -192,6 +200,7 @@ struct Kernel {
   static constexpr int kKT = kHalf ? 2 : 1;  // 16-key tiles of a step
   static constexpr int kKeys = 16 * kKT;
   static constexpr int kThreads = 64 * WR * WK;
+  static constexpr int kWavesPerSimd = DT <= 8 ? 2 : 1;  // that share the registers
   static constexpr int kMaxRow = 16 * DT * T::bytes;             // bytes of a head
   static constexpr int kTile = (16 * kMaxRow + 1023) / 1024 * 1024;  // LDS bytes of 16 keys
   static constexpr int kPieces = kTile / 1024;
@@ -225,7 +234,7 @@ struct Kernel {
   static __device__ void run(const Args& a) {
     const AttentionProblem& p = a.p;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
-    __shared__ int64_t tile_list[kPageList];  // byte offsets of 16-key tiles in keys and values, or -1
+    __shared__ int64_t tile_list[kPageList];  // byte offsets of 16-key tiles in keys and values; 1: of no page
     __shared__ int missing;
     __shared__ float2 join_stats[WK > 1 ? WK * RT * 16 : 1];
 
@@ -358,7 +367,7 @@ struct Kernel {
         const uint32_t page = segment == begin && i < kThreads
                                   ? (early < static_cast<uint32_t>(p.cache.pages) ? early : kNoPage)
                                   : page_of(p.cache, p.batch, b, index);
-        tile_list[i] = page == kNoPage ? -1
+        tile_list[i] = page == kNoPage ? 1
                                        : (static_cast<int64_t>(page) * p.cache.kv_heads + kv) * head_bytes +
                                              static_cast<int64_t>(at - index * p.cache.page_size) * row_bytes;
         if (page == kNoPage) missing = 1;
@@ -377,14 +386,16 @@ struct Kernel {
         const int tile = (first + step * WK) * kKT + kt, last = static_cast<int>((segment_end - segment - 1) / 16);
         return tile_list[min(tile, last)];
       };
-      auto issue = [&](int step, const int64_t (&offsets)[kKT]) {
-        const uint32_t to = ring + (step % STAGES) * kStage;
+      // Starts a step's transfers to a place in LDS.
+      auto issue = [&](int place, const int64_t (&offsets)[kKT]) {
+        const uint32_t to = ring + place * kStage;
 #pragma unroll
         for (int kt = 0; kt < kKT; ++kt) {
-          const int64_t at = static_cast<int64_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt] >> 32))) << 32 |
-                             static_cast<uint32_t>(__builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt])));
-          const uint8_t* key_tile = p.cache.keys + max(at, static_cast<int64_t>(0));
-          const uint8_t* value_tile = p.cache.values + max(at, static_cast<int64_t>(0));
+          const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt] >> 32));
+          const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<int>(offsets[kt]));
+          const int64_t at = static_cast<int64_t>(high) << 32 | (low & ~15u);
+          const uint8_t* key_tile = uniform(p.cache.keys + at);
+          const uint8_t* value_tile = uniform(p.cache.values + at);
 #pragma unroll
           for (int i = 0; i < kPer; ++i) {
             const int piece = min(first_piece + i * WR, 2 * kPieces - 1);
@@ -395,8 +406,8 @@ struct Kernel {
         }
       };
       u32x4_t keys[kKT][kQSteps];
-      auto read_keys = [&](int step) {
-        const uint8_t* from_lds = ring_data + (step % STAGES) * kStage;
+      auto read_keys = [&](int place) {
+        const uint8_t* from_lds = ring_data + place * kStage;
 #pragma unroll
         for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
@@ -461,8 +472,9 @@ struct Kernel {
       read_keys(0);
       multiply_keys();
 
-      for (int step = 0; step < steps; ++step) {
-        const uint8_t* values = ring_data + (step % STAGES) * kStage + kKT * kTile;
+      auto advance = [&](int step, auto place_of_step) {
+        constexpr int place = decltype(place_of_step)::value;
+        const uint8_t* values = ring_data + place * kStage + kKT * kTile;
         const uint32_t key0 = segment + static_cast<uint32_t>(first + step * WK) * kKeys;
         int64_t offsets[kKT];
 #pragma unroll
@@ -479,7 +491,7 @@ struct Kernel {
 #pragma unroll
           for (int kt = 0; kt < kKT; ++kt) {
             const int tile = static_cast<int>((key0 - segment) / 16) + kt;
-            if (segment + tile * 16 < segment_end && __builtin_amdgcn_readfirstlane(static_cast<int>(tile_list[tile] >> 32)) >= 0)
+            if (segment + tile * 16 < segment_end && __builtin_amdgcn_readfirstlane(static_cast<int>(tile_list[tile])) != 1)
               there |= 0xffffu << (16 * kt);
           }
 #pragma unroll
@@ -593,8 +605,8 @@ struct Kernel {
           wait_vmcnt<0>();
         if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        if (step + STAGES < steps) issue(step + STAGES, offsets);
-        read_keys(step + 1);  // after the last step: what lies there, for scores that nothing reads
+        if (step + STAGES < steps) issue(place, offsets);
+        read_keys((place + 1) % STAGES);  // after the last step: what lies there, for scores that nothing reads
 
         // ---- sums of values ----
 #pragma unroll
@@ -636,7 +648,12 @@ struct Kernel {
           }
         }
         multiply_keys();
-      }
+      };
+      // The places follow each other at fixed addresses.
+      for (int step = 0; step < steps; step += STAGES)
+        pipeline::Unroll<0, STAGES>::run([&](auto place) {
+          if (step + place < steps) advance(step + place, place);
+        });
       wait_lds_reads();
     }
 
@@ -739,7 +756,7 @@ struct Kernel {
 };
 
 template <typename K>
-__global__ __launch_bounds__(K::kThreads) void kernel(Args a) {
+__global__ __launch_bounds__(K::kThreads, K::kWavesPerSimd) void kernel(Args a) {
   K::run(a);
 }
 
@@ -758,10 +775,8 @@ void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
   // Waves over the keys: as many as two stages each leave room for.
     constexpr int WK = WR > 1 ? 1 : Probe::kStage > 8192 ? 2 : 4;
-  #ifndef ST4
-#define ST4 3
-#endif
-  constexpr int STAGES = WR == 1 ? 2 : ST4;
+    // Two steps in LDS: three took 457 us against 446 for trees of 64 over up to 16384 tokens, four 720.
+  constexpr int STAGES = 2;
   using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
   hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
 }
@@ -774,11 +789,8 @@ void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
       return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
     }
   }
-  if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
-  if constexpr (T::bytes == 2 && DT <= 8) {
-    if (shape.tiles == 4) return launch_shape<T, DT, EXACT, 4, 4>(a, grid, stream);
-  }
-  return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
+  if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
+  if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
 }
 
 template <typename T>

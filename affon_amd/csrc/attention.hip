@@ -4,7 +4,6 @@
 
 #include <algorithm>
 #include <cmath>
-#include <cstdlib>
 
 #include "attention.h"
 
@@ -64,10 +63,11 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* words, int count) 
 
 // Few rows: waves side by side over the keys; more: over the rows, and where
 // the keys of two waves do not fit in LDS twice to a CU.
-Shape shape_for(int rows, int head_dim, bool half) {
+Shape shape_for(int rows, int head_dim) {
   if (rows <= 16 && head_dim <= 128) return {1, 1};
   if (rows <= 32 && head_dim <= 128) return {2, 1};
-  if (rows <= 64) return {1, 4};
+  // Wide heads of odd sizes leave no registers for a second tile.
+  if (rows <= 64 || (head_dim > 128 && head_dim != 256)) return {1, 4};
   return {2, 4};
 }
 
@@ -83,7 +83,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   if (rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
   const bool half = p.cache.dtype == AFFON_ROCM_BF16;
-  const Shape shape = shape_for(a.rows, p.cache.head_dim, half);
+  const Shape shape = shape_for(a.rows, p.cache.head_dim);
   a.row_groups = (a.rows + shape.rows() - 1) / shape.rows();
   a.row_slots = a.rows;
   a.log2_scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
@@ -101,7 +101,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // where lengths differ (trees of 64 over up to 16384: 541 us in 512
   // workgroups, 450 in 2048), and pieces of fewer keys than rows cost more to
   // join than they read.
-  const int64_t kRound = 512, kEven = getenv("KE") ? atoi(getenv("KE")) : 2048;
+  constexpr int64_t kRound = 512, kEven = 2048;
   int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 16 * own_rows));
   splits = std::min(splits, capacity / std::max<int64_t>(128, (half ? 2 : 1) * own_rows));
   splits = std::max<int64_t>(splits, 1);
