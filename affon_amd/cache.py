@@ -28,6 +28,9 @@ from . import _native
 from .core import _ITEMSIZE, _NATIVE_DTYPE, Session, Tensor
 
 
+_NO_MASK = _native.View()
+
+
 def _positive(name: str, value: int) -> int:
     if not isinstance(value, int) or isinstance(value, bool) or value <= 0:
         raise TypeError(f"{name} must be a positive integer")
@@ -61,6 +64,11 @@ def _output(op: str, out: Tensor | None, session: Session, dtype: str, shape: tu
     return out
 
 
+def _space(out: Tensor) -> int:
+    """Bytes from a tensor's first value to the end of its memory."""
+    return out._buffer.nbytes - out.offset * _ITEMSIZE[out.dtype]
+
+
 class PagedCache:
     """Keys and values ``[layers, pages, kv_heads, page_size, head_dim]`` of one
     Session, f32 or bf16. page_size: a multiple of 16; head_dim: a multiple of
@@ -84,10 +92,10 @@ class PagedCache:
         self._struct = _native.KvCache(self.keys.data_ptr, self.values.data_ptr,
                                        math.prod(self.shape) * _ITEMSIZE[dtype], *self.shape, _NATIVE_DTYPE[dtype])
 
-    def _check(self, op: str, layer: int | None = None) -> _native.KvCache:
+    def _check(self, op: str, layer: int = 0) -> _native.KvCache:
         self.keys._check_live()
         self.values._check_live()
-        if layer is not None and (not isinstance(layer, int) or not 0 <= layer < self.layers):
+        if type(layer) is not int or not 0 <= layer < self.layers:
             raise TypeError(f"{op} layer is out of range")
         return self._struct
 
@@ -112,11 +120,15 @@ class DraftBatch:
         if any(t.session is not self.session for t in self._tensors):
             raise TypeError("DraftBatch tensors must belong to the same Session")
 
-    def _check(self, op: str, cache: PagedCache, *operands: Tensor | None) -> _native.DraftBatch:
+    def _check(self, op: str, cache: PagedCache, operands: tuple[Tensor | None, ...]) -> _native.DraftBatch:
         for t in self._tensors:
             t._check_live()
-        if cache.session is not self.session or any(t is not None and t.session is not self.session for t in operands):
+        session = self.session
+        if cache.session is not session:
             raise TypeError(f"{op} operands must belong to the same Session")
+        for t in operands:
+            if t is not None and (not isinstance(t, Tensor) or t.session is not session):
+                raise TypeError(f"{op} operands must belong to the same Session")
         return self._struct
 
 
@@ -137,6 +149,24 @@ def _query_rows(op: str, cache: PagedCache, batch: DraftBatch, query: Tensor, dt
         raise TypeError(f"{op} query width must be a multiple of kv_heads * head_dim")
 
 
+# The library checks every operand that reaches it as a view, before it
+# enqueues anything. A call whose operands it refuses is explained here, in
+# the terms of this module; one that it takes is not checked twice.
+
+def _refused(status: int, op: str, explain) -> None:
+    if status == _native.INVALID_SHAPE:
+        message = _native.last_error()
+        explain()
+        raise _native.NativeError(status, f"{op}: {message}")
+    _native.check(status, op)
+
+
+def _rank_two(op: str, name: str, t: Tensor) -> _native.View:
+    if len(t.shape) != 2 or t.dtype not in _NATIVE_DTYPE:
+        raise TypeError(f"{op} {name} must be a rank-two f32/bf16/u32 tensor")
+    return t.view()
+
+
 def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tensor, value: Tensor,
                  positions: Tensor | None, rotary: Tensor, *, layer: int = 0, interleaved: bool = False,
                  out: Tensor | None = None) -> Tensor:
@@ -149,20 +179,23 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
     return zeros."""
     op = "cache_append"
     cache_struct = cache._check(op, layer)
-    batch_struct = batch._check(op, cache, query, key, value, positions, rotary)
-    _query_rows(op, cache, batch, query, ("f32", "bf16"))
-    rows = query.shape[0]
-    for name, t in (("key", key), ("value", value)):
-        _matrix(op, name, t, (query.dtype,), (rows, cache.kv_heads * cache.head_dim))
-    _matrix(op, "rotary", rotary, ("f32",), (None, None))
-    if not rotary.is_contiguous() or rotary.shape[1] % 2 or not 2 <= rotary.shape[1] <= cache.head_dim:
-        raise TypeError("cache_append rotary table must be contiguous, its width even and at most head_dim")
+    batch_struct = batch._check(op, cache, (query, key, value, positions, rotary))
+    views = _rank_two(op, "query", query), _rank_two(op, "key", key), _rank_two(op, "value", value)
+    if rotary.dtype != "f32" or len(rotary.shape) != 2 or not rotary.is_contiguous() or rotary.shape[1] % 2 or \
+            not 2 <= rotary.shape[1] <= cache.head_dim:
+        raise TypeError("cache_append rotary table must be a contiguous f32 [*, *] tensor, its width even and at most "
+                        "head_dim")
     out = _output(op, out, cache.session, cache.dtype, query.shape)
-    desc = _native.AppendDesc(query.view(), key.view(), value.view(),
-                              None if positions is None else _words(op, "positions", positions, rows),
-                              rotary.data_ptr, rotary.shape[0], rotary.shape[1], 1 if interleaved else 0, layer,
-                              out.data_ptr, out._buffer.nbytes - out.offset * _ITEMSIZE[out.dtype])
-    _native.check(_native.load().affon_rocm_cache_append(cache.session._handle, cache_struct, batch_struct, desc), op)
+    status = _native.load().affon_rocm_cache_append(
+        cache.session._handle, cache_struct, batch_struct,
+        _native.AppendDesc(*views, None if positions is None else _words(op, "positions", positions, query.shape[0]),
+                           rotary.data_ptr, *rotary.shape, 1 if interleaved else 0, layer, out.data_ptr, _space(out)))
+    if status:
+        def explain():
+            _query_rows(op, cache, batch, query, ("f32", "bf16"))
+            for name, t in (("key", key), ("value", value)):
+                _matrix(op, name, t, (query.dtype,), (query.shape[0], cache.kv_heads * cache.head_dim))
+        _refused(status, op, explain)
     return out
 
 
@@ -176,21 +209,21 @@ def tree_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, mask: Te
     gives zeros."""
     op = "tree_attention"
     cache_struct = cache._check(op, layer)
-    batch_struct = batch._check(op, cache, query, mask)
-    _query_rows(op, cache, batch, query, (cache.dtype,))
-    desc = _native.AttentionDesc()
-    desc.query = query.view()
-    if mask is not None:
-        _matrix(op, "mask", mask, ("u32",), (query.shape[0], None))
-        if mask.shape[1] * 32 < batch.rows:
-            raise TypeError("tree_attention mask must have a bit for every row of a sequence")
-        desc.mask = mask.view()
-    desc.scale = cache.head_dim ** -0.5 if scale is None else scale
-    desc.layer = layer
+    batch_struct = batch._check(op, cache, (query, mask))
+    view = _rank_two(op, "query", query)
     out = _output(op, out, cache.session, cache.dtype, query.shape)
-    desc.output = out.data_ptr
-    desc.output_bytes = out._buffer.nbytes - out.offset * _ITEMSIZE[out.dtype]
-    _native.check(_native.load().affon_rocm_tree_attention(cache.session._handle, cache_struct, batch_struct, desc), op)
+    status = _native.load().affon_rocm_tree_attention(
+        cache.session._handle, cache_struct, batch_struct,
+        _native.AttentionDesc(view, _NO_MASK if mask is None else _rank_two(op, "mask", mask),
+                              cache.head_dim ** -0.5 if scale is None else scale, layer, out.data_ptr, _space(out)))
+    if status:
+        def explain():
+            _query_rows(op, cache, batch, query, (cache.dtype,))
+            if mask is not None:
+                _matrix(op, "mask", mask, ("u32",), (query.shape[0], None))
+                if mask.shape[1] * 32 < batch.rows:
+                    raise TypeError("tree_attention mask must have a bit for every row of a sequence")
+        _refused(status, op, explain)
     return out
 
 
@@ -201,9 +234,13 @@ def cache_commit(cache: PagedCache, batch: DraftBatch, path: Tensor, accepted: T
     ``accepted`` u32 [B]. The caller then adds accepted[b] to lengths[b]."""
     op = "cache_commit"
     cache_struct = cache._check(op)
-    batch_struct = batch._check(op, cache, path, accepted)
-    _matrix(op, "path", path, ("u32",), (batch.sequences, None))
-    if path.shape[1] > batch.rows:
-        raise TypeError("cache_commit path is longer than the batch's rows")
-    _native.check(_native.load().affon_rocm_cache_commit(cache.session._handle, cache_struct, batch_struct, path.view(),
-                                                         _words(op, "accepted", accepted, batch.sequences)), op)
+    batch_struct = batch._check(op, cache, (path, accepted))
+    status = _native.load().affon_rocm_cache_commit(cache.session._handle, cache_struct, batch_struct,
+                                                    _rank_two(op, "path", path),
+                                                    _words(op, "accepted", accepted, batch.sequences))
+    if status:
+        def explain():
+            _matrix(op, "path", path, ("u32",), (batch.sequences, None))
+            if path.shape[1] > batch.rows:
+                raise TypeError("cache_commit path is longer than the batch's rows")
+        _refused(status, op, explain)

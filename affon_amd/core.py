@@ -130,6 +130,7 @@ class Tensor:
         # What every call on the tensor asks for; a tensor's description never changes.
         self.spec = TensorSpec(self.dtype, self.shape)
         self._view: _native.View | None = None
+        self._contiguous: bool | None = None
 
     def _check_live(self) -> None:
         if self._disposed or self._buffer.ptr is None:
@@ -151,12 +152,13 @@ class Tensor:
         return self._buffer.ptr + self.offset * _ITEMSIZE[self.dtype]
 
     def is_contiguous(self) -> bool:
-        expected = 1
-        for dim, stride in zip(reversed(self.shape), reversed(self.strides)):
-            if dim != 1 and stride != expected:
-                return False
-            expected *= dim
-        return True
+        if self._contiguous is None:
+            expected, self._contiguous = 1, True
+            for dim, stride in zip(reversed(self.shape), reversed(self.strides)):
+                if dim != 1 and stride != expected:
+                    self._contiguous = False
+                expected *= dim
+        return self._contiguous
 
     def storage(self) -> np.ndarray:
         """Reads the view back as a host array of the storage dtype (synchronizes)."""

@@ -3,6 +3,7 @@
 // behind the committed ones.
 
 #include <algorithm>
+#include <type_traits>
 
 #include "paged.h"
 
@@ -12,40 +13,47 @@ namespace {
 typedef uint32_t u32x2_t __attribute__((ext_vector_type(2)));
 typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
 
-// V (4 or 1) consecutive values.
+// V (8, 4 or 1) consecutive values.
 template <typename T, int V>
 __device__ __forceinline__ void load_values(const uint8_t* base, int64_t at, float (&v)[V]) {
   if constexpr (V == 1) {
     v[0] = T::load(base, at);
   } else if constexpr (T::bytes == 4) {
-    const u32x4_t raw = *reinterpret_cast<const u32x4_t*>(base + at * 4);
 #pragma unroll
-    for (int e = 0; e < V; ++e) v[e] = __uint_as_float(raw[e]);
+    for (int i = 0; i < V / 4; ++i) {
+      const u32x4_t raw = reinterpret_cast<const u32x4_t*>(base + at * 4)[i];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) v[4 * i + e] = __uint_as_float(raw[e]);
+    }
   } else {
-    const u32x2_t raw = *reinterpret_cast<const u32x2_t*>(base + at * 2);
+    using raw_t = typename std::conditional<V == 8, u32x4_t, u32x2_t>::type;
+    const raw_t raw = *reinterpret_cast<const raw_t*>(base + at * 2);
 #pragma unroll
     for (int e = 0; e < V; ++e) v[e] = __uint_as_float(e % 2 ? raw[e / 2] & 0xffff0000u : raw[e / 2] << 16);
   }
 }
 template <typename T, int V>
 __device__ __forceinline__ void store_values(uint8_t* base, int64_t at, const float (&v)[V]) {
-  if constexpr (T::bytes == 4) {
-    if constexpr (V == 1) {
+  if constexpr (V == 1) {
+    if constexpr (T::bytes == 4)
       reinterpret_cast<float*>(base)[at] = v[0];
-    } else {
+    else
+      reinterpret_cast<uint16_t*>(base)[at] = f32_to_bf16_bits(v[0]);
+  } else if constexpr (T::bytes == 4) {
+#pragma unroll
+    for (int i = 0; i < V / 4; ++i) {
       u32x4_t raw;
 #pragma unroll
-      for (int e = 0; e < V; ++e) raw[e] = __float_as_uint(v[e]);
-      *reinterpret_cast<u32x4_t*>(base + at * 4) = raw;
+      for (int e = 0; e < 4; ++e) raw[e] = __float_as_uint(v[4 * i + e]);
+      reinterpret_cast<u32x4_t*>(base + at * 4)[i] = raw;
     }
-  } else if constexpr (V == 1) {
-    reinterpret_cast<uint16_t*>(base)[at] = f32_to_bf16_bits(v[0]);
   } else {
-    u32x2_t raw;
+    using raw_t = typename std::conditional<V == 8, u32x4_t, u32x2_t>::type;
+    raw_t raw;
 #pragma unroll
-    for (int e = 0; e < 2; ++e)
+    for (int e = 0; e < V / 2; ++e)
       raw[e] = f32_to_bf16_bits(v[2 * e]) | static_cast<uint32_t>(f32_to_bf16_bits(v[2 * e + 1])) << 16;
-    *reinterpret_cast<u32x2_t*>(base + at * 2) = raw;
+    *reinterpret_cast<raw_t*>(base + at * 2) = raw;
   }
 }
 
@@ -165,10 +173,10 @@ __global__ __launch_bounds__(256) void append_kernel(AppendProblem p) {
 }
 
 // Every thread takes one piece of 16 bytes of a token's keys or values of one
-// layer through the accepted tokens in their order, four at a time: the path
+// layer through the accepted tokens in their order, eight at a time: the path
 // ascends strictly, so token path[i] >= i is read before anything is written
 // to its place, and no other thread touches these bytes.
-constexpr int kMoves = 4;
+constexpr int kMoves = 8;
 
 __global__ __launch_bounds__(256) void commit_kernel(PagedCache cache, DraftBatch batch, const uint32_t* path,
                                                      int64_t path_stride, int path_columns, const uint32_t* accepted) {
@@ -209,26 +217,34 @@ __global__ __launch_bounds__(256) void commit_kernel(PagedCache cache, DraftBatc
   }
 }
 
+constexpr int64_t kManyRows = 64;
+
 template <typename X, typename C>
 hipError_t append_typed(const AppendProblem& p, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   const int half = p.rotary_dim / 2;
-  // Four values at a time where every row, half and table row starts at a
-  // multiple of them, else one.
+  // Eight or four values at a time where every row, half and table row starts
+  // at a multiple of them (16-byte accesses need no more than that), else one.
   const uint64_t starts = static_cast<uint64_t>(p.query_stride | p.key_stride | p.value_stride | half |
                                                 (p.cache.head_dim / 2 - half) | p.rotary_dim);
   const uintptr_t bases = reinterpret_cast<uintptr_t>(p.query) | reinterpret_cast<uintptr_t>(p.key) |
                           reinterpret_cast<uintptr_t>(p.value);
   const uintptr_t outs = reinterpret_cast<uintptr_t>(p.out);
-  const bool wide = starts % 4 == 0 && bases % (4 * X::bytes) == 0 && outs % (4 * C::bytes) == 0 &&
-                    reinterpret_cast<uintptr_t>(p.rotary) % 16 == 0;
-  const int64_t units = rows * (p.heads + 2 * p.cache.kv_heads) * (p.cache.head_dim / (wide ? 8 : 2));
+  auto fits = [&](int v) {
+    return starts % v == 0 && bases % std::min(16, v * X::bytes) == 0 && outs % std::min(16, v * C::bytes) == 0 &&
+           reinterpret_cast<uintptr_t>(p.rotary) % 16 == 0 && p.cache.head_dim % (2 * v) == 0;
+  };
+  const int v = fits(8) && rows >= kManyRows ? 8 : fits(4) ? 4 : 1;
+  const int64_t units = rows * (p.heads + 2 * p.cache.kv_heads) * (p.cache.head_dim / (2 * v));
   const int64_t blocks = (units + 255) / 256;
   if (blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
-  if (wide)
-    hipLaunchKernelGGL((append_kernel<X, C, 4>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+  const dim3 grid(static_cast<unsigned>(blocks));
+  if (v == 8)
+    hipLaunchKernelGGL((append_kernel<X, C, 8>), grid, dim3(256), 0, stream, p);
+  else if (v == 4)
+    hipLaunchKernelGGL((append_kernel<X, C, 4>), grid, dim3(256), 0, stream, p);
   else
-    hipLaunchKernelGGL((append_kernel<X, C, 1>), dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, p);
+    hipLaunchKernelGGL((append_kernel<X, C, 1>), grid, dim3(256), 0, stream, p);
   return hipGetLastError();
 }
 

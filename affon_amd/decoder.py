@@ -17,8 +17,11 @@ Each part of the block is a Program whose weights are arguments:
 * ``feed_forward_program``: normalized ``[M, width]`` ->
   ``down(mul(silu(gate), up))``, whose gate/up pair lowers to one fused step
   (one launch at M = 1).
-Norms, RoPE, attention and the residual adds are other ops, not part of this
-path.
+
+``QuantizedDecoderBlock.step`` runs a whole block over drafted tokens: its
+norms (model.ts:64-87 has one before attention and one before the
+feed-forward), the rotation, the append to a paged cache and the attention
+are evaluated ops (cache.py, ``residual_norm``) between those Programs.
 """
 from __future__ import annotations
 
@@ -26,8 +29,9 @@ from dataclasses import dataclass
 from typing import Mapping
 
 from . import checkpoint as ckpt
+from .cache import DraftBatch, PagedCache, cache_append, tree_attention
 from .core import Program, Session, Tensor, TensorSpec, program
-from .ops import add, mul, quantized_matmul, silu
+from .ops import add, mul, quantized_matmul, residual_norm, silu
 
 # (block field of LlamaWeights, Hugging Face module, input side, output side)
 PROJECTIONS = (
@@ -39,6 +43,9 @@ PROJECTIONS = (
     ("up", "mlp.up_proj", "width", "inner_width"),
     ("down", "mlp.down_proj", "inner_width", "width"),
 )
+
+# (norm of a block, Hugging Face module of its weight)
+NORMS = {"attentionNorm": "input_layernorm", "feedForwardNorm": "post_attention_layernorm"}
 
 
 @dataclass(frozen=True)
@@ -73,8 +80,8 @@ class QuantizedDecoderBlock:
     biases, and the Programs that run them."""
 
     def __init__(self, shape: DecoderShape, layers: Mapping[str, ckpt.QuantizedLinear],
-                 output_biases: Mapping[str, Tensor] | None = None):
-        output_biases = dict(output_biases or {})
+                 output_biases: Mapping[str, Tensor] | None = None, norms: Mapping[str, Tensor] | None = None):
+        output_biases, norms = dict(output_biases or {}), dict(norms or {})
         names = [p[0] for p in PROJECTIONS]
         if sorted(layers) != sorted(names):
             raise TypeError(f"a decoder block needs the projections {names}")
@@ -97,6 +104,13 @@ class QuantizedDecoderBlock:
                 raise TypeError("gate and up output biases are not supported (the SiLU-gated product fuses them)")
             if bias.dtype not in ("f32", "bf16") or bias.shape != (shape.features(name)[0],):
                 raise TypeError(f"{name} output bias must be an f32/bf16 [{shape.features(name)[0]}] tensor")
+        for name, weight in norms.items():
+            if name not in NORMS:
+                raise TypeError(f"unknown norm {name}")
+            if weight.dtype not in ("f32", "bf16") or weight.shape != (shape.width,):
+                raise TypeError(f"{name} must be an f32/bf16 [{shape.width}] tensor")
+        self.norms = norms
+        self.unread_norms: tuple[str, ...] = ()  # of a checkpoint, in a type or shape that is not an f32/bf16 [width]
         self.shape = shape
         self.layers = dict(layers)
         self.output_biases = output_biases
@@ -112,16 +126,26 @@ class QuantizedDecoderBlock:
                         group_size: int, prefix: str = "model.layers") -> "QuantizedDecoderBlock":
         """Binds block ``index`` of an MLX-affine checkpoint: ``<prefix>.<index>.
         <module>.weight`` (U32) with ``.scales`` / ``.biases`` per projection,
-        and ``<module>.bias`` as the output bias where present."""
+        and ``<module>.bias`` as the output bias and the norms' weights where present."""
         base = f"{prefix}.{index}"
         modules = {field: f"{base}.{module}" for field, module, _, _ in PROJECTIONS}
         bound = ckpt.quantized_linears(session, path, bits=bits, group_size=group_size, prefixes=modules.values())
         header = ckpt.inspect(path)
         bias_names = [m + ".bias" for m in modules.values() if m + ".bias" in header]
-        loaded = ckpt.load(session, path, bias_names) if bias_names else {}
+        norm_names = {name: f"{base}.{module}.weight" for name, module in NORMS.items() if f"{base}.{module}.weight" in header}
+        # A weight of another type or shape does not keep the projections from
+        # being bound; a step, which needs it, then refuses.
+        unread = [n for n in norm_names if header[norm_names[n]]["dtype"] not in ("F32", "BF16")
+                  or header[norm_names[n]]["shape"] != [shape.width]]
+        for name in unread:
+            del norm_names[name]
+        wanted = bias_names + list(norm_names.values())
+        loaded = ckpt.load(session, path, wanted) if wanted else {}
         layers = {field: bound[module] for field, module in modules.items()}
         biases = {field: loaded[module + ".bias"] for field, module in modules.items() if module + ".bias" in loaded}
-        return cls(shape, layers, biases)
+        block = cls(shape, layers, biases, {name: loaded[module] for name, module in norm_names.items()})
+        block.unread_norms = tuple(unread)
+        return block
 
     # ---- Programs ----
 
@@ -197,3 +221,31 @@ class QuantizedDecoderBlock:
         """down(silu(gate(h)) * up(h)) of normalized activations [M, width]."""
         return self._run(self.feed_forward_program(normalized.shape[0], normalized.dtype), {"normalized": normalized},
                          **options)
+
+    def step(self, stream: Tensor, update: Tensor | None, cache: PagedCache, batch: DraftBatch, rotary: Tensor, *,
+             positions: Tensor | None = None, mask: Tensor | None = None, layer: int = 0, epsilon: float = 1e-5,
+             scale: float | None = None, interleaved: bool = False, **options) -> tuple[Tensor, Tensor]:
+        """The block over a batch's drafted tokens (row b*T + i of ``stream``
+        [B*T, width]: token i of sequence b), whose keys and values it appends to
+        ``layer`` of the cache. ``update`` is what the block before still adds to
+        the stream (None: nothing), and the result (stream, update) what the next
+        one takes: every residual add is part of the norm that follows it. After
+        the last block, ``residual_norm(stream, update, weight=final)`` gives
+        the hidden states, and once their tokens are judged ``cache_commit``
+        keeps the accepted ones.
+
+        ``positions`` and ``mask`` as cache_append and tree_attention take them (a
+        tree's depths and ancestors; None: a chain); ``options``: the
+        projections' compile options."""
+        if self.unread_norms:
+            raise TypeError(f"the checkpoint's {', '.join(self.unread_norms)} is no f32/bf16 [{self.shape.width}] tensor")
+        stream, normalized = residual_norm(stream, update, weight=self.norms.get("attentionNorm"), epsilon=epsilon,
+                                           dtype=cache.dtype)
+        query, key, value = self.attention(normalized, **options)
+        rotated = cache_append(cache, batch, query, key, value, positions, rotary, layer=layer,
+                               interleaved=interleaved)
+        attended = tree_attention(cache, batch, rotated, mask, layer=layer, scale=scale)
+        stream, normalized = residual_norm(stream, self.attention_output(attended, **options),
+                                           weight=self.norms.get("feedForwardNorm"), epsilon=epsilon,
+                                           dtype=cache.dtype)
+        return stream, self.feed_forward(normalized, **options)

@@ -611,27 +611,33 @@ def _run_index_select(x: Tensor, axis: int, indices: Tensor) -> Tensor:
 
 # ---- the norms between blocks (no counterpart op in the reference) ----
 
-def _rows_operand(name: str, t: Any, like: Tensor, rank_one: bool = False) -> Tensor:
-    """An f32/bf16 operand of residual_norm shaped like the stream (rank_one:
-    or of its columns), of its Session and with consecutive columns."""
-    if not isinstance(t, Tensor) or t.dtype not in ("f32", "bf16") or \
-            t.shape != like.shape and not (rank_one and t.shape == like.shape[1:]):
-        raise TypeError(f"residual_norm {name} must be an f32/bf16 tensor of the stream's shape"
-                        + (" or of its columns" if rank_one else ""))
-    if t.shape[-1] > 1 and t.strides[-1] != 1:
-        raise TypeError(f"residual_norm {name} must have consecutive columns")
-    if t.session is not like.session:
-        raise TypeError("residual_norm operands must belong to the same Session")
-    return t
+_FLOAT_CODES = {"f32": _native.F32, "bf16": _native.BF16}
 
 
-def _weight_operand(name: str, t: Any, like: Tensor) -> Tensor:
-    if not isinstance(t, Tensor) or t.dtype not in ("f32", "bf16") or t.shape != like.shape[1:] or \
-            not t.is_contiguous():
+def _rows_operand(name: str, t: Any, like: Tensor, rank_one: bool = False) -> tuple[int, int, int]:
+    """Address, row stride and type of an f32/bf16 operand of residual_norm
+    shaped like the stream (rank_one: or like one of its rows, at stride 0),
+    of its Session and with consecutive columns."""
+    if not isinstance(t, Tensor) or t.session is not like.session:
+        raise TypeError("residual_norm operands must be tensors of the same Session")
+    code = _FLOAT_CODES.get(t.dtype)
+    if code is not None:
+        if t.shape == like.shape:
+            if t.strides[1] == 1 or t.shape[1] == 1:
+                return t.data_ptr, t.strides[0], code
+            raise TypeError(f"residual_norm {name} must have consecutive columns")
+        if rank_one and t.shape == like.shape[1:] and t.is_contiguous():
+            return t.data_ptr, 0, code
+    raise TypeError(f"residual_norm {name} must be " + (
+        f"a contiguous f32/bf16 [{like.shape[1]}] tensor" if name.endswith("weight") else
+        "an f32/bf16 tensor of the stream's shape" + (" or of its columns" if rank_one else "")))
+
+
+def _weight_operand(name: str, t: Any, like: Tensor) -> tuple[int, int]:
+    address, stride, code = _rows_operand(name, t, like, rank_one=True)
+    if len(t.shape) != 1:
         raise TypeError(f"residual_norm {name} must be a contiguous f32/bf16 [{like.shape[1]}] tensor")
-    if t.session is not like.session:
-        raise TypeError("residual_norm operands must belong to the same Session")
-    return t
+    return address, code
 
 
 def residual_norm(stream: Tensor, update: Tensor | None = None, *, gate: Tensor | None = None, scale: float = 1.0,
@@ -652,48 +658,36 @@ def residual_norm(stream: Tensor, update: Tensor | None = None, *, gate: Tensor 
     both results; the first may be the stream itself."""
     if not isinstance(stream, Tensor) or len(stream.shape) != 2:
         raise TypeError("residual_norm requires an evaluated rank-two stream")
-    _rows_operand("stream", stream, stream)
-    epsilon, scale = float(epsilon), float(scale)
-    if not np.isfinite(epsilon) or epsilon <= 0:
-        raise TypeError("invalid residual_norm options: epsilon must be finite and positive")
-    if not np.isfinite(scale):
-        raise TypeError("invalid residual_norm options: scale must be finite")
-    if update is None and (gate is not None or post_norm):
-        raise TypeError("residual_norm without an update takes no gate and no post_norm")
-    if post_weight is not None and not post_norm:
-        raise TypeError("residual_norm post_weight needs post_norm")
-    if post_weight is not None and weight is not None and post_weight.dtype != weight.dtype:
-        raise TypeError("residual_norm weights must have one type")
+    address, stride, code = _rows_operand("stream", stream, stream)
+    rows, cols = stream.shape
+    # The library checks the numbers (epsilon, scale) and what goes with what.
+    desc = _native.ResidualNormDesc()
+    desc.rows, desc.cols, desc.scale, desc.epsilon = rows, cols, scale, epsilon
+    desc.stream, desc.stream_stride, desc.stream_dtype = address, stride, code
+    if update is not None:
+        desc.update, desc.update_stride, desc.update_dtype = _rows_operand("update", update, stream)
+    if gate is not None:
+        desc.gate, desc.gate_stride, desc.gate_dtype = _rows_operand("gate", gate, stream, rank_one=True)
+    if post_norm:
+        desc.post_norm = 1
+    if post_weight is not None:
+        desc.post_weight, desc.weight_dtype = _weight_operand("post_weight", post_weight, stream)
+    if weight is not None:
+        if post_weight is not None and post_weight.dtype != getattr(weight, "dtype", None):
+            raise TypeError("residual_norm weights must have one type")
+        desc.weight, desc.weight_dtype = _weight_operand("weight", weight, stream)
     if dtype not in (None, "f32", "bf16"):
         raise TypeError("residual_norm result must be f32 or bf16")
-    code = {"f32": _native.F32, "bf16": _native.BF16}
-    desc = _native.ResidualNormDesc(rows=stream.shape[0], cols=stream.shape[1], scale=scale, epsilon=epsilon,
-                                    post_norm=1 if post_norm else 0, stream=stream.data_ptr,
-                                    stream_stride=stream.strides[0], stream_dtype=code[stream.dtype])
-    if update is not None:
-        _rows_operand("update", update, stream)
-        desc.update, desc.update_stride, desc.update_dtype = update.data_ptr, update.strides[0], code[update.dtype]
-    if gate is not None:
-        _rows_operand("gate", gate, stream, rank_one=True)
-        desc.gate, desc.gate_dtype = gate.data_ptr, code[gate.dtype]
-        desc.gate_stride = gate.strides[0] if len(gate.shape) == 2 else 0
-    if post_weight is not None:
-        _weight_operand("post_weight", post_weight, stream)
-        desc.post_weight, desc.weight_dtype = post_weight.data_ptr, code[post_weight.dtype]
-    if weight is not None:
-        _weight_operand("weight", weight, stream)
-        desc.weight, desc.weight_dtype = weight.data_ptr, code[weight.dtype]
     if out is None:
         out = (stream if update is None else stream.session.empty(stream.dtype, stream.shape),
                stream.session.empty(dtype or stream.dtype, stream.shape))
     first, normalized = out
-    _rows_operand("output", first, stream)
-    _rows_operand("output", normalized, stream)
-    if first.dtype != stream.dtype or dtype not in (None, normalized.dtype):
+    desc.stream_out, desc.stream_out_stride, first_code = _rows_operand("output", first, stream)
+    desc.normalized, desc.normalized_stride, desc.normalized_dtype = _rows_operand("output", normalized, stream)
+    if first_code != code or dtype not in (None, normalized.dtype):
         raise TypeError("residual_norm outputs must have the stream's type and that of the result")
-    desc.stream_out, desc.stream_out_stride = first.data_ptr, first.strides[0]
-    desc.normalized, desc.normalized_stride = normalized.data_ptr, normalized.strides[0]
-    desc.normalized_dtype = code[normalized.dtype]
-    _native.check(_native.load().affon_rocm_residual_norm(stream.session._handle, ctypes.byref(desc)),
-                  "Program execution failed")
+    status = _native.load().affon_rocm_residual_norm(stream.session._handle, desc)
+    if status == _native.INVALID_SHAPE:
+        raise TypeError(_native.last_error())
+    _native.check(status, "Program execution failed")
     return first, normalized

@@ -100,3 +100,10 @@ def test_infinities_and_nan_stay_in_their_row(session, rng):
     y, n = A.residual_norm(upload(session, stored(x, "f32"), "f32"), upload(session, stored(x, "f32"), "f32"))
     assert np.isnan(n.numpy()[1]).all() and np.isfinite(n.numpy()[[0, 2]]).all()
     assert np.isnan(y.numpy()[1]).sum() == 1
+
+
+@pytest.mark.parametrize("N", [520, 1024, 2000, 4096, 8190, 9000])
+def test_many_wide_rows(session, rng, N):
+    """As many rows as there are two threads' values of, and one fewer."""
+    for M in (511, 512):
+        check(session, rng, M, N, post=True, gate="columns", stream="bf16")
