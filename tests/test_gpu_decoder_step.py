@@ -156,7 +156,7 @@ def test_accepted_tokens_go_on_as_if_they_came_one_by_one(session, blocks, rng):
     close(next_token, single.run(last, T=1))
 
 
-def test_norm_weights_of_other_types(session, tmp_path):
+def test_norm_weights_of_other_shapes(session, tmp_path):
     """They are not read; the projections are, and a step refuses."""
     entries = []
     for field, module, _, _ in PROJECTIONS:
@@ -165,7 +165,7 @@ def test_norm_weights_of_other_types(session, tmp_path):
         entries += [(name + ".weight", "U32", [out, inp // 4], np.zeros((out, inp // 4), np.uint32).tobytes()),
                     (name + ".scales", "BF16", [out, inp // GROUP], np.zeros((out, inp // GROUP), np.uint16).tobytes()),
                     (name + ".biases", "BF16", [out, inp // GROUP], np.zeros((out, inp // GROUP), np.uint16).tobytes())]
-    entries.append(("model.layers.0.input_layernorm.weight", "F16", [256], np.ones(256, np.float16).tobytes()))
+    entries.append(("model.layers.0.input_layernorm.weight", "F32", [1, 256], np.ones(256, np.float32).tobytes()))
     path = write_file(tmp_path / "block.safetensors", entries, metadata={"format": "mlx"})
     block = QuantizedDecoderBlock.from_checkpoint(session, str(path), 0, SHAPE, bits=BITS, group_size=GROUP)
     assert not block.norms and len(block.attention(session.empty("bf16", (1, 256)))) == 3
