@@ -2,7 +2,7 @@
 //
 // The query heads that share a key head, G of them, and the T drafted tokens
 // of a sequence make T*G rows over the same keys and values. A wave holds 16
-// to 64 of these rows and walks over keys 32 (bf16) or 16 (f32) at a time:
+// or 32 of these rows and walks over keys 32 (bf16) or 16 (f32) at a time:
 //   S^T = K Q^T      (MFMA, rows of the queries as columns of the result),
 //   P = e^(S - m)    (one running reference m per row),
 //   O^T += V^T P^T   (MFMA).
@@ -12,12 +12,24 @@
 // keys 4 (lane / 16) .. + 3 of each 16, and the order of the keys inside a
 // product is free as long as V^T is read in the same one.
 //
+// What bounds it (one MI355X, head width 128, bf16): few rows, the memory (32
+// sequences of one token over up to 4096: 68 us, 5.0 TB/s of keys and
+// values, where a large copy reaches 5.2); many rows, the instructions around
+// the products (trees of 64 of 16 sequences over up to 16384, 512 rows to a
+// key head: 432 us, 757 TFLOP/s; a large library product reaches 1272). There
+// the matrix cores are busy a third of the time: without the softmax's
+// exponentials 10% goes, without the products as much, without the transfers
+// 20%, and no one of them alone is the limit. Tried there, us: four row tiles
+// a wave instead of two 552 (a wave to a SIMD), one 516 to 582 in three or
+// four waves; the two tiles' products and softmax in turns within a wave 459;
+// a wave priority for either 434 to 443.
+//
 // m follows the largest score only where a score passes it by more than
 // kSlack: e^(S - m) then stays below 2^kSlack, the sums and O are in f32 and
 // a later m only scales them, so that most steps neither reduce across lanes
 // nor touch O.
 //
-// Keys and values reach LDS by direct transfers, several steps ahead; 16
+// Keys and values reach LDS by direct transfers, a step ahead; 16
 // keys of one head and page are consecutive in memory, and every transfer
 // moves whole 1 KiB pieces of them. LDS keeps their order, its 16-byte pieces
 // permuted inside each row where the row is a power of two long (the banks

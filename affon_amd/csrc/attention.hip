@@ -97,13 +97,15 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // One round of workgroups, two to a CU: a second round of shorter ones costs
   // more in starts and joins than it evens out (32 sequences of one token over
   // up to 4096 tokens: 68.0 us in 512 workgroups, 76.8 in 768; trees of 24 of
-  // 8 sequences 57.8 and 69.6). Longer pieces than kEven leave the GPU uneven
-  // where lengths differ (trees of 64 over up to 16384: 541 us in 512
-  // workgroups, 450 in 2048), and pieces of fewer keys than rows cost more to
-  // join than they read.
+  // 8 sequences 57.8 and 69.6). Much longer pieces leave the GPU uneven where
+  // lengths differ, but the results of many rows weigh more (trees of 64 of
+  // 16 sequences over up to 16384: 541 us in 512 workgroups, 445 in pieces of
+  // 4096 keys, 463 of 2048). Pieces of fewer keys than rows cost more to join
+  // than they read (trees of 64 of one sequence over 2000 tokens: 20.2 us in
+  // pieces of as many keys as rows, 24.4 in twice that, 44.6 in eight times).
   constexpr int64_t kRound = 512, kEven = 2048;
-  int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 16 * own_rows));
-  splits = std::min(splits, capacity / std::max<int64_t>(128, (half ? 2 : 1) * own_rows));
+  int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 32 * own_rows));
+  splits = std::min(splits, capacity / std::max<int64_t>(128, own_rows));
   splits = std::max<int64_t>(splits, 1);
   a.chunk = static_cast<uint32_t>((capacity + splits - 1) / splits + 127) / 128 * 128;
   a.splits = static_cast<int>((capacity + a.chunk - 1) / a.chunk);
