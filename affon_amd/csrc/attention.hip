@@ -102,12 +102,18 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   // 16 sequences over up to 16384: 541 us in 512 workgroups, 445 in pieces of
   // 4096 keys, 463 of 2048). Pieces of fewer keys than rows cost more to join
   // than they read (trees of 64 of one sequence over 2000 tokens: 20.2 us in
-  // pieces of as many keys as rows, 24.4 in twice that, 44.6 in eight times).
+  // pieces of as many keys as rows, 24.4 in twice that, 44.6 in eight times);
+  // f32, whose products take eight times as long, is cut finer (trees of 32 of
+  // 4 sequences over up to 2000 tokens 38.6 us against 51.5 with bf16's sizes).
   constexpr int64_t kRound = 512, kEven = 2048;
-  int64_t splits = std::max(kRound / (units * a.row_groups), capacity / std::max(kEven, 32 * own_rows));
-  splits = std::min(splits, capacity / std::max<int64_t>(128, own_rows));
+  const int64_t groups_whole = units * a.row_groups;
+  // Four rounds of workgroups are even enough, and hold the partial results of no more.
+  const int64_t even = std::min(capacity / std::max(kEven, 32 * own_rows), (4 * kRound + groups_whole - 1) / groups_whole);
+  int64_t splits = std::max(kRound / groups_whole, even);
+  const int64_t unit = half ? 128 : 64;  // keys, at least
+  splits = std::min(splits, capacity / std::max<int64_t>(unit, half ? own_rows : own_rows / 2));
   splits = std::max<int64_t>(splits, 1);
-  a.chunk = static_cast<uint32_t>((capacity + splits - 1) / splits + 127) / 128 * 128;
+  a.chunk = static_cast<uint32_t>((capacity + splits - 1) / splits + unit - 1) / unit * unit;
   a.splits = static_cast<int>((capacity + a.chunk - 1) / a.chunk);
   if (a.splits > 1) {
     const size_t slots = static_cast<size_t>(units) * a.splits * a.row_slots;

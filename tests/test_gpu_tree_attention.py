@@ -184,3 +184,46 @@ def test_captured_calls_follow_new_lengths(session, rng):
             np.testing.assert_array_equal(out.storage(), replayed)
     finally:
         hip.destroy(graph)
+
+
+@pytest.mark.parametrize("dtype,T", [("bf16", 1), ("bf16", 20), ("f32", 3)])
+def test_a_capture_without_scratch(rng, dtype, T):
+    """A session's first call, captured: no memory for partial results can be
+    had, and every workgroup walks a whole context of several page lists."""
+    hip = HipRuntime()
+    with A.Session("rocm") as session:
+        step = Step(rng, B=2, T=T, heads=8, kv=2, dim=64, lengths=(9000, 4095), dtype=dtype, spread=2.0).device(session)
+        query = upload(session, step.query, dtype)
+        out = session.empty(dtype, query.shape)
+        graph = hip.capture(session.stream, lambda: A.tree_attention(step.cache, step.batch, query, out=out))
+        try:
+            for _ in range(3):
+                hip.replay(session.stream, graph)
+                replayed = out.storage()
+                step.check(replayed)
+                warm = A.tree_attention(step.cache, step.batch, query).storage()  # in pieces
+                step.check(warm)
+        finally:
+            hip.destroy(graph)
+
+
+def test_calls_from_several_threads(session, rng):
+    """Threads share a session's partial results and counters one call at a time."""
+    import threading
+    steps = [Step(rng, B=1, T=1, heads=8, kv=2, dim=128, lengths=(n,)).device(session) for n in (3000, 900, 5000, 1700)]
+    queries = [upload(session, s.query, "bf16") for s in steps]
+    results = [[] for _ in steps]
+
+    def work(i):
+        for _ in range(20):
+            results[i].append(A.tree_attention(steps[i].cache, steps[i].batch, queries[i]))
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(len(steps))]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    for s, outs in zip(steps, results):
+        first = outs[0].storage()
+        s.check(first)
+        for other in outs[1:]:
+            np.testing.assert_array_equal(other.storage(), first)
