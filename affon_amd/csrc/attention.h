@@ -262,8 +262,10 @@ struct Kernel {
     id = id / a.row_groups * 8 + (blockIdx.x & 7);
     const int kv = id % p.cache.kv_heads;
     id /= p.cache.kv_heads;
-    const int b = id % p.batch.sequences, split = id / p.batch.sequences;
-    if (split >= a.splits) return;
+    // The last pieces first: only the longest sequences have them, and a piece
+    // that starts when the others end holds the whole call up.
+    const int b = id % p.batch.sequences, split = a.splits - 1 - id / p.batch.sequences;
+    if (split < 0) return;
 
     // The page list's first part, whose loads need not wait for the lengths.
     const uint32_t start = static_cast<uint32_t>(split) * a.chunk;

@@ -138,7 +138,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   }
   const int64_t groups = units * a.splits;
   const int64_t blocks = (groups + 7) / 8 * 8 * a.row_groups;
-  if (blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
   (half ? launch_bf16 : launch_f32)(a, shape, grid, l.stream);
   hipError_t e = hipGetLastError();
@@ -148,7 +148,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   const int shares = std::min((a.splits + 7) / 8, 256 / pieces);
   const int64_t per = 256 / (pieces * shares);
   const int64_t join_blocks = (static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads + per - 1) / per;
-  if (join_blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  if (join_blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 join_grid(static_cast<unsigned>(join_blocks));
   if (half)
     hipLaunchKernelGGL(join_kernel<BF16>, join_grid, dim3(256), 0, l.stream, a, shares);

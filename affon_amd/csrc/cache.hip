@@ -237,7 +237,7 @@ hipError_t append_typed(const AppendProblem& p, hipStream_t stream) {
   const int v = fits(8) && rows >= kManyRows ? 8 : fits(4) ? 4 : 1;
   const int64_t units = rows * (p.heads + 2 * p.cache.kv_heads) * (p.cache.head_dim / (2 * v));
   const int64_t blocks = (units + 255) / 256;
-  if (blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (v == 8)
     hipLaunchKernelGGL((append_kernel<X, C, 8>), grid, dim3(256), 0, stream, p);
@@ -261,7 +261,7 @@ hipError_t commit_launch(const PagedCache& cache, const DraftBatch& batch, const
   const int line_pieces = cache.head_dim * (cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
   const int64_t units = static_cast<int64_t>(cache.layers) * batch.sequences * 2 * cache.kv_heads * line_pieces;
   const int64_t blocks = (units + 255) / 256;
-  if (blocks > (int64_t(1) << 31) - 1) return hipErrorInvalidValue;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
   hipLaunchKernelGGL(commit_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, cache, batch, path,
                      path_stride, path_columns, accepted);
   return hipGetLastError();

@@ -17,6 +17,9 @@ __device__ __forceinline__ uint32_t drafted(const DraftBatch& batch, int b) {
   return batch.counts != nullptr ? min(batch.counts[b], rows) : rows;
 }
 
+// Workgroups of up to 256 threads that a launch takes: 2^32 threads.
+constexpr int64_t kMaxBlocks = (int64_t(1) << 24) - 1;
+
 constexpr uint32_t kNoPage = 0xffffffffu;
 
 // The page that holds page `index` of sequence b, or kNoPage.

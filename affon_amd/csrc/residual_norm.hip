@@ -254,7 +254,9 @@ void launch_held(const NormArgs& a, hipStream_t stream) {
 
 }  // namespace
 
-hipError_t residual_norm_launch(const affon_rocm_residual_norm_desc& d, hipStream_t stream) {
+namespace {
+
+void launch_rows(const affon_rocm_residual_norm_desc& d, hipStream_t stream) {
   const NormArgs a{d,
                    d.stream_dtype == AFFON_ROCM_BF16,
                    d.update_dtype == AFFON_ROCM_BF16,
@@ -287,7 +289,32 @@ hipError_t residual_norm_launch(const affon_rocm_residual_norm_desc& d, hipStrea
     launch_held<1024, 2>(a, stream);
   else
     hipLaunchKernelGGL(long_kernel, dim3(static_cast<unsigned>(d.rows)), dim3(kLongThreads), 0, stream, a);
-  return hipGetLastError();
+}
+
+}  // namespace
+
+// A workgroup a row, and as many rows as a grid holds to a launch (a loop over
+// rows in the kernel: 2048 x 8192 f32 with a gate 78 us against 53).
+hipError_t residual_norm_launch(const affon_rocm_residual_norm_desc& d, hipStream_t stream) {
+  constexpr int64_t kMaxGrid = int64_t(1) << 20;
+  auto skip = [](const void* base, int64_t rows, int64_t stride, int dtype) {
+    return base == nullptr ? nullptr
+                           : const_cast<uint8_t*>(static_cast<const uint8_t*>(base)) +
+                                 rows * stride * (dtype == AFFON_ROCM_BF16 ? 2 : 4);
+  };
+  for (int64_t row = 0; row < d.rows; row += kMaxGrid) {
+    affon_rocm_residual_norm_desc part = d;
+    part.rows = std::min(kMaxGrid, d.rows - row);
+    part.stream = skip(d.stream, row, d.stream_stride, d.stream_dtype);
+    part.update = skip(d.update, row, d.update_stride, d.update_dtype);
+    part.gate = skip(d.gate, row, d.gate_stride, d.gate_dtype);
+    part.stream_out = skip(d.stream_out, row, d.stream_out_stride, d.stream_dtype);
+    part.normalized = skip(d.normalized, row, d.normalized_stride, d.normalized_dtype);
+    launch_rows(part, stream);
+    const hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+  }
+  return hipSuccess;
 }
 
 }  // namespace affon

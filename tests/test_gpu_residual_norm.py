@@ -107,3 +107,7 @@ def test_many_wide_rows(session, rng, N):
     """As many rows as there are two threads' values of, and one fewer."""
     for M in (511, 512):
         check(session, rng, M, N, post=True, gate="columns", stream="bf16")
+
+
+def test_more_rows_than_a_grid_holds(session, rng):
+    check(session, rng, (1 << 20) + 3, 9, update="bf16", post=True)
