@@ -787,9 +787,13 @@ void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 template <typename T, int DT, bool EXACT, int RT, int WR>
 void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
-  // Waves over the keys: as many as two stages each leave room for.
-    constexpr int WK = WR > 1 ? 1 : Probe::kStage > 8192 ? 2 : 4;
-    // Two steps in LDS: three took 457 us against 446 for trees of 64 over up to 16384 tokens, four 720.
+  // Waves over the keys: as many as leave room in LDS for two workgroups of
+  // two steps a wave; f32, which has more to compute in the same bytes, gains
+  // by a third wave at widths of 65 to 96 (32 sequences of one token over up to
+  // 4096, width 80: 109 us against 139), bf16 does not (48.1 and 48.0, width 96
+  // 58.1 and 57.1).
+  constexpr int WK = WR > 1 ? 1 : Probe::kStage <= 8192 ? 4 : Probe::kStage <= 12288 && !Probe::kHalf ? 3 : 2;
+  // Two steps in LDS: three took 457 us against 446 for trees of 64 over up to 16384 tokens, four 720.
   constexpr int STAGES = 2;
   using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
   hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
@@ -802,6 +806,9 @@ void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
       if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1>(a, grid, stream);
       return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
     }
+  }
+  if constexpr (DT > 8) {
+    if (shape.waves == 2) return launch_shape<T, DT, EXACT, 1, 2>(a, grid, stream);
   }
   if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
   if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
@@ -816,6 +823,9 @@ void launch_head(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
   if (D < 64) return launch_width<T, 4, false>(a, shape, grid, stream);
   if (D <= 96) return launch_width<T, 6, false>(a, shape, grid, stream);
   if (D < 128) return launch_width<T, 8, false>(a, shape, grid, stream);
+  // Tiles that 256 columns would waste, 32 sequences of one token over up to
+  // 4096: width 192 bf16 108 us against 114, f32 322 and 477.
+  if (D <= 192) return launch_width<T, 12, false>(a, shape, grid, stream);
   launch_width<T, 16, false>(a, shape, grid, stream);
 }
 

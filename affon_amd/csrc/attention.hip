@@ -62,10 +62,14 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* words, int count) 
 }
 
 // Few rows: waves side by side over the keys; more: over the rows, and where
-// the keys of two waves do not fit in LDS twice to a CU.
+// the keys of two waves do not fit in LDS twice to a CU. There two waves, as
+// the ones past the last row still repeat its work: 32 sequences of one token
+// over up to 4096, width 256, bf16 133 us in two waves and 169 in four, f32 306
+// and 614.
 Shape shape_for(int rows, int head_dim) {
   if (rows <= 16 && head_dim <= 128) return {1, 1};
   if (rows <= 32 && head_dim <= 128) return {2, 1};
+  if (rows <= 32) return {1, 2};
   // Wide heads of odd sizes leave no registers for a second tile.
   if (rows <= 64 || (head_dim > 128 && head_dim != 256)) return {1, 4};
   return {2, 4};

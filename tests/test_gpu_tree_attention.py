@@ -5,7 +5,7 @@ import numpy as np
 import pytest
 
 import affon_amd as A
-from tests.drafts import NO_PAGE, Step, mask_words, set_tensor, stored, tree, upload
+from tests.drafts import NO_PAGE, Step, mask_words, set_tensor, stored, tree, upload, widened
 from tests.helpers import HipRuntime
 
 pytestmark = pytest.mark.gpu
@@ -93,6 +93,30 @@ def test_masked_infinities_and_nan_stay_out(session, rng, dtype, T, length):
         if key == 1.0:  # a seen infinity or NaN is what the sum says
             from tests.drafts import widened
             assert not np.isfinite(widened(got[~blind])).any()
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("dim", [24, 72, 80, 96, 112, 160, 192])
+@pytest.mark.parametrize("T", [5, 21])
+def test_odd_widths(session, rng, T, dtype, dim):
+    """Heads whose rows lie in the banks in other orders: trees over a few
+    steps, and a value that is not finite for the rows that do not see it."""
+    step = Step(rng, T=T, heads=6, kv=2, dim=dim, lengths=(75,), dtype=dtype, spread=2.0).device(session)
+    mask = tree(rng, 1, T, wide=0.9)
+    clean = attend(session, step, mask)
+    step.check(clean, mask)
+    for j in range(1, T, 3):
+        blind = ~mask[:, j]
+        page, line = step.place(0, 75 + j)
+        values = step.values.copy()
+        values[0, page, :, line, j] = stored(np.inf, dtype)
+        set_tensor(step.cache.values, values)
+        got = attend(session, step, mask)
+        assert blind.any()
+        np.testing.assert_array_equal(got[blind], clean[blind])
+        seen = widened(got[~blind]).reshape(-1, 6, dim)
+        assert np.isposinf(seen[..., j]).all()
+        assert np.isfinite(np.delete(seen, j, axis=-1)).all()
 
 
 def test_scores_far_apart(session, rng):
