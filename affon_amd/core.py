@@ -153,11 +153,13 @@ class Tensor:
 
     def is_contiguous(self) -> bool:
         if self._contiguous is None:
-            expected, self._contiguous = 1, True
+            # Stored once it is known: another thread may be asking.
+            expected, contiguous = 1, True
             for dim, stride in zip(reversed(self.shape), reversed(self.strides)):
                 if dim != 1 and stride != expected:
-                    self._contiguous = False
+                    contiguous = False
                 expected *= dim
+            self._contiguous = contiguous
         return self._contiguous
 
     def storage(self) -> np.ndarray:
