@@ -21,6 +21,7 @@
 
 #include "affon_rocm.h"
 #include "internal.h"
+#include "overlap.h"
 
 struct affon_rocm_session {
   int device = 0;
@@ -1116,6 +1117,11 @@ int affon_rocm_residual_norm(affon_rocm_session* session, const affon_rocm_resid
     return fail(AFFON_ROCM_INVALID_SHAPE, "%s without an update takes no gate and no post_norm", op);
   if (d->post_norm == 0 && d->post_weight != nullptr)
     return fail(AFFON_ROCM_INVALID_SHAPE, "%s post_weight needs post_norm", op);
+  // Without an update a stream that is its own output is left alone, whatever its stride.
+  const bool kept = d->update == nullptr && d->stream_out == d->stream &&
+                    (d->rows == 1 || d->stream_out_stride == d->stream_stride);
+  affon_rocm_residual_norm_desc run = *d;
+  if (kept) run.stream_out = nullptr;
   const struct {
     const void* data;
     int dtype;
@@ -1125,7 +1131,7 @@ int affon_rocm_residual_norm(affon_rocm_session* session, const affon_rocm_resid
                   {d->gate, d->gate_dtype, d->gate_stride, 0},
                   {d->post_weight, d->weight_dtype, 0, 0},
                   {d->weight, d->weight_dtype, 0, 0},
-                  {d->stream_out, d->stream_dtype, d->stream_out_stride, d->cols},
+                  {run.stream_out, d->stream_dtype, d->stream_out_stride, d->cols},
                   {d->normalized, d->normalized_dtype, d->normalized_stride, d->cols}};
   for (const auto& o : operands) {
     if (o.data == nullptr) continue;
@@ -1140,7 +1146,27 @@ int affon_rocm_residual_norm(affon_rocm_session* session, const affon_rocm_resid
   if (!(d->scale - d->scale == 0.0f)) return fail(AFFON_ROCM_INVALID_SHAPE, "invalid residual_norm options: scale must be finite");
   int status = check_session(session);
   if (status != AFFON_ROCM_OK) return status;
-  const hipError_t e = affon::residual_norm_launch(*d, session->stream);
+
+  // An output may be the stream, update or gate itself: a thread reads its
+  // values of a row before it writes them. What overlaps in another way would
+  // be read by threads and rows after others have written there.
+  auto rows = [&](const void* data, int dtype, int64_t stride) {
+    const int size = element_size(dtype);
+    return affon::rows_of(data, d->rows, d->cols * size, stride * size);
+  };
+  const affon::Rows stream = rows(d->stream, d->stream_dtype, d->stream_stride);
+  const affon::Rows stream_out = rows(run.stream_out, d->stream_dtype, d->stream_out_stride);
+  const affon::Rows normalized = rows(d->normalized, d->normalized_dtype, d->normalized_stride);
+  if (affon::rows_meet(kept ? stream : stream_out, normalized))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s outputs overlap", op);
+  const affon::Rows inputs[] = {stream, rows(d->update, d->update_dtype, d->update_stride),
+                                rows(d->gate, d->gate_dtype, d->gate_stride),
+                                rows(d->post_weight, d->weight_dtype, 0), rows(d->weight, d->weight_dtype, 0)};
+  for (const auto& in : inputs)
+    for (const auto& out : {stream_out, normalized})
+      if (affon::rows_meet(in, out) && !affon::same_rows(in, out))
+        return fail(AFFON_ROCM_INVALID_SHAPE, "%s output overlaps an operand that it is not", op);
+  const hipError_t e = affon::residual_norm_launch(run, session->stream);
   if (e != hipSuccess) return hip_fail(e, op);
   return AFFON_ROCM_OK;
 }

@@ -186,7 +186,7 @@ __global__ __launch_bounds__(THREADS) void held_kernel(NormArgs a) {
       add_update(a, r, at, inverse, u[j], x[j]);
       store_chunk(r.stream_out, a.stream_half, at, cols, x[j]);
     }
-  } else if (a.d.stream_out != nullptr && a.d.stream_out != a.d.stream) {
+  } else if (a.d.stream_out != nullptr) {
 #pragma unroll
     for (int j = 0; j < HELD; ++j)
       store_chunk(r.stream_out, a.stream_half, (threadIdx.x + j * THREADS) * kChunk, cols, x[j]);
@@ -237,8 +237,7 @@ __global__ __launch_bounds__(kLongThreads) void long_kernel(NormArgs a) {
   for (int64_t at = threadIdx.x * kChunk; at < cols; at += kLongThreads * kChunk) {
     float x[kChunk];
     summed(at, x);
-    if (a.d.stream_out != nullptr && (r.update != nullptr || a.d.stream_out != a.d.stream))
-      store_chunk(r.stream_out, a.stream_half, at, cols, x);
+    if (a.d.stream_out != nullptr) store_chunk(r.stream_out, a.stream_half, at, cols, x);
     write_normalized(a, r, at, last, x);
   }
 }

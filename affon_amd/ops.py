@@ -655,7 +655,8 @@ def residual_norm(stream: Tensor, update: Tensor | None = None, *, gate: Tensor 
     rows at any stride; ``gate`` [M, N] or [N]; weights [N], both of one type.
     Without an update the stream is only normalized, and returned as it is.
     ``dtype`` of normalized: by default the stream's. ``out``: tensors for
-    both results; the first may be the stream itself."""
+    both results, each of which may be the stream, the update or the gate
+    itself, and overlaps nothing else."""
     if not isinstance(stream, Tensor) or len(stream.shape) != 2:
         raise TypeError("residual_norm requires an evaluated rank-two stream")
     address, stride, code = _rows_operand("stream", stream, stream)

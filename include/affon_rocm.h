@@ -418,7 +418,8 @@ int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cac
  *   normalized = stream' / sqrt(mean(stream'^2) + epsilon) * weight
  * of each row, in f32 (normalized from stream' before it is rounded). A null
  * update leaves the stream as it is (stream_out may then be null); null weights and gates are ones. Every
- * operand is f32 or bf16 by itself; row strides are in elements. stream_out may be the stream itself. */
+ * operand is f32 or bf16 by itself; row strides are in elements. An output may be the stream, the update or the
+ * gate itself (its address, type and stride), and otherwise overlaps no operand and no other output. */
 typedef struct {
   const void* stream;
   const void* update;
