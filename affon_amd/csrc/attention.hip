@@ -119,6 +119,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   splits = std::max<int64_t>(splits, 1);
   a.chunk = static_cast<uint32_t>((capacity + splits - 1) / splits + unit - 1) / unit * unit;
   a.splits = static_cast<int>((capacity + a.chunk - 1) / a.chunk);
+  bool few = false;
   if (a.splits > 1) {
     const size_t slots = static_cast<size_t>(units) * a.splits * a.row_slots;
     const size_t sums = (slots * p.cache.head_dim * sizeof(float) + 255) / 256 * 256;
@@ -130,10 +131,12 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
       // Few results are joined by the workgroup that is last to end (one token
       // over 777: 9.4 us against 11.8 with a second launch; 32 sequences 67.7
       // and 70.2), more by a launch of their own (one token over 32000, 129 KB
-      // a head: 36.6 and 34.6; trees of 24 94 and 62).
+      // a head: 36.6 and 34.6; trees of 24 94 and 62). Captured calls get no
+      // tickets, and join few results in a launch too, in the same order (one
+      // token over 777 in a graph: 10.3 us against 8.3 with tickets).
       constexpr int64_t kJoined = 32768;
-      if (own_rows * p.cache.head_dim * 4 * a.splits <= kJoined && units * a.row_groups <= Workspace::kTickets &&
-          l.workspace != nullptr)
+      few = own_rows * p.cache.head_dim * 4 * a.splits <= kJoined;
+      if (few && units * a.row_groups <= Workspace::kTickets && l.workspace != nullptr)
         a.tickets = l.workspace->tickets(&fresh);
       if (fresh) hipLaunchKernelGGL(clear_kernel, dim3(64), dim3(256), 0, l.stream, a.tickets, Workspace::kTickets);
     } else {  // a captured stream whose workspace cannot grow
@@ -149,7 +152,7 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   if (e != hipSuccess || a.splits == 1 || a.tickets != nullptr) return e;
   // A share takes the eight splits that a thread has in flight.
   const int pieces = p.cache.head_dim / 4;
-  const int shares = std::min((a.splits + 7) / 8, 256 / pieces);
+  const int shares = few ? 1 : std::min((a.splits + 7) / 8, 256 / pieces);
   const int64_t per = 256 / (pieces * shares);
   const int64_t join_blocks = (static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads + per - 1) / per;
   if (join_blocks > kMaxBlocks) return hipErrorInvalidValue;

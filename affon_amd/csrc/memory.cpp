@@ -17,7 +17,8 @@ bool Workspace::capturing() const {
 
 uint32_t* Workspace::tickets(bool* fresh) {
   *fresh = false;
-  if (tickets_ == nullptr && !capturing()) {
+  if (capturing()) return nullptr;
+  if (tickets_ == nullptr) {
     if (hipMalloc(&tickets_, kTickets * sizeof(uint32_t)) == hipSuccess) {
       *fresh = true;
     } else {

@@ -26,7 +26,10 @@ class Workspace {
   void* get(size_t bytes);
   // kTickets words for workgroups of one launch to count each other, which
   // every launch leaves at 0; *fresh: they were allocated now, and the caller
-  // clears them on the stream. Null when they cannot be allocated now.
+  // clears them on the stream. Null when they cannot be allocated, and for
+  // captured launches: a graph replayed beside other work of the session would
+  // mix both counts and leave words raised for every later call. Only launches
+  // that the session's stream orders count in them.
   static constexpr int kTickets = 65536;
   uint32_t* tickets(bool* fresh);
   size_t retired() const { return retired_.size(); }
