@@ -110,7 +110,7 @@ class QuantizedDecoderBlock:
             if weight.dtype not in ("f32", "bf16") or weight.shape != (shape.width,):
                 raise TypeError(f"{name} must be an f32/bf16 [{shape.width}] tensor")
         self.norms = norms
-        self.unread_norms: tuple[str, ...] = ()  # of a checkpoint, in a type or shape that is not an f32/bf16 [width]
+        self.unread_norms: tuple[str, ...] = ()  # that a checkpoint does not hold as f32/bf16 [width]
         self.shape = shape
         self.layers = dict(layers)
         self.output_biases = output_biases
@@ -126,25 +126,27 @@ class QuantizedDecoderBlock:
                         group_size: int, prefix: str = "model.layers") -> "QuantizedDecoderBlock":
         """Binds block ``index`` of an MLX-affine checkpoint: ``<prefix>.<index>.
         <module>.weight`` (U32) with ``.scales`` / ``.biases`` per projection,
-        and ``<module>.bias`` as the output bias and the norms' weights where present."""
+        and ``<module>.bias`` as the output bias where present. Norms' weights
+        are read where they are f32/bf16 ``[width]``; without them the block runs
+        its projections and refuses a ``step``. (A block that is made without
+        ``norms`` has norms of ones.)"""
         base = f"{prefix}.{index}"
         modules = {field: f"{base}.{module}" for field, module, _, _ in PROJECTIONS}
         bound = ckpt.quantized_linears(session, path, bits=bits, group_size=group_size, prefixes=modules.values())
         header = ckpt.inspect(path)
         bias_names = [m + ".bias" for m in modules.values() if m + ".bias" in header]
         norm_names = {name: f"{base}.{module}.weight" for name, module in NORMS.items() if f"{base}.{module}.weight" in header}
-        # A weight of another type or shape does not keep the projections from
-        # being bound; a step, which needs it, then refuses.
-        unread = [n for n in norm_names if header[norm_names[n]]["dtype"] not in ("F32", "BF16")
-                  or header[norm_names[n]]["shape"] != [shape.width]]
-        for name in unread:
+        # A weight that is not there, or of another type or shape, does not keep
+        # the projections from being bound; a step, which needs it, then refuses.
+        for name in [n for n in norm_names if header[norm_names[n]]["dtype"] not in ("F32", "BF16")
+                     or header[norm_names[n]]["shape"] != [shape.width]]:
             del norm_names[name]
         wanted = bias_names + list(norm_names.values())
         loaded = ckpt.load(session, path, wanted) if wanted else {}
         layers = {field: bound[module] for field, module in modules.items()}
         biases = {field: loaded[module + ".bias"] for field, module in modules.items() if module + ".bias" in loaded}
         block = cls(shape, layers, biases, {name: loaded[module] for name, module in norm_names.items()})
-        block.unread_norms = tuple(unread)
+        block.unread_norms = tuple(n for n in NORMS if n not in norm_names)
         return block
 
     # ---- Programs ----
@@ -238,7 +240,7 @@ class QuantizedDecoderBlock:
         tree's depths and ancestors; None: a chain); ``options``: the
         projections' compile options."""
         if self.unread_norms:
-            raise TypeError(f"the checkpoint's {', '.join(self.unread_norms)} is no f32/bf16 [{self.shape.width}] tensor")
+            raise TypeError(f"the checkpoint holds no f32/bf16 [{self.shape.width}] tensor for {', '.join(self.unread_norms)}")
         stream, normalized = residual_norm(stream, update, weight=self.norms.get("attentionNorm"), epsilon=epsilon,
                                            dtype=cache.dtype)
         query, key, value = self.attention(normalized, **options)
