@@ -176,7 +176,8 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
     u32 [B*T] (None: lengths[b] + i); ``rotary``: a ``rotary_table``, whose
     rotary_dim may be less than head_dim; pairs are dims (j, j + rotary_dim/2),
     or neighbours with ``interleaved``. Rows not in use append nothing and
-    return zeros."""
+    return zeros. ``out`` may be the query itself, and overlaps no operand
+    otherwise."""
     op = "cache_append"
     cache_struct = cache._check(op, layer)
     batch_struct = batch._check(op, cache, (query, key, value, positions, rotary))
@@ -206,7 +207,8 @@ def tree_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, mask: Te
     committed tokens and drafted token j where bit j % 32 of ``mask``[b*T + i,
     j // 32] is set (u32; None: a chain, j <= i). ``scale`` of the scores: by
     default head_dim ** -0.5. A row that sees nothing, or is not in use,
-    gives zeros."""
+    gives zeros. ``out`` may be the query itself, and overlaps no operand
+    otherwise."""
     op = "tree_attention"
     cache_struct = cache._check(op, layer)
     batch_struct = batch._check(op, cache, (query, mask))

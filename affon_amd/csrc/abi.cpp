@@ -1004,6 +1004,33 @@ int check_query(const affon_rocm_view& q, const affon::PagedCache& cache, const 
   return AFFON_ROCM_OK;
 }
 
+affon::Rows rows_of_view(const affon_rocm_view& v) {
+  if (v.data == nullptr) return affon::Rows{nullptr, 0, 0, 0};
+  const int64_t size = element_size(v.dtype);
+  return affon::rows_of(origin(v), v.shape[0], v.shape[1] * size, v.stride[0] * size);
+}
+
+affon::Rows words(const void* data, int64_t count) { return affon::rows_of(data, 1, count * 4, 0); }
+
+// The output of the queries' shape: it may be the query itself, as whoever
+// writes a value there has read it before, and otherwise overlaps nothing.
+int check_output(const void* output, const affon_rocm_view& query, const affon_rocm_kv_cache& cache,
+                 const affon_rocm_draft_batch& batch, const affon::DraftBatch& b, const char* op,
+                 std::initializer_list<affon::Rows> others) {
+  const int64_t bytes = query.shape[1] * element_size(cache.dtype);
+  const affon::Rows out = affon::rows_of(output, query.shape[0], bytes, bytes);
+  const affon::Rows q = rows_of_view(query);
+  bool clear = !affon::rows_meet(q, out) || affon::same_rows(q, out);
+  const int64_t cache_bytes = cache.layers * cache.pages * cache.kv_heads * cache.page_size * cache.head_dim *
+                              element_size(cache.dtype);
+  for (const auto& held : {affon::rows_of(cache.keys, 1, cache_bytes, 0), affon::rows_of(cache.values, 1, cache_bytes, 0),
+                           rows_of_view(batch.page_table), words(b.lengths, b.sequences), words(b.counts, b.sequences)})
+    clear = clear && !affon::rows_meet(held, out);
+  for (const auto& other : others) clear = clear && !affon::rows_meet(other, out);
+  if (!clear) return fail(AFFON_ROCM_INVALID_SHAPE, "%s output overlaps an operand that it is not", op);
+  return AFFON_ROCM_OK;
+}
+
 }  // namespace
 
 int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
@@ -1041,7 +1068,11 @@ int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cac
   p.rotary_dim = static_cast<int>(d->rotary_dim);
   p.interleaved = d->interleaved != 0;
   p.out = static_cast<uint8_t*>(d->output);
-  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  if ((status = check_session(session)) != AFFON_ROCM_OK ||
+      (status = check_output(d->output, d->query, *cache, *batch, p.batch, op,
+                             {rows_of_view(d->key), rows_of_view(d->value), words(d->positions, rows),
+                              words(d->rotary, d->rotary_rows * d->rotary_dim)})) != AFFON_ROCM_OK)
+    return status;
   const hipError_t e = affon::append_launch(p, session->stream);
   if (e != hipSuccess) return hip_fail(e, op);
   return AFFON_ROCM_OK;
@@ -1072,7 +1103,9 @@ int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_c
   p.query_stride = d->query.stride[0];
   p.scale = d->scale;
   p.out = static_cast<uint8_t*>(d->output);
-  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  if ((status = check_session(session)) != AFFON_ROCM_OK ||
+      (status = check_output(d->output, d->query, *cache, *batch, p.batch, op, {rows_of_view(d->mask)})) != AFFON_ROCM_OK)
+    return status;
   affon::Launch launch;
   launch.stream = session->stream;
   launch.workspace = session->workspace;

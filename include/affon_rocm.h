@@ -376,7 +376,8 @@ typedef struct {
   int64_t rotary_rows, rotary_dim; /* rotary_dim: even, at most head_dim */
   int32_t interleaved;
   int64_t layer;
-  void* output; /* rotated queries [B*T, heads*head_dim], contiguous, the cache's type */
+  void* output; /* rotated queries [B*T, heads*head_dim], contiguous, the cache's type: the query itself, or
+                   memory of no operand */
   size_t output_bytes;
 } affon_rocm_append_desc;
 int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
@@ -397,7 +398,7 @@ typedef struct {
   affon_rocm_view mask;  /* [B*T, >= T/32 rounded up] u32, unit inner stride; data null: a chain */
   float scale;
   int64_t layer;
-  void* output; /* [B*T, heads*head_dim], contiguous, the cache's type */
+  void* output; /* [B*T, heads*head_dim], contiguous, the cache's type: the query itself, or memory of no operand */
   size_t output_bytes;
 } affon_rocm_attention_desc;
 int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,

@@ -5,7 +5,7 @@ import pytest
 
 import affon_amd as A
 from affon_amd.core import Tensor
-from tests.drafts import stored, upload
+from tests.drafts import Step, stored, upload
 
 pytestmark = pytest.mark.gpu
 
@@ -81,3 +81,57 @@ def test_norms_without_an_update(session, rng):
     assert same is row
     one = A.residual_norm(view(whole, (1, 64), (64, 1)))[1].numpy()
     np.testing.assert_array_equal(n.numpy(), np.repeat(one, 4, axis=0))
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+@pytest.mark.parametrize("T,lengths", [(1, (700, 3)), (40, (50, 0)), (70, (2500, 900))])
+def test_attention_and_append_in_place_of_the_query(session, rng, dtype, T, lengths):
+    step = Step(rng, B=2, T=T, heads=8, kv=2, dim=64, lengths=lengths, dtype=dtype).device(session)
+    query = lambda: upload(session, step.query, dtype)
+    want = A.tree_attention(step.cache, step.batch, query()).storage()
+    step.check(want)
+    q = query()
+    assert A.tree_attention(step.cache, step.batch, q, out=q) is q
+    np.testing.assert_array_equal(q.storage(), want)
+    for interleaved in (False, True):
+        args = (query(), query(), None, A.rotary_table(session, 4000, 64))
+        kv = [upload(session, step.query[:, i * 128:(i + 1) * 128], dtype) for i in range(2)]
+        want = A.cache_append(step.cache, step.batch, query(), *kv, *args[2:], interleaved=interleaved).storage()
+        q = query()
+        A.cache_append(step.cache, step.batch, q, *kv, *args[2:], interleaved=interleaved, out=q)
+        np.testing.assert_array_equal(q.storage(), want)
+
+
+def test_outputs_that_overlap_operands(session, rng):
+    step = Step(rng, B=2, T=3, heads=4, kv=2, dim=64, lengths=(20, 7)).device(session)
+    wide = session.empty("bf16", (20, 512))
+    columns = view(wide, (6, 256), (512, 1))
+    refused = lambda: pytest.raises(Exception, match="overlaps an operand")
+    with refused():  # the same first row, another stride
+        A.tree_attention(step.cache, step.batch, columns, out=view(wide, (6, 256), (256, 1)))
+    query = view(wide, (6, 256), (256, 1))
+    with refused():  # a row further
+        A.tree_attention(step.cache, step.batch, query, out=view(wide, (6, 256), (256, 1), 256))
+    whole = step.cache.keys
+    flat = view(whole, (6, 256), (256, 1), 64)
+    keys = whole.storage()
+    kv = [upload(session, step.query[:, :128], "bf16") for _ in range(2)]
+    rotary = A.rotary_table(session, 64, 64)
+    for out in (flat, view(step.cache.values, (6, 256), (256, 1))):
+        with refused():
+            A.tree_attention(step.cache, step.batch, query, out=out)
+        with refused():
+            A.cache_append(step.cache, step.batch, query, *kv, None, rotary, out=out)
+    with refused():  # a value that is part of the output
+        A.cache_append(step.cache, step.batch, upload(session, step.query, "bf16"), kv[0], view(wide, (6, 128), (512, 1), 128),
+                       None, rotary, out=query)
+    with refused():  # f32 queries where bf16 ones go
+        f32 = session.empty("f32", (6, 256))
+        A.cache_append(step.cache, step.batch, f32, *(view(session.empty("f32", (6, 128)), (6, 128), (128, 1)) for _ in "kv"),
+                       None, rotary, out=view(f32, (6, 256), (256, 1), 0, "bf16"))
+    np.testing.assert_array_equal(whole.storage(), keys)
+    # Columns beside the query's are no part of it.
+    data = np.zeros((6, 512), np.uint16)
+    data[:, :256] = step.query
+    part = upload(session, data, "bf16")
+    A.tree_attention(step.cache, step.batch, view(part, (6, 256), (512, 1)), out=view(wide, (6, 256), (256, 1)))
