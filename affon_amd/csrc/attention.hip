@@ -3,6 +3,7 @@
 // results (attention.h holds the kernels).
 
 #include <algorithm>
+#include <cfloat>
 #include <cmath>
 
 #include "attention.h"
@@ -90,7 +91,8 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   const Shape shape = shape_for(a.rows, p.cache.head_dim);
   a.row_groups = (a.rows + shape.rows() - 1) / shape.rows();
   a.row_slots = a.rows;
-  a.log2_scale = p.scale == 0.0f ? 1.0f : std::fabs(p.scale) * 1.44269504088896340736f;
+  // Finite for every finite scale: infinite, it would make NaN of scores of 0.
+  a.log2_scale = p.scale == 0.0f ? 1.0f : std::min(std::fabs(p.scale) * 1.44269504088896340736f, FLT_MAX);
   a.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
 
   // Pieces of the context: enough workgroups for the GPU, none so short that

@@ -389,7 +389,7 @@ int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cac
  * j / 32] is set (no mask: j <= i). For each of its heads, with key head
  * head / (heads / kv_heads):
  *   out = sum_n e^(scale q.k_n - m) v_n / sum_n e^(scale q.k_n - m),
- * m the largest score seen; a row that sees nothing gives zeros, whatever
+ * m the largest score seen; a row that sees nothing (or only scores of -infinity) gives zeros, and whatever
  * unseen slots hold, infinities and NaN included, does not reach its output. Scores, the
  * softmax and sums in f32; for bf16 the probabilities are rounded to bf16
  * for the product with v. */
