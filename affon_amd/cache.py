@@ -106,7 +106,7 @@ class DraftBatch:
     entry >= pages names none); ``lengths`` u32 [B]: committed tokens;
     ``counts`` u32 [B]: drafted tokens in use (default: all). Drafted token i of
     sequence b is its token lengths[b] + i. The tensors are read when a call
-    runs: write new values into them for the next step."""
+    runs: ``Tensor.write`` puts new values into them for the next step."""
 
     def __init__(self, page_table: Tensor, lengths: Tensor, rows: int, *, counts: Tensor | None = None):
         _matrix("DraftBatch", "page_table", page_table, ("u32",), (None, None))

@@ -173,6 +173,21 @@ class Tensor:
         return np.lib.stride_tricks.as_strided(raw[self.offset:], shape=self.shape,
                                                strides=tuple(s * item for s in self.strides)).copy()
 
+    def write(self, values: Any) -> "Tensor":
+        """Replaces the values of a contiguous tensor by host values of its
+        shape, after the calls made so far and before later ones: how a step's
+        lengths, tables or masks get new values where calls, and captured ones,
+        read them."""
+        self._check_live()
+        storage = host_storage(values, self.dtype)
+        if storage.shape != self.shape:
+            raise TypeError(f"write requires values of shape {list(self.shape)}")
+        if not self.is_contiguous():
+            raise TypeError("write requires a contiguous tensor")
+        _native.check(_native.load().affon_rocm_memcpy_h2d(self.session._handle, self.data_ptr, storage.ctypes.data,
+                                                           storage.nbytes), "upload")
+        return self
+
     def numpy(self) -> np.ndarray:
         """Host values: f32 for f32/bf16 (bf16 widened exactly), u32 for u32."""
         values = self.storage()

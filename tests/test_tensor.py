@@ -56,3 +56,21 @@ def test_contiguous_of_many_tensors_in_threads():
         assert not wrong
     finally:
         sys.setswitchinterval(interval)
+
+
+class Memory:
+    ptr, nbytes = 1 << 20, 1 << 10
+
+
+@pytest.mark.parametrize("shape,strides,values,message", [
+    ((3, 4), (4, 1), [1, 2, 3], "shape"), ((3, 4), (5, 1), [[0] * 4] * 3, "contiguous"), ((2,), (1,), 5, "shape")])
+def test_what_a_write_refuses(shape, strides, values, message):
+    with pytest.raises(TypeError, match=message):
+        Tensor(None, Memory, "u32", shape, strides).write(values)
+
+
+def test_a_disposed_tensor_takes_no_values():
+    t = Tensor(None, Memory, "f32", (2,), (1,))
+    t.dispose()
+    with pytest.raises(RuntimeError, match="disposed"):
+        t.write([1, 2])
