@@ -37,9 +37,12 @@ COMMON_FLAGS = [
 EXACT_FLAGS = {"quantize.hip": ["-ffp-contract=off"], "generic.hip": ["-ffp-contract=off"]}
 # Decode-batch kernels whose MFMA results feed VALU scaling every step: the
 # MFMAs write ordinary VGPRs, so no accumulator-register read
-# (v_accvgpr_read) sits between each MFMA and its scaling. No kernel in
-# these files needs scratch memory with it. The attention kernels' softmax
-# reads every product's result the same way.
+# (v_accvgpr_read) sits between each MFMA and its scaling. The attention
+# kernels' softmax reads every product's result the same way. With it no kernel
+# of gemv_mfma and vrow needs scratch memory; of the xgemm files 16 of 102 do,
+# 8 to 100 bytes a lane, and of the attention's 54 three, all of two row tiles a
+# wave and more than 64 rows: bf16 of width 128 (12 bytes), bf16 (52) and f32
+# (160) of widths 104 to 120.
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 UNIT_FLAGS = {**EXACT_FLAGS, **{f: VGPR_MFMA for f in ("gemv_mfma.hip", "vrow_b2.hip", "vrow_b4.hip", "vrow_b8.hip",
                                                      "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip", "attention_bf16.hip",

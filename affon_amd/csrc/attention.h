@@ -16,13 +16,14 @@
 // sequences of one token over up to 4096: 68 us, 5.0 TB/s of keys and
 // values, where a large copy reaches 5.2); many rows, the instructions around
 // the products (trees of 64 of 16 sequences over up to 16384, 512 rows to a
-// key head: 432 us, 757 TFLOP/s; a large library product reaches 1272). There
-// the matrix cores are busy a third of the time: without the softmax's
-// exponentials 10% goes, without the products as much, without the transfers
-// 20%, and no one of them alone is the limit. Tried there, us: four row tiles
-// a wave instead of two 552 (a wave to a SIMD), one 516 to 582 in three or
-// four waves; the two tiles' products and softmax in turns within a wave 459;
-// a wave priority for either 434 to 443.
+// key head: 424 to 437 us with the join, 750 to 770 TFLOP/s; a large library
+// product reaches 1272). There the matrix cores are busy a third of the time:
+// without the softmax's exponentials 10% goes, without the products as much,
+// without the transfers 20%, and no one of them alone is the limit. Tried
+// there, us: four row tiles a wave instead of two 552 (a wave to a SIMD), one
+// 516 to 582 in three or four waves, and the two tiles' products and softmax in
+// turns within a wave 459, all against 447 at the time; a wave priority for
+// either 434 to 443 against 437 to 442.
 //
 // m follows the largest score only where a score passes it by more than
 // kSlack: e^(S - m) then stays below 2^kSlack, the sums and O are in f32 and
@@ -605,6 +606,12 @@ struct Kernel {
               s[rt][kt][i] = __builtin_amdgcn_exp2f(fmaf(s[rt][kt][i], a.log2_scale, -m[rt]));
               l[rt] += s[rt][kt][i];
             }
+          // The matrix cores take bf16: each probability is rounded once for its
+          // product, their sum l is of the unrounded ones, and O stays f32. That is
+          // one rounding of 2^-9 a term, averaged over the terms: against 64 bits a
+          // result is off by 1.4e-3 to 2.4e-3 where f32 throughout, rounded at the
+          // end, gives 1.0e-3 to 1.6e-3. A second product for the rounded part would
+          // double the instructions of this half.
           if constexpr (kHalf)
             packed[rt] = u32x4_t{pack_bf16(s[rt][0][0], s[rt][0][1]), pack_bf16(s[rt][0][2], s[rt][0][3]),
                                  pack_bf16(s[rt][kKT - 1][0], s[rt][kKT - 1][1]),

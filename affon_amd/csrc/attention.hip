@@ -96,7 +96,11 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   a.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
 
   // Pieces of the context: enough workgroups for the GPU, none so short that
-  // its results weigh against the keys it reads.
+  // its results weigh against the keys it reads. The lengths are on the device,
+  // so pieces are cut from what the table holds; under a table wider than the
+  // contexts they are longer and fewer, and the rest of the workgroups leave at
+  // once (one token over 777 8.8 us under a table of 784 tokens, 10.9 of 8192
+  // and 15.2 of 131072; 8 sequences of 2000 17.1 us, 17.3 and 28.8).
   const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
   const int64_t capacity = p.batch.capacity;
   const int64_t own_rows = std::min(a.rows, shape.rows());

@@ -349,7 +349,8 @@ typedef struct {
 /* `rows` (T) drafted tokens of each sequence: row b*T + i of the operands is
  * token i of sequence b. Sequence b holds lengths[b] tokens; its token n lies
  * in line n % page_size of page page_table[b, n / page_size], and drafted token i is
- * its token lengths[b] + i. A table entry that names no page (>= pages) and
+ * its token lengths[b] + i. A table no wider than the longest context lets
+ * attention cut its work finest. A table entry that names no page (>= pages) and
  * tokens past the table hold nothing: appends to them are dropped, attention
  * does not see them. Only the first counts[b] rows are in use (null: all);
  * the others append nothing, and their outputs are zeros. */
