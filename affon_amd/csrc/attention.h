@@ -314,15 +314,20 @@ struct Kernel {
     f32x4_t o[RT][DT];
     float m[RT], l[RT];
 
-    auto place_queries = [&] {  // dims past the head are 0, and the scale's sign is theirs
-      const uint32_t keep = a.sign == 0.0f ? 0u : ~0u, flip = a.sign < 0.0f ? (kHalf ? 0x80008000u : 0x80000000u) : 0u;
+    // Dims past the head are 0, and the scale's sign is theirs. So are rows not
+    // in use: a NaN there would leave sums that are not finite (below).
+    auto place_queries = [&] {
+      const uint32_t flip = a.sign < 0.0f ? (kHalf ? 0x80008000u : 0x80000000u) : 0u;
 #pragma unroll
-      for (int rt = 0; rt < RT; ++rt)
+      for (int rt = 0; rt < RT; ++rt) {
+        const bool used = min(row0 + rt * 16 + col, a.rows - 1) / a.group < static_cast<int>(count);
+        const uint32_t keep = a.sign == 0.0f || !used ? 0u : ~0u;
 #pragma unroll
         for (int s = 0; s < kQSteps; ++s)
 #pragma unroll
           for (int e = 0; e < 4; ++e)
             q[rt][s][e] = !EXACT && s * 64 + quad * 16 >= row_bytes ? 0u : (q[rt][s][e] & keep) ^ flip;
+      }
     };
 
     // Transfers: where this lane's 16 bytes of every piece come from.
