@@ -114,6 +114,33 @@ class AppendDesc(ctypes.Structure):
     ]
 
 
+class HeadNorm(ctypes.Structure):
+    """affon_rocm_head_norm."""
+    _fields_ = [
+        ("query_weight", c_void_p),
+        ("key_weight", c_void_p),
+        ("query_weight_stride", c_int64),
+        ("key_weight_stride", c_int64),
+        ("query_weight_dtype", c_int32),
+        ("key_weight_dtype", c_int32),
+        ("epsilon", ctypes.c_float),
+        ("axes", c_int32),
+        ("axis", ctypes.c_uint8 * 128),
+    ]
+
+
+class WeightsDesc(ctypes.Structure):
+    """affon_rocm_weights_desc."""
+    _fields_ = [
+        ("query", View),
+        ("mask", View),
+        ("scale", ctypes.c_float),
+        ("layer", c_int64),
+        ("weights", c_void_p),
+        ("weights_bytes", c_size_t),
+    ]
+
+
 class AttentionDesc(ctypes.Structure):
     """affon_rocm_attention_desc."""
     _fields_ = [
@@ -184,6 +211,16 @@ SIGNATURES = {
                                         ctypes.POINTER(AppendDesc)]),
     "affon_rocm_tree_attention": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
                                           ctypes.POINTER(AttentionDesc)]),
+    "affon_rocm_cache_append_normed": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                               ctypes.POINTER(AppendDesc), ctypes.POINTER(HeadNorm)]),
+    "affon_rocm_shared_attention": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                            ctypes.POINTER(AttentionDesc), c_void_p, c_int64]),
+    "affon_rocm_attention_weights": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                             ctypes.POINTER(WeightsDesc)]),
+    "affon_rocm_cache_evict": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch), c_void_p, c_void_p,
+                                       c_size_t, c_void_p, c_void_p]),
+    "affon_rocm_weights_commit": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
+                                          ctypes.POINTER(View), c_void_p, c_void_p, c_size_t]),
     "affon_rocm_cache_commit": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
                                         ctypes.POINTER(View), c_void_p]),
     "affon_rocm_residual_norm": (c_int, [c_void_p, ctypes.POINTER(ResidualNormDesc)]),

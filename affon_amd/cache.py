@@ -10,7 +10,10 @@ tree: speculative decoding).
   and values to a layer;
 * ``tree_attention`` attends over the committed tokens and, by a mask, the drafted
   ones;
-* ``cache_commit`` keeps the accepted tokens of the draft, in all layers.
+* ``shared_attention`` does so where sequences share a prefix, read once for all;
+* ``cache_commit`` keeps the accepted tokens of the draft, in all layers;
+* ``attention_weights`` adds up what attention every token of a layer gathers, and
+  ``cache_evict`` keeps those that gathered most.
 
 Row ``b * T + i`` of an operand is drafted token i of sequence b. All calls
 enqueue on the Session's stream and read lengths, tables and masks on the
@@ -143,6 +146,42 @@ def rotary_table(session: Session, positions: int, rotary_dim: int, *, theta: fl
     return session.tensor(np.concatenate([np.cos(angle), np.sin(angle)], 1), "f32")
 
 
+class RotaryAxes:
+    """Which of up to four axes of the positions each pair of a head's rotated dims turns by."""
+
+    def __init__(self, axes):
+        self.axes = tuple(axes)
+        if not 1 <= len(self.axes) <= 128 or any(type(a) is not int or not 0 <= a < 4 for a in self.axes):
+            raise TypeError("RotaryAxes takes 1 to 128 axes from 0 to 3")
+        self.count = max(self.axes) + 1
+        self._packed = (ctypes.c_uint8 * 128)(*self.axes)
+
+
+def rotary_axes(sections, *, interleaved: bool = False) -> RotaryAxes:
+    """The axes of sections[0] + sections[1] + .. pairs (together rotary_dim / 2):
+    the first sections[0] pairs turn by axis 0 (say, time), the next by axis 1
+    (height), and so on; ``interleaved``: the axes take pairs in turn, while
+    each has some left."""
+    sections = [_positive("a section", n) for n in sections]
+    if not 1 <= len(sections) <= 4 or sum(sections) > 128:
+        raise TypeError("rotary_axes takes one to four sections of together at most 128 pairs")
+    if not interleaved:
+        return RotaryAxes(a for a, n in enumerate(sections) for _ in range(n))
+    return RotaryAxes(a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n)
+
+
+_ONE_AXIS = (ctypes.c_uint8 * 128)()
+
+
+def _norm_weight(name: str, t: Tensor | None, heads: int, dim: int) -> tuple[int | None, int, int]:
+    """Address, elements from head to head and type of a norm's weights."""
+    if t is None:
+        return None, 0, 0
+    if t.dtype not in ("f32", "bf16") or t.shape not in ((dim,), (heads * dim,)) or not t.is_contiguous():
+        raise TypeError(f"cache_append {name} must be a contiguous f32/bf16 [{dim}] or [{heads * dim}] tensor")
+    return t.data_ptr, dim if t.shape[0] > dim else 0, _NATIVE_DTYPE[t.dtype]
+
+
 def _query_rows(op: str, cache: PagedCache, batch: DraftBatch, query: Tensor, dtypes: tuple[str, ...]) -> None:
     _matrix(op, "query", query, dtypes, (batch.sequences * batch.rows, None))
     if query.shape[1] % (cache.kv_heads * cache.head_dim):
@@ -169,7 +208,8 @@ def _rank_two(op: str, name: str, t: Tensor) -> _native.View:
 
 def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tensor, value: Tensor,
                  positions: Tensor | None, rotary: Tensor, *, layer: int = 0, interleaved: bool = False,
-                 out: Tensor | None = None) -> Tensor:
+                 query_norm: Tensor | None = None, key_norm: Tensor | None = None, epsilon: float = 1e-5,
+                 axes: RotaryAxes | None = None, out: Tensor | None = None) -> Tensor:
     """Appends the drafted tokens' keys [B*T, kv_heads*head_dim], rotated by
     their positions, and values to a layer of the cache, and returns the
     rotated queries [B*T, heads*head_dim] in the cache's type. ``positions``
@@ -177,7 +217,13 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
     rotary_dim may be less than head_dim; pairs are dims (j, j + rotary_dim/2),
     or neighbours with ``interleaved``. Rows not in use append nothing and
     return zeros. ``out`` may be the query itself, and overlaps no operand
-    otherwise."""
+    otherwise.
+
+    ``query_norm``, ``key_norm``: f32/bf16 weights [head_dim], or [heads*head_dim]
+    with each head's own, of norms before the rotation: x / sqrt(mean(x^2) +
+    epsilon) * weight of every query (key) head. ``axes`` (``rotary_axes``):
+    ``positions`` are then [axes, B*T], and each pair turns by those of its
+    axis."""
     op = "cache_append"
     cache_struct = cache._check(op, layer)
     batch_struct = batch._check(op, cache, (query, key, value, positions, rotary))
@@ -187,10 +233,27 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
         raise TypeError("cache_append rotary table must be a contiguous f32 [*, *] tensor, its width even and at most "
                         "head_dim")
     out = _output(op, out, cache.session, cache.dtype, query.shape)
-    status = _native.load().affon_rocm_cache_append(
-        cache.session._handle, cache_struct, batch_struct,
-        _native.AppendDesc(*views, None if positions is None else _words(op, "positions", positions, query.shape[0]),
-                           rotary.data_ptr, *rotary.shape, 1 if interleaved else 0, layer, out.data_ptr, _space(out)))
+    if axes is None:
+        place = None if positions is None else _words(op, "positions", positions, query.shape[0])
+    else:
+        if not isinstance(axes, RotaryAxes) or 2 * len(axes.axes) != rotary.shape[1]:
+            raise TypeError("cache_append axes must be a RotaryAxes of rotary_dim / 2 pairs")
+        if positions is not None and (positions.dtype != "u32" or positions.shape != (axes.count, query.shape[0]) or
+                                      not positions.is_contiguous()):
+            raise TypeError(f"cache_append positions must be a contiguous u32 [{axes.count}, {query.shape[0]}] tensor")
+        place = None if positions is None else positions.data_ptr
+    desc = _native.AppendDesc(*views, place, rotary.data_ptr, *rotary.shape, 1 if interleaved else 0, layer, out.data_ptr,
+                              _space(out))
+    native = _native.load()
+    if axes is None and query_norm is None and key_norm is None:
+        status = native.affon_rocm_cache_append(cache.session._handle, cache_struct, batch_struct, desc)
+    else:
+        batch._check(op, cache, (query_norm, key_norm))
+        q_data, q_stride, q_dtype = _norm_weight("query_norm", query_norm, query.shape[1] // cache.head_dim, cache.head_dim)
+        k_data, k_stride, k_dtype = _norm_weight("key_norm", key_norm, cache.kv_heads, cache.head_dim)
+        norm = _native.HeadNorm(q_data, k_data, q_stride, k_stride, q_dtype, k_dtype, epsilon,
+                                1 if axes is None else axes.count, _ONE_AXIS if axes is None else axes._packed)
+        status = native.affon_rocm_cache_append_normed(cache.session._handle, cache_struct, batch_struct, desc, norm)
     if status:
         def explain():
             _query_rows(op, cache, batch, query, ("f32", "bf16"))
@@ -218,28 +281,124 @@ def tree_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, mask: Te
         cache.session._handle, cache_struct, batch_struct,
         _native.AttentionDesc(view, _NO_MASK if mask is None else _rank_two(op, "mask", mask),
                               cache.head_dim ** -0.5 if scale is None else scale, layer, out.data_ptr, _space(out)))
+    _attention_status(status, op, cache, batch, query, mask)
+    return out
+
+
+def _attention_status(status: int, op: str, cache: PagedCache, batch: DraftBatch, query: Tensor, mask: Tensor | None) -> None:
     if status:
         def explain():
             _query_rows(op, cache, batch, query, (cache.dtype,))
             if mask is not None:
                 _matrix(op, "mask", mask, ("u32",), (query.shape[0], None))
                 if mask.shape[1] * 32 < batch.rows:
-                    raise TypeError("tree_attention mask must have a bit for every row of a sequence")
+                    raise TypeError(f"{op} mask must have a bit for every row of a sequence")
         _refused(status, op, explain)
+
+
+def shared_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, shared: Tensor, mask: Tensor | None = None, *,
+                     layer: int = 0, scale: float | None = None, out: Tensor | None = None) -> Tensor:
+    """``tree_attention`` of sequences that share a prefix, which is read once
+    for all of them. ``shared`` u32 [groups]: the B sequences are `groups`
+    groups of B / groups one after the other, and each sequence of group g with
+    lengths[b] >= shared[g] holds the same first shared[g] tokens as its group's
+    others, in the same pages or in copies of them. (Sequences with fewer
+    tokens share nothing.) A prompt's samples are one group; answers to one
+    system prompt another."""
+    op = "shared_attention"
+    cache_struct = cache._check(op, layer)
+    batch_struct = batch._check(op, cache, (query, shared, mask))
+    if len(shared.shape) != 1 or shared.shape[0] == 0 or batch.sequences % shared.shape[0]:
+        raise TypeError("shared_attention shared must be a u32 tensor of as many values as there are groups of equal size")
+    view, groups = _rank_two(op, "query", query), shared.shape[0]
+    out = _output(op, out, cache.session, cache.dtype, query.shape)
+    status = _native.load().affon_rocm_shared_attention(
+        cache.session._handle, cache_struct, batch_struct,
+        _native.AttentionDesc(view, _NO_MASK if mask is None else _rank_two(op, "mask", mask),
+                              cache.head_dim ** -0.5 if scale is None else scale, layer, out.data_ptr, _space(out)),
+        _words(op, "shared", shared, groups), groups)
+    _attention_status(status, op, cache, batch, query, mask)
     return out
 
 
-def cache_commit(cache: PagedCache, batch: DraftBatch, path: Tensor, accepted: Tensor) -> None:
+def token_weights(cache: PagedCache, batch: DraftBatch) -> Tensor:
+    """Gathered weights of tokens that have gathered none: f32 zeros [layers, B,
+    kv_heads, columns * page_size]. A row of them belongs to a row of the page table."""
+    batch._check("token_weights", cache, ())
+    return cache.session.tensor(np.zeros(_weights_shape(cache, batch), np.float32), "f32")
+
+
+def _weights_shape(cache: PagedCache, batch: DraftBatch) -> tuple[int, ...]:
+    return cache.layers, batch.sequences, cache.kv_heads, batch.page_table.shape[1] * cache.page_size
+
+
+def _weights(op: str, name: str, t: Tensor, cache: PagedCache, batch: DraftBatch) -> int:
+    shape = _weights_shape(cache, batch)
+    if not isinstance(t, Tensor) or t.dtype != "f32" or t.shape != shape or not t.is_contiguous():
+        raise TypeError(f"{op} {name} must be a contiguous f32 {list(shape)} tensor")
+    return t.data_ptr
+
+
+def attention_weights(cache: PagedCache, batch: DraftBatch, query: Tensor, weights: Tensor, mask: Tensor | None = None, *,
+                      layer: int = 0, scale: float | None = None) -> None:
+    """Adds the attention that the drafted tokens' rows in use give every token of
+    their sequence, summed over the rows and the heads of each key head, to
+    ``weights`` (``token_weights``) of the layer: to those of committed tokens
+    it is added, those of drafted ones in use it replaces, as they begin.
+    Operands as ``tree_attention``'s."""
+    op = "attention_weights"
+    cache_struct = cache._check(op, layer)
+    batch_struct = batch._check(op, cache, (query, weights, mask))
+    view = _rank_two(op, "query", query)
+    status = _native.load().affon_rocm_attention_weights(
+        cache.session._handle, cache_struct, batch_struct,
+        _native.WeightsDesc(view, _NO_MASK if mask is None else _rank_two(op, "mask", mask),
+                            cache.head_dim ** -0.5 if scale is None else scale, layer,
+                            _weights(op, "weights", weights, cache, batch), _space(weights)))
+    _attention_status(status, op, cache, batch, query, mask)
+
+
+def cache_evict(cache: PagedCache, batch: DraftBatch, weights: Tensor, keep: Tensor, recent: Tensor, *,
+                out: Tensor | None = None) -> Tensor:
+    """Cuts sequences down to ``keep`` u32 [B] tokens, in every layer and for each
+    key head by itself: the ``recent`` u32 [B] last ones stay, and of those
+    before the ones of the largest ``weights`` (equal ones: the first). They move
+    up in their order, keys and values in their pages, and so do the weights, with zeros
+    behind them: the result, in ``out``, which may be ``weights`` itself. The caller then sets
+    lengths[b] to min(keep[b], lengths[b]). Keys are turned by the positions
+    that they were appended with, so later ones need ``positions`` of their own.
+    No page of a sequence may be another's."""
+    op = "cache_evict"
+    cache_struct = cache._check(op)
+    batch_struct = batch._check(op, cache, (weights, keep, recent))
+    data = _weights(op, "weights", weights, cache, batch)
+    out = _output(op, out, cache.session, "f32", weights.shape)
+    status = _native.load().affon_rocm_cache_evict(
+        cache.session._handle, cache_struct, batch_struct, data, out.data_ptr, min(_space(weights), _space(out)),
+        _words(op, "keep", keep, batch.sequences), _words(op, "recent", recent, batch.sequences))
+    if status:
+        _refused(status, op, lambda: None)
+    return out
+
+
+def cache_commit(cache: PagedCache, batch: DraftBatch, path: Tensor, accepted: Tensor, *,
+                 weights: Tensor | None = None) -> None:
     """Keeps the accepted tokens of the draft, in every layer: drafted token
     i < accepted[b] of sequence b becomes what drafted token path[b, i] was.
     ``path`` u32 [B, n], n <= rows, ascends strictly along its accepted part;
-    ``accepted`` u32 [B]. The caller then adds accepted[b] to lengths[b]."""
+    ``accepted`` u32 [B]. ``weights``: gathered weights (``token_weights``) that
+    follow their tokens, with zeros for the drafted ones that are not kept. The
+    caller then adds accepted[b] to lengths[b]."""
     op = "cache_commit"
     cache_struct = cache._check(op)
-    batch_struct = batch._check(op, cache, (path, accepted))
-    status = _native.load().affon_rocm_cache_commit(cache.session._handle, cache_struct, batch_struct,
-                                                    _rank_two(op, "path", path),
-                                                    _words(op, "accepted", accepted, batch.sequences))
+    batch_struct = batch._check(op, cache, (path, accepted, weights))
+    view, count = _rank_two(op, "path", path), _words(op, "accepted", accepted, batch.sequences)
+    native, status = _native.load(), 0
+    if weights is not None:
+        status = native.affon_rocm_weights_commit(cache.session._handle, cache_struct, batch_struct, view, count,
+                                                  _weights(op, "weights", weights, cache, batch), _space(weights))
+    if not status:
+        status = native.affon_rocm_cache_commit(cache.session._handle, cache_struct, batch_struct, view, count)
     if status:
         def explain():
             _matrix(op, "path", path, ("u32",), (batch.sequences, None))

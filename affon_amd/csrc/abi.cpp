@@ -986,9 +986,9 @@ int check_batch(const affon_rocm_draft_batch* b, const affon::PagedCache& cache,
   return AFFON_ROCM_OK;
 }
 
-// The queries of a batch: [B*T, heads*head_dim], heads a multiple of kv_heads; and an output of their shape.
+// The queries of a batch: [B*T, heads*head_dim], heads a multiple of kv_heads; and (`has_output`) an output of their shape.
 int check_query(const affon_rocm_view& q, const affon::PagedCache& cache, const affon::DraftBatch& batch,
-                const void* output, size_t output_bytes, const char* op, int* heads) {
+                const void* output, size_t output_bytes, const char* op, int* heads, bool has_output = true) {
   const int64_t rows = static_cast<int64_t>(batch.sequences) * batch.rows;
   const int64_t unit = static_cast<int64_t>(cache.kv_heads) * cache.head_dim;
   if (q.shape[1] <= 0 || q.shape[1] % unit != 0 || q.shape[1] / cache.head_dim > 65535)
@@ -997,10 +997,11 @@ int check_query(const affon_rocm_view& q, const affon::PagedCache& cache, const 
   if (status != AFFON_ROCM_OK) return status;
   uint64_t count = 0;
   if (!extent({rows, q.shape[1]}, &count)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s query size overflows", op);
+  *heads = static_cast<int>(q.shape[1] / cache.head_dim);
+  if (!has_output) return AFFON_ROCM_OK;
   if (output == nullptr || output_bytes < count * static_cast<uint64_t>(element_size(cache.dtype)) ||
       !aligned(output, element_size(cache.dtype)))
     return fail(AFFON_ROCM_INVALID_SHAPE, "%s output buffer is smaller than the query", op);
-  *heads = static_cast<int>(q.shape[1] / cache.head_dim);
   return AFFON_ROCM_OK;
 }
 
@@ -1012,6 +1013,19 @@ affon::Rows rows_of_view(const affon_rocm_view& v) {
 
 affon::Rows words(const void* data, int64_t count) { return affon::rows_of(data, 1, count * 4, 0); }
 
+// Whether `out` shares memory with the cache, the batch or one of `others`.
+bool meets(const affon::Rows& out, const affon_rocm_kv_cache& cache, const affon_rocm_draft_batch& batch,
+           const affon::DraftBatch& b, std::initializer_list<affon::Rows> others) {
+  const int64_t cache_bytes = cache.layers * cache.pages * cache.kv_heads * cache.page_size * cache.head_dim *
+                              element_size(cache.dtype);
+  for (const auto& held : {affon::rows_of(cache.keys, 1, cache_bytes, 0), affon::rows_of(cache.values, 1, cache_bytes, 0),
+                           rows_of_view(batch.page_table), words(b.lengths, b.sequences), words(b.counts, b.sequences)})
+    if (affon::rows_meet(held, out)) return true;
+  for (const auto& other : others)
+    if (affon::rows_meet(other, out)) return true;
+  return false;
+}
+
 // The output of the queries' shape: it may be the query itself, as whoever
 // writes a value there has read it before, and otherwise overlaps nothing.
 int check_output(const void* output, const affon_rocm_view& query, const affon_rocm_kv_cache& cache,
@@ -1020,25 +1034,15 @@ int check_output(const void* output, const affon_rocm_view& query, const affon_r
   const int64_t bytes = query.shape[1] * element_size(cache.dtype);
   const affon::Rows out = affon::rows_of(output, query.shape[0], bytes, bytes);
   const affon::Rows q = rows_of_view(query);
-  bool clear = !affon::rows_meet(q, out) || affon::same_rows(q, out);
-  const int64_t cache_bytes = cache.layers * cache.pages * cache.kv_heads * cache.page_size * cache.head_dim *
-                              element_size(cache.dtype);
-  for (const auto& held : {affon::rows_of(cache.keys, 1, cache_bytes, 0), affon::rows_of(cache.values, 1, cache_bytes, 0),
-                           rows_of_view(batch.page_table), words(b.lengths, b.sequences), words(b.counts, b.sequences)})
-    clear = clear && !affon::rows_meet(held, out);
-  for (const auto& other : others) clear = clear && !affon::rows_meet(other, out);
+  const bool clear = (!affon::rows_meet(q, out) || affon::same_rows(q, out)) && !meets(out, cache, batch, b, others);
   if (!clear) return fail(AFFON_ROCM_INVALID_SHAPE, "%s output overlaps an operand that it is not", op);
   return AFFON_ROCM_OK;
 }
 
-}  // namespace
-
-int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
-                            const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* d) {
-  clear_error();
-  const char* op = "cache_append";
-  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
-  affon::AppendProblem p{};
+// An append's operands, but for what its output overlaps.
+int check_append(const affon_rocm_kv_cache* cache, const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* d,
+                 const char* op, affon::AppendProblem* out) {
+  affon::AppendProblem& p = *out;
   if (d->layer < 0) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
   int status = check_cache(cache, d->layer, op, &p.cache);
   if (status != AFFON_ROCM_OK || (status = check_batch(batch, p.cache, op, &p.batch)) != AFFON_ROCM_OK) return status;
@@ -1068,6 +1072,71 @@ int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cac
   p.rotary_dim = static_cast<int>(d->rotary_dim);
   p.interleaved = d->interleaved != 0;
   p.out = static_cast<uint8_t*>(d->output);
+  return AFFON_ROCM_OK;
+}
+
+// An attention's operands but for its output: query, mask, scale and layer.
+int check_attention(const affon_rocm_kv_cache* cache, const affon_rocm_draft_batch* batch, const affon_rocm_view& query,
+                    const affon_rocm_view& mask, float scale, int64_t layer, const void* output, size_t output_bytes,
+                    const char* op, affon::AttentionProblem* out, bool has_output = true) {
+  affon::AttentionProblem& p = *out;
+  if (layer < 0) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
+  int status = check_cache(cache, layer, op, &p.cache);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, p.cache, op, &p.batch)) != AFFON_ROCM_OK) return status;
+  if (query.dtype != p.cache.dtype)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires query and cache of one type", op);
+  if ((status = check_query(query, p.cache, p.batch, output, output_bytes, op, &p.heads, has_output)) != AFFON_ROCM_OK)
+    return status;
+  if (mask.data != nullptr) {
+    if (mask.dtype != AFFON_ROCM_U32 || mask.shape[1] < (p.batch.rows + 31) / 32)
+      return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 mask with a bit for every row of a sequence", op);
+    if ((status = check_matrix(mask, query.shape[0], mask.shape[1], "mask", op)) != AFFON_ROCM_OK) return status;
+    p.mask = reinterpret_cast<const uint32_t*>(origin(mask));
+    p.mask_stride = mask.stride[0];
+  }
+  if (!(scale - scale == 0.0f)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s scale must be finite", op);
+  p.query = origin(query);
+  p.query_stride = query.stride[0];
+  p.scale = scale;
+  return AFFON_ROCM_OK;
+}
+
+// Gathered weights f32 [layers, B, kv_heads, columns * page_size].
+int check_weights(const affon_rocm_kv_cache& cache, const affon::DraftBatch& b, const void* weights, size_t bytes,
+                  const char* op, affon::Rows* out) {
+  uint64_t count = 0;
+  if (!extent({cache.layers, b.sequences, cache.kv_heads, static_cast<int64_t>(b.capacity)}, &count))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s weights' size overflows", op);
+  if (weights == nullptr || !aligned(weights, 4) || bytes < count * 4)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires f32 weights [layers, sequences, kv_heads, columns * page_size]", op);
+  *out = affon::rows_of(weights, 1, static_cast<int64_t>(count) * 4, 0);
+  return AFFON_ROCM_OK;
+}
+
+// A commit's operands: the cache's every layer, and the accepted tokens' path.
+int check_commit(const affon_rocm_kv_cache* cache, const affon_rocm_draft_batch* batch, const affon_rocm_view* path,
+                 const uint32_t* accepted, const char* op, affon::PagedCache* c, affon::DraftBatch* b) {
+  int status = check_cache(cache, -1, op, c);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, *c, op, b)) != AFFON_ROCM_OK) return status;
+  if (path == nullptr || path->dtype != AFFON_ROCM_U32 || path->shape[1] > b->rows)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 path of at most the batch's rows", op);
+  if ((status = check_matrix(*path, b->sequences, path->shape[1], "path", op)) != AFFON_ROCM_OK) return status;
+  if (accepted == nullptr || !aligned(accepted, 4))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 counts of accepted tokens", op);
+  return AFFON_ROCM_OK;
+}
+
+}  // namespace
+
+int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                            const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* d) {
+  clear_error();
+  const char* op = "cache_append";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AppendProblem p{};
+  int status = check_append(cache, batch, d, op, &p);
+  if (status != AFFON_ROCM_OK) return status;
+  const int64_t rows = d->query.shape[0];
   if ((status = check_session(session)) != AFFON_ROCM_OK ||
       (status = check_output(d->output, d->query, *cache, *batch, p.batch, op,
                              {rows_of_view(d->key), rows_of_view(d->value), words(d->positions, rows),
@@ -1078,30 +1147,57 @@ int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cac
   return AFFON_ROCM_OK;
 }
 
+int affon_rocm_cache_append_normed(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                   const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* d,
+                                   const affon_rocm_head_norm* norm) {
+  clear_error();
+  const char* op = "cache_append";
+  if (d == nullptr || norm == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AppendNormProblem q{};
+  int status = check_append(cache, batch, d, op, &q.base);
+  if (status != AFFON_ROCM_OK) return status;
+  const affon::AppendProblem& p = q.base;
+  const int64_t rows = d->query.shape[0], D = p.cache.head_dim;
+  affon::Rows weights[2];
+  for (int k = 0; k < 2; ++k) {
+    affon::HeadNorm& n = k == 0 ? q.query_norm : q.key_norm;
+    n.weight = static_cast<const uint8_t*>(k == 0 ? norm->query_weight : norm->key_weight);
+    n.stride = k == 0 ? norm->query_weight_stride : norm->key_weight_stride;
+    n.dtype = k == 0 ? norm->query_weight_dtype : norm->key_weight_dtype;
+    weights[k] = words(nullptr, 0);
+    if (n.weight == nullptr) continue;
+    if (!is_float_dtype(n.dtype) || (n.stride != 0 && n.stride != D) || !aligned(n.weight, element_size(n.dtype)))
+      return fail(AFFON_ROCM_INVALID_SHAPE, "%s norm weights must be f32 or bf16, of one head or of each", op);
+    const int64_t heads = n.stride == 0 ? 1 : k == 0 ? p.heads : p.cache.kv_heads;
+    weights[k] = affon::rows_of(n.weight, 1, heads * D * element_size(n.dtype), 0);
+  }
+  q.epsilon = norm->epsilon;
+  if (!(q.epsilon > 0.0f) || q.epsilon == std::numeric_limits<float>::infinity())
+    return fail(AFFON_ROCM_INVALID_SHAPE, "invalid cache_append options: epsilon must be finite and positive");
+  q.axes = norm->axes;
+  if (q.axes < 1 || q.axes > 4) return fail(AFFON_ROCM_INVALID_SHAPE, "%s takes positions of one to four axes", op);
+  for (int j = 0; j < p.rotary_dim / 2; ++j) {
+    if (norm->axis[j] >= q.axes) return fail(AFFON_ROCM_INVALID_SHAPE, "%s pair has an axis that the positions have not", op);
+    q.axis[j / 16] |= static_cast<uint32_t>(norm->axis[j]) << 2 * (j % 16);
+  }
+  if ((status = check_session(session)) != AFFON_ROCM_OK ||
+      (status = check_output(d->output, d->query, *cache, *batch, p.batch, op,
+                             {rows_of_view(d->key), rows_of_view(d->value), words(d->positions, q.axes * rows),
+                              words(d->rotary, d->rotary_rows * d->rotary_dim), weights[0], weights[1]})) != AFFON_ROCM_OK)
+    return status;
+  const hipError_t e = affon::append_norm_launch(q, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
 int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                               const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* d) {
   clear_error();
   const char* op = "tree_attention";
   if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
   affon::AttentionProblem p{};
-  if (d->layer < 0) return fail(AFFON_ROCM_INVALID_SHAPE, "%s layer is out of range", op);
-  int status = check_cache(cache, d->layer, op, &p.cache);
-  if (status != AFFON_ROCM_OK || (status = check_batch(batch, p.cache, op, &p.batch)) != AFFON_ROCM_OK) return status;
-  if (d->query.dtype != p.cache.dtype)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires query and cache of one type", op);
-  if ((status = check_query(d->query, p.cache, p.batch, d->output, d->output_bytes, op, &p.heads)) != AFFON_ROCM_OK)
-    return status;
-  if (d->mask.data != nullptr) {
-    if (d->mask.dtype != AFFON_ROCM_U32 || d->mask.shape[1] < (p.batch.rows + 31) / 32)
-      return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 mask with a bit for every row of a sequence", op);
-    if ((status = check_matrix(d->mask, d->query.shape[0], d->mask.shape[1], "mask", op)) != AFFON_ROCM_OK) return status;
-    p.mask = reinterpret_cast<const uint32_t*>(origin(d->mask));
-    p.mask_stride = d->mask.stride[0];
-  }
-  if (!(d->scale - d->scale == 0.0f)) return fail(AFFON_ROCM_INVALID_SHAPE, "%s scale must be finite", op);
-  p.query = origin(d->query);
-  p.query_stride = d->query.stride[0];
-  p.scale = d->scale;
+  int status = check_attention(cache, batch, d->query, d->mask, d->scale, d->layer, d->output, d->output_bytes, op, &p);
+  if (status != AFFON_ROCM_OK) return status;
   p.out = static_cast<uint8_t*>(d->output);
   if ((status = check_session(session)) != AFFON_ROCM_OK ||
       (status = check_output(d->output, d->query, *cache, *batch, p.batch, op, {rows_of_view(d->mask)})) != AFFON_ROCM_OK)
@@ -1114,6 +1210,80 @@ int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_c
   return AFFON_ROCM_OK;
 }
 
+int affon_rocm_shared_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* d,
+                                const uint32_t* shared, int64_t groups) {
+  clear_error();
+  const char* op = "shared_attention";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AttentionProblem p{};
+  int status = check_attention(cache, batch, d->query, d->mask, d->scale, d->layer, d->output, d->output_bytes, op, &p);
+  if (status != AFFON_ROCM_OK) return status;
+  p.out = static_cast<uint8_t*>(d->output);
+  if (shared == nullptr || !aligned(shared, 4) || groups <= 0 || p.batch.sequences % groups != 0)
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 numbers of shared tokens, of groups of equal size", op);
+  if ((status = check_session(session)) != AFFON_ROCM_OK ||
+      (status = check_output(d->output, d->query, *cache, *batch, p.batch, op,
+                             {rows_of_view(d->mask), words(shared, groups)})) != AFFON_ROCM_OK)
+    return status;
+  affon::Launch launch;
+  launch.stream = session->stream;
+  launch.workspace = session->workspace;
+  const hipError_t e = affon::shared_attention_launch(p, shared, static_cast<int>(groups), launch);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_attention_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                 const affon_rocm_draft_batch* batch, const affon_rocm_weights_desc* d) {
+  clear_error();
+  const char* op = "attention_weights";
+  if (d == nullptr) return fail(AFFON_ROCM_INVALID_SHAPE, "%s descriptor is null", op);
+  affon::AttentionProblem p{};
+  int status = check_attention(cache, batch, d->query, d->mask, d->scale, d->layer, nullptr, 0, op, &p, false);
+  if (status != AFFON_ROCM_OK) return status;
+  affon::Rows weights;
+  if ((status = check_weights(*cache, p.batch, d->weights, d->weights_bytes, op, &weights)) != AFFON_ROCM_OK ||
+      (status = check_session(session)) != AFFON_ROCM_OK)
+    return status;
+  if (meets(weights, *cache, *batch, p.batch, {rows_of_view(d->query), rows_of_view(d->mask)}))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s weights overlap an operand", op);
+  float* layer = d->weights + d->layer * p.batch.sequences * p.cache.kv_heads * static_cast<int64_t>(p.batch.capacity);
+  affon::Launch launch;
+  launch.stream = session->stream;
+  launch.workspace = session->workspace;
+  const hipError_t e = affon::attention_weights_launch(p, layer, launch);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_cache_evict(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                           const affon_rocm_draft_batch* batch, const float* weights, float* out, size_t bytes,
+                           const uint32_t* keep, const uint32_t* recent) {
+  clear_error();
+  const char* op = "cache_evict";
+  affon::PagedCache c{};
+  affon::DraftBatch b{};
+  int status = check_cache(cache, -1, op, &c);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, c, op, &b)) != AFFON_ROCM_OK) return status;
+  affon::Rows in, to;
+  if ((status = check_weights(*cache, b, weights, bytes, op, &in)) != AFFON_ROCM_OK ||
+      (status = check_weights(*cache, b, out, bytes, op, &to)) != AFFON_ROCM_OK)
+    return status;
+  if (keep == nullptr || recent == nullptr || !aligned(keep, 4) || !aligned(recent, 4))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 numbers of tokens to keep, and of recent ones", op);
+  if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
+  const affon::Rows k = words(keep, b.sequences), r = words(recent, b.sequences);
+  if ((weights != out && affon::rows_meet(in, to)) || meets(to, *cache, *batch, b, {k, r}))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s output overlaps an operand that it is not", op);
+  affon::Launch launch;
+  launch.stream = session->stream;
+  launch.workspace = session->workspace;
+  const hipError_t e = affon::evict_launch(c, b, weights, out, keep, recent, launch);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
 int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                             const affon_rocm_draft_batch* batch, const affon_rocm_view* path,
                             const uint32_t* accepted) {
@@ -1121,16 +1291,33 @@ int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cac
   const char* op = "cache_commit";
   affon::PagedCache c{};
   affon::DraftBatch b{};
-  int status = check_cache(cache, -1, op, &c);
-  if (status != AFFON_ROCM_OK || (status = check_batch(batch, c, op, &b)) != AFFON_ROCM_OK) return status;
-  if (path == nullptr || path->dtype != AFFON_ROCM_U32 || path->shape[1] > b.rows)
-    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires a u32 path of at most the batch's rows", op);
-  if ((status = check_matrix(*path, b.sequences, path->shape[1], "path", op)) != AFFON_ROCM_OK) return status;
-  if (accepted == nullptr || !aligned(accepted, 4))
-    return fail(AFFON_ROCM_INVALID_SHAPE, "%s requires u32 counts of accepted tokens", op);
+  int status = check_commit(cache, batch, path, accepted, op, &c, &b);
+  if (status != AFFON_ROCM_OK) return status;
   if ((status = check_session(session)) != AFFON_ROCM_OK) return status;
   const hipError_t e = affon::commit_launch(c, b, reinterpret_cast<const uint32_t*>(origin(*path)), path->stride[0],
                                             static_cast<int>(path->shape[1]), accepted, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
+int affon_rocm_weights_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                              const affon_rocm_draft_batch* batch, const affon_rocm_view* path,
+                              const uint32_t* accepted, float* weights, size_t weights_bytes) {
+  clear_error();
+  const char* op = "cache_commit";
+  affon::PagedCache c{};
+  affon::DraftBatch b{};
+  int status = check_commit(cache, batch, path, accepted, op, &c, &b);
+  if (status != AFFON_ROCM_OK) return status;
+  affon::Rows to;
+  if ((status = check_weights(*cache, b, weights, weights_bytes, op, &to)) != AFFON_ROCM_OK ||
+      (status = check_session(session)) != AFFON_ROCM_OK)
+    return status;
+  if (meets(to, *cache, *batch, b, {rows_of_view(*path), words(accepted, b.sequences)}))
+    return fail(AFFON_ROCM_INVALID_SHAPE, "%s weights overlap an operand", op);
+  const hipError_t e = affon::commit_weights_launch(b, c.layers, c.kv_heads, weights,
+                                                    reinterpret_cast<const uint32_t*>(origin(*path)), path->stride[0],
+                                                    static_cast<int>(path->shape[1]), accepted, session->stream);
   if (e != hipSuccess) return hip_fail(e, op);
   return AFFON_ROCM_OK;
 }

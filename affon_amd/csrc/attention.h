@@ -73,7 +73,44 @@ struct Args {
   // One per unit and row group, 0 between calls: the workgroup that raises it
   // to the number of splits in use joins their results. Null: a second launch does.
   uint32_t* tickets;
+  // Of a call over shared prefixes (part 1 or 2): `per` sequences to a group,
+  // shared[group] tokens of each in the same pages.
+  const uint32_t* shared;
+  int per;
 };
+
+// Parts of the keys that a launch takes: all of a sequence; the prefixes that
+// the sequences of a group share, whose rows are then the rows of one sequence
+// (p.batch: groups for sequences); or what each has after its prefix.
+enum Part { kAllKeys = 0, kPrefix = 1, kOwnKeys = 2 };
+
+// Tokens of a prefix that are taken once for its group: whole steps of every
+// kernel, so that the own tokens start at one too. The rest is each sequence's own.
+constexpr uint32_t kPrefixUnit = 64;
+__device__ __forceinline__ uint32_t prefix_tokens(const Args& a, const DraftBatch& batch, int group) {
+  return min(a.shared[group], batch.capacity) / kPrefixUnit * kPrefixUnit;
+}
+// Whether sequence b holds the prefix of its group.
+__device__ __forceinline__ bool takes_prefix(const Args& a, const DraftBatch& batch, int b, int group) {
+  return batch.lengths[b] >= a.shared[group] && drafted(batch, b) > 0;
+}
+// The first sequence of a group that does, whose pages are read for all; -1: none. For whole waves.
+__device__ __forceinline__ int prefix_holder(const Args& a, int group) {
+  const int lane = threadIdx.x & 63;
+  DraftBatch batch = a.p.batch;  // of the sequences themselves
+  batch.rows /= a.per;
+  for (int i = 0; i < a.per; i += 64) {
+    const int b = group * a.per + min(i + lane, a.per - 1);
+    const uint64_t held = __ballot(takes_prefix(a, batch, b, group));
+    if (held != 0) return group * a.per + min(i + __builtin_ctzll(held), a.per - 1);
+  }
+  return -1;
+}
+// Keys of a piece where n keys are cut into at most `splits` of them.
+__device__ __forceinline__ uint32_t piece_of(uint32_t n, int splits, uint32_t unit) {
+  const uint32_t each = (n + splits - 1) / splits;
+  return max(unit, (each + unit - 1) / unit * unit);
+}
 
 constexpr float kSlack = 8.0f;
 constexpr float kLowest = -3.0e38f;  // m before the first score
@@ -207,7 +244,7 @@ __device__ __forceinline__ f32x4_t joined_sums(const Args& a, int64_t slot, int 
 // head is 16 * DT wide, 64, 128 or 256, else at most that; RT: 16-row tiles
 // of a wave; WR: waves side by side over the rows, sharing the keys in LDS;
 // WK: waves side by side over the keys, each with its own; STAGES: steps in LDS.
-template <typename T, int DT, bool EXACT, int RT, int WR, int WK, int STAGES>
+template <typename T, int DT, bool EXACT, int RT, int WR, int WK, int STAGES, int PART>
 struct Kernel {
   static constexpr bool kHalf = T::bytes == 2;
   static constexpr int kKT = kHalf ? 2 : 1;  // 16-key tiles of a step
@@ -269,19 +306,38 @@ struct Kernel {
     if (split < 0) return;
 
     // The page list's first part, whose loads need not wait for the lengths.
-    const uint32_t start = static_cast<uint32_t>(split) * a.chunk;
-    const uint32_t early_at = start + threadIdx.x * 16;
+    uint32_t start = static_cast<uint32_t>(split) * a.chunk;
     uint32_t early = kNoPage;
-    if (early_at < p.batch.capacity) early = p.batch.table[b * p.batch.table_stride + early_at / p.cache.page_size];
+    if constexpr (PART == kAllKeys) {
+      const uint32_t early_at = start + threadIdx.x * 16;
+      if (early_at < p.batch.capacity) early = p.batch.table[b * p.batch.table_stride + early_at / p.cache.page_size];
+    }
 
-    const uint32_t length = committed(p.batch, b);
-    const uint32_t count = drafted(p.batch, b);
-    const uint32_t n = min(length + count, p.batch.capacity);
+    uint32_t length, count, n, chunk = a.chunk;
+    int table_row = b;
+    if constexpr (PART == kPrefix) {
+      // All keys are committed, and all rows are done: those of sequences that
+      // do not take the prefix are not read again.
+      length = n = prefix_tokens(a, p.batch, b);
+      count = static_cast<uint32_t>(p.batch.rows);
+      if (n == 0) return;
+      table_row = prefix_holder(a, b);
+      if (table_row < 0) return;
+      chunk = piece_of(n, a.splits, a.chunk);
+      start = static_cast<uint32_t>(split) * chunk;
+    } else {
+      length = committed(p.batch, b);
+      count = drafted(p.batch, b);
+      n = min(length + count, p.batch.capacity);
+      if constexpr (PART == kOwnKeys) {
+        if (takes_prefix(a, p.batch, b, b / a.per)) start += prefix_tokens(a, p.batch, b / a.per);
+      }
+    }
     const uint32_t begin = min(start, n);
-    const uint32_t end = split == a.splits - 1 ? n : min(begin + a.chunk, n);
-    if (begin >= end && split > 0) return;
+    const uint32_t end = split == a.splits - 1 ? n : min(begin + chunk, n);
+    if (begin >= end && (split > 0 || PART == kPrefix)) return;
     const uint32_t used = max(1u, (n + a.chunk - 1) / a.chunk);  // splits that hold keys
-    const bool whole = a.splits == 1 || used == 1;               // the result is this workgroup's
+    const bool whole = PART == kAllKeys && (a.splits == 1 || used == 1);  // the result is this workgroup's
 
     // This wave's rows, as columns of its results.
     const int row0 = (rg * WR + (WR > 1 ? wave : 0)) * RT * 16;
@@ -384,9 +440,9 @@ struct Kernel {
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < kPageList && segment + i * 16 < segment_end; i += kThreads) {
         const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
-        const uint32_t page = segment == begin && i < kThreads
+        const uint32_t page = PART == kAllKeys && segment == begin && i < kThreads
                                   ? (early < static_cast<uint32_t>(p.cache.pages) ? early : kNoPage)
-                                  : page_of(p.cache, p.batch, b, index);
+                                  : page_of(p.cache, p.batch, table_row, index);
         tile_list[i] = page == kNoPage ? 1
                                        : (static_cast<int64_t>(page) * p.cache.kv_heads + kv) * head_bytes +
                                              static_cast<int64_t>(at - index * p.cache.page_size) * row_bytes;
@@ -686,7 +742,7 @@ struct Kernel {
       wait_lds_reads();
     }
 
-    if (end > length && !careful) {  // the drafted tokens are among the keys
+    if (PART != kPrefix && end > length && !careful) {  // the drafted tokens are among the keys
       float odd = 0.0f;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -798,10 +854,15 @@ struct Shape {
 
 void launch_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_prefix_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_prefix_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_own_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_own_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+Shape shape_for(int rows, int head_dim);
 
-template <typename T, int DT, bool EXACT, int RT, int WR>
+template <typename T, int DT, bool EXACT, int RT, int WR, int PART>
 void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
-  using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2>;
+  using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2, PART>;
   // Waves over the keys: as many as leave room in LDS for two workgroups of
   // two steps a wave; f32, which has more to compute in the same bytes, gains
   // by a third wave at widths of 65 to 96 (32 sequences of one token over up to
@@ -810,38 +871,38 @@ void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   constexpr int WK = WR > 1 ? 1 : Probe::kStage <= 8192 ? 4 : Probe::kStage <= 12288 && !Probe::kHalf ? 3 : 2;
   // Two steps in LDS: three took 457 us against 446 for trees of 64 over up to 16384 tokens, four 720.
   constexpr int STAGES = 2;
-  using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES>;
+  using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES, PART>;
   hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
 }
 
-template <typename T, int DT, bool EXACT>
+template <typename T, int DT, bool EXACT, int PART>
 void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
   if constexpr (DT <= 8) {
     if (shape.waves == 1) {
-      if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1>(a, grid, stream);
-      return launch_shape<T, DT, EXACT, 2, 1>(a, grid, stream);
+      if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1, PART>(a, grid, stream);
+      return launch_shape<T, DT, EXACT, 2, 1, PART>(a, grid, stream);
     }
   }
   if constexpr (DT > 8) {
-    if (shape.waves == 2) return launch_shape<T, DT, EXACT, 1, 2>(a, grid, stream);
+    if (shape.waves == 2) return launch_shape<T, DT, EXACT, 1, 2, PART>(a, grid, stream);
   }
-  if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4>(a, grid, stream);
-  if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4>(a, grid, stream);
+  if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4, PART>(a, grid, stream);
+  if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4, PART>(a, grid, stream);
 }
 
-template <typename T>
+template <typename T, int PART>
 void launch_head(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
   const int D = a.p.cache.head_dim;
-  if (D == 64) return launch_width<T, 4, true>(a, shape, grid, stream);
-  if (D == 128) return launch_width<T, 8, true>(a, shape, grid, stream);
-  if (D == 256) return launch_width<T, 16, true>(a, shape, grid, stream);
-  if (D < 64) return launch_width<T, 4, false>(a, shape, grid, stream);
-  if (D <= 96) return launch_width<T, 6, false>(a, shape, grid, stream);
-  if (D < 128) return launch_width<T, 8, false>(a, shape, grid, stream);
+  if (D == 64) return launch_width<T, 4, true, PART>(a, shape, grid, stream);
+  if (D == 128) return launch_width<T, 8, true, PART>(a, shape, grid, stream);
+  if (D == 256) return launch_width<T, 16, true, PART>(a, shape, grid, stream);
+  if (D < 64) return launch_width<T, 4, false, PART>(a, shape, grid, stream);
+  if (D <= 96) return launch_width<T, 6, false, PART>(a, shape, grid, stream);
+  if (D < 128) return launch_width<T, 8, false, PART>(a, shape, grid, stream);
   // Tiles that 256 columns would waste, 32 sequences of one token over up to
   // 4096: width 192 bf16 108 us against 114, f32 322 and 477.
-  if (D <= 192) return launch_width<T, 12, false>(a, shape, grid, stream);
-  launch_width<T, 16, false>(a, shape, grid, stream);
+  if (D <= 192) return launch_width<T, 12, false, PART>(a, shape, grid, stream);
+  launch_width<T, 16, false, PART>(a, shape, grid, stream);
 }
 
 }  // namespace attention

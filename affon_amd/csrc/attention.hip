@@ -62,6 +62,8 @@ __global__ __launch_bounds__(256) void clear_kernel(uint32_t* words, int count) 
   for (int i = blockIdx.x * 256 + threadIdx.x; i < count; i += gridDim.x * 256) words[i] = 0;
 }
 
+}  // namespace
+
 // Few rows: waves side by side over the keys; more: over the rows, and where
 // the keys of two waves do not fit in LDS twice to a CU. There two waves, as
 // the ones past the last row still repeat its work: 32 sequences of one token
@@ -76,7 +78,6 @@ Shape shape_for(int rows, int head_dim) {
   return {2, 4};
 }
 
-}  // namespace
 }  // namespace attention
 
 hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {

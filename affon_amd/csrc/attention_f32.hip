@@ -4,7 +4,7 @@
 namespace affon {
 namespace attention {
 
-void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream) { launch_head<F32>(a, shape, grid, stream); }
+void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream) { launch_head<F32, kAllKeys>(a, shape, grid, stream); }
 
 }  // namespace attention
 }  // namespace affon

@@ -1,0 +1,311 @@
+// Eviction: of each row (layer, sequence, key head) the `recent` last tokens
+// stay, and of the others those of the largest weights, ties to the lowest
+// index; they move up in their order, keys and values in their pages.
+//
+// One launch selects (a workgroup a row: the threshold by its digits, then the
+// tokens that stay as bits, and their weights in place), another moves.
+
+#include <algorithm>
+
+#include "lds_pipeline.h"
+#include "paged.h"
+
+namespace affon {
+namespace {
+
+typedef uint32_t u32x4_t __attribute__((ext_vector_type(4)));
+
+struct EvictArgs {
+  PagedCache cache;
+  DraftBatch batch;
+  const float* weights;  // [layer][sequence][key head][capacity]
+  float* out;
+  const uint32_t* keep;
+  const uint32_t* recent;
+  uint64_t* kept;  // bit n % 64 of word n / 64 of a row: token n stays
+  int words;       // of a row
+};
+
+// Tokens of a sequence, and how many of them stay.
+struct Plan {
+  uint32_t length, left, recent;
+  __device__ __forceinline__ Plan(const EvictArgs& a, int b) {
+    length = committed(a.batch, b);
+    left = min(a.keep[b], length);
+    recent = min(a.recent[b], left);
+  }
+};
+
+// In the order of the weights; 0s are equal, and a NaN is below all.
+__device__ __forceinline__ uint32_t order_of(float w) {
+  if (w != w) return 0u;
+  const uint32_t u = __float_as_uint(w + 0.0f);
+  return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kThreads = 1024, kWaves = kThreads / 64;
+
+__global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
+  __shared__ uint32_t bins[2048];
+  __shared__ uint32_t counts[64];  // of each wave and part of a window
+  __shared__ uint32_t found_bin, found_above;
+  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  const int64_t row = blockIdx.x;
+  const int b = static_cast<int>(row / a.cache.kv_heads % a.batch.sequences);
+  const Plan plan(a, b);
+  const float* w = a.weights + row * a.batch.capacity;
+  float* out = a.out + row * a.batch.capacity;
+  const uint32_t others = plan.length - plan.recent;  // that stay by their weight
+  const uint32_t wanted = plan.left - plan.recent;
+
+  // The `wanted`-th largest of the others, digit by digit from the highest.
+  uint32_t threshold = 0, ties = 0;  // those above stay, and the first `ties` of those equal
+  if (plan.left < plan.length && wanted > 0) {
+    uint32_t left = wanted;
+    const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
+    for (int pass = 0; pass < 3; ++pass) {
+      const int shift = shifts[pass];
+      const uint32_t size = 1u << widths[pass], high = pass == 0 ? 0u : ~0u << shifts[pass - 1];
+      for (uint32_t i = threadIdx.x; i < size; i += kThreads) bins[i] = 0;
+      __syncthreads();
+      for (uint32_t n = threadIdx.x; n < others; n += kThreads) {
+        const uint32_t key = order_of(w[n]);
+        if ((key & high) == threshold) atomicAdd(&bins[key >> shift & (size - 1)], 1u);
+      }
+      __syncthreads();
+      // Sums from the highest bin down: thread i has bins 2i and 2i + 1 of the reversed order.
+      const uint32_t per = size / kThreads;  // 2 or 1
+      uint32_t mine[2] = {0, 0};
+      for (uint32_t j = 0; j < per; ++j) mine[j] = bins[size - 1 - (threadIdx.x * per + j)];
+      uint32_t sum = mine[0] + mine[1];
+#pragma unroll
+      for (int offset = 1; offset < 64; offset <<= 1) {
+        const uint32_t other = __shfl_up(sum, offset);
+        if (lane >= offset) sum += other;
+      }
+      if (lane == 63) counts[wave] = sum;
+      __syncthreads();
+      uint32_t above = sum - mine[0] - mine[1];
+      for (int i = 0; i < wave; ++i) above += counts[i];
+      for (uint32_t j = 0; j < per; ++j) {
+        if (above < left && above + mine[j] >= left) {
+          found_bin = size - 1 - (threadIdx.x * per + j);
+          found_above = above;
+        }
+        above += mine[j];
+      }
+      __syncthreads();
+      threshold |= found_bin << shift;
+      left -= found_above;
+      __syncthreads();
+    }
+    ties = left;
+  }
+
+  // Windows of four parts of 1024 tokens.
+  uint32_t before = 0, ties_before = 0;  // tokens that stay, and equal ones
+  for (uint32_t window = 0; window < plan.length; window += 4 * kThreads) {
+    float v[4];
+    uint32_t equal = 0, stays = 0;
+    uint64_t ballots[4];
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t n = window + j * kThreads + threadIdx.x;
+      v[j] = n < plan.length ? w[n] : 0.0f;
+      const uint32_t key = order_of(v[j]);
+      if (n < others && plan.left < plan.length) {
+        if (wanted > 0 && key > threshold) stays |= 1u << j;
+        if (wanted > 0 && key == threshold) equal |= 1u << j;
+      } else if (n < plan.length) {
+        stays |= 1u << j;
+      }
+      ballots[j] = __ballot(equal >> j & 1);
+      if (lane == 0) counts[j * kWaves + wave] = __popcll(ballots[j]);
+    }
+    __syncthreads();
+    // Sums over the parts and waves before, in the tokens' order.
+    auto scan = [&](uint32_t* total) {
+      uint32_t sum = counts[lane];
+      const uint32_t own = sum;
+#pragma unroll
+      for (int offset = 1; offset < 64; offset <<= 1) {
+        const uint32_t other = __shfl_up(sum, offset);
+        if (lane >= offset) sum += other;
+      }
+      *total = __shfl(sum, 63);
+      return sum - own;
+    };
+    const uint64_t below = (uint64_t(1) << lane) - 1;
+    uint32_t total;
+    uint32_t base = scan(&total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const uint32_t rank = ties_before + __shfl(base, j * kWaves + wave) + __popcll(ballots[j] & below);
+      if ((equal >> j & 1) && rank < ties) stays |= 1u << j;
+    }
+    ties_before += total;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      ballots[j] = __ballot(stays >> j & 1);
+      if (lane == 0) {
+        counts[j * kWaves + wave] = __popcll(ballots[j]);
+        const uint32_t word = window / 64 + j * kWaves + wave;
+        if (word < static_cast<uint32_t>(a.words)) a.kept[row * a.words + word] = ballots[j];
+      }
+    }
+    __syncthreads();
+    base = scan(&total);
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      // Where out is the weights themselves: this window has been read, and no token moves down.
+      const uint32_t to = before + __shfl(base, j * kWaves + wave) + __popcll(ballots[j] & below);
+      if (stays >> j & 1) out[to] = v[j];
+    }
+    before += total;
+    __syncthreads();
+  }
+  for (uint32_t n = plan.left + threadIdx.x; n < a.batch.capacity; n += kThreads) out[n] = 0.0f;
+}
+
+// A workgroup moves up to 128 bytes of every line of a row, keys or values,
+// 256 lines at a time: all of them are read before one is written, and a line
+// is written only after every line of its place or before has been read.
+constexpr int kMoveThreads = 256, kLanes = 8, kDeep = 8, kLines = kMoveThreads / kLanes * kDeep;
+constexpr uint32_t kWindow = 4096;
+
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int parts) {
+  __shared__ uint16_t list[kWindow];  // sources, from the window's first token on
+  __shared__ uint32_t starts[64];
+  __shared__ uint32_t in_window;
+  int64_t id = blockIdx.x;
+  const int part = static_cast<int>(id % parts);
+  id /= parts;
+  const bool is_value = id % 2 != 0;
+  const int64_t row = id / 2;
+  const int kv = static_cast<int>(row % a.cache.kv_heads);
+  const int64_t above = row / a.cache.kv_heads;
+  const int b = static_cast<int>(above % a.batch.sequences);
+  const int64_t layer = above / a.batch.sequences;
+  const Plan plan(a, b);
+  if (plan.left == plan.length) return;
+  const int line_pieces = a.cache.head_dim * (a.cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
+  const int piece = part * kLanes + threadIdx.x % kLanes;
+  const bool works = piece < line_pieces;
+  auto* data = reinterpret_cast<u32x4_t*>((is_value ? a.cache.values : a.cache.keys) + layer * a.cache.layer_bytes);
+  const int64_t head_lines = static_cast<int64_t>(kv) * a.cache.page_size;
+  const uint64_t* kept = a.kept + row * a.words;
+  uint32_t before = 0;  // tokens that stay before the window
+  for (uint32_t window = 0; window < plan.length && before < plan.left; window += kWindow) {
+    // The window's tokens that stay, in their order.
+    const uint32_t word = threadIdx.x / 4;
+    const uint64_t bits = window / 64 + word < static_cast<uint32_t>(a.words) && window + word * 64 < plan.length
+                              ? kept[window / 64 + word] : 0;
+    if (threadIdx.x % 4 == 0) starts[word] = __popcll(bits);
+    __syncthreads();
+    if (threadIdx.x < 64) {
+      uint32_t sum = starts[threadIdx.x];
+      const uint32_t own = sum;
+#pragma unroll
+      for (int offset = 1; offset < 64; offset <<= 1) {
+        const uint32_t other = __shfl_up(sum, offset);
+        if (static_cast<int>(threadIdx.x) >= offset) sum += other;
+      }
+      starts[threadIdx.x] = sum - own;
+      if (threadIdx.x == 63) in_window = sum;
+    }
+    __syncthreads();
+    const uint32_t shift = threadIdx.x % 4 * 16;
+    uint32_t to = starts[word] + __popcll(bits & ((uint64_t(1) << shift) - 1));
+    for (uint32_t i = shift; i < shift + 16; ++i)
+      if (bits >> i & 1) list[to++] = static_cast<uint16_t>(word * 64 + i);
+    __syncthreads();
+    const uint32_t total = in_window;
+    for (uint32_t i0 = 0; i0 < total; i0 += kLines) {
+      u32x4_t v[kDeep];
+      int64_t place[kDeep];
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j) {
+        const uint32_t i = i0 + j * (kMoveThreads / kLanes) + threadIdx.x / kLanes;
+        place[j] = -1;
+        if (!works || i >= total) continue;
+        const uint32_t source = window + list[i], target = before + i;
+        if (source == target) continue;
+        const int64_t from = line_of(a.cache, a.batch, b, source);
+        if (from < 0) continue;
+        const int64_t line = line_of(a.cache, a.batch, b, target);
+        if (line < 0) continue;
+        place[j] = (line + head_lines) * line_pieces + piece;
+        v[j] = data[(from + head_lines) * line_pieces + piece];
+      }
+      pipeline::wait_vmcnt<0>();
+      __syncthreads();
+#pragma unroll
+      for (int j = 0; j < kDeep; ++j)
+        if (place[j] >= 0) data[place[j]] = v[j];
+    }
+    before += total;
+    __syncthreads();  // the list is free
+  }
+}
+
+}  // namespace
+
+hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const float* weights, float* out,
+                        const uint32_t* keep, const uint32_t* recent, const Launch& l) {
+  EvictArgs a{cache, batch, weights, out, keep, recent, nullptr, static_cast<int>((batch.capacity + 63) / 64)};
+  const int64_t rows = static_cast<int64_t>(cache.layers) * batch.sequences * cache.kv_heads;
+  const int line_pieces = cache.head_dim * (cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
+  const int parts = (line_pieces + kLanes - 1) / kLanes;
+  if (rows * 2 * parts > kMaxBlocks / (kThreads / 256)) return hipErrorInvalidValue;
+  a.kept = static_cast<uint64_t*>(l.scratch(static_cast<size_t>(rows) * a.words * sizeof(uint64_t)));
+  if (a.kept == nullptr) return hipErrorOutOfMemory;
+  hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, l.stream, a);
+  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(rows * 2 * parts)), dim3(kMoveThreads), 0, l.stream, a, parts);
+  return hipGetLastError();
+}
+
+namespace {
+
+// The weights of accepted tokens follow them: a thread for each layer,
+// sequence and key head, eight at a time as the path ascends. The other
+// drafted tokens' places have gathered nothing.
+__global__ __launch_bounds__(256) void commit_weights_kernel(DraftBatch batch, int64_t total, int kv_heads, float* weights,
+                                                             const uint32_t* path, int64_t path_stride, int path_columns,
+                                                             const uint32_t* accepted) {
+  constexpr int kMoves = 8;
+  const int64_t row = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
+  if (row >= total) return;
+  const int b = static_cast<int>(row / kv_heads % batch.sequences);
+  const uint32_t length = batch.lengths[b];
+  if (length >= batch.capacity) return;
+  float* w = weights + row * batch.capacity + length;
+  const uint32_t room = min(batch.capacity - length, static_cast<uint32_t>(batch.rows));
+  const uint32_t count = min(min(accepted[b], static_cast<uint32_t>(path_columns)), room);
+  for (uint32_t i0 = 0; i0 < count; i0 += kMoves) {
+    float v[kMoves];
+#pragma unroll
+    for (int j = 0; j < kMoves; ++j) {
+      const uint32_t i = min(i0 + j, count - 1), from = path[b * path_stride + i];
+      v[j] = from < room ? w[from] : w[i];
+    }
+#pragma unroll
+    for (int j = 0; j < kMoves; ++j)
+      if (i0 + j < count) w[i0 + j] = v[j];
+  }
+  for (uint32_t i = count; i < room; ++i) w[i] = 0.0f;
+}
+
+}  // namespace
+
+hipError_t commit_weights_launch(const DraftBatch& batch, int layers, int kv_heads, float* weights, const uint32_t* path,
+                                 int64_t path_stride, int path_columns, const uint32_t* accepted, hipStream_t stream) {
+  const int64_t total = static_cast<int64_t>(layers) * batch.sequences * kv_heads;
+  const int64_t blocks = (total + 255) / 256;
+  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  hipLaunchKernelGGL(commit_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, batch, total,
+                     kv_heads, weights, path, path_stride, path_columns, accepted);
+  return hipGetLastError();
+}
+
+}  // namespace affon

@@ -133,6 +133,22 @@ struct AppendProblem {
 };
 hipError_t append_launch(const AppendProblem& p, hipStream_t stream);
 
+// The same with norms of the query and key heads, and positions of several axes.
+struct HeadNorm {
+  const uint8_t* weight;  // or null: no norm
+  int64_t stride;         // elements from one head's weights to the next's
+  int dtype;
+};
+constexpr int kAxisWords = 8;  // 128 pairs, two bits each
+struct AppendNormProblem {
+  AppendProblem base;  // positions: [axes][rows]
+  HeadNorm query_norm, key_norm;
+  float epsilon;
+  int axes;  // 1 to 4
+  uint32_t axis[kAxisWords];
+};
+hipError_t append_norm_launch(const AppendNormProblem& q, hipStream_t stream);
+
 struct AttentionProblem {
   PagedCache cache;
   DraftBatch batch;
@@ -145,9 +161,17 @@ struct AttentionProblem {
   uint8_t* out;
 };
 hipError_t attention_launch(const AttentionProblem& p, const Launch& l);
+// Over prefixes that the sequences of each of `groups` groups share.
+hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* shared, int groups, const Launch& l);
+// Adds the attention weights to those of the layer, [sequence][key head][capacity]. (p.out is not used.)
+hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, const Launch& l);
 
 hipError_t commit_launch(const PagedCache& cache, const DraftBatch& batch, const uint32_t* path, int64_t path_stride,
                          int path_columns, const uint32_t* accepted, hipStream_t stream);
+hipError_t commit_weights_launch(const DraftBatch& batch, int layers, int kv_heads, float* weights, const uint32_t* path,
+                                 int64_t path_stride, int path_columns, const uint32_t* accepted, hipStream_t stream);
+hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const float* weights, float* out,
+                        const uint32_t* keep, const uint32_t* recent, const Launch& l);
 
 hipError_t residual_norm_launch(const affon_rocm_residual_norm_desc& d, hipStream_t stream);
 

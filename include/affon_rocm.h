@@ -384,6 +384,25 @@ typedef struct {
 int affon_rocm_cache_append(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                             const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* desc);
 
+/* affon_rocm_cache_append of heads that are normed first, and of positions of
+ * several axes (time, height and width of images and video). For each query
+ * head h (and key head, with its weights) and its values x:
+ *   x' = x / sqrt(mean(x^2) + epsilon) * query_weight[h * query_weight_stride + ..]
+ * in f32, of which pair j then turns by position positions[axis[j], row].
+ * Values are not normed. */
+typedef struct {
+  const void* query_weight; /* null: queries are not normed */
+  const void* key_weight;   /* null: keys are not normed */
+  int64_t query_weight_stride, key_weight_stride; /* elements: 0 (one head_dim of weights for all heads) or head_dim */
+  int32_t query_weight_dtype, key_weight_dtype;   /* f32 or bf16 */
+  float epsilon;                                  /* finite and positive */
+  int32_t axes;      /* of the positions, [axes, B*T] (null: lengths[b] + i on every axis): 1 to 4 */
+  uint8_t axis[128]; /* of pair j < rotary_dim / 2: below axes */
+} affon_rocm_head_norm;
+int affon_rocm_cache_append_normed(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                   const affon_rocm_draft_batch* batch, const affon_rocm_append_desc* desc,
+                                   const affon_rocm_head_norm* norm);
+
 /* Attention of drafted tokens over one layer of the cache, which already
  * holds their own keys and values. Row (b, i) sees the lengths[b] tokens
  * before and drafted token j < counts[b] where bit j % 32 of mask[b*T + i,
@@ -405,6 +424,48 @@ typedef struct {
 int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                               const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* desc);
 
+/* affon_rocm_tree_attention where sequences share a prefix, which is read and
+ * multiplied once for all of them. The B sequences are `groups` groups of B /
+ * groups one after the other; sequence b of group g with lengths[b] >=
+ * shared[g] holds the same first shared[g] tokens as the others, in the same
+ * pages or in copies of them. Sequences with fewer tokens share nothing. The
+ * result is tree_attention's, up to the order of its sums. */
+int affon_rocm_shared_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* desc,
+                                const uint32_t* shared /* [groups] device words */, int64_t groups);
+
+/* The attention weights that tokens gather. With p(b, i, h, n) the probability
+ * that row (b, i) and its head h give token n of its sequence, as in
+ * affon_rocm_tree_attention, the sum over the rows in use and the heads of key head k
+ *   s = sum_{i, h} p(b, i, h, n)
+ * is added to weights[layer, b, k, n] for the committed tokens n < lengths[b],
+ * and stored there for the drafted ones in use, which begin. Other weights stay as they are.
+ * Weights: f32 [layers, B, kv_heads, columns * page_size], contiguous: a row
+ * of them belongs to a row of the page table. All in f32. */
+typedef struct {
+  affon_rocm_view query; /* [B*T, heads*head_dim] of the cache's type, unit inner stride */
+  affon_rocm_view mask;  /* as affon_rocm_attention_desc's */
+  float scale;
+  int64_t layer;
+  float* weights; /* of all layers; memory of no operand */
+  size_t weights_bytes;
+} affon_rocm_weights_desc;
+int affon_rocm_attention_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                                 const affon_rocm_draft_batch* batch, const affon_rocm_weights_desc* desc);
+
+/* Evicts tokens, in every layer: of sequence b's lengths[b] tokens min(keep[b],
+ * lengths[b]) stay for each layer and key head by itself: the recent[b] last
+ * ones, and of those before the ones of the largest weights (equal ones: the
+ * first; a NaN is below all). They become tokens 0, 1, .. in their order, keys and values in their
+ * pages; out[layer, b, k, i] is the weight of the i-th of them, and 0 from
+ * there on. The caller then sets lengths[b] = min(keep[b], lengths[b]). Every
+ * token's pages have to be its sequence's own: nothing moves from or to a place that no page holds. */
+int affon_rocm_cache_evict(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                           const affon_rocm_draft_batch* batch, const float* weights /* as affon_rocm_weights_desc's */,
+                           float* out /* of the same shape: the weights themselves, or memory of no operand */,
+                           size_t bytes /* of each */, const uint32_t* keep /* [B] device words */,
+                           const uint32_t* recent /* [B] device words */);
+
 /* Keeps the accepted tokens: in every layer, drafted token i < accepted[b] of
  * sequence b becomes what drafted token path[b, i] was. path[b, :accepted[b]]
  * ascends strictly (a walk down a tree whose tokens follow their parents), which
@@ -413,6 +474,12 @@ int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_c
 int affon_rocm_cache_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                             const affon_rocm_draft_batch* batch, const affon_rocm_view* path /* [B, n] u32 */,
                             const uint32_t* accepted /* [B] device words */);
+
+/* affon_rocm_cache_commit's part for gathered weights: those of accepted tokens
+ * follow them, and the drafted tokens that are not kept have gathered nothing. */
+int affon_rocm_weights_commit(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                              const affon_rocm_draft_batch* batch, const affon_rocm_view* path /* [B, n] u32 */,
+                              const uint32_t* accepted /* [B] device words */, float* weights, size_t weights_bytes);
 
 /* The norms before and after a block, with its gate and residual scale:
  *   u = update, or update / sqrt(mean(update^2) + epsilon) * post_weight (post_norm),
