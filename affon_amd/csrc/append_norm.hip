@@ -4,181 +4,264 @@
 
 #include <algorithm>
 
+#include "lds_pipeline.h"
 #include "paged.h"
 #include "values.h"
 
 namespace affon {
 namespace {
 
+template <int CTRL>
+__device__ __forceinline__ float plus_lane(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), CTRL, 0xf, 0xf, true));
+}
+// The sum over each group of 2^lanes_log lanes, in all of them.
+__device__ __forceinline__ float group_sum(float v, int lanes_log) {
+  if (lanes_log > 0) v = plus_lane<0xB1>(v);   // lane ^ 1
+  if (lanes_log > 1) v = plus_lane<0x4E>(v);   // lane ^ 2
+  if (lanes_log > 2) v = plus_lane<0x141>(v);  // the other four of eight
+  if (lanes_log > 3) v = plus_lane<0x140>(v);  // the other eight of sixteen
+  if (lanes_log > 4) v += __shfl_xor(v, 16);
+  if (lanes_log > 5) v += __shfl_xor(v, 32);
+  return v;
+}
+
+template <typename C, int V>
+__device__ __forceinline__ void store_rounded(uint8_t* base, int64_t at, const float (&v)[V]) {
+  if constexpr (C::bytes == 2 && V == 8) {
+    *reinterpret_cast<u32x4_t*>(base + at * 2) = u32x4_t{pipeline::pack_bf16(v[0], v[1]), pipeline::pack_bf16(v[2], v[3]),
+                                                         pipeline::pack_bf16(v[4], v[5]), pipeline::pack_bf16(v[6], v[7])};
+  } else if constexpr (C::bytes == 2 && V == 4) {
+    *reinterpret_cast<u32x2_t*>(base + at * 2) = u32x2_t{pipeline::pack_bf16(v[0], v[1]), pipeline::pack_bf16(v[2], v[3])};
+  } else {
+    store_values<C, V>(base, at, v);
+  }
+}
+
 // 2^lanes_log lanes hold a head, V pairs of it each (V = 1: two where a wave
-// holds fewer than half the head's values): the first and the second value of the pairs are V consecutive
-// ones each, interleaved pairs 2V consecutive values. A head's lanes meet in
-// its sum of squares without LDS, and lanes past an odd head's end idle.
-template <typename X, typename C, int V>
-__global__ __launch_bounds__(256) void append_norm_kernel(AppendNormProblem q, int lanes_log) {
+// holds fewer than half the head's values): the first and the second value of
+// the pairs are V consecutive ones each, interleaved pairs 2V consecutive
+// values. A head's lanes meet in its sum of squares without LDS, and lanes past
+// an odd head's end idle. `parts` workgroups take the heads of one row, H at a
+// time to a group of lanes: what belongs to the row (its place, positions and
+// pages) is in scalar registers, its cosines and sines are read once.
+template <typename X, typename C, int V, bool INTERLEAVED, int H>
+__global__ __launch_bounds__(512) void append_norm_kernel(AppendNormProblem q, int lanes_log, uint32_t parts) {
   constexpr int kChunks = V == 1 ? 2 : 1;
   const AppendProblem& p = q.base;
-  const int D = p.cache.head_dim, heads = p.heads, kv = p.cache.kv_heads;
-  const uint32_t slots = static_cast<uint32_t>(heads + 2 * kv);  // heads of a row
-  const int lanes = 1 << lanes_log, lane = threadIdx.x & (lanes - 1);
-  const uint32_t per = 256u >> lanes_log;
-  int64_t row = static_cast<int64_t>(blockIdx.x) * per / slots;
-  uint32_t head = static_cast<uint32_t>(static_cast<int64_t>(blockIdx.x) * per - row * slots) + (threadIdx.x >> lanes_log);
-  if (head >= slots) {
-    row += head / slots;
-    head %= slots;
-  }
-  if (row >= static_cast<int64_t>(p.batch.sequences) * p.batch.rows) return;
+  const int D = p.cache.head_dim, half = p.rotary_dim / 2;
+  const uint32_t heads = p.heads, kv = p.cache.kv_heads, slots = heads + 2 * kv;
+  const int64_t row = blockIdx.x / parts, rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   const int b = static_cast<int>(row / p.batch.rows);
   const uint32_t i = static_cast<uint32_t>(row - static_cast<int64_t>(b) * p.batch.rows);
+  const uint32_t groups = blockDim.x >> lanes_log;
+  const uint32_t first_head = (blockIdx.x - static_cast<uint32_t>(row) * parts) * groups + (threadIdx.x >> lanes_log);
+  const uint32_t stride = groups * parts;
+  const int lane = threadIdx.x & ((1 << lanes_log) - 1);
 
-  const int half = p.rotary_dim / 2;
-  const bool is_query = head < static_cast<uint32_t>(heads), is_value = head >= static_cast<uint32_t>(heads + kv);
-  const uint32_t h = is_query ? head : is_value ? head - heads - kv : head - heads;
-  const uint8_t* in = is_query ? p.query + row * p.query_stride * X::bytes
-                      : is_value ? p.value + row * p.value_stride * X::bytes
-                                 : p.key + row * p.key_stride * X::bytes;
-  int first[kChunks], second[kChunks], w[kChunks];
+  // Places in a query or key (its pairs, or the halves of its kept dims), and in a value (its halves).
+  int w[kChunks], first[kChunks], second[kChunks];
   bool there[kChunks], turns[kChunks];
-  float x[kChunks][V], y[kChunks][V];
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    w[c] = (c * lanes + lane) * V;  // pairs before
+    w[c] = ((c << lanes_log) + lane) * V;  // pairs before
     there[c] = w[c] < D / 2;
-    turns[c] = !is_value && w[c] < half;
-    if (is_value) {  // the halves of what is kept
-      first[c] = w[c];
-      second[c] = D / 2 + w[c];
-    } else if (turns[c]) {
-      first[c] = p.interleaved ? 2 * w[c] : w[c];
-      second[c] = p.interleaved ? 2 * w[c] + V : half + w[c];
+    turns[c] = w[c] < half;
+    if (turns[c]) {
+      first[c] = INTERLEAVED ? 2 * w[c] : w[c];
+      second[c] = INTERLEAVED ? 2 * w[c] + V : half + w[c];
     } else {
       first[c] = p.rotary_dim + (w[c] - half);
       second[c] = first[c] + (D / 2 - half);
     }
-#pragma unroll
-    for (int e = 0; e < V; ++e) x[c][e] = y[c][e] = 0.0f;
-    if (there[c]) {
-      load_values<X, V>(in, static_cast<int64_t>(h) * D + first[c], x[c]);
-      load_values<X, V>(in, static_cast<int64_t>(h) * D + second[c], y[c]);
-    }
   }
-  const uint32_t length = p.batch.lengths[b];
-  const bool used = i < drafted(p.batch, b);
-
-  const HeadNorm& norm = is_query ? q.query_norm : q.key_norm;
-  if (!is_value && norm.weight != nullptr) {
-    float wx[kChunks][V], wy[kChunks][V];
-    const int64_t at = static_cast<int64_t>(h) * norm.stride;
+  const uint8_t* in[3] = {p.query + row * p.query_stride * X::bytes, p.key + row * p.key_stride * X::bytes,
+                          p.value + row * p.value_stride * X::bytes};
+  float x[H][kChunks][V], y[H][kChunks][V];
+  auto load = [&](uint32_t head, float (&to_x)[kChunks][V], float (&to_y)[kChunks][V]) {
+    const bool is_query = head < heads, is_value = head >= heads + kv;
+    const uint32_t h = is_query ? head : is_value ? head - heads - kv : head - heads;
+    const uint8_t* from = (is_query ? in[0] : is_value ? in[2] : in[1]) + h * static_cast<uint32_t>(D * X::bytes);
 #pragma unroll
     for (int c = 0; c < kChunks; ++c) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) wx[c][e] = wy[c][e] = 0.0f;
+      for (int e = 0; e < V; ++e) to_x[c][e] = to_y[c][e] = 0.0f;
       if (!there[c]) continue;
-      if (norm.dtype == AFFON_ROCM_BF16) {
-        load_values<BF16, V>(norm.weight, at + first[c], wx[c]);
-        load_values<BF16, V>(norm.weight, at + second[c], wy[c]);
-      } else {
-        load_values<F32, V>(norm.weight, at + first[c], wx[c]);
-        load_values<F32, V>(norm.weight, at + second[c], wy[c]);
-      }
+      load_values<X, V>(from, is_value ? w[c] : first[c], to_x[c]);
+      load_values<X, V>(from, is_value ? D / 2 + w[c] : second[c], to_y[c]);
     }
-    float sum = 0.0f;
+  };
 #pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int e = 0; e < V; ++e) sum = fmaf(x[c][e], x[c][e], fmaf(y[c][e], y[c][e], sum));
-    for (int offset = lanes >> 1; offset > 0; offset >>= 1) sum += __shfl_xor(sum, offset);
-    const float scale = 1.0f / sqrtf(sum / static_cast<float>(D) + q.epsilon);
-#pragma unroll
-    for (int c = 0; c < kChunks; ++c)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[c][e] = x[c][e] * scale * wx[c][e];
-        y[c][e] = y[c][e] * scale * wy[c][e];
-      }
-  }
+  for (int k = 0; k < H; ++k)
+    if (first_head + k * stride < slots) load(first_head + k * stride, x[k], y[k]);
 
-  // Where the head goes.
-  uint8_t* to = p.out;
-  int64_t at = (row * heads + h) * D;
-  if (!is_query) {
-    if (!used || length >= p.batch.capacity) return;
-    const int64_t line = line_of(p.cache, p.batch, b, length + i);
-    if (line < 0) return;
-    to = is_value ? p.cache.values : p.cache.keys;
-    at = (line + static_cast<int64_t>(h) * p.cache.page_size) * D;
-  }
-  const int64_t rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
+  const uint32_t length = p.batch.lengths[b];
+  const bool used = i < drafted(p.batch, b);
+  const int64_t line = used && length < p.batch.capacity ? line_of(p.cache, p.batch, b, length + i) : -1;
+  float cosine[kChunks][V], sine[kChunks][V];
+  uint32_t axes[kChunks];  // two bits a pair, of a table of words in the arguments
 #pragma unroll
   for (int c = 0; c < kChunks; ++c) {
-    if (!there[c]) continue;
-    if (turns[c]) {
-      // The axes that these pairs have, one after the other: mostly one.
-      float cosine[V], sine[V];
+    axes[c] = 0;
+    if (q.axes > 1) {
 #pragma unroll
-      for (int e = 0; e < V; ++e) cosine[e] = sine[e] = 0.0f;
-      uint32_t axes = 0;  // two bits a pair, of a table of words in the arguments
-      if (q.axes > 1) {
+      for (int word = 0; word < kAxisWords; ++word)
+        if (w[c] / 16 == word) axes[c] = q.axis[word];
+      axes[c] >>= 2 * (w[c] % 16);
+    }
 #pragma unroll
-        for (int k = 0; k < kAxisWords; ++k)
-          if (w[c] / 16 == k) axes = q.axis[k];
-        axes >>= 2 * (w[c] % 16);
-      }
-      for (int axis = 0; axis < q.axes; ++axis) {
-        bool any = false;
+    for (int e = 0; e < V; ++e) cosine[c][e] = sine[c][e] = 0.0f;
+  }
+  uint32_t place[4];  // the row's positions
 #pragma unroll
-        for (int e = 0; e < V; ++e) any |= static_cast<int>(axes >> (2 * e) & 3) == axis;
-        if (!any) continue;
-        const uint32_t position = p.positions != nullptr ? p.positions[axis * rows + row] : length + i;
-        if (position >= p.rotary_rows) continue;
-        const auto* table = reinterpret_cast<const uint8_t*>(p.rotary + static_cast<int64_t>(position) * p.rotary_dim);
-        float co[V], si[V];
-        load_values<F32, V>(table, w[c], co);
-        load_values<F32, V>(table, half + w[c], si);
+  for (int axis = 0; axis < 4; ++axis) {
+    place[axis] = length + i;
+    if (p.positions != nullptr && axis < q.axes) place[axis] = p.positions[axis * rows + row];
+  }
+  auto table_at = [&](uint32_t position, int c, float (&co)[V], float (&si)[V]) {
+    if (position >= p.rotary_rows) return;  // zeros
+    const auto* table = reinterpret_cast<const uint8_t*>(p.rotary + static_cast<int64_t>(position) * p.rotary_dim);
+    load_values<F32, V>(table, w[c], co);
+    load_values<F32, V>(table, half + w[c], si);
+  };
 #pragma unroll
-        for (int e = 0; e < V; ++e)
-          if (static_cast<int>(axes >> (2 * e) & 3) == axis) {
-            cosine[e] = co[e];
-            sine[e] = si[e];
-          }
-      }
-      float v[2 * V];
+  for (int c = 0; c < kChunks; ++c) {
+    constexpr uint32_t kPairs = (uint32_t(1) << 2 * V) - 1;
+    const uint32_t axis = axes[c] & 3;
+    if (__all((axes[c] & kPairs) == axis * (0x5555u & kPairs) || !turns[c])) {  // each lane's pairs have one axis
+      const uint32_t position = axis < 2 ? (axis == 0 ? place[0] : place[1]) : (axis == 2 ? place[2] : place[3]);
+      if (turns[c]) table_at(position, c, cosine[c], sine[c]);
+      continue;
+    }
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        v[e] = x[c][e];
-        v[V + e] = y[c][e];
-      }
+    for (int a = 0; a < 4; ++a) {
+      bool any = false;
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        // Interleaved: pair e is the two neighbours 2e, 2e + 1 of the 2V values.
-        const float x1 = p.interleaved ? v[2 * e] : x[c][e], x2 = p.interleaved ? v[2 * e + 1] : y[c][e];
-        const float y1 = x1 * cosine[e] - x2 * sine[e], y2 = x2 * cosine[e] + x1 * sine[e];
-        if (p.interleaved) {
-          v[2 * e] = y1;
-          v[2 * e + 1] = y2;
+      for (int e = 0; e < V; ++e) any |= static_cast<int>(axes[c] >> (2 * e) & 3) == a;
+      if (!any || !turns[c]) continue;
+      float co[V] = {}, si[V] = {};
+      table_at(place[a], c, co, si);
+#pragma unroll
+      for (int e = 0; e < V; ++e)
+        if (static_cast<int>(axes[c] >> (2 * e) & 3) == a) {
+          cosine[c][e] = co[e];
+          sine[c][e] = si[e];
+        }
+    }
+  }
+
+  auto finish = [&](uint32_t head, float (&hx)[kChunks][V], float (&hy)[kChunks][V]) {
+    const bool is_query = head < heads, is_value = head >= heads + kv;
+    const uint32_t h = is_query ? head : is_value ? head - heads - kv : head - heads;
+    const uint8_t* weight = is_query ? q.query_norm.weight : q.key_norm.weight;
+    if (!is_value && weight != nullptr) {
+      const bool half_weight = (is_query ? q.query_norm.dtype : q.key_norm.dtype) == AFFON_ROCM_BF16;
+      const uint32_t at = h * static_cast<uint32_t>(is_query ? q.query_norm.stride : q.key_norm.stride);
+      float wx[kChunks][V], wy[kChunks][V], sum = 0.0f;
+#pragma unroll
+      for (int c = 0; c < kChunks; ++c) {
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          wx[c][e] = wy[c][e] = 0.0f;
+          sum = fmaf(hx[c][e], hx[c][e], fmaf(hy[c][e], hy[c][e], sum));
+        }
+        if (!there[c]) continue;
+        if (half_weight) {
+          load_values<BF16, V>(weight, at + first[c], wx[c]);
+          load_values<BF16, V>(weight, at + second[c], wy[c]);
         } else {
-          v[e] = y1;
-          v[V + e] = y2;
+          load_values<F32, V>(weight, at + first[c], wx[c]);
+          load_values<F32, V>(weight, at + second[c], wy[c]);
         }
       }
+      sum = group_sum(sum, lanes_log);
+      const float scale = 1.0f / sqrtf(sum / static_cast<float>(D) + q.epsilon);
 #pragma unroll
-      for (int e = 0; e < V; ++e) {
-        x[c][e] = v[e];
-        y[c][e] = v[V + e];
+      for (int c = 0; c < kChunks; ++c)
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          hx[c][e] = hx[c][e] * scale * wx[c][e];
+          hy[c][e] = hy[c][e] * scale * wy[c][e];
+        }
+    }
+    if (!is_query && line < 0) return;
+    uint8_t* to = is_query   ? p.out + (row * heads + h) * D * C::bytes
+                  : is_value ? p.cache.values + (line + static_cast<int64_t>(h) * p.cache.page_size) * D * C::bytes
+                             : p.cache.keys + (line + static_cast<int64_t>(h) * p.cache.page_size) * D * C::bytes;
+#pragma unroll
+    for (int c = 0; c < kChunks; ++c) {
+      if (!there[c]) continue;
+      if (is_value) {
+        store_rounded<C, V>(to, w[c], hx[c]);
+        store_rounded<C, V>(to, D / 2 + w[c], hy[c]);
+        continue;
       }
-    }
-    if (is_query && !used) {
+      if (!used) {  // a query: keys have left
 #pragma unroll
-      for (int e = 0; e < V; ++e) x[c][e] = y[c][e] = 0.0f;
+        for (int e = 0; e < V; ++e) hx[c][e] = hy[c][e] = 0.0f;
+      } else if (turns[c]) {
+        float v[2 * V];
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          v[e] = hx[c][e];
+          v[V + e] = hy[c][e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          // Interleaved: pair e is the two neighbours 2e, 2e + 1 of the 2V values.
+          const int one = INTERLEAVED ? 2 * e : e, two = INTERLEAVED ? 2 * e + 1 : V + e;
+          const float x1 = v[one], x2 = v[two];
+          v[one] = x1 * cosine[c][e] - x2 * sine[c][e];
+          v[two] = x2 * cosine[c][e] + x1 * sine[c][e];
+        }
+#pragma unroll
+        for (int e = 0; e < V; ++e) {
+          hx[c][e] = v[e];
+          hy[c][e] = v[V + e];
+        }
+      }
+      store_rounded<C, V>(to, first[c], hx[c]);
+      store_rounded<C, V>(to, second[c], hy[c]);
     }
-    store_values<C, V>(to, at + first[c], x[c]);
-    store_values<C, V>(to, at + second[c], y[c]);
+  };
+  for (uint32_t head = first_head; head < slots; head += H * stride) {
+#pragma unroll
+    for (int k = 0; k < H; ++k) {
+      const uint32_t now = head + k * stride;
+      if (now >= slots) break;
+      finish(now, x[k], y[k]);
+      if (now + H * stride < slots) load(now + H * stride, x[k], y[k]);
+    }
   }
 }
 
 // As the plain append: eight values at a time for many rows.
 constexpr int64_t kManyRows = 64;
+
+template <typename X, typename C, int V, int H>
+hipError_t launch_wide(const AppendNormProblem& q, hipStream_t stream) {
+  const AppendProblem& p = q.base;
+  const int64_t rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
+  int lanes_log = 0;
+  while (lanes_log < 6 && (V << lanes_log) < p.cache.head_dim / 2) ++lanes_log;
+  // Few rows: a head to every group of lanes. Many: a workgroup to a row, of
+  // as few waves as take its heads in the same number of turns: bf16 operands,
+  // where the instructions bound it, in more turns, to set the row up less
+  // often (2738 rows of 48 heads 15.6 us in waves of three heads, 17.3 of two;
+  // f32, 4096 rows of 80 heads, 54.3 us in waves of five heads, 51.2 of two).
+  const int64_t waves = ((static_cast<int64_t>(p.heads + 2 * p.cache.kv_heads) << lanes_log) + 63) / 64;
+  const int64_t most = X::bytes == 2 ? 2 : 5;
+  const int64_t turns = rows < kManyRows ? 1 : (waves + most - 1) / most;
+  const int64_t each = rows < kManyRows ? std::min<int64_t>(waves, 4) : (waves + turns - 1) / turns;
+  const int64_t parts = rows < kManyRows ? (waves + each - 1) / each : 1;
+  if (rows * parts * each > kMaxBlocks * 4) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(rows * parts)), block(static_cast<unsigned>(64 * each));
+  if (p.interleaved)
+    hipLaunchKernelGGL((append_norm_kernel<X, C, V, true, H>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
+  else
+    hipLaunchKernelGGL((append_norm_kernel<X, C, V, false, H>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
+  return hipGetLastError();
+}
 
 template <typename X, typename C>
 hipError_t launch_typed(const AppendNormProblem& q, hipStream_t stream) {
@@ -201,20 +284,9 @@ hipError_t launch_typed(const AppendNormProblem& q, hipStream_t stream) {
            weights_fit(q.query_norm, v) && weights_fit(q.key_norm, v) &&
            reinterpret_cast<uintptr_t>(p.rotary) % 16 == 0 && D % (2 * v) == 0;
   };
-  const int v = fits(8) && rows >= kManyRows ? 8 : fits(4) ? 4 : 1;
-  int lanes_log = 0;
-  while (lanes_log < 6 && (v << lanes_log) < D / 2) ++lanes_log;
-  const int64_t per = 256 >> lanes_log;
-  const int64_t blocks = (rows * (p.heads + 2 * p.cache.kv_heads) + per - 1) / per;
-  if (blocks > kMaxBlocks) return hipErrorInvalidValue;
-  const dim3 grid(static_cast<unsigned>(blocks));
-  if (v == 8)
-    hipLaunchKernelGGL((append_norm_kernel<X, C, 8>), grid, dim3(256), 0, stream, q, lanes_log);
-  else if (v == 4)
-    hipLaunchKernelGGL((append_norm_kernel<X, C, 4>), grid, dim3(256), 0, stream, q, lanes_log);
-  else
-    hipLaunchKernelGGL((append_norm_kernel<X, C, 1>), grid, dim3(256), 0, stream, q, lanes_log);
-  return hipGetLastError();
+  if (fits(8) && rows >= kManyRows) return launch_wide<X, C, 8, 1>(q, stream);
+  if (fits(4)) return launch_wide<X, C, 4, 1>(q, stream);
+  return launch_wide<X, C, 1, 1>(q, stream);
 }
 
 }  // namespace

@@ -168,13 +168,14 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
   for (uint32_t n = plan.left + threadIdx.x; n < a.batch.capacity; n += kThreads) out[n] = 0.0f;
 }
 
-// A workgroup moves up to 128 bytes of every line of a row, keys or values,
-// 256 lines at a time: all of them are read before one is written, and a line
-// is written only after every line of its place or before has been read.
-constexpr int kMoveThreads = 256, kLanes = 8, kDeep = 8, kLines = kMoveThreads / kLanes * kDeep;
+// A workgroup moves 2^lanes_log pieces of 16 bytes of every line of a row, keys or
+// values, as many lines at a time as its threads hold eight pieces of: all of
+// them are read before one is written, and a line is written only after every
+// line of its place or before has been read.
+constexpr int kMoveThreads = 256, kDeep = 8;
 constexpr uint32_t kWindow = 4096;
 
-__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int parts) {
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int parts, int lanes_log) {
   __shared__ uint16_t list[kWindow];  // sources, from the window's first token on
   __shared__ uint32_t starts[64];
   __shared__ uint32_t in_window;
@@ -190,7 +191,8 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
   const Plan plan(a, b);
   if (plan.left == plan.length) return;
   const int line_pieces = a.cache.head_dim * (a.cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
-  const int piece = part * kLanes + threadIdx.x % kLanes;
+  const int piece = (part << lanes_log) + (threadIdx.x & ((1 << lanes_log) - 1));
+  const uint32_t lines = kMoveThreads >> lanes_log, line_of_thread = threadIdx.x >> lanes_log;
   const bool works = piece < line_pieces;
   auto* data = reinterpret_cast<u32x4_t*>((is_value ? a.cache.values : a.cache.keys) + layer * a.cache.layer_bytes);
   const int64_t head_lines = static_cast<int64_t>(kv) * a.cache.page_size;
@@ -221,12 +223,12 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
       if (bits >> i & 1) list[to++] = static_cast<uint16_t>(word * 64 + i);
     __syncthreads();
     const uint32_t total = in_window;
-    for (uint32_t i0 = 0; i0 < total; i0 += kLines) {
+    for (uint32_t i0 = 0; i0 < total; i0 += lines * kDeep) {
       u32x4_t v[kDeep];
       int64_t place[kDeep];
 #pragma unroll
       for (int j = 0; j < kDeep; ++j) {
-        const uint32_t i = i0 + j * (kMoveThreads / kLanes) + threadIdx.x / kLanes;
+        const uint32_t i = i0 + j * lines + line_of_thread;
         place[j] = -1;
         if (!works || i >= total) continue;
         const uint32_t source = window + list[i], target = before + i;
@@ -256,12 +258,16 @@ hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const 
   EvictArgs a{cache, batch, weights, out, keep, recent, nullptr, static_cast<int>((batch.capacity + 63) / 64)};
   const int64_t rows = static_cast<int64_t>(cache.layers) * batch.sequences * cache.kv_heads;
   const int line_pieces = cache.head_dim * (cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
-  const int parts = (line_pieces + kLanes - 1) / kLanes;
+  // Whole lines, or parts of them side by side until there is work for every CU.
+  int lanes_log = 0;
+  while ((1 << lanes_log) < line_pieces && lanes_log < 6) ++lanes_log;
+  while (lanes_log > 0 && rows * 2 * ((line_pieces + (1 << lanes_log) - 1) >> lanes_log) < 512) --lanes_log;
+  const int parts = (line_pieces + (1 << lanes_log) - 1) >> lanes_log;
   if (rows * 2 * parts > kMaxBlocks / (kThreads / 256)) return hipErrorInvalidValue;
   a.kept = static_cast<uint64_t*>(l.scratch(static_cast<size_t>(rows) * a.words * sizeof(uint64_t)));
   if (a.kept == nullptr) return hipErrorOutOfMemory;
   hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, l.stream, a);
-  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(rows * 2 * parts)), dim3(kMoveThreads), 0, l.stream, a, parts);
+  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(rows * 2 * parts)), dim3(kMoveThreads), 0, l.stream, a, parts, lanes_log);
   return hipGetLastError();
 }
 
