@@ -175,13 +175,18 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
 constexpr int kMoveThreads = 256, kDeep = 8;
 constexpr uint32_t kWindow = 4096;
 
-__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int parts, int lanes_log) {
+__global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int parts, int lanes_log, uint32_t per_page) {
   __shared__ uint16_t list[kWindow];  // sources, from the window's first token on
   __shared__ uint32_t starts[64];
   __shared__ uint32_t in_window;
-  int64_t id = blockIdx.x;
-  const int part = static_cast<int>(id % parts);
-  id /= parts;
+  // Pages of the window's tokens and of their new places: looked up beside the
+  // lines' own loads, they kept every chunk waiting (8 sequences of up to 4096
+  // tokens, 32 layers: 836 us, against 482 without any lookup).
+  __shared__ uint32_t pages[2][kWindow / 16 + 1];
+  // Parts of a line at workgroups as far apart as there are rows: mostly on one
+  // XCD, whose L2 then holds the line for them.
+  const int64_t each = static_cast<int64_t>(gridDim.x) / parts, id = blockIdx.x % each;
+  const int part = static_cast<int>(blockIdx.x / each);
   const bool is_value = id % 2 != 0;
   const int64_t row = id / 2;
   const int kv = static_cast<int>(row % a.cache.kv_heads);
@@ -197,6 +202,13 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
   auto* data = reinterpret_cast<u32x4_t*>((is_value ? a.cache.values : a.cache.keys) + layer * a.cache.layer_bytes);
   const int64_t head_lines = static_cast<int64_t>(kv) * a.cache.page_size;
   const uint64_t* kept = a.kept + row * a.words;
+  const uint32_t size = static_cast<uint32_t>(a.cache.page_size);
+  // Line of the token that lies `at` tokens after the start of the page whose number is list[0]; -1: nowhere.
+  auto line_at = [&](const uint32_t* list, uint32_t at) {
+    const uint32_t index = static_cast<uint32_t>(static_cast<uint64_t>(at / 16) * per_page >> 31), page = list[index];
+    return page < static_cast<uint32_t>(a.cache.pages)
+               ? static_cast<int64_t>(page) * a.cache.kv_heads * size + (at - index * size) : -1;
+  };
   uint32_t before = 0;  // tokens that stay before the window
   for (uint32_t window = 0; window < plan.length && before < plan.left; window += kWindow) {
     // The window's tokens that stay, in their order.
@@ -221,8 +233,14 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
     uint32_t to = starts[word] + __popcll(bits & ((uint64_t(1) << shift) - 1));
     for (uint32_t i = shift; i < shift + 16; ++i)
       if (bits >> i & 1) list[to++] = static_cast<uint16_t>(word * 64 + i);
-    __syncthreads();
     const uint32_t total = in_window;
+    const uint32_t first_page[2] = {window / size, before / size};
+    const uint32_t last_token[2] = {min(window + kWindow, plan.length) - 1, before + (total > 0 ? total - 1 : 0)};
+    for (int k = 0; k < 2; ++k)
+      for (uint32_t j = first_page[k] + threadIdx.x; j <= last_token[k] / size; j += kMoveThreads)
+        pages[k][j - first_page[k]] = a.batch.table[b * a.batch.table_stride + j];
+    __syncthreads();
+    const uint32_t window_phase = window - first_page[0] * size, before_phase = before - first_page[1] * size;
     for (uint32_t i0 = 0; i0 < total; i0 += lines * kDeep) {
       u32x4_t v[kDeep];
       int64_t place[kDeep];
@@ -231,12 +249,9 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
         const uint32_t i = i0 + j * lines + line_of_thread;
         place[j] = -1;
         if (!works || i >= total) continue;
-        const uint32_t source = window + list[i], target = before + i;
-        if (source == target) continue;
-        const int64_t from = line_of(a.cache, a.batch, b, source);
-        if (from < 0) continue;
-        const int64_t line = line_of(a.cache, a.batch, b, target);
-        if (line < 0) continue;
+        if (window + list[i] == before + i) continue;
+        const int64_t from = line_at(pages[0], window_phase + list[i]), line = line_at(pages[1], before_phase + i);
+        if (from < 0 || line < 0) continue;
         place[j] = (line + head_lines) * line_pieces + piece;
         v[j] = data[(from + head_lines) * line_pieces + piece];
       }
@@ -263,11 +278,14 @@ hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const 
   while ((1 << lanes_log) < line_pieces && lanes_log < 6) ++lanes_log;
   while (lanes_log > 0 && rows * 2 * ((line_pieces + (1 << lanes_log) - 1) >> lanes_log) < 512) --lanes_log;
   const int parts = (line_pieces + (1 << lanes_log) - 1) >> lanes_log;
+  // t * per_page >> 31 is t / (page_size / 16), for the t up to 4351 of a window and a page.
+  const uint32_t unit = static_cast<uint32_t>(cache.page_size / 16), per_page = ((uint32_t(1) << 31) + unit - 1) / unit;
   if (rows * 2 * parts > kMaxBlocks / (kThreads / 256)) return hipErrorInvalidValue;
   a.kept = static_cast<uint64_t*>(l.scratch(static_cast<size_t>(rows) * a.words * sizeof(uint64_t)));
   if (a.kept == nullptr) return hipErrorOutOfMemory;
   hipLaunchKernelGGL(select_kernel, dim3(static_cast<unsigned>(rows)), dim3(kThreads), 0, l.stream, a);
-  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(rows * 2 * parts)), dim3(kMoveThreads), 0, l.stream, a, parts, lanes_log);
+  hipLaunchKernelGGL(move_kernel, dim3(static_cast<unsigned>(rows * 2 * parts)), dim3(kMoveThreads), 0, l.stream, a, parts,
+                     lanes_log, per_page);
   return hipGetLastError();
 }
 
