@@ -3,11 +3,13 @@
 // share the key head.
 //
 // A row's probabilities need its largest score and the sum of its exponentials
-// first, so the scores are computed twice: once for these two (stats_kernel,
-// queries in registers, keys walked over), and once for the sums over the rows
-// (gather_kernel, keys in registers, rows walked over). Both products are
-// S^T = K Q^T on the matrix cores: lane % 16 is a row, and a lane's four results
-// are keys 4 (lane / 16) .. + 3 of a tile of 16.
+// first (stats_kernel). For up to 16 rows of a key head the scores are then kept
+// and summed over the rows by sum_kernel: the keys are read once. With more rows
+// the scores would be more to write and read than the keys, and are computed
+// again (gather_kernel). Products are S^T = K Q^T on the matrix cores: lane % 16
+// is a row, and a lane's four results are keys 4 (lane / 16) .. + 3 of a tile of
+// 16. stats_kernel holds queries in registers and walks over the keys,
+// gather_kernel holds keys and walks over the rows.
 
 #include <algorithm>
 #include <cfloat>
@@ -24,23 +26,85 @@ struct WeightArgs {
   int group;         // query heads per key head
   int rows;          // T * group
   int row_groups;    // workgroups of stats_kernel that share a piece's keys
-  uint32_t unit;     // keys of a piece, at least
-  int splits;        // pieces of a context, at most
+  int tiles;         // 16-row tiles of a wave there
+  bool over_rows;    // its waves are side by side over the rows
+  int pieces;        // of all contexts, for each key head: about so many, and one a sequence more at most
+  int gather_pieces; // the same for gather_kernel
   float log2_scale;  // |scale| * log2(e)
   float sign;        // of the scale: a factor of the queries
-  float2* stats;     // (m, l) [unit][split][row]
-  float2* ready;     // (m, 1 / l) [unit][row]; 1 / l = 0: the row takes no part
+  float2* stats;     // (m, l) [piece][row]
+  float* ready;      // m + log2(l) [unit][row]; infinite: the row takes no part
+  u32x4_t* packed;   // the queries as gather_kernel's operands
+  float* scores;     // [unit][row][capacity], or null: computed again
   float* weights;    // of the layer, [sequence][key head][capacity]
-  int blocks;        // workgroups of gather_kernel along a context
+  int blocks;        // workgroups of sum_kernel along a context
 };
 
-// What a sequence holds, and where this workgroup's piece of it lies.
+// What a sequence holds.
 struct Context {
   uint32_t length, count, n;
   __device__ __forceinline__ Context(const AttentionProblem& p, int b) {
     length = committed(p.batch, b);
     count = drafted(p.batch, b);
     n = min(length + count, p.batch.capacity);
+  }
+};
+
+// All contexts, cut into pieces of about the same number of keys by the lengths
+// that are there: workgroups that are numbered through them have equal work,
+// whatever the lengths and the table's width, and one round of them pays for its
+// start (lengths, table, queries: 5 us) once. For whole waves.
+constexpr uint32_t kPieceUnit = 128;
+struct Pieces {
+  const DraftBatch& batch;
+  uint32_t chunk;  // keys of a piece
+  __device__ __forceinline__ uint32_t keys_of(int b) const {
+    const uint32_t count = drafted(batch, b);
+    return count == 0 ? 0u : min(committed(batch, b) + count, batch.capacity);
+  }
+  __device__ __forceinline__ Pieces(const DraftBatch& batch, int pieces) : batch(batch) {
+    uint64_t all = 0;
+    for (int b = threadIdx.x & 63; b < batch.sequences; b += 64) all += keys_of(b);
+#pragma unroll
+    for (int offset = 1; offset < 64; offset <<= 1) all += __shfl_xor(static_cast<unsigned long long>(all), offset);
+    const uint64_t each = min(all / static_cast<uint32_t>(pieces) + 1, static_cast<uint64_t>(batch.capacity));
+    chunk = __builtin_amdgcn_readfirstlane(
+        static_cast<int>((static_cast<uint32_t>(each) + kPieceUnit - 1) / kPieceUnit * kPieceUnit));
+  }
+  // Piece `id` of [sequence][key head][piece of the sequence]; false: there are fewer.
+  __device__ __forceinline__ bool find(int64_t id, int kv_heads, int* b, int* kv, uint32_t* piece) const {
+    const int lane = threadIdx.x & 63;
+    int64_t before = 0;
+    for (int base = 0; base < batch.sequences; base += 64) {
+      const uint32_t own = base + lane < batch.sequences ? (keys_of(base + lane) + chunk - 1) / chunk : 0u;
+      uint32_t sum = own;
+#pragma unroll
+      for (int offset = 1; offset < 64; offset <<= 1) {
+        const uint32_t other = __shfl_up(sum, offset);
+        if (lane >= offset) sum += other;
+      }
+      const uint64_t past = __ballot((before + sum) * kv_heads > id);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        const uint32_t pieces = __builtin_amdgcn_readlane(static_cast<int>(own), at);
+        const int64_t start = before + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), at)) - pieces;
+        const uint32_t rest = static_cast<uint32_t>(id - start * kv_heads);
+        *b = base + at;
+        *kv = static_cast<int>(rest / pieces);
+        *piece = rest - static_cast<uint32_t>(*kv) * pieces;
+        return true;
+      }
+      before += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+    }
+    return false;
+  }
+  // Number of the first piece of a sequence's key head.
+  __device__ __forceinline__ int64_t first_of(int b, int kv, int kv_heads) const {
+    uint64_t before = 0;
+    for (int i = threadIdx.x & 63; i < b; i += 64) before += (keys_of(i) + chunk - 1) / chunk;
+#pragma unroll
+    for (int offset = 1; offset < 64; offset <<= 1) before += __shfl_xor(static_cast<unsigned long long>(before), offset);
+    return static_cast<int64_t>(before) * kv_heads + static_cast<int64_t>(kv) * ((keys_of(b) + chunk - 1) / chunk);
   }
 };
 
@@ -83,29 +147,50 @@ struct Tiles {
     }
   }
 
-  // The 16 keys at `tile` as an operand.
-  static __device__ __forceinline__ void load_keys(const WeightArgs& a, const uint8_t* tile, u32x4_t (&k)[KS]) {
-    const int lane = threadIdx.x & 63, col = lane & 15, quad = lane >> 4;
-    const int row_bytes = a.p.cache.head_dim * T::bytes;
+  // A tile of 16 keys is consecutive in memory and comes by whole lines, a lane
+  // the 16-byte pieces lane, lane + 64, .. (`from`), through a place of the wave's
+  // own in LDS, whose rows are padded against bank conflicts and hold zeros past the head.
+  // (An operand's own lanes would ask for 64 bytes of 16 keys at a time.)
+  static constexpr int kRow = 64 * KS + 16, kPlace = 16 * kRow + 16;  // the last 16 bytes: for pieces past the tile
+  int from[KS], to[KS], at;
+  __device__ __forceinline__ explicit Tiles(const WeightArgs& a) {
+    const int lane = threadIdx.x & 63, row_bytes = a.p.cache.head_dim * T::bytes;
 #pragma unroll
-    for (int s = 0; s < KS; ++s)
-      k[s] = *reinterpret_cast<const u32x4_t*>(tile + col * row_bytes + min(s * 64 + quad * 16, row_bytes - 16));
+    for (int s = 0; s < KS; ++s) {
+      const int byte = s * 1024 + lane * 16, key = byte / row_bytes;
+      from[s] = min(byte, 16 * row_bytes - 16);
+      to[s] = key < 16 ? key * kRow + byte - key * row_bytes : 16 * kRow;
+    }
+    at = (lane & 15) * kRow + (lane >> 4) * 16;
+  }
+  static __device__ __forceinline__ void clear(uint8_t* place, int tiles) {
+    for (int i = threadIdx.x & 63; i < tiles * kPlace / 16; i += 64) reinterpret_cast<u32x4_t*>(place)[i] = u32x4_t{0, 0, 0, 0};
+  }
+  __device__ __forceinline__ void fetch(const uint8_t* tile, u32x4_t (&k)[KS]) const {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k[s] = *reinterpret_cast<const u32x4_t*>(tile + from[s]);
+  }
+  __device__ __forceinline__ void put(uint8_t* place, const u32x4_t (&k)[KS]) const {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) *reinterpret_cast<u32x4_t*>(place + to[s]) = k[s];
+  }
+  // The tile as an operand (a wave's own LDS accesses keep their order).
+  __device__ __forceinline__ void get(const uint8_t* place, u32x4_t (&k)[KS]) const {
+#pragma unroll
+    for (int s = 0; s < KS; ++s) k[s] = *reinterpret_cast<const u32x4_t*>(place + at + s * 64);
   }
 
-  static __device__ __forceinline__ f32x4_t scores(const WeightArgs& a, const u32x4_t (&k)[KS], const u32x4_t (&q)[KS]) {
-    const int quad = (threadIdx.x & 63) >> 4, row_bytes = a.p.cache.head_dim * T::bytes;
+  static __device__ __forceinline__ f32x4_t scores(const u32x4_t (&k)[KS], const u32x4_t (&q)[KS]) {
     f32x4_t s{0, 0, 0, 0};
 #pragma unroll
     for (int i = 0; i < KS; ++i) {
-      // Past the head: zeros, as the queries hold there.
-      const u32x4_t ki = i * 64 + quad * 16 < row_bytes ? k[i] : u32x4_t{0, 0, 0, 0};
       if constexpr (kHalf) {
-        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, ki), __builtin_bit_cast(bf16x8_t, q[i]), s,
+        s = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, k[i]), __builtin_bit_cast(bf16x8_t, q[i]), s,
                                                     0, 0, 0);
       } else {
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const uint32_t ke = ki[e], qe = q[i][e];
+          const uint32_t ke = k[i][e], qe = q[i][e];
           s = __builtin_amdgcn_mfma_f32_16x16x4f32(__uint_as_float(ke), __uint_as_float(qe), s, 0, 0, 0);
         }
       }
@@ -113,13 +198,12 @@ struct Tiles {
     return s;
   }
 
-  // Address of the tile that starts at token `at` of sequence b; *there: it
-  // lies somewhere (else some tile's, to be loaded and not looked at).
-  static __device__ __forceinline__ const uint8_t* tile_of(const WeightArgs& a, int kv, uint32_t page, uint32_t at, bool* there) {
+  // Byte offset in the keys of the tile that starts at token n of sequence b; 1: it lies nowhere.
+  static __device__ __forceinline__ int64_t tile_of(const WeightArgs& a, int b, int kv, uint32_t n) {
     const PagedCache& c = a.p.cache;
-    *there = page < static_cast<uint32_t>(c.pages);
-    const int64_t line = (static_cast<int64_t>(*there ? page : 0) * c.kv_heads + kv) * c.page_size + at % c.page_size;
-    return c.keys + line * c.head_dim * T::bytes;
+    const uint32_t index = n / c.page_size, page = page_of(c, a.p.batch, b, index);
+    if (page == kNoPage) return 1;
+    return ((static_cast<int64_t>(page) * c.kv_heads + kv) * c.page_size + (n - index * c.page_size)) * c.head_dim * T::bytes;
   }
 
   // Bits of the 16 keys from `at` on that row t of the sequence sees.
@@ -129,163 +213,443 @@ struct Tiles {
   }
 };
 
-// Four waves side by side over the keys of a piece, 16 rows each.
-template <typename T, int KS>
+// Four waves side by side over the keys of a piece, RT tiles of 16 rows each; or
+// (ROWS) over the rows, which then fetch a tile of four each for all of them:
+// the L2s answer some 68 requests of 128 bytes a ns, and four row groups that
+// fetch the keys by themselves are bound by that.
+template <typename T, int KS, int RT, bool KEEP, bool ROWS>
 __global__ __launch_bounds__(256) void stats_kernel(WeightArgs a) {
   using Ops = Tiles<T, KS>;
-  constexpr int KT = KS <= 8 ? 2 : 1;  // tiles of a step
+  constexpr int KT = KS <= 4 && RT <= 2 && !ROWS ? 2 : 1;             // tiles of a step
+  constexpr int kAhead = ROWS || KEEP ? 1 : RT > 2 ? 3 : KS <= 8 ? 2 : 1;  // steps on their way from memory
+  constexpr int kOwn = ROWS ? 4 : 1;                                  // waves over the rows
   const AttentionProblem& p = a.p;
-  __shared__ float2 parts[4][16];
+  __shared__ __attribute__((aligned(16))) uint8_t lds[(ROWS ? 8 : 4 * KT) * Ops::kPlace];
+  __shared__ float2 parts[ROWS ? 1 : 4][16 * RT];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  int id = blockIdx.x;
+  // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow each other there.
+  int id = blockIdx.x >> 3;
   const int rg = id % a.row_groups;
-  id /= a.row_groups;
-  const int split = id % a.splits, unit = id / a.splits;
-  const int b = unit / p.cache.kv_heads, kv = unit - b * p.cache.kv_heads;
+  id = id / a.row_groups * 8 + (blockIdx.x & 7);
+  const Pieces pieces(p.batch, a.pieces);
+  const uint32_t chunk = pieces.chunk;
+  int b, kv;
+  uint32_t piece;
+  if (!pieces.find(id, p.cache.kv_heads, &b, &kv, &piece)) return;
+  const int unit = b * p.cache.kv_heads + kv;
   const Context c(p, b);
-  const uint32_t chunk = piece_of(c.n, a.splits, a.unit), begin = split * chunk;
-  if (begin >= c.n) return;
+  const uint32_t begin = piece * chunk;
   const uint32_t end = min(begin + chunk, c.n);
-  const uint32_t sub = ((end - begin + 3) / 4 + 31) / 32 * 32;
-  const uint32_t first = min(begin + wave * sub, end), last = min(first + sub, end);
+  const uint32_t sub = ROWS ? chunk : ((end - begin + 3) / 4 + 31) / 32 * 32;
+  const uint32_t first = min(begin + (ROWS ? 0 : wave * sub), end), last = min(first + sub, end);
 
-  u32x4_t q[KS];
-  Ops::load_rows(a, b, kv, c.count, rg * 16, q);
-  const int t = min(rg * 16 + col, a.rows - 1) / a.group;
-  float m = kLowest, l = 0.0f;
+  const int row0 = (rg * kOwn + (ROWS ? wave : 0)) * 16 * RT;
+  u32x4_t q[RT][KS];
+  int t[RT];
+  float m[RT], l[RT];
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    Ops::load_rows(a, b, kv, c.count, row0 + 16 * rt, q[rt]);
+    t[rt] = min(row0 + 16 * rt + col, a.rows - 1) / a.group;
+    m[rt] = kLowest;
+    l[rt] = 0.0f;
+  }
 
-  uint32_t list = kNoPage;  // of 64 tiles, a lane each
-  u32x4_t keys[2][KT][KS];
-  bool there[2][KT];
-  auto load = [&](uint32_t at, auto place) {
-    constexpr int to = decltype(place)::value;
+  // A step: its pieces come from memory (`raw`) while the step before it is
+  // multiplied and the one before that goes through its exponentials.
+  uint8_t* place = lds + (ROWS ? 0 : wave * KT * Ops::kPlace);
+  const Ops ops(a);
+  Ops::clear(ROWS ? lds + wave * 2 * Ops::kPlace : place, ROWS ? 2 : KT);
+  int64_t list = 1;  // places of 64 tiles, a lane each
+  u32x4_t raw[kAhead][KT][KS];
+  uint32_t raw_there[kAhead];  // bit kt: tile kt lies somewhere
+  auto fetch = [&](uint32_t at, auto spot) {
+    constexpr int into = decltype(spot)::value;
     if ((at - first) % 1024 == 0) {
       const uint32_t mine = at + lane * 16;
-      list = mine < last ? page_of(p.cache, p.batch, b, mine / p.cache.page_size) : kNoPage;
+      list = mine < last ? Ops::tile_of(a, b, kv, mine) : 1;
     }
+    raw_there[into] = 0;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const uint32_t page = __builtin_amdgcn_readlane(static_cast<int>(list), (at - first) / 16 % 64 + kt);
-      Ops::load_keys(a, Ops::tile_of(a, kv, page, at + 16 * kt, &there[to][kt]), keys[to][kt]);
+      const int i = static_cast<int>((at - first) / 16 % 64) + kt;
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(list), i);
+      const uint32_t high = __builtin_amdgcn_readlane(static_cast<int>(list >> 32), i);
+      ops.fetch(p.cache.keys + (static_cast<int64_t>(high) << 32 | (low & ~15u)), raw[into][kt]);
+      raw_there[into] |= low & 1 ? 0u : 1u << kt;
     }
   };
-  auto take = [&](uint32_t at, auto place) {
-    constexpr int from = decltype(place)::value;
-    f32x4_t s[KT];
-    float top = -INFINITY;
+  f32x4_t s[RT][KT];
+  auto multiply = [&](f32x4_t (&into)[RT][KT], const uint8_t* from) {
+    u32x4_t keys[KT][KS];
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt) {
-      s[kt] = Ops::scores(a, keys[from][kt], q);
-      const uint32_t key0 = at + 16 * kt;
-      if (!there[from][kt] || key0 + 16 > c.length) {
-        const uint32_t seen = there[from][kt] ? Ops::seen(a, c, b, t, key0) : 0u;
+    for (int kt = 0; kt < KT; ++kt) ops.get(from + kt * Ops::kPlace, keys[kt]);
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-          if (!(seen >> (4 * quad + i) & 1)) s[kt][i] = -INFINITY;
+    for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt) into[rt][kt] = Ops::scores(keys[kt], q[rt]);
+  };
+  // Scores that a row does not see, the kept ones, and the reference of the exponentials.
+  auto settle = [&](uint32_t at, uint32_t there) {
+    if (there != (1u << KT) - 1 || at + 16 * KT > c.length) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int rt = 0; rt < RT; ++rt) {
+          const uint32_t seen = there >> kt & 1 ? Ops::seen(a, c, b, t[rt], at + 16 * kt) : 0u;
+#pragma unroll
+          for (int i = 0; i < 4; ++i)
+            if (!(seen >> (4 * quad + i) & 1)) s[rt][kt][i] = -INFINITY;
+        }
+    }
+    if constexpr (KEEP) {
+#pragma unroll
+      for (int kt = 0; kt < KT; ++kt)
+        if (row0 + col < a.rows && at + 16 * kt < c.n)
+          *reinterpret_cast<f32x4_t*>(a.scores + (static_cast<int64_t>(unit) * a.rows + row0 + col) * p.batch.capacity + at +
+                                      16 * kt + 4 * quad) = s[0][kt];
+    }
+    float top[RT];
+    bool above = false;
+#pragma unroll
+    for (int rt = 0; rt < RT; ++rt) {
+      top[rt] = fmaxf(fmaxf(s[rt][0][0], s[rt][0][1]), fmaxf(s[rt][0][2], s[rt][0][3]));
+#pragma unroll
+      for (int kt = 1; kt < KT; ++kt)
+        top[rt] = fmaxf(top[rt], fmaxf(fmaxf(s[rt][kt][0], s[rt][kt][1]), fmaxf(s[rt][kt][2], s[rt][kt][3])));
+      top[rt] *= a.log2_scale;
+      above |= top[rt] > m[rt] + kSlack;
+    }
+    if (__any(above)) {
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt) {
+        top[rt] = fmaxf(top[rt], __shfl_xor(top[rt], 16));
+        top[rt] = fmaxf(fmaxf(top[rt], __shfl_xor(top[rt], 32)), m[rt]);
+        l[rt] *= __builtin_amdgcn_exp2f(m[rt] - top[rt]);
+        m[rt] = top[rt];
       }
-#pragma unroll
-      for (int i = 0; i < 4; ++i) top = fmaxf(top, s[kt][i]);
     }
-    top *= a.log2_scale;
-    if (__any(top > m + kSlack)) {
-      top = fmaxf(top, __shfl_xor(top, 16));
-      top = fmaxf(fmaxf(top, __shfl_xor(top, 32)), m);
-      l *= __builtin_amdgcn_exp2f(m - top);
-      m = top;
-    }
+  };
+  auto exponentials = [&] {
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int rt = 0; rt < RT; ++rt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) l += __builtin_amdgcn_exp2f(fmaf(s[kt][i], a.log2_scale, -m));
+      for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l[rt] += __builtin_amdgcn_exp2f(fmaf(s[rt][kt][i], a.log2_scale, -m[rt]));
+  };
+  auto put = [&](auto spot) {
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) ops.put(place + kt * Ops::kPlace, raw[decltype(spot)::value][kt]);
   };
   constexpr uint32_t kStep = 16 * KT;
-  if (first < last) load(first, std::integral_constant<int, 0>{});
-  for (uint32_t at = first; at < last; at += 2 * kStep) {
-    if (at + kStep < last) load(at + kStep, std::integral_constant<int, 1>{});
-    take(at, std::integral_constant<int, 0>{});
-    if (at + kStep >= last) break;
-    if (at + 2 * kStep < last) load(at + 2 * kStep, std::integral_constant<int, 0>{});
-    take(at + kStep, std::integral_constant<int, 1>{});
+  if constexpr (ROWS) {
+    // Four tiles at a time, one of each wave, in one half of the LDS while the other fills.
+    __syncthreads();  // the halves are cleared
+    f32x4_t next[RT][KT];
+    auto fetch_own = [&](uint32_t four) {
+      if ((four - first) % 1024 == 0) {
+        const uint32_t mine = four + lane * 16;
+        list = mine < last ? Ops::tile_of(a, b, kv, mine) : 1;
+      }
+      const int i = static_cast<int>((four - first) / 16 % 64) + wave;
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(list), i);
+      const uint32_t high = __builtin_amdgcn_readlane(static_cast<int>(list >> 32), i);
+      ops.fetch(p.cache.keys + (static_cast<int64_t>(high) << 32 | (low & ~15u)), raw[0][0]);
+      uint32_t there = 0;  // bit i: tile i of the four lies somewhere
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        there |= __builtin_amdgcn_readlane(static_cast<int>(list), (four - first) / 16 % 64 + j) & 1 ? 0u : 1u << j;
+      return there;
+    };
+    uint32_t coming = fetch_own(first), half = 0;
+    for (uint32_t four = first; four < last; four += 64, half ^= 1) {
+      uint8_t* tiles = lds + half * 4 * Ops::kPlace;
+      ops.put(tiles + wave * Ops::kPlace, raw[0][0]);
+      const uint32_t there = coming;
+      coming = fetch_own(four + 64);  // past the last: some page's, and not looked at
+      wait_lds_reads();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      multiply(s, tiles);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        settle(four + 16 * i, four + 16 * i < last ? there >> i & 1 : 0u);
+        if (i < 3) multiply(next, tiles + (i + 1) * Ops::kPlace);
+        exponentials();
+        if (i < 3) {
+#pragma unroll
+          for (int rt = 0; rt < RT; ++rt) s[rt][0] = next[rt][0];
+        }
+      }
+    }
+  } else if (first < last) {
+    using First = std::integral_constant<int, 0>;
+    // Steps past the last one are fetched from some page and multiplied too, and
+    // not looked at: with fetches under conditions, the loads' count is not known,
+    // and every step would wait for all of them.
+    pipeline::Unroll<0, kAhead>::run([&](auto spot) { fetch(first + spot * kStep, spot); });
+    put(First{});
+    uint32_t there = raw_there[0];
+    fetch(first + kAhead * kStep, First{});
+    multiply(s, place);
+    uint32_t at = first;
+    // A step, while the next one, whose pieces are in `spot`, is multiplied; false: it was the last.
+    auto advance = [&](auto spot) {
+      settle(at, there);
+      put(spot);
+      there = raw_there[decltype(spot)::value];
+      fetch(at + (kAhead + 1) * kStep, spot);
+      f32x4_t next[RT][KT];
+      multiply(next, place);
+      exponentials();
+#pragma unroll
+      for (int rt = 0; rt < RT; ++rt)
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[rt][kt] = next[rt][kt];
+      at += kStep;
+      return at < last;
+    };
+    for (;;) {
+      if (!advance(std::integral_constant<int, 1 % kAhead>{})) break;
+      if constexpr (kAhead > 1)
+        if (!advance(std::integral_constant<int, 2 % kAhead>{})) break;
+      if constexpr (kAhead > 2)
+        if (!advance(std::integral_constant<int, 3 % kAhead>{})) break;
+    }
   }
-  l += __shfl_xor(l, 16);
-  l += __shfl_xor(l, 32);
-  if (quad == 0) parts[wave][col] = float2{m, l};
+#pragma unroll
+  for (int rt = 0; rt < RT; ++rt) {
+    l[rt] += __shfl_xor(l[rt], 16);
+    l[rt] += __shfl_xor(l[rt], 32);
+    const int r = row0 + 16 * rt + col;
+    if constexpr (ROWS) {
+      if (quad == 0 && r < a.rows) a.stats[static_cast<int64_t>(id) * a.rows + r] = float2{m[rt], l[rt]};
+    } else {
+      if (quad == 0) parts[wave][16 * rt + col] = float2{m[rt], l[rt]};
+    }
+  }
+  if constexpr (ROWS) return;
   __syncthreads();
-  const int r = rg * 16 + static_cast<int>(threadIdx.x);
-  if (threadIdx.x >= 16 || r >= a.rows) return;
+  const int own = static_cast<int>(threadIdx.x), r = row0 + own;
+  if (own >= 16 * RT || r >= a.rows) return;
   float top = kLowest, sum = 0.0f;
-  for (int w = 0; w < 4; ++w) top = fmaxf(top, parts[w][threadIdx.x].x);
-  for (int w = 0; w < 4; ++w) sum = fmaf(parts[w][threadIdx.x].y, __builtin_amdgcn_exp2f(parts[w][threadIdx.x].x - top), sum);
-  a.stats[(static_cast<int64_t>(unit) * a.splits + split) * a.rows + r] = float2{top, sum};
+  for (int w = 0; w < 4; ++w) top = fmaxf(top, parts[w][own].x);
+  for (int w = 0; w < 4; ++w) sum = fmaf(parts[w][own].y, __builtin_amdgcn_exp2f(parts[w][own].x - top), sum);
+  a.stats[static_cast<int64_t>(id) * a.rows + r] = float2{top, sum};
 }
 
-// Joins the pieces of a row: a thread each.
-__global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t total) {
-  const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x;
-  if (i >= total) return;
-  const int64_t unit = i / a.rows;
-  const int r = static_cast<int>(i - unit * a.rows);
-  const Context c(a.p, static_cast<int>(unit / a.p.cache.kv_heads));
-  const uint32_t used = c.n == 0 ? 0u : (c.n + piece_of(c.n, a.splits, a.unit) - 1) / piece_of(c.n, a.splits, a.unit);
+// What a row's exponents start from, m + log2(l), of its joined pieces.
+__device__ __forceinline__ float ready_of(float m, float l, bool used) {
+  return l == 0.0f || !used ? INFINITY : m + __builtin_amdgcn_logf(l);
+}
+
+// Joins the pieces of a row, a thread each, and lays the queries out as
+// gather_kernel's operands: [unit][tile of 16 rows][piece][lane].
+template <typename T, int KS>
+__global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t packs) {
+  if (blockIdx.x < packs) {
+    const int row_tiles = (a.rows + 15) / 16;
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * 4 + (threadIdx.x >> 6);  // a wave a tile
+    const int64_t unit = i / row_tiles;
+    if (unit >= static_cast<int64_t>(a.p.batch.sequences) * a.p.cache.kv_heads) return;
+    const int tile = static_cast<int>(i - unit * row_tiles), b = static_cast<int>(unit / a.p.cache.kv_heads);
+    u32x4_t q[KS];
+    Tiles<T, KS>::load_rows(a, b, static_cast<int>(unit - static_cast<int64_t>(b) * a.p.cache.kv_heads),
+                            drafted(a.p.batch, b), tile * 16, q);
+#pragma unroll
+    for (int s = 0; s < KS; ++s) a.packed[(i * KS + s) * 64 + (threadIdx.x & 63)] = q[s];
+    return;
+  }
+  const int parts = (a.rows + 255) / 256;
+  const int unit = static_cast<int>((blockIdx.x - packs) / parts);
+  const int r = static_cast<int>(blockIdx.x - packs - static_cast<int64_t>(unit) * parts) * 256 + threadIdx.x;
+  const int b = unit / a.p.cache.kv_heads, kv = unit - b * a.p.cache.kv_heads;
+  const Context c(a.p, b);
+  if (c.n == 0 || c.count == 0) return;
+  const Pieces pieces(a.p.batch, a.pieces);
+  const int64_t first = pieces.first_of(b, kv, a.p.cache.kv_heads);
+  const uint32_t used = (c.n + pieces.chunk - 1) / pieces.chunk;
+  if (r >= a.rows) return;
   float m = kLowest, l = 0.0f;
-  for (uint32_t s = 0; s < used; ++s) {
-    const float2 st = a.stats[(unit * a.splits + s) * a.rows + r];
-    const float top = fmaxf(m, st.x);
-    l = fmaf(st.y, __builtin_amdgcn_exp2f(st.x - top), l * __builtin_amdgcn_exp2f(m - top));
+  constexpr uint32_t kAtOnce = 8;  // pieces whose loads are in flight together
+  for (uint32_t s0 = 0; s0 < used; s0 += kAtOnce) {
+    float2 st[kAtOnce];
+    float top = m;
+#pragma unroll
+    for (uint32_t i = 0; i < kAtOnce; ++i) st[i] = a.stats[(first + min(s0 + i, used - 1)) * a.rows + r];
+#pragma unroll
+    for (uint32_t i = 0; i < kAtOnce; ++i) top = fmaxf(top, st[i].x);
+    l *= __builtin_amdgcn_exp2f(m - top);
+    m = top;
+#pragma unroll
+    for (uint32_t i = 0; i < kAtOnce; ++i)
+      if (s0 + i < used) l = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - m), l);
+  }
+  a.ready[static_cast<int64_t>(unit) * a.rows + r] = ready_of(m, l, r / a.group < static_cast<int>(c.count));
+}
+
+// Sums of up to 16 rows' kept scores: a thread four keys, 16 lanes the pieces of a row.
+__global__ __launch_bounds__(256) void sum_kernel(WeightArgs a) {
+  __shared__ float ready[16];
+  const AttentionProblem& p = a.p;
+  const int unit = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
+  const Context c(p, unit / p.cache.kv_heads);
+  if (c.count == 0 || static_cast<uint32_t>(block) * 1024 >= c.n) return;
+  const Pieces pieces(p.batch, a.pieces);
+  const int64_t first = pieces.first_of(unit / p.cache.kv_heads, unit % p.cache.kv_heads, p.cache.kv_heads);
+  const uint32_t used = (c.n + pieces.chunk - 1) / pieces.chunk;
+  const int r = threadIdx.x / 16;
+  float m = kLowest, l = 0.0f;
+  if (r < a.rows) {
+    for (uint32_t s = threadIdx.x % 16; s < used; s += 16) {
+      const float2 st = a.stats[(first + s) * a.rows + r];
+      const float top = fmaxf(m, st.x);
+      l = fmaf(st.y, __builtin_amdgcn_exp2f(st.x - top), l * __builtin_amdgcn_exp2f(m - top));
+      m = top;
+    }
+  }
+#pragma unroll
+  for (int offset = 1; offset < 16; offset <<= 1) {
+    const float other_m = __shfl_xor(m, offset), other_l = __shfl_xor(l, offset), top = fmaxf(m, other_m);
+    l = l * __builtin_amdgcn_exp2f(m - top) + other_l * __builtin_amdgcn_exp2f(other_m - top);
     m = top;
   }
-  const bool none = l == 0.0f || r / a.group >= static_cast<int>(c.count);
-  a.ready[i] = float2{m, none ? 0.0f : 1.0f / l};
+  if (threadIdx.x % 16 == 0) ready[r] = ready_of(m, l, r < a.rows && r / a.group < static_cast<int>(c.count));
+  __syncthreads();
+  float* weights = a.weights + static_cast<int64_t>(unit) * p.batch.capacity;
+  const float* scores = a.scores + static_cast<int64_t>(unit) * a.rows * p.batch.capacity;
+  const bool aligned = reinterpret_cast<uintptr_t>(a.weights) % 16 == 0;
+  for (uint32_t n = (block * 256 + threadIdx.x) * 4; n < c.n; n += a.blocks * 1024) {
+    f32x4_t before{0, 0, 0, 0}, v{0, 0, 0, 0};
+    const bool whole = aligned && n + 4 <= c.length;
+    if (whole) before = *reinterpret_cast<const f32x4_t*>(weights + n);
+    for (int row = 0; row < a.rows; ++row) {
+      const float from = ready[row];
+      if (from == INFINITY) continue;
+      const f32x4_t s = *reinterpret_cast<const f32x4_t*>(scores + static_cast<int64_t>(row) * p.batch.capacity + n);
+#pragma unroll
+      for (int i = 0; i < 4; ++i) v[i] += __builtin_amdgcn_exp2f(fmaf(s[i], a.log2_scale, -from));
+    }
+    if (whole) {
+      *reinterpret_cast<f32x4_t*>(weights + n) = before + v;
+    } else {
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (n + i < c.n) weights[n + i] = n + i < c.length ? weights[n + i] + v[i] : v[i];
+    }
+  }
 }
 
 // Four waves side by side over the keys, KT tiles each, all rows one after the other.
 template <typename T, int KS>
 __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
   using Ops = Tiles<T, KS>;
-  constexpr int KT = KS <= 4 ? 4 : KS <= 8 ? 2 : 1;
+  constexpr int KT = KS <= 4 ? 2 : 1;
   constexpr uint32_t kKeys = 16 * KT;
+  constexpr int kTiles = KS <= 4 ? 4 : 2;  // of rows that go through LDS at a time
   const AttentionProblem& p = a.p;
+  __shared__ __attribute__((aligned(16))) uint8_t lds[4 * Ops::kPlace];
+  __shared__ __attribute__((aligned(16))) uint8_t queries[2][kTiles * KS * 1024];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
-  const int unit = blockIdx.x / a.blocks, block = blockIdx.x % a.blocks;
-  const int b = unit / p.cache.kv_heads, kv = unit - b * p.cache.kv_heads;
+  const Pieces pieces(p.batch, a.gather_pieces);
+  int b, kv;
+  uint32_t piece;
+  if (!pieces.find(blockIdx.x, p.cache.kv_heads, &b, &kv, &piece)) return;
+  const int unit = b * p.cache.kv_heads + kv;
   const Context c(p, b);
-  if (c.count == 0) return;
-  for (uint32_t at = (block * 4 + wave) * kKeys; at < c.n; at += a.blocks * 4 * kKeys) {
-    u32x4_t keys[KT][KS];
-    bool there[KT], all = at + kKeys <= c.length;
+  // Rows past the last one in use take no part.
+  const int rows = min(a.rows, static_cast<int>(c.count) * a.group);
+  const float* all_ready = a.ready + static_cast<int64_t>(unit) * a.rows;
+  const u32x4_t* packed = a.packed + static_cast<int64_t>(unit) * ((a.rows + 15) / 16) * KS * 64;
+  uint8_t* place = lds + wave * Ops::kPlace;
+  const Ops ops(a);
+  Ops::clear(place, 1);
+  const uint32_t begin = piece * pieces.chunk, end = min(begin + pieces.chunk, c.n);
+  // This wave's keys of the next step, on their way while a step's rows are gone through.
+  u32x4_t raw[KT][KS];
+  uint32_t raw_there = 0;
+  auto fetch = [&](uint32_t at) {  // past the last key: some page's, and not looked at
+    int64_t tile[KT];
+    raw_there = 0;
+#pragma unroll
+    for (int kt = 0; kt < KT; ++kt) tile[kt] = at + 16 * kt < c.n ? Ops::tile_of(a, b, kv, at + 16 * kt) : 1;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      const uint32_t key0 = at + 16 * kt;
-      const uint32_t page = key0 < c.n ? page_of(p.cache, p.batch, b, key0 / p.cache.page_size) : kNoPage;
-      Ops::load_keys(a, Ops::tile_of(a, kv, page, key0, &there[kt]), keys[kt]);
-      all = all && there[kt];
+      raw_there |= (tile[kt] & 1) == 0 ? 1u << kt : 0u;
+      ops.fetch(uniform(p.cache.keys + (tile[kt] & ~int64_t(15))), raw[kt]);
     }
+  };
+  fetch(begin + wave * kKeys);
+  for (uint32_t at4 = begin; at4 < end; at4 += 4 * kKeys) {
+    const uint32_t at = at4 + wave * kKeys, there = raw_there;
+    const bool all = at + kKeys <= c.length && __builtin_amdgcn_readfirstlane(static_cast<int>(there)) == (1 << KT) - 1;
+    u32x4_t keys[KT][KS];
     f32x4_t sums[KT];
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) sums[kt] = f32x4_t{0, 0, 0, 0};
-    for (int r0 = 0; r0 < a.rows; r0 += 16) {
-      const int r = min(r0 + col, a.rows - 1);
-      const float2 ready = a.ready[static_cast<int64_t>(unit) * a.rows + r];
-      const float inverse = r0 + col < a.rows ? ready.y : 0.0f;
-      u32x4_t q[KS];
-      Ops::load_rows(a, b, kv, c.count, r0, q);
-      f32x4_t s[KT];
+    // Tiles of rows through LDS, a group of them ahead.
+    const int groups = (rows + 16 * kTiles - 1) / (16 * kTiles);
+    auto issue = [&](int group) {
+      const u32x4_t* from = packed + static_cast<int64_t>(group) * kTiles * KS * 64;
+      const uint32_t into = __builtin_amdgcn_readfirstlane(static_cast<int>(lds_address(queries[group % 2])));
+      const int pieces = min(kTiles, (rows + 15) / 16 - group * kTiles) * KS;
+      for (int i = wave; i < pieces; i += 4)
+        dma16(uniform(reinterpret_cast<const uint8_t*>(from + i * 64)), lane * 16, into + i * 1024);
+    };
+    auto ready_at = [&](int r0) { return r0 + col < rows ? all_ready[r0 + col] : INFINITY; };
+    float coming[kTiles];
+    auto prepare = [&](int group) {
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) s[kt] = Ops::scores(a, keys[kt], q);
-      const bool edge = !all || __any(inverse == 0.0f);
+      for (int i = 0; i < kTiles; ++i) coming[i] = ready_at((group * kTiles + i) * 16);
+    };
+    __syncthreads();  // the queries before have been read
+    issue(0);
+    prepare(0);
 #pragma unroll
-      for (int kt = 0; kt < KT; ++kt) {
-        const uint32_t seen = !edge ? ~0u : !there[kt] || inverse == 0.0f ? 0u : Ops::seen(a, c, b, r / a.group, at + 16 * kt);
+    for (int kt = 0; kt < KT; ++kt) {
+      ops.put(place, raw[kt]);
+      ops.get(place, keys[kt]);
+    }
+    for (int group = 0; group < groups; ++group) {
+      float ready[kTiles];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const float e = __builtin_amdgcn_exp2f(fmaf(s[kt][i], a.log2_scale, -ready.x)) * inverse;
-          sums[kt][i] += seen >> (4 * quad + i) & 1 ? e : 0.0f;
+      for (int i = 0; i < kTiles; ++i) ready[i] = coming[i];
+      wait_vmcnt<0>();
+      __syncthreads();
+      if (group + 1 < groups) prepare(group + 1);
+      if (group + 1 < groups) issue(group + 1);
+      if (group == 0 && at4 + 4 * kKeys < end) fetch(at + 4 * kKeys);
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        const int r0 = (group * kTiles + i) * 16;
+        if (r0 >= rows) break;
+        u32x4_t q[KS];
+#pragma unroll
+        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(queries[group % 2] + (i * KS + s) * 1024 + lane * 16);
+        f32x4_t s[KT];
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt) s[kt] = Ops::scores(keys[kt], q);
+        if (!all || __any(ready[i] == INFINITY)) {
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) {
+            const uint32_t seen = !(there >> kt & 1) || ready[i] == INFINITY
+                                      ? 0u : Ops::seen(a, c, b, min(r0 + col, a.rows - 1) / a.group, at + 16 * kt);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (!(seen >> (4 * quad + e) & 1)) s[kt][e] = -INFINITY;
+          }
+          if (ready[i] == INFINITY) ready[i] = 0.0f;  // every score is -infinity
         }
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sums[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.log2_scale, -ready[i]));
       }
     }
-    float* to = a.weights + static_cast<int64_t>(unit) * p.batch.capacity;
+    float* weights = a.weights + static_cast<int64_t>(unit) * p.batch.capacity;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt)
 #pragma unroll
@@ -294,19 +658,49 @@ __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
 #pragma unroll
         for (int offset = 1; offset < 16; offset <<= 1) v += __shfl_xor(v, offset);
         const uint32_t n = at + 16 * kt + 4 * quad + i;
-        if (col == i && n < c.n) to[n] = n < c.length ? to[n] + v : v;
+        if (col == i && n < c.n) weights[n] = n < c.length ? weights[n] + v : v;
       }
   }
 }
 
+template <typename T, int KS, int RT>
+void launch_stats(const WeightArgs& a, dim3 grid, hipStream_t stream) {
+  if (a.over_rows)
+    hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, true>), grid, dim3(256), 0, stream, a);
+  else
+    hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, false>), grid, dim3(256), 0, stream, a);
+}
+
+constexpr int64_t kMaxInt = 2147483647;
+constexpr int64_t kKeepRound = 1280, kStatsRound = 512, kGatherRound = 768;
+
+// Tiles of 16 rows that a wave of stats_kernel holds beside its keys, at most.
+constexpr int most_tiles(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 2 : 1; }
+
 template <typename T, int KS>
 hipError_t launch(const WeightArgs& a, int64_t units, hipStream_t stream) {
-  const int64_t stats_blocks = units * a.splits * a.row_groups, total = units * a.rows;
-  if (stats_blocks > kMaxBlocks || (total + 255) / 256 > kMaxBlocks || units * a.blocks > kMaxBlocks)
-    return hipErrorInvalidValue;
-  hipLaunchKernelGGL((stats_kernel<T, KS>), dim3(static_cast<unsigned>(stats_blocks)), dim3(256), 0, stream, a);
-  hipLaunchKernelGGL(ready_kernel, dim3(static_cast<unsigned>((total + 255) / 256)), dim3(256), 0, stream, a, total);
-  hipLaunchKernelGGL((gather_kernel<T, KS>), dim3(static_cast<unsigned>(units * a.blocks)), dim3(256), 0, stream, a);
+  const int64_t kv = a.p.cache.kv_heads, sequences = a.p.batch.sequences;
+  const int64_t stats_blocks = (kv * (a.pieces + sequences) + 7) / 8 * 8 * a.row_groups;
+  const int64_t gather_blocks = kv * (a.gather_pieces + sequences);
+  if (stats_blocks > kMaxBlocks || gather_blocks > kMaxBlocks || units * a.blocks > kMaxBlocks) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(stats_blocks));
+  const dim3 along(static_cast<unsigned>(units * a.blocks));
+  if (a.scores != nullptr) {
+    hipLaunchKernelGGL((stats_kernel<T, KS, 1, true, false>), grid, dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(sum_kernel, along, dim3(256), 0, stream, a);
+    return hipGetLastError();
+  }
+  if (a.tiles == 1) launch_stats<T, KS, 1>(a, grid, stream);
+  if constexpr (most_tiles(KS) >= 2) {
+    if (a.tiles == 2) launch_stats<T, KS, 2>(a, grid, stream);
+  }
+  if constexpr (most_tiles(KS) >= 4) {
+    if (a.tiles == 4) launch_stats<T, KS, 4>(a, grid, stream);
+  }
+  const int64_t packs = (units * ((a.rows + 15) / 16) + 3) / 4, ready_blocks = packs + units * ((a.rows + 255) / 256);
+  if (ready_blocks > kMaxBlocks) return hipErrorInvalidValue;
+  hipLaunchKernelGGL((ready_kernel<T, KS>), dim3(static_cast<unsigned>(ready_blocks)), dim3(256), 0, stream, a, packs);
+  hipLaunchKernelGGL((gather_kernel<T, KS>), dim3(static_cast<unsigned>(gather_blocks)), dim3(256), 0, stream, a);
   return hipGetLastError();
 }
 
@@ -321,22 +715,41 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   const int64_t rows = static_cast<int64_t>(p.batch.rows) * a.group;
   if (rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
-  a.row_groups = (a.rows + 15) / 16;
+  const int pieces = (p.cache.head_dim * (p.cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) + 63) / 64;
+  a.tiles = 1;
+  a.over_rows = a.rows > 16 * most_tiles(pieces);
+  const int side = a.over_rows ? 64 : 16;  // rows of a workgroup for each tile of a wave
+  while (a.tiles < most_tiles(pieces) && side * a.tiles < a.rows) a.tiles *= 2;
+  a.row_groups = (a.rows + side * a.tiles - 1) / (side * a.tiles);
   a.log2_scale = p.scale == 0.0f ? 1.0f : std::min(std::fabs(p.scale) * 1.44269504088896340736f, FLT_MAX);
   a.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
   a.weights = weights;
   const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
   const int64_t capacity = p.batch.capacity;
-  a.unit = 256;
-  a.splits = static_cast<int>(std::max<int64_t>(1, std::min(1024 / (units * a.row_groups), capacity / a.unit)));
-  a.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / units, (capacity + 63) / 64)));
-  const size_t stats = static_cast<size_t>(units) * a.splits * a.rows * sizeof(float2);
-  const size_t ready = static_cast<size_t>(units) * a.rows * sizeof(float2);
-  auto* scratch = static_cast<uint8_t*>(l.scratch(stats + ready));
-  if (scratch == nullptr) return hipErrorOutOfMemory;
+  // One round of workgroups, or two for every key head and sequence.
+  auto pieces_for = [&](int64_t round, int64_t groups) {
+    const int64_t least = p.batch.sequences;
+    return static_cast<int>(std::min<int64_t>(std::max(round / (p.cache.kv_heads * groups) - least, least), kMaxInt / 2));
+  };
+  a.pieces = pieces_for(a.rows <= 16 ? kKeepRound : kStatsRound, a.row_groups);
+  a.gather_pieces = pieces_for(kGatherRound, 1);
+  const size_t stats = (static_cast<size_t>(a.pieces + p.batch.sequences) * p.cache.kv_heads * a.rows * sizeof(float2) + 255) / 256 * 256;
+  // Up to 16 rows' scores are kept, where they find room.
+  constexpr size_t kMostScores = size_t(1) << 30;
+  const size_t scores = static_cast<size_t>(units) * a.rows * capacity * sizeof(float);
+  uint8_t* scratch = nullptr;
+  if (a.rows <= 16 && scores <= kMostScores) scratch = static_cast<uint8_t*>(l.scratch(stats + scores));
+  if (scratch != nullptr) {
+    a.scores = reinterpret_cast<float*>(scratch + stats);
+  } else {
+    const size_t ready = (static_cast<size_t>(units) * a.rows * sizeof(float) + 255) / 256 * 256;
+    scratch = static_cast<uint8_t*>(l.scratch(stats + ready + static_cast<size_t>(units) * ((a.rows + 15) / 16) * 1024 * 16));
+    if (scratch == nullptr) return hipErrorOutOfMemory;
+    a.ready = reinterpret_cast<float*>(scratch + stats);
+    a.packed = reinterpret_cast<u32x4_t*>(scratch + stats + ready);
+  }
   a.stats = reinterpret_cast<float2*>(scratch);
-  a.ready = reinterpret_cast<float2*>(scratch + stats);
-  const int pieces = (p.cache.head_dim * (p.cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) + 63) / 64;
+  a.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / units, (capacity + 1023) / 1024)));
   if (p.cache.dtype == AFFON_ROCM_BF16) {
     if (pieces <= 2) return launch<BF16, 2>(a, units, l.stream);
     if (pieces <= 3) return launch<BF16, 3>(a, units, l.stream);
