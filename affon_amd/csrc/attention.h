@@ -859,6 +859,8 @@ void launch_prefix_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream
 void launch_own_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 void launch_own_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 Shape shape_for(int rows, int head_dim);
+// Heads of 64 or 128 in bf16, workgroups of 4 or 8 waves of 32 rows.
+void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream);
 
 template <typename T, int DT, bool EXACT, int RT, int WR, int PART>
 void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {

@@ -1,0 +1,315 @@
+// A prefix that many rows share, on the matrix cores: bf16, heads of 64 or 128.
+//
+// All its keys are committed and seen by every row, so nothing is masked: a
+// workgroup of W waves holds 32 W rows and walks over a piece of the keys 32 at
+// a time,
+//   S^T = K Q^T,  P = e^(S - m),  O^T += V^T P^T   (32x32x16 products).
+// A query row is the column lane % 32 of both results; a lane's sixteen scores
+// are the keys 8 (i / 4) + 4 (lane / 32) + i % 4 of the 32, and the values are read in that order.
+//
+// What bounds it: per 32 rows and keys the matrix cores have 512 cycles of
+// products, the vector unit about 400 of exponentials, sums and conversions,
+// and LDS 128 per CU and wave. They overlap within a wave: a step's exponentials run
+// between the scores of the step after it and the values' products of the one
+// before it, none of which waits for them.
+#pragma once
+
+#include "attention.h"
+
+namespace affon {
+namespace attention {
+
+typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+// DT: 32-wide tiles of the head; W: waves, 32 rows each; STAGES: steps in LDS.
+template <int DT, int W, int STAGES>
+struct PrefixKernel {
+  using Swizzle = Kernel<BF16, 2 * DT, true, 1, 1, 1, 2, kPrefix>;
+  static constexpr int D = 32 * DT, kRowBytes = 2 * D, kThreads = 64 * W;
+  static constexpr int kTile = 16 * kRowBytes, kPieces = kTile / 1024;  // of 16 keys, or values
+  static constexpr int kStage = 2 * kTile;                              // keys of a step; the values' lie in a ring of their own
+  static constexpr int kValues = STAGES * kStage;
+  static constexpr int kPer = 4 * kPieces / W;                          // transfers of a wave and step, all of one tile
+  static constexpr int kLead = STAGES - 2;                              // steps from a transfer's start to its use, and one
+  static constexpr float kMostSum = 1024.0f;  // of a lane's sixteen probabilities: each is 1 at most where m is the largest score
+  static constexpr int kList = 512;                                     // tiles of a segment
+  static_assert(4 * kPieces % W == 0 && kPieces % kPer == 0 && kLead >= 2 && kLead * kPer < 64, "transfers in flight");
+  static_assert(kValues <= 65536, "places are offsets in the instructions");
+  static constexpr int kGroups = 2 * DT, kExps = 16 / kGroups;  // products of each kind in a step, exponentials beside one of each
+
+  static __device__ void run(const Args& a) {
+    const AttentionProblem& p = a.p;
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kValues];
+    __shared__ int64_t tile_list[kList];  // byte offsets of the segment's tiles that lie somewhere
+    __shared__ int listed[W];
+
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, side = lane >> 5;
+    // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow each other there.
+    int id = blockIdx.x >> 3;
+    const int rg = id % a.row_groups;
+    id = id / a.row_groups * 8 + (blockIdx.x & 7);
+    const int kv = id % p.cache.kv_heads;
+    id /= p.cache.kv_heads;
+    const int group = id % p.batch.sequences, split = id / p.batch.sequences;
+    if (split >= a.splits) return;
+    const uint32_t n = prefix_tokens(a, p.batch, group);
+    if (n == 0) return;
+    const int holder = prefix_holder(a, group);
+    if (holder < 0) return;
+    const uint32_t chunk = piece_of(n, a.splits, a.chunk), begin = split * chunk;
+    if (begin >= n) return;
+    const uint32_t end = min(begin + chunk, n);
+
+    // This wave's rows.
+    const int row0 = (rg * W + wave) * 32;
+    const bool active = row0 < a.rows;
+    u32x4_t q[2 * DT];
+    {
+      const int r = min(row0 + col, a.rows - 1), t = r / a.group;
+      const uint8_t* from = p.query + ((static_cast<int64_t>(group) * p.batch.rows + t) * p.query_stride +
+                                       static_cast<int64_t>(kv * a.group + r - t * a.group) * D) * 2;
+      const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * 2)) % 16 == 0;
+      const uint32_t flip = a.sign < 0.0f ? 0x80008000u : 0u, keep = a.sign == 0.0f ? 0u : ~0u;
+#pragma unroll
+      for (int c = 0; c < 2 * DT; ++c) {
+        const uint8_t* piece = from + c * 32 + side * 16;
+        if (aligned) {
+          q[c] = *reinterpret_cast<const u32x4_t*>(piece);
+        } else {
+          const auto* h = reinterpret_cast<const uint16_t*>(piece);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[c][e] = h[2 * e] | static_cast<uint32_t>(h[2 * e + 1]) << 16;
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[c][e] = (q[c][e] & keep) ^ flip;
+      }
+    }
+
+    // A wave moves pieces of one tile of a step: of the keys' first or second, or the values'.
+    const int which = wave * kPer / kPieces, first_piece = wave * kPer % kPieces;
+    const uint8_t* source = which >= 2 ? p.cache.values : p.cache.keys;
+    // Where this lane's 16 bytes of them come from, and where it reads.
+    uint32_t from[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int at = (first_piece + i) * 1024 + lane * 16, k = at / kRowBytes, c = at % kRowBytes / 16;
+      from[i] = k * kRowBytes + (c ^ (which >= 2 ? Swizzle::value_swizzle(k) : Swizzle::key_swizzle(k))) * 16;
+    }
+    const uint32_t into = __builtin_amdgcn_readfirstlane(
+        static_cast<int>(lds_address(lds) + (which >= 2 ? kValues : 0) + which % 2 * kTile + first_piece * 1024));
+    int key_at[2 * DT], value_at[2][DT];
+    const int key = lane & 15;
+#pragma unroll
+    for (int c = 0; c < 2 * DT; ++c)
+      key_at[c] = pinned((col >> 4) * kTile + key * kRowBytes + ((2 * c + side) ^ Swizzle::key_swizzle(key)) * 16);
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int dt = 0; dt < DT; ++dt) {
+        // Lanes 4e .. 4e + 3 of 16 address key 8 h + 4 side + e; lane j gets column j of the four.
+        const int k = 8 * h + 4 * side + (lane >> 2 & 3);
+        value_at[h][dt] = pinned(kValues + k * kRowBytes +
+                                 ((4 * dt + 2 * (lane >> 4 & 1) + (lane >> 1 & 1)) ^ Swizzle::value_swizzle(k)) * 16 + (lane & 1) * 8);
+      }
+
+    f32x16_t o[DT];
+    float m = kLowest, l = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16_t{};
+
+    for (uint32_t segment = begin; segment < end; segment += kList * 16) {
+      // The tiles that lie somewhere, in their order: others hold no keys.
+      const int wanted = static_cast<int>(min(end - segment, static_cast<uint32_t>(kList * 16)) / 16);
+      int tiles = 0;
+      for (int i0 = 0; i0 < kList && i0 < wanted; i0 += kThreads) {
+        const int i = i0 + static_cast<int>(threadIdx.x);
+        int64_t offset = -1;
+        if (i < wanted) {
+          const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
+          const uint32_t page = page_of(p.cache, p.batch, holder, index);
+          if (page != kNoPage)
+            offset = ((static_cast<int64_t>(page) * p.cache.kv_heads + kv) * p.cache.page_size + (at - index * p.cache.page_size)) *
+                     kRowBytes;
+        }
+        const uint64_t lies = __ballot(offset >= 0);
+        __syncthreads();  // the list, and `listed`, are free
+        if (lane == 0) listed[wave] = __popcll(lies);
+        __syncthreads();
+        int before = tiles;
+        for (int w = 0; w < W; ++w) {
+          if (w < wave) before += listed[w];
+          tiles += listed[w];
+        }
+        if (offset >= 0) tile_list[before + __popcll(lies & ((uint64_t(1) << lane) - 1))] = offset;
+      }
+      __syncthreads();
+      tiles = __builtin_amdgcn_readfirstlane(tiles);
+      if (tiles == 0) continue;
+      const int steps = (tiles + 1) / 2;
+      const bool odd = tiles % 2 != 0;  // the last step's second tile holds no keys
+
+      // Transfers of a step; past the last one the last tile's again, so that their number is known.
+      auto offset_of = [&](int step) { return tile_list[min(2 * step + which % 2, tiles - 1)]; };
+      auto issue = [&](int place, int64_t offset) {
+        const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<int>(offset));
+        const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<int>(offset >> 32));
+        const uint8_t* tile = uniform(source + (static_cast<int64_t>(high) << 32 | low));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) dma16(tile, from[i], into + place * kStage + i * 1024);
+      };
+      auto read_key = [&](int place, int c) { return *reinterpret_cast<const u32x4_t*>(lds + key_at[c] + place * kStage); };
+      // Product g of a step's values: of 16 keys and 32 dims.
+      auto read_value = [&](int place, int g) {
+        u32x2_t half[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const uint32_t address = lds_address(lds + value_at[h][g % DT] + place * kStage + g / DT * kTile);
+          half[h] = __builtin_bit_cast(u32x2_t, __builtin_amdgcn_ds_read_tr16_b64_v4i16(
+                                                    reinterpret_cast<lds_s16x4>(static_cast<uintptr_t>(address))));
+        }
+        return u32x4_t{half[0][0], half[0][1], half[1][0], half[1][1]};
+      };
+      f32x16_t s{};
+      // The largest score of this lane's row, in both its lanes.
+      auto largest = [&] {
+        float top = s[0];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+        top *= a.log2_scale;
+        return fmaxf(top, __shfl_xor(top, 32));
+      };
+      u32x4_t packed[2] = {u32x4_t{0, 0, 0, 0}, u32x4_t{0, 0, 0, 0}};
+#pragma unroll
+      for (int i = 0; i < kLead; ++i) issue(i, offset_of(i));
+      int64_t coming = offset_of(kLead);
+      wait_vmcnt<(kLead - 1) * kPer>();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (odd && steps == 1) clear(lds + kValues + kTile);
+#pragma unroll
+      for (int c = 0; c < 2 * DT; ++c)
+        s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, read_key(0, c)), __builtin_bit_cast(bf16x8_t, q[c]), s,
+                                                    0, 0, 0);
+
+      // A step, in place `place`: its exponentials between the next one's scores
+      // and the last one's values. The values of step -1 are what lies there, times 0: so
+      // FIRST leaves them out, as they may be infinite.
+      auto advance = [&](int step, auto place_of_step, auto first_step) {
+        constexpr int place = decltype(place_of_step)::value, ahead = (place + 1) % STAGES, behind = (place + STAGES - 1) % STAGES;
+        constexpr bool FIRST = decltype(first_step)::value;
+        wait_lds_reads();
+        wait_vmcnt<(kLead - 2) * kPer>();  // step + 1 is there, and the place of step - 2 is free
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        issue((place + kLead) % STAGES, coming);
+        coming = offset_of(step + kLead + 1);
+        if (odd && step + 1 == steps - 1) clear(lds + kValues + ahead * kStage + kTile);
+        if (!active) return;
+        u32x4_t k = read_key(ahead, 0), v{};
+        if constexpr (!FIRST) v = read_value(behind, 0);
+        if (odd && step == steps - 1) {
+          asm volatile("" ::: "memory");  // a branch, not eight selections in every step
+#pragma unroll
+          for (int i = 8; i < 16; ++i) s[i] = -INFINITY;
+        }
+        if constexpr (FIRST) {
+          if (m == kLowest) m = fmaxf(m, largest());  // else the reference of the segment before
+        }
+        float sum = 0.0f;
+        auto probabilities = [&](int i, u32x4_t (&to)[2]) {
+          const float x = __builtin_amdgcn_exp2f(fmaf(s[i], a.log2_scale, -m));
+          const float y = __builtin_amdgcn_exp2f(fmaf(s[i + 1], a.log2_scale, -m));
+          sum += x;
+          sum += y;
+          // As in the other attention kernels, a probability is rounded once
+          // for its product, by 2^-8 at most, and their sum is of the unrounded ones.
+          to[i / 8][i % 8 / 2] = pack_bf16(x, y);
+        };
+        f32x16_t next{};
+        u32x4_t done[2];
+        pipeline::Unroll<0, kGroups>::run([&](auto group_of) {
+          constexpr int g = decltype(group_of)::value;
+          __builtin_amdgcn_sched_barrier(0);
+          u32x4_t next_k = k, next_v = v;
+          if constexpr (g + 1 < kGroups) {
+            next_k = read_key(ahead, g + 1);
+            if constexpr (!FIRST) next_v = read_value(behind, g + 1);
+          }
+          next = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, k), __builtin_bit_cast(bf16x8_t, q[g]), next, 0, 0, 0);
+          if constexpr (!FIRST)
+            o[g % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, v),
+                                                                __builtin_bit_cast(bf16x8_t, packed[g / DT]), o[g % DT], 0, 0, 0);
+#pragma unroll
+          for (int e = 0; e < kExps; e += 2) probabilities(g * kExps + e, done);
+          k = next_k;
+          v = next_v;
+        });
+        __builtin_amdgcn_sched_barrier(0);
+        // A score far past the reference shows in the sum, where no probability
+        // has been multiplied yet: then, and only then, the reference moves.
+        if (__any(sum > kMostSum)) {
+          const float top = fmaxf(m, largest()), keep = __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          l *= keep;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] *= keep;
+          sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; i += 2) probabilities(i, done);
+        }
+        l += sum;
+        s = next;
+        packed[0] = done[0];
+        packed[1] = done[1];
+      };
+      advance(0, std::integral_constant<int, 0>{}, std::true_type{});
+      int last_place = 0;
+      for (int step = 1; step < steps; step += STAGES)
+        pipeline::Unroll<0, STAGES>::run([&](auto i) {
+          constexpr int place = (decltype(i)::value + 1) % STAGES;
+          if (step + i < steps) {
+            advance(step + i, std::integral_constant<int, place>{}, std::false_type{});
+            last_place = place;
+          }
+        });
+      if (active) {
+#pragma unroll
+        for (int g = 0; g < kGroups; ++g)
+          o[g % DT] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8_t, read_value(last_place, g)),
+                                                              __builtin_bit_cast(bf16x8_t, packed[g / DT]), o[g % DT], 0, 0, 0);
+      }
+      wait_lds_reads();
+      wait_vmcnt<0>();  // transfers past the last step end before their places are used again
+    }
+    if (!active) return;
+    l += __shfl_xor(l, 32);
+    const int r = row0 + col;
+    if (r >= a.rows) return;
+    const int64_t slot = ((static_cast<int64_t>(group) * p.cache.kv_heads + kv) * a.splits + split) * a.row_slots + r;
+    float* to = a.sums + slot * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        *reinterpret_cast<f32x4_t*>(to + 32 * dt + 8 * j + 4 * side) =
+            f32x4_t{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    if (side == 0) *reinterpret_cast<float2*>(a.stats + 2 * slot) = float2{m, l};
+  }
+
+  // Zeros for a tile of values that holds no keys; for whole workgroups.
+  static __device__ __forceinline__ void clear(uint8_t* tile) {
+    for (int i = threadIdx.x; i < kTile / 16; i += kThreads) reinterpret_cast<u32x4_t*>(tile)[i] = u32x4_t{0, 0, 0, 0};
+    wait_lds_reads();
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+};
+
+template <typename K>
+__global__ __launch_bounds__(K::kThreads, 2) void prefix_kernel(Args a) {
+  K::run(a);
+}
+
+}  // namespace attention
+}  // namespace affon

@@ -77,6 +77,7 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   if (prefix_rows * (p.heads / p.cache.kv_heads) > (int64_t(1) << 30)) return hipErrorInvalidValue;
   j.prefix.p.batch.rows = static_cast<int>(prefix_rows);
   Shape shapes[2];
+  int tiles = 0;  // waves of the kernel for prefixes of many rows, or 0: the other one
   size_t bytes = 0, sums[2], stats[2];
   for (int part = 0; part < 2; ++part) {
     Args& a = part == 0 ? j.prefix : j.own;
@@ -84,11 +85,17 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
     a.rows = a.p.batch.rows * a.group;
     a.row_slots = a.rows;
     shapes[part] = shape_for(a.rows, p.cache.head_dim);
-    a.row_groups = (a.rows + shapes[part].rows() - 1) / shapes[part].rows();
+    int64_t round = kRound;
+    if (part == 0 && half && (p.cache.head_dim == 64 || p.cache.head_dim == 128) && a.rows > 64) {
+      tiles = a.rows > 128 ? 8 : 4;
+      if (tiles == 8) round /= 2;
+    }
+    const int group_rows = part == 0 && tiles > 0 ? 32 * tiles : shapes[part].rows();
+    a.row_groups = (a.rows + group_rows - 1) / group_rows;
     a.log2_scale = p.scale == 0.0f ? 1.0f : std::min(std::fabs(p.scale) * 1.44269504088896340736f, FLT_MAX);
     a.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
     const int64_t units = static_cast<int64_t>(a.p.batch.sequences) * p.cache.kv_heads;
-    int64_t splits = std::min(kRound / (units * a.row_groups), capacity / unit);
+    int64_t splits = std::min(round / (units * a.row_groups), capacity / unit);
     splits = std::max<int64_t>(splits, 1);
     // The prefix is cut on the device, in pieces of `chunk` at least.
     a.chunk = part == 0 ? static_cast<uint32_t>(unit)
@@ -109,7 +116,9 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
     a.sums = reinterpret_cast<float*>(scratch + sums[part]);
     a.stats = reinterpret_cast<float*>(scratch + stats[part]);
     const dim3 grid(static_cast<unsigned>(blocks_of(a, static_cast<int64_t>(a.p.batch.sequences) * p.cache.kv_heads)));
-    if (part == 0)
+    if (part == 0 && tiles > 0)
+      launch_prefix_tiles(a, tiles, grid, l.stream);
+    else if (part == 0)
       (half ? launch_prefix_bf16 : launch_prefix_f32)(a, shapes[part], grid, l.stream);
     else
       (half ? launch_own_bf16 : launch_own_f32)(a, shapes[part], grid, l.stream);

@@ -139,3 +139,68 @@ def test_it_is_tree_attention(session, rng):
     got = A.shared_attention(step.cache, step.batch, query, shared).storage()
     step.check(got)
     step.check(plain)
+
+
+def copies(rng, B, T, tokens, own, **options):
+    """Sequences whose first `tokens` are the first one's, each with `own` more."""
+    return share(Step(rng, B=B, T=T, lengths=[tokens + n for n in own], spread=2.0, **options), 1, [tokens])
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("B,T,heads,kv,tokens,page", [
+    (17, 1, 8, 2, 64, 16), (18, 2, 4, 2, 128, 16), (5, 9, 2, 1, 1000, 48), (9, 4, 16, 2, 640, 80), (30, 3, 4, 1, 2048, 64),
+    (3, 30, 8, 1, 9000, 256), (33, 1, 2, 1, 17000, 64)])
+def test_many_rows(session, rng, dim, B, T, heads, kv, tokens, page):
+    """From 65 to hundreds of rows over a prefix, of several thousand keys to a workgroup too."""
+    own = [(13 * b) % 31 for b in range(B)]
+    step = copies(rng, B, T, tokens, own, heads=heads, kv=kv, dim=dim, page=page).device(session)
+    for scale in (None, -0.1):
+        step.check(run(session, step, [tokens], scale=scale), scale=scale)
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("missing", [[0], [3, 4], [1, 2, 3], [8], list(range(12)), list(range(1, 12, 2))])
+@pytest.mark.parametrize("page", [16, 48])
+def test_gaps_under_many_rows(session, rng, dim, missing, page):
+    """An odd number of 16-key tiles too, infinities and NaNs in the pages that lie behind."""
+    step = copies(rng, 20, 1, 12 * page, [3 * b for b in range(20)], heads=8, kv=2, dim=dim, page=page)
+    step.table[:, missing] = NO_PAGE
+    step.device(session)
+    step.check(run(session, step, [12 * page]))
+
+
+def test_peaks_that_move(session, rng):
+    """Scores that grow along the prefix: every row's reference moves many times."""
+    step = copies(rng, 24, 1, 1024, [5] * 24, heads=4, kv=1, dim=128)
+    query = stored(np.full((24, 4 * 128), 1.0) + rng.standard_normal((24, 4 * 128)) * 0.1, "bf16")
+    step.query = query
+    for n in range(1024):
+        page, line = step.place(0, n)
+        for b in range(24):
+            step.keys[0, step.table[b, n // 16], :, line] = stored(np.full(128, n / 64.0), "bf16")
+    step.device(session)
+    step.check(run(session, step, [1024]))
+
+
+@pytest.mark.parametrize("value", [0x7F80, 0xFF80, 0x7FC0])
+def test_committed_values_that_are_not_finite(session, rng, value):
+    """They reach every row, as the formula has it: infinities as such, NaN as NaN."""
+    step = copies(rng, 20, 1, 256, [2] * 20, heads=8, kv=2, dim=64)
+    page, line = step.place(0, 100)
+    step.values[0, page, 1, line, 7] = value
+    step.device(session)
+    got = run(session, step, [256]).reshape(20, 8, 64)
+    # Head 4 is the first of key head 1.
+    odd = got[:, 4:, 7]
+    assert (odd == value).all() if value != 0x7FC0 else ((odd & 0x7FFF) > 0x7F80).all()
+    finite = got.copy()
+    finite[:, 4:, 7] = 0
+    assert ((finite & 0x7F80) != 0x7F80).all()
+
+
+def test_odd_strides_of_many_rows(session, rng):
+    step = copies(rng, 20, 1, 320, [9] * 20, heads=8, kv=2, dim=128).device(session)
+    wide = np.zeros((20, 8 * 128 + 3), np.uint16)
+    wide[:, 1:-2] = step.query
+    query = A.slice(upload(session, wide, "bf16"), [{}, {"start": 1, "stop": 8 * 128 + 1}])
+    step.check(A.shared_attention(step.cache, step.batch, query, upload(session, np.array([320], np.uint32), "u32")).storage())
