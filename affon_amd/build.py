@@ -45,7 +45,7 @@ EXACT_FLAGS = {"quantize.hip": ["-ffp-contract=off"], "generic.hip": ["-ffp-cont
 # (160) of widths 104 to 120.
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
 UNIT_FLAGS = {**EXACT_FLAGS, **{f: VGPR_MFMA for f in ("gemv_mfma.hip", "vrow_b2.hip", "vrow_b4.hip", "vrow_b8.hip",
-                                                     "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip", "attention_weights.hip", "attention_prefix_tiles.hip", *(f"attention_{part}{t}.hip" for part in ("", "prefix_", "own_") for t in ("bf16", "f32")))}}
+                                                     "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip", "attention_weights.hip", "attention_prefix_tiles.hip", *(f"attention_{part}{t}.hip" for part in ("", "parts_") for t in ("bf16", "f32")))}}
 
 
 def _sources() -> list[pathlib.Path]:

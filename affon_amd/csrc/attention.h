@@ -79,10 +79,34 @@ struct Args {
   int per;
 };
 
-// Parts of the keys that a launch takes: all of a sequence; the prefixes that
-// the sequences of a group share, whose rows are then the rows of one sequence
-// (p.batch: groups for sequences); or what each has after its prefix.
-enum Part { kAllKeys = 0, kPrefix = 1, kOwnKeys = 2 };
+// A call over shared prefixes: the part of its own keys, and what is another one's in
+// the part of the prefixes.
+struct Parts : Args {
+  int groups, group_rows;  // sequences and their drafted tokens there
+  int prefix_rows, prefix_row_groups, prefix_splits, prefix_slots;
+  uint32_t prefix_chunk;   // the least keys of a piece: both parts are cut on the device
+  float *prefix_sums, *prefix_stats;
+  unsigned prefix_blocks;  // workgroups of a launch that take prefixes, before the others
+  __host__ __device__ Args prefix() const {
+    Args a = *this;
+    a.p.batch.sequences = groups;
+    a.p.batch.rows = group_rows;
+    a.p.mask = nullptr;
+    a.rows = prefix_rows;
+    a.row_groups = prefix_row_groups;
+    a.splits = prefix_splits;
+    a.row_slots = prefix_slots;
+    a.chunk = prefix_chunk;
+    a.sums = prefix_sums;
+    a.stats = prefix_stats;
+    return a;
+  }
+};
+
+// Keys that a launch takes: all of a sequence; or, by its workgroups, the prefixes
+// that the sequences of a group share, whose rows are then the rows of one
+// sequence (p.batch: groups for sequences), and what each has after its prefix.
+enum Keys { kAllKeys = 0, kParts = 1 };
 
 // Tokens of a prefix that are taken once for its group: whole steps of every
 // kernel, so that the own tokens start at one too. The rest is each sequence's own.
@@ -240,11 +264,11 @@ __device__ __forceinline__ f32x4_t joined_sums(const Args& a, int64_t slot, int 
   return v;
 }
 
-// T: element type; DT: 16-wide tiles of the head (an even number); EXACT: the
+// T: element type; DT: 16-wide tiles of the head (an even number in bf16); EXACT: the
 // head is 16 * DT wide, 64, 128 or 256, else at most that; RT: 16-row tiles
 // of a wave; WR: waves side by side over the rows, sharing the keys in LDS;
 // WK: waves side by side over the keys, each with its own; STAGES: steps in LDS.
-template <typename T, int DT, bool EXACT, int RT, int WR, int WK, int STAGES, int PART>
+template <typename T, int DT, bool EXACT, int RT, int WR, int WK, int STAGES, int KEYS>
 struct Kernel {
   static constexpr bool kHalf = T::bytes == 2;
   static constexpr int kKT = kHalf ? 2 : 1;  // 16-key tiles of a step
@@ -281,8 +305,10 @@ struct Kernel {
     return (k >> 2 & 1) << 2;
   }
 
-  static __device__ void run(const Args& a) {
+  // `block` of the launch; `shares`: it takes a prefix (KEYS = kParts).
+  static __device__ void run(const Args& a, unsigned block, bool shares) {
     const AttentionProblem& p = a.p;
+    const bool prefix = KEYS == kParts && shares;
     __shared__ __attribute__((aligned(16))) uint8_t lds[kLds];
     __shared__ int64_t tile_list[kPageList];  // byte offsets of 16-key tiles in keys and values; 1: of no page
     __shared__ int missing;
@@ -295,9 +321,9 @@ struct Kernel {
 
     // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow
     // each other there, to find them in its L2.
-    int id = blockIdx.x >> 3;
+    int id = block >> 3;
     const int rg = id % a.row_groups;
-    id = id / a.row_groups * 8 + (blockIdx.x & 7);
+    id = id / a.row_groups * 8 + (block & 7);
     const int kv = id % p.cache.kv_heads;
     id /= p.cache.kv_heads;
     // The last pieces first: only the longest sequences have them, and a piece
@@ -308,14 +334,14 @@ struct Kernel {
     // The page list's first part, whose loads need not wait for the lengths.
     uint32_t start = static_cast<uint32_t>(split) * a.chunk;
     uint32_t early = kNoPage;
-    if constexpr (PART == kAllKeys) {
+    if constexpr (KEYS == kAllKeys) {
       const uint32_t early_at = start + threadIdx.x * 16;
       if (early_at < p.batch.capacity) early = p.batch.table[b * p.batch.table_stride + early_at / p.cache.page_size];
     }
 
     uint32_t length, count, n, chunk = a.chunk;
     int table_row = b;
-    if constexpr (PART == kPrefix) {
+    if (prefix) {
       // All keys are committed, and all rows are done: those of sequences that
       // do not take the prefix are not read again.
       length = n = prefix_tokens(a, p.batch, b);
@@ -329,18 +355,23 @@ struct Kernel {
       length = committed(p.batch, b);
       count = drafted(p.batch, b);
       n = min(length + count, p.batch.capacity);
-      if constexpr (PART == kOwnKeys) {
-        if (takes_prefix(a, p.batch, b, b / a.per)) start += prefix_tokens(a, p.batch, b / a.per);
+      if constexpr (KEYS == kParts) {
+        if (count == 0) return;  // zeros, without a look at its results
+        const uint32_t first = takes_prefix(a, p.batch, b, b / a.per) ? prefix_tokens(a, p.batch, b / a.per) : 0u;
+        chunk = piece_of(n - first, a.splits, a.chunk);
+        start = first + static_cast<uint32_t>(split) * chunk;
       }
     }
     const uint32_t begin = min(start, n);
     const uint32_t end = split == a.splits - 1 ? n : min(begin + chunk, n);
-    if (begin >= end && (split > 0 || PART == kPrefix)) return;
+    if (begin >= end && (split > 0 || prefix)) return;
     const uint32_t used = max(1u, (n + a.chunk - 1) / a.chunk);  // splits that hold keys
-    const bool whole = PART == kAllKeys && (a.splits == 1 || used == 1);  // the result is this workgroup's
+    const bool whole = KEYS == kAllKeys && (a.splits == 1 || used == 1);  // the result is this workgroup's
 
     // This wave's rows, as columns of its results.
     const int row0 = (rg * WR + (WR > 1 ? wave : 0)) * RT * 16;
+    // Waves past the last row bring keys, and leave the rest out.
+    const bool idle = KEYS == kParts && WR > 1 && row0 >= a.rows;
     const uint8_t* queries = p.query + static_cast<int64_t>(b) * p.batch.rows * p.query_stride * T::bytes;
     const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * T::bytes)) % 16 == 0;
     u32x4_t q[RT][kQSteps];
@@ -440,7 +471,7 @@ struct Kernel {
       __syncthreads();
       for (uint32_t i = threadIdx.x; i < kPageList && segment + i * 16 < segment_end; i += kThreads) {
         const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
-        const uint32_t page = PART == kAllKeys && segment == begin && i < kThreads
+        const uint32_t page = KEYS == kAllKeys && segment == begin && i < kThreads
                                   ? (early < static_cast<uint32_t>(p.cache.pages) ? early : kNoPage)
                                   : page_of(p.cache, p.batch, table_row, index);
         tile_list[i] = page == kNoPage ? 1
@@ -545,8 +576,10 @@ struct Kernel {
         wait_vmcnt<0>();
       if constexpr (WR > 1) __builtin_amdgcn_s_barrier();
       asm volatile("" ::: "memory");
-      read_keys(0);
-      multiply_keys();
+      if (!idle) {
+        read_keys(0);
+        multiply_keys();
+      }
 
       auto advance = [&](int step, auto place_of_step) {
         constexpr int place = decltype(place_of_step)::value;
@@ -617,6 +650,14 @@ struct Kernel {
             else
               wait_lds_reads();
           }
+        }
+
+        if (idle) {
+          wait_vmcnt<0>();
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+          if (step + STAGES < steps) issue(place, offsets);
+          return;
         }
 
         // ---- values, on the way beside the softmax ----
@@ -742,7 +783,7 @@ struct Kernel {
       wait_lds_reads();
     }
 
-    if (PART != kPrefix && end > length && !careful) {  // the drafted tokens are among the keys
+    if (!prefix && end > length && !careful) {  // the drafted tokens are among the keys
       float odd = 0.0f;
 #pragma unroll
       for (int rt = 0; rt < RT; ++rt)
@@ -842,7 +883,13 @@ struct Kernel {
 
 template <typename K>
 __global__ __launch_bounds__(K::kThreads, K::kWavesPerSimd) void kernel(Args a) {
-  K::run(a);
+  K::run(a, blockIdx.x, false);
+}
+template <typename K>
+__global__ __launch_bounds__(K::kThreads, K::kWavesPerSimd) void parts_kernel(Parts parts) {
+  const bool shares = blockIdx.x < parts.prefix_blocks;
+  const Args a = shares ? parts.prefix() : parts;
+  K::run(a, shares ? blockIdx.x : blockIdx.x - parts.prefix_blocks, shares);
 }
 
 // Shape of the kernel that takes `rows` rows: 16-row tiles of a wave, waves
@@ -854,17 +901,15 @@ struct Shape {
 
 void launch_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
-void launch_prefix_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
-void launch_prefix_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
-void launch_own_bf16(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
-void launch_own_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
+void launch_parts_bf16(const Parts& parts, Shape shape, dim3 grid, hipStream_t stream);
+void launch_parts_f32(const Parts& parts, Shape shape, dim3 grid, hipStream_t stream);
 Shape shape_for(int rows, int head_dim);
 // Heads of 64 or 128 in bf16, workgroups of 4 or 8 waves of 32 rows.
 void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream);
 
-template <typename T, int DT, bool EXACT, int RT, int WR, int PART>
-void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
-  using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2, PART>;
+template <typename T, int DT, bool EXACT, int RT, int WR, int KEYS, typename Launched>
+void launch_shape(const Launched& a, dim3 grid, hipStream_t stream) {
+  using Probe = Kernel<T, DT, EXACT, RT, WR, 1, 2, KEYS>;
   // Waves over the keys: as many as leave room in LDS for two workgroups of
   // two steps a wave; f32, which has more to compute in the same bytes, gains
   // by a third wave at widths of 65 to 96 (32 sequences of one token over up to
@@ -873,38 +918,45 @@ void launch_shape(const Args& a, dim3 grid, hipStream_t stream) {
   constexpr int WK = WR > 1 ? 1 : Probe::kStage <= 8192 ? 4 : Probe::kStage <= 12288 && !Probe::kHalf ? 3 : 2;
   // Two steps in LDS: three took 457 us against 446 for trees of 64 over up to 16384 tokens, four 720.
   constexpr int STAGES = 2;
-  using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES, PART>;
-  hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
+  using K = Kernel<T, DT, EXACT, RT, WR, WK, STAGES, KEYS>;
+  if constexpr (KEYS == kAllKeys)
+    hipLaunchKernelGGL((kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
+  else
+    hipLaunchKernelGGL((parts_kernel<K>), grid, dim3(K::kThreads), 0, stream, a);
 }
 
-template <typename T, int DT, bool EXACT, int PART>
-void launch_width(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
+template <typename T, int DT, bool EXACT, int KEYS, typename Launched>
+void launch_width(const Launched& a, Shape shape, dim3 grid, hipStream_t stream) {
   if constexpr (DT <= 8) {
     if (shape.waves == 1) {
-      if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1, PART>(a, grid, stream);
-      return launch_shape<T, DT, EXACT, 2, 1, PART>(a, grid, stream);
+      if (shape.tiles == 1) return launch_shape<T, DT, EXACT, 1, 1, KEYS>(a, grid, stream);
+      return launch_shape<T, DT, EXACT, 2, 1, KEYS>(a, grid, stream);
     }
   }
   if constexpr (DT > 8) {
-    if (shape.waves == 2) return launch_shape<T, DT, EXACT, 1, 2, PART>(a, grid, stream);
+    if (shape.waves == 2) return launch_shape<T, DT, EXACT, 1, 2, KEYS>(a, grid, stream);
   }
-  if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4, PART>(a, grid, stream);
-  if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4, PART>(a, grid, stream);
+  if (shape.tiles == 1 || (!EXACT && DT > 8)) return launch_shape<T, DT, EXACT, 1, 4, KEYS>(a, grid, stream);
+  if constexpr (EXACT || DT <= 8) return launch_shape<T, DT, EXACT, 2, 4, KEYS>(a, grid, stream);
 }
 
-template <typename T, int PART>
-void launch_head(const Args& a, Shape shape, dim3 grid, hipStream_t stream) {
+template <typename T, int KEYS, typename Launched>
+void launch_head(const Launched& a, Shape shape, dim3 grid, hipStream_t stream) {
   const int D = a.p.cache.head_dim;
-  if (D == 64) return launch_width<T, 4, true, PART>(a, shape, grid, stream);
-  if (D == 128) return launch_width<T, 8, true, PART>(a, shape, grid, stream);
-  if (D == 256) return launch_width<T, 16, true, PART>(a, shape, grid, stream);
-  if (D < 64) return launch_width<T, 4, false, PART>(a, shape, grid, stream);
-  if (D <= 96) return launch_width<T, 6, false, PART>(a, shape, grid, stream);
-  if (D < 128) return launch_width<T, 8, false, PART>(a, shape, grid, stream);
+  if (D == 64) return launch_width<T, 4, true, KEYS>(a, shape, grid, stream);
+  if (D == 128) return launch_width<T, 8, true, KEYS>(a, shape, grid, stream);
+  if (D == 256) return launch_width<T, 16, true, KEYS>(a, shape, grid, stream);
+  if (D < 64) return launch_width<T, 4, false, KEYS>(a, shape, grid, stream);
+  // Five tiles of 16 columns in f32, whose products cost the most.
+  if constexpr (KEYS == kParts && T::bytes == 4) {
+    if (D <= 80) return launch_width<T, 5, false, KEYS>(a, shape, grid, stream);
+  }
+  if (D <= 96) return launch_width<T, 6, false, KEYS>(a, shape, grid, stream);
+  if (D < 128) return launch_width<T, 8, false, KEYS>(a, shape, grid, stream);
   // Tiles that 256 columns would waste, 32 sequences of one token over up to
   // 4096: width 192 bf16 108 us against 114, f32 322 and 477.
-  if (D <= 192) return launch_width<T, 12, false, PART>(a, shape, grid, stream);
-  launch_width<T, 16, false, PART>(a, shape, grid, stream);
+  if (D <= 192) return launch_width<T, 12, false, KEYS>(a, shape, grid, stream);
+  launch_width<T, 16, false, KEYS>(a, shape, grid, stream);
 }
 
 }  // namespace attention

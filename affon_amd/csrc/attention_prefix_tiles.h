@@ -24,7 +24,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // DT: 32-wide tiles of the head; W: waves, 32 rows each; STAGES: steps in LDS.
 template <int DT, int W, int STAGES>
 struct PrefixKernel {
-  using Swizzle = Kernel<BF16, 2 * DT, true, 1, 1, 1, 2, kPrefix>;
+  using Swizzle = Kernel<BF16, 2 * DT, true, 1, 1, 1, 2, kParts>;
   static constexpr int D = 32 * DT, kRowBytes = 2 * D, kThreads = 64 * W;
   static constexpr int kTile = 16 * kRowBytes, kPieces = kTile / 1024;  // of 16 keys, or values
   static constexpr int kStage = 2 * kTile;                              // keys of a step; the values' lie in a ring of their own

@@ -11,53 +11,75 @@ namespace affon {
 namespace attention {
 namespace {
 
-// Partial results of one part, as its kernels leave them.
-struct Joined {
-  Args prefix, own;
-};
-
-// head_dim / 4 threads for every row and head, which take the pieces of the
-// prefix and then the own ones in their order; several rows and heads to a workgroup.
+// Joins the pieces of the prefix and the own ones, in their order: head_dim / 4
+// threads for each of `shares` shares of the pieces of a row and head, which then
+// meet in LDS; several rows and heads to a workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void join_parts_kernel(Joined j) {
-  const AttentionProblem& p = j.own.p;
-  const int D = p.cache.head_dim, pieces = D / 4, per = 256 / pieces;
-  const int local = threadIdx.x / pieces, d = 4 * static_cast<int>(threadIdx.x - local * pieces);
+__global__ __launch_bounds__(256) void join_parts_kernel(Parts parts, int shares) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[256];
+  __shared__ float2 stats[256];
+  const AttentionProblem& p = parts.p;
+  const int D = p.cache.head_dim, pieces = D / 4, each = pieces * shares, per = 256 / each;
+  const int local = threadIdx.x / each, share = (threadIdx.x - local * each) / pieces;
+  const int d = 4 * static_cast<int>(threadIdx.x % pieces);
   const int64_t slot = static_cast<int64_t>(blockIdx.x) * per + local;  // of [row][head]
   const int64_t row = slot / p.heads;
-  if (local >= per || row >= static_cast<int64_t>(p.batch.sequences) * p.batch.rows) return;
-  const int head = static_cast<int>(slot - row * p.heads), kv = head / j.own.group, g = head - kv * j.own.group;
-  const int b = static_cast<int>(row / p.batch.rows);
+  const bool there = local < per && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
+  const int head = static_cast<int>(slot - row * p.heads), kv = head / parts.group, g = head - kv * parts.group;
+  const int b = there ? static_cast<int>(row / p.batch.rows) : 0;
   const int t = static_cast<int>(row - static_cast<int64_t>(b) * p.batch.rows);
-  const int group = b / j.own.per;
   const uint32_t count = drafted(p.batch, b);
-  const uint32_t n = min(committed(p.batch, b) + count, p.batch.capacity);
-  const uint32_t prefix = prefix_tokens(j.own, p.batch, group);
-  const bool takes = prefix > 0 && takes_prefix(j.own, p.batch, b, group);
-
   float top = kLowest, sum = 0.0f;
   f32x4_t v{0, 0, 0, 0};
-  if (takes) {
-    const uint32_t chunk = piece_of(prefix, j.prefix.splits, j.prefix.chunk);
-    const int64_t r = static_cast<int64_t>(row - static_cast<int64_t>(group) * j.own.per * p.batch.rows) * j.own.group + g;
-    const int64_t first = (static_cast<int64_t>(group) * p.cache.kv_heads + kv) * j.prefix.splits * j.prefix.row_slots + r;
-    v = joined_sums<false>(j.prefix, first, d, D, 0, (prefix + chunk - 1) / chunk, 1, &top, &sum);
+  if (there && t < static_cast<int>(count)) {
+    const int group = b / parts.per;
+    const uint32_t n = min(committed(p.batch, b) + count, p.batch.capacity);
+    const uint32_t prefix = takes_prefix(parts, p.batch, b, group) ? prefix_tokens(parts, p.batch, group) : 0u;
+    if (prefix > 0) {
+      const Args a = parts.prefix();
+      const uint32_t chunk = piece_of(prefix, a.splits, a.chunk), used = (prefix + chunk - 1) / chunk;
+      const int64_t r = (row - static_cast<int64_t>(group) * parts.group_rows) * parts.group + g;
+      if (share < static_cast<int>(used))
+        v = joined_sums<false>(a, (static_cast<int64_t>(group) * p.cache.kv_heads + kv) * a.splits * a.row_slots + r, d, D, share,
+                               used, shares, &top, &sum);
+    }
+    const uint32_t chunk = piece_of(n - prefix, parts.splits, parts.chunk), used = max(1u, (n - prefix + chunk - 1) / chunk);
+    const uint32_t own_share = static_cast<uint32_t>(shares - 1 - share);  // the prefix's last ones have fewer pieces
+    if (own_share < used) {
+      float own_top, own_sum;
+      const f32x4_t w = joined_sums<false>(parts, (static_cast<int64_t>(b) * p.cache.kv_heads + kv) * parts.splits * parts.row_slots +
+                                           static_cast<int64_t>(t) * parts.group + g, d, D, own_share, used, shares, &own_top, &own_sum);
+      const float peak = fmaxf(top, own_top);
+      const float keep = __builtin_amdgcn_exp2f(top - peak), own_keep = __builtin_amdgcn_exp2f(own_top - peak);
+      sum = fmaf(sum, keep, own_sum * own_keep);
+      v = v * keep + w * own_keep;
+      top = peak;
+    }
   }
-  const uint32_t own = n - min(n, takes ? prefix : 0u);
-  const uint32_t used = max(1u, (own + j.own.chunk - 1) / j.own.chunk);
-  const int64_t first = (static_cast<int64_t>(b) * p.cache.kv_heads + kv) * j.own.splits * j.own.row_slots +
-                        static_cast<int64_t>(t) * j.own.group + g;
-  float own_top, own_sum;
-  const f32x4_t w = joined_sums<false>(j.own, first, d, D, 0, used, 1, &own_top, &own_sum);
-  const float peak = fmaxf(top, own_top);
-  const float keep = __builtin_amdgcn_exp2f(top - peak), own_keep = __builtin_amdgcn_exp2f(own_top - peak);
-  sum = fmaf(sum, keep, own_sum * own_keep);
-  v = v * keep + w * own_keep;
-  store_result<T>(p.out, slot * D + d, v, t < static_cast<int>(count) ? sum : 0.0f);
+  if (shares > 1) {
+    part[threadIdx.x] = v;
+    stats[threadIdx.x] = float2{top, sum};
+    __syncthreads();
+    if (share != 0) return;
+    for (int s = 1; s < shares; ++s) top = fmaxf(top, stats[threadIdx.x + s * pieces].x);
+    v = f32x4_t{0, 0, 0, 0};
+    sum = 0.0f;
+    for (int s = 0; s < shares; ++s) {
+      const float2 st = stats[threadIdx.x + s * pieces];
+      const float keep = __builtin_amdgcn_exp2f(st.x - top);
+      sum = fmaf(st.y, keep, sum);
+      v += part[threadIdx.x + s * pieces] * keep;
+    }
+  }
+  if (there) store_result<T>(p.out, slot * D + d, v, sum);
 }
 
-// Workgroups of a launch over `units` x row groups x splits.
-int64_t blocks_of(const Args& a, int64_t units) { return (units * a.splits + 7) / 8 * 8 * a.row_groups; }
+// Workgroups over `units` x row groups x splits.
+int64_t blocks_of(int64_t units, int splits, int row_groups) { return (units * splits + 7) / 8 * 8 * row_groups; }
+
+int64_t splits_for(int64_t round, int64_t groups, int64_t most) {
+  return std::max<int64_t>(1, std::min((round + groups - 1) / groups, most));
+}
 
 }  // namespace
 }  // namespace attention
@@ -65,73 +87,85 @@ int64_t blocks_of(const Args& a, int64_t units) { return (units * a.splits + 7) 
 hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* shared, int groups, const Launch& l) {
   using namespace attention;
   const bool half = p.cache.dtype == AFFON_ROCM_BF16;
-  const int64_t capacity = p.batch.capacity, unit = half ? 128 : 64;
-  constexpr int64_t kRound = 512;  // workgroups, two to a CU
-  Joined j{};
-  j.own.p = j.prefix.p = p;
-  j.own.shared = j.prefix.shared = shared;
-  j.own.per = j.prefix.per = p.batch.sequences / groups;
-  j.prefix.p.batch.sequences = groups;
-  j.prefix.p.mask = nullptr;
-  const int64_t prefix_rows = static_cast<int64_t>(p.batch.rows) * j.own.per;
-  if (prefix_rows * (p.heads / p.cache.kv_heads) > (int64_t(1) << 30)) return hipErrorInvalidValue;
-  j.prefix.p.batch.rows = static_cast<int>(prefix_rows);
-  Shape shapes[2];
-  int tiles = 0;  // waves of the kernel for prefixes of many rows, or 0: the other one
-  size_t bytes = 0, sums[2], stats[2];
-  for (int part = 0; part < 2; ++part) {
-    Args& a = part == 0 ? j.prefix : j.own;
-    a.group = p.heads / p.cache.kv_heads;
-    a.rows = a.p.batch.rows * a.group;
-    a.row_slots = a.rows;
-    shapes[part] = shape_for(a.rows, p.cache.head_dim);
-    int64_t round = kRound;
-    if (part == 0 && half && (p.cache.head_dim == 64 || p.cache.head_dim == 128) && a.rows > 64) {
-      tiles = a.rows > 128 ? 8 : 4;
-      if (tiles == 8) round /= 2;
-    }
-    const int group_rows = part == 0 && tiles > 0 ? 32 * tiles : shapes[part].rows();
-    a.row_groups = (a.rows + group_rows - 1) / group_rows;
-    a.log2_scale = p.scale == 0.0f ? 1.0f : std::min(std::fabs(p.scale) * 1.44269504088896340736f, FLT_MAX);
-    a.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
-    const int64_t units = static_cast<int64_t>(a.p.batch.sequences) * p.cache.kv_heads;
-    int64_t splits = std::min(round / (units * a.row_groups), capacity / unit);
-    splits = std::max<int64_t>(splits, 1);
-    // The prefix is cut on the device, in pieces of `chunk` at least.
-    a.chunk = part == 0 ? static_cast<uint32_t>(unit)
-                        : static_cast<uint32_t>((capacity + splits - 1) / splits + unit - 1) / unit * unit;
-    a.splits = part == 0 ? static_cast<int>(splits) : static_cast<int>((capacity + a.chunk - 1) / a.chunk);
-    const size_t slots = static_cast<size_t>(units) * a.splits * a.row_slots;
-    sums[part] = bytes;
-    bytes += (slots * p.cache.head_dim * sizeof(float) + 255) / 256 * 256;
-    stats[part] = bytes;
-    bytes += (slots * sizeof(float2) + 255) / 256 * 256;
-    if (blocks_of(a, units) > kMaxBlocks) return hipErrorInvalidValue;
-  }
-  auto* scratch = static_cast<uint8_t*>(l.scratch(bytes));
+  const int D = p.cache.head_dim;
+  const int64_t unit = half ? 128 : 64;  // the least keys of a piece
+  constexpr int64_t kRound = 512;        // workgroups, two to a CU
+  Parts parts{};
+  parts.p = p;
+  parts.shared = shared;
+  parts.per = p.batch.sequences / groups;
+  parts.group = p.heads / p.cache.kv_heads;
+  parts.log2_scale = p.scale == 0.0f ? 1.0f : std::min(std::fabs(p.scale) * 1.44269504088896340736f, FLT_MAX);
+  parts.sign = p.scale > 0.0f ? 1.0f : p.scale < 0.0f ? -1.0f : 0.0f;
+  parts.groups = groups;
+  const int64_t group_rows = static_cast<int64_t>(p.batch.rows) * parts.per, prefix_rows = group_rows * parts.group;
+  if (prefix_rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
+  parts.group_rows = static_cast<int>(group_rows);
+  parts.rows = parts.row_slots = p.batch.rows * parts.group;
+  parts.prefix_rows = parts.prefix_slots = static_cast<int>(prefix_rows);
+
+  // Waves of the kernel for prefixes of many rows, or 0: the general one takes them.
+  const int tiles = !half || (D != 64 && D != 128) || prefix_rows <= 64 ? 0 : prefix_rows > 128 ? 8 : 4;
+  const Shape own_shape = shape_for(parts.rows, D), prefix_shape = shape_for(parts.prefix_rows, D);
+  const int64_t at_once = tiles > 0 ? 32 * tiles : prefix_shape.rows();
+  parts.row_groups = (parts.rows + own_shape.rows() - 1) / own_shape.rows();
+  parts.prefix_row_groups = static_cast<int>((prefix_rows + at_once - 1) / at_once);
+  const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
+  const int64_t prefix_units = static_cast<int64_t>(groups) * p.cache.kv_heads;
+  const int64_t most = std::max<int64_t>(1, p.batch.capacity / unit);
+  parts.chunk = parts.prefix_chunk = static_cast<uint32_t>(unit);
+  parts.splits = static_cast<int>(splits_for(kRound, units * parts.row_groups, most));
+  parts.prefix_splits = static_cast<int>(splits_for(tiles == 8 ? kRound / 2 : kRound, prefix_units * parts.prefix_row_groups, most));
+  const int64_t own_blocks = blocks_of(units, parts.splits, parts.row_groups);
+  const int64_t prefix_blocks = blocks_of(prefix_units, parts.prefix_splits, parts.prefix_row_groups);
+  if (own_blocks + prefix_blocks > kMaxBlocks) return hipErrorInvalidValue;
+
+  auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
+  const size_t own_slots = static_cast<size_t>(units) * parts.splits * parts.row_slots;
+  const size_t prefix_slots = static_cast<size_t>(prefix_units) * parts.prefix_splits * parts.prefix_slots;
+  const size_t sums = whole(own_slots * D * sizeof(float)), stats = whole(own_slots * sizeof(float2));
+  const size_t prefix_sums = whole(prefix_slots * D * sizeof(float)), prefix_stats = prefix_slots * sizeof(float2);
+  auto* scratch = static_cast<uint8_t*>(l.scratch(sums + stats + prefix_sums + prefix_stats));
   // A captured stream whose workspace cannot grow: every sequence by itself.
   if (scratch == nullptr) return attention_launch(p, l);
-  for (int part = 0; part < 2; ++part) {
-    Args& a = part == 0 ? j.prefix : j.own;
-    a.sums = reinterpret_cast<float*>(scratch + sums[part]);
-    a.stats = reinterpret_cast<float*>(scratch + stats[part]);
-    const dim3 grid(static_cast<unsigned>(blocks_of(a, static_cast<int64_t>(a.p.batch.sequences) * p.cache.kv_heads)));
-    if (part == 0 && tiles > 0)
-      launch_prefix_tiles(a, tiles, grid, l.stream);
-    else if (part == 0)
-      (half ? launch_prefix_bf16 : launch_prefix_f32)(a, shapes[part], grid, l.stream);
-    else
-      (half ? launch_own_bf16 : launch_own_f32)(a, shapes[part], grid, l.stream);
-    const hipError_t e = hipGetLastError();
-    if (e != hipSuccess) return e;
+  parts.sums = reinterpret_cast<float*>(scratch);
+  parts.stats = reinterpret_cast<float*>(scratch + sums);
+  parts.prefix_sums = reinterpret_cast<float*>(scratch + sums + stats);
+  parts.prefix_stats = reinterpret_cast<float*>(scratch + sums + stats + prefix_sums);
+
+  auto launch = half ? launch_parts_bf16 : launch_parts_f32;
+  auto run = [&](Shape shape, int64_t of_prefix, int64_t of_own) {
+    parts.prefix_blocks = static_cast<unsigned>(of_prefix);
+    launch(parts, shape, dim3(static_cast<unsigned>(of_prefix + of_own)), l.stream);
+    return hipGetLastError();
+  };
+  hipError_t e = hipSuccess;
+  if (tiles == 0 && prefix_shape.tiles == own_shape.tiles && prefix_shape.waves == own_shape.waves) {
+    // One launch for both parts (four sequences of 40 tokens after 1008 @@ us, in two launches 19.8).
+    e = run(own_shape, prefix_blocks, own_blocks);
+  } else {
+    if (tiles > 0) {
+      launch_prefix_tiles(parts.prefix(), tiles, dim3(static_cast<unsigned>(prefix_blocks)), l.stream);
+      e = hipGetLastError();
+    } else {
+      e = run(prefix_shape, prefix_blocks, 0);
+    }
+    if (e == hipSuccess) e = run(own_shape, 0, own_blocks);
   }
-  const int64_t per = 256 / (p.cache.head_dim / 4);
-  const int64_t blocks = (static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads + per - 1) / per;
+  if (e != hipSuccess) return e;
+  // A share takes the eight pieces that a thread has in flight, or fewer where
+  // there are not enough workgroups.
+  const int64_t results = static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads;
+  const int threads = D / 4;
+  int shares = std::min((std::max(parts.prefix_splits, parts.splits) + 7) / 8, 256 / threads);
+  while (shares * 2 <= 256 / threads && shares * 2 <= parts.prefix_splits && results * threads * shares < 256 * 512) shares *= 2;
+  const int64_t per = 256 / (threads * shares), blocks = (results + per - 1) / per;
   if (blocks > kMaxBlocks) return hipErrorInvalidValue;
+  const dim3 grid(static_cast<unsigned>(blocks));
   if (half)
-    hipLaunchKernelGGL(join_parts_kernel<BF16>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, l.stream, j);
+    hipLaunchKernelGGL(join_parts_kernel<BF16>, grid, dim3(256), 0, l.stream, parts, shares);
   else
-    hipLaunchKernelGGL(join_parts_kernel<F32>, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, l.stream, j);
+    hipLaunchKernelGGL(join_parts_kernel<F32>, grid, dim3(256), 0, l.stream, parts, shares);
   return hipGetLastError();
 }
 
