@@ -20,8 +20,9 @@ Each part of the block is a Program whose weights are arguments:
 
 ``QuantizedDecoderBlock.step`` runs a whole block over drafted tokens: its
 norms (model.ts:64-87 has one before attention and one before the
-feed-forward), the rotation, the append to a paged cache and the attention
-are evaluated ops (cache.py, ``residual_norm``) between those Programs.
+feed-forward), the rotation with the heads' norms, the append to a paged cache
+and the attention, over shared prefixes too, are evaluated ops (cache.py,
+``residual_norm``) between those Programs.
 """
 from __future__ import annotations
 
@@ -29,7 +30,8 @@ from dataclasses import dataclass
 from typing import Mapping
 
 from . import checkpoint as ckpt
-from .cache import DraftBatch, PagedCache, cache_append, tree_attention
+from .cache import (DraftBatch, PagedCache, RotaryAxes, attention_weights, cache_append, shared_attention,
+                    tree_attention)
 from .core import Program, Session, Tensor, TensorSpec, program
 from .ops import add, mul, quantized_matmul, residual_norm, silu
 
@@ -46,6 +48,8 @@ PROJECTIONS = (
 
 # (norm of a block, Hugging Face module of its weight)
 NORMS = {"attentionNorm": "input_layernorm", "feedForwardNorm": "post_attention_layernorm"}
+# (norm of a block's query or key heads, Hugging Face module of its weight)
+HEAD_NORMS = {"queryNorm": "self_attn.q_norm", "keyNorm": "self_attn.k_norm"}
 
 
 @dataclass(frozen=True)
@@ -80,8 +84,9 @@ class QuantizedDecoderBlock:
     biases, and the Programs that run them."""
 
     def __init__(self, shape: DecoderShape, layers: Mapping[str, ckpt.QuantizedLinear],
-                 output_biases: Mapping[str, Tensor] | None = None, norms: Mapping[str, Tensor] | None = None):
-        output_biases, norms = dict(output_biases or {}), dict(norms or {})
+                 output_biases: Mapping[str, Tensor] | None = None, norms: Mapping[str, Tensor] | None = None,
+                 head_norms: Mapping[str, Tensor] | None = None):
+        output_biases, norms, head_norms = dict(output_biases or {}), dict(norms or {}), dict(head_norms or {})
         names = [p[0] for p in PROJECTIONS]
         if sorted(layers) != sorted(names):
             raise TypeError(f"a decoder block needs the projections {names}")
@@ -109,7 +114,13 @@ class QuantizedDecoderBlock:
                 raise TypeError(f"unknown norm {name}")
             if weight.dtype not in ("f32", "bf16") or weight.shape != (shape.width,):
                 raise TypeError(f"{name} must be an f32/bf16 [{shape.width}] tensor")
-        self.norms = norms
+        for name, weight in head_norms.items():
+            if name not in HEAD_NORMS:
+                raise TypeError(f"unknown head norm {name}")
+            if weight.dtype not in ("f32", "bf16") or weight.shape not in self._head_norm_shapes(shape, name):
+                raise TypeError(f"{name} must be an f32/bf16 tensor of one of the shapes "
+                                f"{[list(s) for s in self._head_norm_shapes(shape, name)]}")
+        self.norms, self.head_norms = norms, head_norms
         self.unread_norms: tuple[str, ...] = ()  # that a checkpoint does not hold as f32/bf16 [width]
         self.shape = shape
         self.layers = dict(layers)
@@ -119,17 +130,24 @@ class QuantizedDecoderBlock:
         self.session: Session = session
         self._programs: dict[tuple[str, int, str], Program] = {}
 
+    @staticmethod
+    def _head_norm_shapes(shape: DecoderShape, name: str) -> tuple[tuple[int], tuple[int]]:
+        """Of one weight for all heads, or of each head's own."""
+        return (shape.width // shape.heads,), (shape.width if name == "queryNorm" else shape.kv_width,)
+
     # ---- construction from a checkpoint ----
 
     @classmethod
     def from_checkpoint(cls, session: Session, path: str, index: int, shape: DecoderShape, *, bits: int,
-                        group_size: int, prefix: str = "model.layers") -> "QuantizedDecoderBlock":
+                        group_size: int, prefix: str = "model.layers",
+                        head_norms: bool = False) -> "QuantizedDecoderBlock":
         """Binds block ``index`` of an MLX-affine checkpoint: ``<prefix>.<index>.
         <module>.weight`` (U32) with ``.scales`` / ``.biases`` per projection,
         and ``<module>.bias`` as the output bias where present. Norms' weights
         are read where they are f32/bf16 ``[width]``; without them the block runs
         its projections and refuses a ``step``. (A block that is made without
-        ``norms`` has norms of ones.)"""
+        ``norms`` has norms of ones.) ``head_norms``: the model norms its query
+        and key heads, whose weights are read and needed likewise."""
         base = f"{prefix}.{index}"
         modules = {field: f"{base}.{module}" for field, module, _, _ in PROJECTIONS}
         bound = ckpt.quantized_linears(session, path, bits=bits, group_size=group_size, prefixes=modules.values())
@@ -141,12 +159,17 @@ class QuantizedDecoderBlock:
         for name in [n for n in norm_names if header[norm_names[n]]["dtype"] not in ("F32", "BF16")
                      or header[norm_names[n]]["shape"] != [shape.width]]:
             del norm_names[name]
-        wanted = bias_names + list(norm_names.values())
+        heads = {name: f"{base}.{module}.weight" for name, module in HEAD_NORMS.items()} if head_norms else {}
+        head_names = {name: tensor for name, tensor in heads.items() if tensor in header and
+                      header[tensor]["dtype"] in ("F32", "BF16") and
+                      tuple(header[tensor]["shape"]) in cls._head_norm_shapes(shape, name)}
+        wanted = bias_names + list(norm_names.values()) + list(head_names.values())
         loaded = ckpt.load(session, path, wanted) if wanted else {}
         layers = {field: bound[module] for field, module in modules.items()}
         biases = {field: loaded[module + ".bias"] for field, module in modules.items() if module + ".bias" in loaded}
-        block = cls(shape, layers, biases, {name: loaded[module] for name, module in norm_names.items()})
-        block.unread_norms = tuple(n for n in NORMS if n not in norm_names)
+        block = cls(shape, layers, biases, {name: loaded[module] for name, module in norm_names.items()},
+                    {name: loaded[module] for name, module in head_names.items()})
+        block.unread_norms = tuple(n for n in NORMS if n not in norm_names) + tuple(n for n in heads if n not in head_names)
         return block
 
     # ---- Programs ----
@@ -226,7 +249,8 @@ class QuantizedDecoderBlock:
 
     def step(self, stream: Tensor, update: Tensor | None, cache: PagedCache, batch: DraftBatch, rotary: Tensor, *,
              positions: Tensor | None = None, mask: Tensor | None = None, layer: int = 0, epsilon: float = 1e-5,
-             scale: float | None = None, interleaved: bool = False, **options) -> tuple[Tensor, Tensor]:
+             scale: float | None = None, interleaved: bool = False, axes: RotaryAxes | None = None,
+             shared: Tensor | None = None, weights: Tensor | None = None, **options) -> tuple[Tensor, Tensor]:
         """The block over a batch's drafted tokens (row b*T + i of ``stream``
         [B*T, width]: token i of sequence b), whose keys and values it appends to
         ``layer`` of the cache. ``update`` is what the block before still adds to
@@ -237,16 +261,26 @@ class QuantizedDecoderBlock:
         keeps the accepted ones.
 
         ``positions`` and ``mask`` as cache_append and tree_attention take them (a
-        tree's depths and ancestors; None: a chain); ``options``: the
-        projections' compile options."""
+        tree's depths and ancestors; None: a chain); ``axes``: of positions with
+        several; ``shared``: tokens that groups of sequences share, as
+        shared_attention takes them; ``weights``: gathered ones, to which
+        attention_weights adds the rows'. ``options``: the projections' compile
+        options."""
         if self.unread_norms:
-            raise TypeError(f"the checkpoint holds no f32/bf16 [{self.shape.width}] tensor for {', '.join(self.unread_norms)}")
+            shape = f"[{self.shape.width}] " if set(self.unread_norms) <= set(NORMS) else ""
+            raise TypeError(f"the checkpoint holds no f32/bf16 {shape}tensor for {', '.join(self.unread_norms)}")
         stream, normalized = residual_norm(stream, update, weight=self.norms.get("attentionNorm"), epsilon=epsilon,
                                            dtype=cache.dtype)
         query, key, value = self.attention(normalized, **options)
         rotated = cache_append(cache, batch, query, key, value, positions, rotary, layer=layer,
-                               interleaved=interleaved)
-        attended = tree_attention(cache, batch, rotated, mask, layer=layer, scale=scale)
+                               interleaved=interleaved, query_norm=self.head_norms.get("queryNorm"),
+                               key_norm=self.head_norms.get("keyNorm"), epsilon=epsilon, axes=axes)
+        if shared is None:
+            attended = tree_attention(cache, batch, rotated, mask, layer=layer, scale=scale)
+        else:
+            attended = shared_attention(cache, batch, rotated, shared, mask, layer=layer, scale=scale)
+        if weights is not None:
+            attention_weights(cache, batch, rotated, weights, mask, layer=layer, scale=scale)
         stream, normalized = residual_norm(stream, self.attention_output(attended, **options),
                                            weight=self.norms.get("feedForwardNorm"), epsilon=epsilon,
                                            dtype=cache.dtype)
