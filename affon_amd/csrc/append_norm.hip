@@ -42,11 +42,11 @@ __device__ __forceinline__ void store_rounded(uint8_t* base, int64_t at, const f
 // holds fewer than half the head's values): the first and the second value of
 // the pairs are V consecutive ones each, interleaved pairs 2V consecutive
 // values. A head's lanes meet in its sum of squares without LDS, and lanes past
-// an odd head's end idle. `parts` workgroups take the heads of one row, H at a
-// time to a group of lanes: what belongs to the row (its place, positions and
+// an odd head's end idle. `parts` workgroups take the heads of one row, one
+// after the other in a group of lanes: what belongs to the row (its place, positions and
 // pages) is in scalar registers, its cosines and sines are read once.
-template <typename X, typename C, int V, bool INTERLEAVED, int H>
-__global__ __launch_bounds__(512) void append_norm_kernel(AppendNormProblem q, int lanes_log, uint32_t parts) {
+template <typename X, typename C, int V, bool INTERLEAVED>
+__global__ __launch_bounds__(320) void append_norm_kernel(AppendNormProblem q, int lanes_log, uint32_t parts) {
   constexpr int kChunks = V == 1 ? 2 : 1;
   const AppendProblem& p = q.base;
   const int D = p.cache.head_dim, half = p.rotary_dim / 2;
@@ -77,7 +77,7 @@ __global__ __launch_bounds__(512) void append_norm_kernel(AppendNormProblem q, i
   }
   const uint8_t* in[3] = {p.query + row * p.query_stride * X::bytes, p.key + row * p.key_stride * X::bytes,
                           p.value + row * p.value_stride * X::bytes};
-  float x[H][kChunks][V], y[H][kChunks][V];
+  float x[kChunks][V], y[kChunks][V];
   auto load = [&](uint32_t head, float (&to_x)[kChunks][V], float (&to_y)[kChunks][V]) {
     const bool is_query = head < heads, is_value = head >= heads + kv;
     const uint32_t h = is_query ? head : is_value ? head - heads - kv : head - heads;
@@ -91,9 +91,7 @@ __global__ __launch_bounds__(512) void append_norm_kernel(AppendNormProblem q, i
       load_values<X, V>(from, is_value ? D / 2 + w[c] : second[c], to_y[c]);
     }
   };
-#pragma unroll
-  for (int k = 0; k < H; ++k)
-    if (first_head + k * stride < slots) load(first_head + k * stride, x[k], y[k]);
+  if (first_head < slots) load(first_head, x, y);
 
   const uint32_t length = p.batch.lengths[b];
   const bool used = i < drafted(p.batch, b);
@@ -224,21 +222,16 @@ __global__ __launch_bounds__(512) void append_norm_kernel(AppendNormProblem q, i
       store_rounded<C, V>(to, second[c], hy[c]);
     }
   };
-  for (uint32_t head = first_head; head < slots; head += H * stride) {
-#pragma unroll
-    for (int k = 0; k < H; ++k) {
-      const uint32_t now = head + k * stride;
-      if (now >= slots) break;
-      finish(now, x[k], y[k]);
-      if (now + H * stride < slots) load(now + H * stride, x[k], y[k]);
-    }
+  for (uint32_t head = first_head; head < slots; head += stride) {
+    finish(head, x, y);
+    if (head + stride < slots) load(head + stride, x, y);
   }
 }
 
 // As the plain append: eight values at a time for many rows.
 constexpr int64_t kManyRows = 64;
 
-template <typename X, typename C, int V, int H>
+template <typename X, typename C, int V>
 hipError_t launch_wide(const AppendNormProblem& q, hipStream_t stream) {
   const AppendProblem& p = q.base;
   const int64_t rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
@@ -257,9 +250,9 @@ hipError_t launch_wide(const AppendNormProblem& q, hipStream_t stream) {
   if (rows * parts * each > kMaxBlocks * 4) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(rows * parts)), block(static_cast<unsigned>(64 * each));
   if (p.interleaved)
-    hipLaunchKernelGGL((append_norm_kernel<X, C, V, true, H>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
+    hipLaunchKernelGGL((append_norm_kernel<X, C, V, true>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
   else
-    hipLaunchKernelGGL((append_norm_kernel<X, C, V, false, H>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
+    hipLaunchKernelGGL((append_norm_kernel<X, C, V, false>), grid, block, 0, stream, q, lanes_log, static_cast<uint32_t>(parts));
   return hipGetLastError();
 }
 
@@ -284,9 +277,9 @@ hipError_t launch_typed(const AppendNormProblem& q, hipStream_t stream) {
            weights_fit(q.query_norm, v) && weights_fit(q.key_norm, v) &&
            reinterpret_cast<uintptr_t>(p.rotary) % 16 == 0 && D % (2 * v) == 0;
   };
-  if (fits(8) && rows >= kManyRows) return launch_wide<X, C, 8, 1>(q, stream);
-  if (fits(4)) return launch_wide<X, C, 4, 1>(q, stream);
-  return launch_wide<X, C, 1, 1>(q, stream);
+  if (fits(8) && rows >= kManyRows) return launch_wide<X, C, 8>(q, stream);
+  if (fits(4)) return launch_wide<X, C, 4>(q, stream);
+  return launch_wide<X, C, 1>(q, stream);
 }
 
 }  // namespace

@@ -58,6 +58,11 @@ constexpr uint32_t kPieceUnit = 128;
 struct Pieces {
   const DraftBatch& batch;
   uint32_t chunk;  // keys of a piece
+  // A whole wave's sum of numbers below 2^56.
+  static __device__ __forceinline__ uint64_t sum_of(uint64_t v) {
+    const uint32_t low = scanned(static_cast<uint32_t>(v) & 0xffffffu), high = scanned(static_cast<uint32_t>(v >> 24));
+    return (static_cast<uint64_t>(lane_of(high, 63)) << 24) + lane_of(low, 63);
+  }
   __device__ __forceinline__ uint32_t keys_of(int b) const {
     const uint32_t count = drafted(batch, b);
     return count == 0 ? 0u : min(committed(batch, b) + count, batch.capacity);
@@ -65,8 +70,7 @@ struct Pieces {
   __device__ __forceinline__ Pieces(const DraftBatch& batch, int pieces) : batch(batch) {
     uint64_t all = 0;
     for (int b = threadIdx.x & 63; b < batch.sequences; b += 64) all += keys_of(b);
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) all += __shfl_xor(static_cast<unsigned long long>(all), offset);
+    all = sum_of(all);
     const uint64_t each = min(all / static_cast<uint32_t>(pieces) + 1, static_cast<uint64_t>(batch.capacity));
     chunk = __builtin_amdgcn_readfirstlane(
         static_cast<int>((static_cast<uint32_t>(each) + kPieceUnit - 1) / kPieceUnit * kPieceUnit));
@@ -77,24 +81,19 @@ struct Pieces {
     int64_t before = 0;
     for (int base = 0; base < batch.sequences; base += 64) {
       const uint32_t own = base + lane < batch.sequences ? (keys_of(base + lane) + chunk - 1) / chunk : 0u;
-      uint32_t sum = own;
-#pragma unroll
-      for (int offset = 1; offset < 64; offset <<= 1) {
-        const uint32_t other = __shfl_up(sum, offset);
-        if (lane >= offset) sum += other;
-      }
+      const uint32_t sum = scanned(own);
       const uint64_t past = __ballot((before + sum) * kv_heads > id);
       if (past != 0) {
         const int at = __builtin_ctzll(past);
-        const uint32_t pieces = __builtin_amdgcn_readlane(static_cast<int>(own), at);
-        const int64_t start = before + static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), at)) - pieces;
+        const uint32_t pieces = lane_of(own, at);
+        const int64_t start = before + lane_of(sum, at) - pieces;
         const uint32_t rest = static_cast<uint32_t>(id - start * kv_heads);
         *b = base + at;
         *kv = static_cast<int>(rest / pieces);
         *piece = rest - static_cast<uint32_t>(*kv) * pieces;
         return true;
       }
-      before += static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(sum), 63));
+      before += lane_of(sum, 63);
     }
     return false;
   }
@@ -102,8 +101,7 @@ struct Pieces {
   __device__ __forceinline__ int64_t first_of(int b, int kv, int kv_heads) const {
     uint64_t before = 0;
     for (int i = threadIdx.x & 63; i < b; i += 64) before += (keys_of(i) + chunk - 1) / chunk;
-#pragma unroll
-    for (int offset = 1; offset < 64; offset <<= 1) before += __shfl_xor(static_cast<unsigned long long>(before), offset);
+    before = sum_of(before);
     return static_cast<int64_t>(before) * kv_heads + static_cast<int64_t>(kv) * ((keys_of(b) + chunk - 1) / chunk);
   }
 };
@@ -709,13 +707,16 @@ hipError_t launch(const WeightArgs& a, int64_t units, hipStream_t stream) {
 
 hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, const Launch& l) {
   using namespace attention;
+  const bool half = p.cache.dtype == AFFON_ROCM_BF16;
   WeightArgs a{};
   a.p = p;
   a.group = p.heads / p.cache.kv_heads;
   const int64_t rows = static_cast<int64_t>(p.batch.rows) * a.group;
   if (rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
-  const int pieces = (p.cache.head_dim * (p.cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) + 63) / 64;
+  const int pieces = (p.cache.head_dim * (half ? 2 : 4) + 63) / 64;
+  int held = half ? 2 : 4;  // pieces of the instance that takes them
+  while (held < pieces) held += held % 3 == 0 ? held / 3 : held > 2 ? held / 2 : 1;
   a.tiles = 1;
   a.over_rows = a.rows > 16 * most_tiles(pieces);
   const int side = a.over_rows ? 64 : 16;  // rows of a workgroup for each tile of a wave
@@ -743,25 +744,22 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
     a.scores = reinterpret_cast<float*>(scratch + stats);
   } else {
     const size_t ready = (static_cast<size_t>(units) * a.rows * sizeof(float) + 255) / 256 * 256;
-    scratch = static_cast<uint8_t*>(l.scratch(stats + ready + static_cast<size_t>(units) * ((a.rows + 15) / 16) * 1024 * 16));
+    scratch = static_cast<uint8_t*>(l.scratch(stats + ready + static_cast<size_t>(units) * ((a.rows + 15) / 16) * 1024 * held));
     if (scratch == nullptr) return hipErrorOutOfMemory;
     a.ready = reinterpret_cast<float*>(scratch + stats);
     a.packed = reinterpret_cast<u32x4_t*>(scratch + stats + ready);
   }
   a.stats = reinterpret_cast<float2*>(scratch);
   a.blocks = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(2048 / units, (capacity + 1023) / 1024)));
-  if (p.cache.dtype == AFFON_ROCM_BF16) {
-    if (pieces <= 2) return launch<BF16, 2>(a, units, l.stream);
-    if (pieces <= 3) return launch<BF16, 3>(a, units, l.stream);
-    if (pieces <= 4) return launch<BF16, 4>(a, units, l.stream);
-    if (pieces <= 6) return launch<BF16, 6>(a, units, l.stream);
-    return launch<BF16, 8>(a, units, l.stream);
+  switch (held) {
+    case 2: return launch<BF16, 2>(a, units, l.stream);
+    case 3: return launch<BF16, 3>(a, units, l.stream);
+    case 4: return half ? launch<BF16, 4>(a, units, l.stream) : launch<F32, 4>(a, units, l.stream);
+    case 6: return half ? launch<BF16, 6>(a, units, l.stream) : launch<F32, 6>(a, units, l.stream);
+    case 8: return half ? launch<BF16, 8>(a, units, l.stream) : launch<F32, 8>(a, units, l.stream);
+    case 12: return launch<F32, 12>(a, units, l.stream);
+    default: return launch<F32, 16>(a, units, l.stream);
   }
-  if (pieces <= 4) return launch<F32, 4>(a, units, l.stream);
-  if (pieces <= 6) return launch<F32, 6>(a, units, l.stream);
-  if (pieces <= 8) return launch<F32, 8>(a, units, l.stream);
-  if (pieces <= 12) return launch<F32, 12>(a, units, l.stream);
-  return launch<F32, 16>(a, units, l.stream);
 }
 
 }  // namespace affon

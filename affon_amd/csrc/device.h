@@ -35,4 +35,21 @@ struct BF16 {
 
 __device__ __forceinline__ unsigned lane_id() { return __lane_id(); }
 
+template <int CTRL, int ROWS>
+__device__ __forceinline__ uint32_t plus_lanes(uint32_t v) {
+  return v + static_cast<uint32_t>(__builtin_amdgcn_update_dpp(0, static_cast<int>(v), CTRL, ROWS, 0xf, true));
+}
+// The sum over a whole wave's lanes up to each.
+__device__ __forceinline__ uint32_t scanned(uint32_t v) {
+  v = plus_lanes<0x111, 0xf>(v);  // 1, 2, 4 and 8 lanes before, of 16
+  v = plus_lanes<0x112, 0xf>(v);
+  v = plus_lanes<0x114, 0xf>(v);
+  v = plus_lanes<0x118, 0xf>(v);
+  v = plus_lanes<0x142, 0xa>(v);         // the 16 before, in every second 16
+  return plus_lanes<0x143, 0xc>(v);      // the 32 before, in the upper 32
+}
+__device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
+  return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
+}
+
 }  // namespace affon

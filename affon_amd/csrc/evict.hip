@@ -45,21 +45,37 @@ __device__ __forceinline__ uint32_t order_of(float w) {
 
 constexpr int kThreads = 1024, kWaves = kThreads / 64;
 
+// A pass over a digit counts the keys that share the digits before in as many
+// bins as the digit has values; the bin that the `wanted`-th largest lies in ends
+// the search where all of it stays, which two of the three passes mostly find. A
+// row's first 4096 weights stay in registers meanwhile. What bounds it is this
+// chain of passes, each between barriers, and not memory: 2048 rows of up to
+// 4096 weights 34 us, 8 rows 6.8 (with three passes always, reading the weights
+// in each, and sums over lanes through LDS 53 and 9). Two or four sets of bins
+// for neighbouring lanes, whose additions to one bin wait for each other, take
+// as long as one.
+constexpr int kDeepWindow = 4;  // tokens of a thread in a window
+constexpr uint32_t kSelectWindow = kDeepWindow * kThreads;
+
 __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
   __shared__ uint32_t bins[2048];
   __shared__ uint32_t counts[64];  // of each wave and part of a window
-  __shared__ uint32_t found_bin, found_above;
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+  __shared__ uint32_t found_bin, found_above, found_count;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int64_t row = blockIdx.x;
   const int b = static_cast<int>(row / a.cache.kv_heads % a.batch.sequences);
-  const Plan plan(a, b);
   const float* w = a.weights + row * a.batch.capacity;
   float* out = a.out + row * a.batch.capacity;
+  float first[kDeepWindow];  // of the first window, on their way beside the plan
+#pragma unroll
+  for (int j = 0; j < kDeepWindow; ++j) first[j] = w[min(j * kThreads + threadIdx.x, a.batch.capacity - 1)];
+  const Plan plan(a, b);
   const uint32_t others = plan.length - plan.recent;  // that stay by their weight
   const uint32_t wanted = plan.left - plan.recent;
 
   // The `wanted`-th largest of the others, digit by digit from the highest.
-  uint32_t threshold = 0, ties = 0;  // those above stay, and the first `ties` of those equal
+  uint32_t threshold = 0, ties = 0;  // the first `ties` of those equal to it stay
+  uint32_t least = 0xffffffffu;      // and all from here on
   if (plan.left < plan.length && wanted > 0) {
     uint32_t left = wanted;
     const int shifts[3] = {21, 10, 0}, widths[3] = {11, 11, 10};
@@ -68,54 +84,58 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
       const uint32_t size = 1u << widths[pass], high = pass == 0 ? 0u : ~0u << shifts[pass - 1];
       for (uint32_t i = threadIdx.x; i < size; i += kThreads) bins[i] = 0;
       __syncthreads();
-      for (uint32_t n = threadIdx.x; n < others; n += kThreads) {
-        const uint32_t key = order_of(w[n]);
+      auto count = [&](float weight) {
+        const uint32_t key = order_of(weight);
         if ((key & high) == threshold) atomicAdd(&bins[key >> shift & (size - 1)], 1u);
-      }
+      };
+#pragma unroll
+      for (int j = 0; j < kDeepWindow; ++j)
+        if (j * kThreads + threadIdx.x < others) count(first[j]);
+      for (uint32_t n = kSelectWindow + threadIdx.x; n < others; n += kThreads) count(w[n]);
       __syncthreads();
       // Sums from the highest bin down: thread i has bins 2i and 2i + 1 of the reversed order.
       const uint32_t per = size / kThreads;  // 2 or 1
       uint32_t mine[2] = {0, 0};
       for (uint32_t j = 0; j < per; ++j) mine[j] = bins[size - 1 - (threadIdx.x * per + j)];
-      uint32_t sum = mine[0] + mine[1];
-#pragma unroll
-      for (int offset = 1; offset < 64; offset <<= 1) {
-        const uint32_t other = __shfl_up(sum, offset);
-        if (lane >= offset) sum += other;
-      }
+      const uint32_t sum = scanned(mine[0] + mine[1]);
       if (lane == 63) counts[wave] = sum;
       __syncthreads();
-      uint32_t above = sum - mine[0] - mine[1];
-      for (int i = 0; i < wave; ++i) above += counts[i];
+      uint32_t above = sum - mine[0] - mine[1] + lane_of(scanned(lane < wave ? counts[lane] : 0u), 63);
       for (uint32_t j = 0; j < per; ++j) {
         if (above < left && above + mine[j] >= left) {
           found_bin = size - 1 - (threadIdx.x * per + j);
           found_above = above;
+          found_count = mine[j];
         }
         above += mine[j];
       }
       __syncthreads();
       threshold |= found_bin << shift;
       left -= found_above;
-      __syncthreads();
+      if (left == found_count) {
+        least = threshold;
+        left = 0;
+        break;
+      }
     }
     ties = left;
+    if (ties > 0) least = threshold + 1;
   }
 
   // Windows of four parts of 1024 tokens.
   uint32_t before = 0, ties_before = 0;  // tokens that stay, and equal ones
-  for (uint32_t window = 0; window < plan.length; window += 4 * kThreads) {
-    float v[4];
+  for (uint32_t window = 0; window < plan.length; window += kSelectWindow) {
+    float v[kDeepWindow];
     uint32_t equal = 0, stays = 0;
-    uint64_t ballots[4];
+    uint64_t ballots[kDeepWindow];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kDeepWindow; ++j) {
       const uint32_t n = window + j * kThreads + threadIdx.x;
-      v[j] = n < plan.length ? w[n] : 0.0f;
+      v[j] = window == 0 ? first[j] : n < plan.length ? w[n] : 0.0f;
       const uint32_t key = order_of(v[j]);
       if (n < others && plan.left < plan.length) {
-        if (wanted > 0 && key > threshold) stays |= 1u << j;
-        if (wanted > 0 && key == threshold) equal |= 1u << j;
+        if (key >= least) stays |= 1u << j;
+        if (ties > 0 && key == threshold) equal |= 1u << j;
       } else if (n < plan.length) {
         stays |= 1u << j;
       }
@@ -125,28 +145,22 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
     __syncthreads();
     // Sums over the parts and waves before, in the tokens' order.
     auto scan = [&](uint32_t* total) {
-      uint32_t sum = counts[lane];
-      const uint32_t own = sum;
-#pragma unroll
-      for (int offset = 1; offset < 64; offset <<= 1) {
-        const uint32_t other = __shfl_up(sum, offset);
-        if (lane >= offset) sum += other;
-      }
-      *total = __shfl(sum, 63);
+      const uint32_t own = counts[lane], sum = scanned(own);
+      *total = lane_of(sum, 63);
       return sum - own;
     };
     const uint64_t below = (uint64_t(1) << lane) - 1;
     uint32_t total;
     uint32_t base = scan(&total);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const uint32_t rank = ties_before + __shfl(base, j * kWaves + wave) + __popcll(ballots[j] & below);
+    for (int j = 0; j < kDeepWindow; ++j) {
+      const uint32_t rank = ties_before + lane_of(base, j * kWaves + wave) + __popcll(ballots[j] & below);
       if ((equal >> j & 1) && rank < ties) stays |= 1u << j;
     }
     ties_before += total;
     __syncthreads();
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kDeepWindow; ++j) {
       ballots[j] = __ballot(stays >> j & 1);
       if (lane == 0) {
         counts[j * kWaves + wave] = __popcll(ballots[j]);
@@ -157,9 +171,9 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
     __syncthreads();
     base = scan(&total);
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < kDeepWindow; ++j) {
       // Where out is the weights themselves: this window has been read, and no token moves down.
-      const uint32_t to = before + __shfl(base, j * kWaves + wave) + __popcll(ballots[j] & below);
+      const uint32_t to = before + lane_of(base, j * kWaves + wave) + __popcll(ballots[j] & below);
       if (stays >> j & 1) out[to] = v[j];
     }
     before += total;
@@ -171,7 +185,10 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
 // A workgroup moves 2^lanes_log pieces of 16 bytes of every line of a row, keys or
 // values, as many lines at a time as its threads hold eight pieces of: all of
 // them are read before one is written, and a line is written only after every
-// line of its place or before has been read.
+// line of its place or before has been read. Memory bounds it: 2048 rows of up to
+// 4096 tokens cut to 1024 (bf16, heads of 128) 445 us, 4.8 TB/s. (Accesses that
+// leave no lines in the caches took 15 us less there, but 3 more of 16 for 8 rows
+// of up to 2000.)
 constexpr int kMoveThreads = 256, kDeep = 8;
 constexpr uint32_t kWindow = 4096;
 
@@ -218,13 +235,7 @@ __global__ __launch_bounds__(kMoveThreads) void move_kernel(EvictArgs a, int par
     if (threadIdx.x % 4 == 0) starts[word] = __popcll(bits);
     __syncthreads();
     if (threadIdx.x < 64) {
-      uint32_t sum = starts[threadIdx.x];
-      const uint32_t own = sum;
-#pragma unroll
-      for (int offset = 1; offset < 64; offset <<= 1) {
-        const uint32_t other = __shfl_up(sum, offset);
-        if (static_cast<int>(threadIdx.x) >= offset) sum += other;
-      }
+      const uint32_t own = starts[threadIdx.x], sum = scanned(own);
       starts[threadIdx.x] = sum - own;
       if (threadIdx.x == 63) in_window = sum;
     }
@@ -273,7 +284,10 @@ hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const 
   EvictArgs a{cache, batch, weights, out, keep, recent, nullptr, static_cast<int>((batch.capacity + 63) / 64)};
   const int64_t rows = static_cast<int64_t>(cache.layers) * batch.sequences * cache.kv_heads;
   const int line_pieces = cache.head_dim * (cache.dtype == AFFON_ROCM_BF16 ? 2 : 4) / 16;
-  // Whole lines, or parts of them side by side until there is work for every CU.
+  // Whole lines, or parts of them side by side until there are two workgroups for
+  // every CU: 8 rows of up to 2000 tokens cut to 1024 (bf16, heads of 128) take 15.7 us
+  // with 512 of them, 16.5 with 128, 19.5 with 64 and 25.8 with 32; 2048 rows
+  // of up to 4096 by whole lines 479, quarters of them 875.
   int lanes_log = 0;
   while ((1 << lanes_log) < line_pieces && lanes_log < 6) ++lanes_log;
   while (lanes_log > 0 && rows * 2 * ((line_pieces + (1 << lanes_log) - 1) >> lanes_log) < 512) --lanes_log;
