@@ -307,7 +307,7 @@ def shared_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, shared
     op = "shared_attention"
     cache_struct = cache._check(op, layer)
     batch_struct = batch._check(op, cache, (query, shared, mask))
-    if len(shared.shape) != 1 or shared.shape[0] == 0 or batch.sequences % shared.shape[0]:
+    if not isinstance(shared, Tensor) or len(shared.shape) != 1 or shared.shape[0] == 0 or batch.sequences % shared.shape[0]:
         raise TypeError("shared_attention shared must be a u32 tensor of as many values as there are groups of equal size")
     view, groups = _rank_two(op, "query", query), shared.shape[0]
     out = _output(op, out, cache.session, cache.dtype, query.shape)

@@ -81,6 +81,14 @@ int hip_fail(hipError_t error, const char* what) {
   return fail(AFFON_ROCM_HIP_ERROR, "%s: %s", what, hipGetErrorString(error));
 }
 
+// Of a launch that does nothing without the session's workspace.
+int workspace_fail(hipError_t error, const char* what) {
+  if (error != hipErrorOutOfMemory) return hip_fail(error, what);
+  return fail(AFFON_ROCM_HIP_ERROR,
+              "%s needs a larger workspace, which there is no memory for, or which a stream that is captured cannot get: run "
+              "the call once before the capture", what);
+}
+
 void clear_error() { g_last_error.clear(); }
 
 bool mul_ok(uint64_t a, uint64_t b, uint64_t* out) {
@@ -1253,7 +1261,7 @@ int affon_rocm_attention_weights(affon_rocm_session* session, const affon_rocm_k
   launch.stream = session->stream;
   launch.workspace = session->workspace;
   const hipError_t e = affon::attention_weights_launch(p, layer, launch);
-  if (e != hipSuccess) return hip_fail(e, op);
+  if (e != hipSuccess) return workspace_fail(e, op);
   return AFFON_ROCM_OK;
 }
 
@@ -1280,7 +1288,7 @@ int affon_rocm_cache_evict(affon_rocm_session* session, const affon_rocm_kv_cach
   launch.stream = session->stream;
   launch.workspace = session->workspace;
   const hipError_t e = affon::evict_launch(c, b, weights, out, keep, recent, launch);
-  if (e != hipSuccess) return hip_fail(e, op);
+  if (e != hipSuccess) return workspace_fail(e, op);
   return AFFON_ROCM_OK;
 }
 
