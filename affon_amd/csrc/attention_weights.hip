@@ -33,7 +33,8 @@ struct WeightArgs {
   float log2_scale;  // |scale| * log2(e)
   float sign;        // of the scale: a factor of the queries
   float2* stats;     // (m, l) [piece][row]
-  float* ready;      // m + log2(l) [unit][row]; infinite: the row takes no part
+  float* ready;      // m + log2(l) [unit][row_slots]; infinite: the row takes no part
+  int row_slots;     // rows, up to a whole 64
   u32x4_t* packed;   // the queries as gather_kernel's operands
   float* scores;     // [unit][row][capacity], or null: computed again
   float* weights;    // of the layer, [sequence][key head][capacity]
@@ -460,7 +461,7 @@ __global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t packs)
     for (int s = 0; s < KS; ++s) a.packed[(i * KS + s) * 64 + (threadIdx.x & 63)] = q[s];
     return;
   }
-  const int parts = (a.rows + 255) / 256;
+  const int parts = (a.row_slots + 255) / 256;
   const int unit = static_cast<int>((blockIdx.x - packs) / parts);
   const int r = static_cast<int>(blockIdx.x - packs - static_cast<int64_t>(unit) * parts) * 256 + threadIdx.x;
   const int b = unit / a.p.cache.kv_heads, kv = unit - b * a.p.cache.kv_heads;
@@ -469,7 +470,11 @@ __global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t packs)
   const Pieces pieces(a.p.batch, a.pieces);
   const int64_t first = pieces.first_of(b, kv, a.p.cache.kv_heads);
   const uint32_t used = (c.n + pieces.chunk - 1) / pieces.chunk;
-  if (r >= a.rows) return;
+  if (r >= a.row_slots) return;
+  if (r >= a.rows) {
+    a.ready[static_cast<int64_t>(unit) * a.row_slots + r] = INFINITY;
+    return;
+  }
   float m = kLowest, l = 0.0f;
   constexpr uint32_t kAtOnce = 8;  // pieces whose loads are in flight together
   for (uint32_t s0 = 0; s0 < used; s0 += kAtOnce) {
@@ -485,7 +490,7 @@ __global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t packs)
     for (uint32_t i = 0; i < kAtOnce; ++i)
       if (s0 + i < used) l = fmaf(st[i].y, __builtin_amdgcn_exp2f(st[i].x - m), l);
   }
-  a.ready[static_cast<int64_t>(unit) * a.rows + r] = ready_of(m, l, r / a.group < static_cast<int>(c.count));
+  a.ready[static_cast<int64_t>(unit) * a.row_slots + r] = ready_of(m, l, r / a.group < static_cast<int>(c.count));
 }
 
 // Sums of up to 16 rows' kept scores: a thread four keys, 16 lanes the pieces of a row.
@@ -540,16 +545,30 @@ __global__ __launch_bounds__(256) void sum_kernel(WeightArgs a) {
   }
 }
 
-// Four waves side by side over the keys, KT tiles each, all rows one after the other.
+// The sum over each 16 lanes, in all of them.
+template <int CTRL>
+__device__ __forceinline__ float plus_other(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), CTRL, 0xf, 0xf, true));
+}
+__device__ __forceinline__ float sum_of_16(float v) {
+  v = plus_other<0xB1>(v);          // lane ^ 1
+  v = plus_other<0x4E>(v);          // lane ^ 2
+  v = plus_other<0x141>(v);         // the other four of eight
+  return plus_other<0x140>(v);      // the other eight of sixteen
+}
+
+// Four waves side by side over the keys, KT tiles each, all rows one after the
+// other, kTiles tiles of them at a time through LDS.
 template <typename T, int KS>
 __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
   using Ops = Tiles<T, KS>;
   constexpr int KT = KS <= 4 ? 2 : 1;
   constexpr uint32_t kKeys = 16 * KT;
-  constexpr int kTiles = KS <= 4 ? 4 : 2;  // of rows that go through LDS at a time
+  constexpr int kTiles = KS <= 4 ? 4 : 2;
+  constexpr int kQueries = kTiles * KS * 1024;
   const AttentionProblem& p = a.p;
   __shared__ __attribute__((aligned(16))) uint8_t lds[4 * Ops::kPlace];
-  __shared__ __attribute__((aligned(16))) uint8_t queries[2][kTiles * KS * 1024];
+  __shared__ __attribute__((aligned(16))) uint8_t queries[2][kQueries + 1024];  // and what their exponents start from
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int col = lane & 15, quad = lane >> 4;
   const Pieces pieces(p.batch, a.gather_pieces);
@@ -559,105 +578,138 @@ __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
   const int unit = b * p.cache.kv_heads + kv;
   const Context c(p, b);
   // Rows past the last one in use take no part.
-  const int rows = min(a.rows, static_cast<int>(c.count) * a.group);
-  const float* all_ready = a.ready + static_cast<int64_t>(unit) * a.rows;
+  const int rows = min(a.rows, static_cast<int>(c.count) * a.group), tiles = (rows + 15) / 16;
+  const int groups = (tiles + kTiles - 1) / kTiles;
+  const auto* all_ready = reinterpret_cast<const uint8_t*>(a.ready + static_cast<int64_t>(unit) * a.row_slots);
   const u32x4_t* packed = a.packed + static_cast<int64_t>(unit) * ((a.rows + 15) / 16) * KS * 64;
+  float* weights = a.weights + static_cast<int64_t>(unit) * p.batch.capacity;
   uint8_t* place = lds + wave * Ops::kPlace;
   const Ops ops(a);
   Ops::clear(place, 1);
   const uint32_t begin = piece * pieces.chunk, end = min(begin + pieces.chunk, c.n);
-  // This wave's keys of the next step, on their way while a step's rows are gone through.
+  auto issue = [&](int group, int turn) {
+    const u32x4_t* from = packed + static_cast<int64_t>(group) * kTiles * KS * 64;
+    const uint32_t into = __builtin_amdgcn_readfirstlane(static_cast<int>(lds_address(queries[turn])));
+    const int pieces = min(kTiles, tiles - group * kTiles) * KS;
+    for (int i = wave; i < pieces; i += 4) dma16(uniform(reinterpret_cast<const uint8_t*>(from + i * 64)), lane * 16, into + i * 1024);
+    if (wave == 3) dma16(uniform(all_ready + group * kTiles * 64), min(lane, 4 * kTiles - 1) * 16, into + kQueries);
+  };
+  // This wave's keys of the next step, on their way while a step's rows are gone
+  // through; past the last one some page's, which are not looked at.
+  int64_t list = 1;  // places of 64 tiles, a lane each
   u32x4_t raw[KT][KS];
-  uint32_t raw_there = 0;
-  auto fetch = [&](uint32_t at) {  // past the last key: some page's, and not looked at
-    int64_t tile[KT];
-    raw_there = 0;
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) tile[kt] = at + 16 * kt < c.n ? Ops::tile_of(a, b, kv, at + 16 * kt) : 1;
+  uint32_t coming = 0;  // bit kt: tile kt lies somewhere
+  auto fetch = [&](uint32_t four) {
+    if ((four - begin) % 1024 == 0) {
+      const uint32_t mine = four + lane * 16;
+      list = mine < end ? Ops::tile_of(a, b, kv, mine) : 1;
+    }
+    coming = 0;
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
-      raw_there |= (tile[kt] & 1) == 0 ? 1u << kt : 0u;
-      ops.fetch(uniform(p.cache.keys + (tile[kt] & ~int64_t(15))), raw[kt]);
+      const int i = static_cast<int>((four - begin) / 16 % 64) + wave * KT + kt;
+      const uint32_t low = __builtin_amdgcn_readlane(static_cast<int>(list), i);
+      const uint32_t high = __builtin_amdgcn_readlane(static_cast<int>(list >> 32), i);
+      ops.fetch(p.cache.keys + (static_cast<int64_t>(high) << 32 | (low & ~15u)), raw[kt]);
+      coming |= low & 1 ? 0u : 1u << kt;
     }
   };
-  fetch(begin + wave * kKeys);
-  for (uint32_t at4 = begin; at4 < end; at4 += 4 * kKeys) {
-    const uint32_t at = at4 + wave * kKeys, there = raw_there;
-    const bool all = at + kKeys <= c.length && __builtin_amdgcn_readfirstlane(static_cast<int>(there)) == (1 << KT) - 1;
+  int turn = 0;
+  issue(0, turn);
+  fetch(begin);
+  for (uint32_t four = begin; four < end; four += 4 * kKeys) {
+    const uint32_t at = four + wave * kKeys, there = coming;
+    const bool all = at + kKeys <= c.length && there == (1 << KT) - 1;
     u32x4_t keys[KT][KS];
     f32x4_t sums[KT];
-#pragma unroll
-    for (int kt = 0; kt < KT; ++kt) sums[kt] = f32x4_t{0, 0, 0, 0};
-    // Tiles of rows through LDS, a group of them ahead.
-    const int groups = (rows + 16 * kTiles - 1) / (16 * kTiles);
-    auto issue = [&](int group) {
-      const u32x4_t* from = packed + static_cast<int64_t>(group) * kTiles * KS * 64;
-      const uint32_t into = __builtin_amdgcn_readfirstlane(static_cast<int>(lds_address(queries[group % 2])));
-      const int pieces = min(kTiles, (rows + 15) / 16 - group * kTiles) * KS;
-      for (int i = wave; i < pieces; i += 4)
-        dma16(uniform(reinterpret_cast<const uint8_t*>(from + i * 64)), lane * 16, into + i * 1024);
-    };
-    auto ready_at = [&](int r0) { return r0 + col < rows ? all_ready[r0 + col] : INFINITY; };
-    float coming[kTiles];
-    auto prepare = [&](int group) {
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) coming[i] = ready_at((group * kTiles + i) * 16);
-    };
-    __syncthreads();  // the queries before have been read
-    issue(0);
-    prepare(0);
+    float before[KT];  // the weights that lanes 0 to 3 of each 16 add to
 #pragma unroll
     for (int kt = 0; kt < KT; ++kt) {
+      sums[kt] = f32x4_t{0, 0, 0, 0};
       ops.put(place, raw[kt]);
       ops.get(place, keys[kt]);
     }
-    for (int group = 0; group < groups; ++group) {
-      float ready[kTiles];
+    for (int group = 0; group < groups; ++group, turn ^= 1) {
+      // The queries of this group were sent before the loads of the next keys and weights.
+      if (group == 1)
+        wait_vmcnt<KT * KS + KT>();
+      else
+        wait_vmcnt<0>();
+      wait_lds_reads();
+      __builtin_amdgcn_s_barrier();
+      asm volatile("" ::: "memory");
+      if (group + 1 < groups)
+        issue(group + 1, turn ^ 1);
+      else if (four + 4 * kKeys < end)
+        issue(0, turn ^ 1);
+      if (group == 0) {
+        fetch(four + 4 * kKeys);
 #pragma unroll
-      for (int i = 0; i < kTiles; ++i) ready[i] = coming[i];
-      wait_vmcnt<0>();
-      __syncthreads();
-      if (group + 1 < groups) prepare(group + 1);
-      if (group + 1 < groups) issue(group + 1);
-      if (group == 0 && at4 + 4 * kKeys < end) fetch(at + 4 * kKeys);
-#pragma unroll
-      for (int i = 0; i < kTiles; ++i) {
-        const int r0 = (group * kTiles + i) * 16;
-        if (r0 >= rows) break;
+        for (int kt = 0; kt < KT; ++kt) before[kt] = weights[min(at + 16 * kt + 4 * quad + min(col, 3), c.n - 1)];
+      }
+      const uint8_t* queries_now = queries[turn];
+      auto multiply = [&](int i, f32x4_t (&s)[KT]) {
         u32x4_t q[KS];
 #pragma unroll
-        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(queries[group % 2] + (i * KS + s) * 1024 + lane * 16);
-        f32x4_t s[KT];
+        for (int s = 0; s < KS; ++s) q[s] = *reinterpret_cast<const u32x4_t*>(queries_now + (i * KS + s) * 1024 + lane * 16);
 #pragma unroll
         for (int kt = 0; kt < KT; ++kt) s[kt] = Ops::scores(keys[kt], q);
+      };
+      auto add = [&](const f32x4_t (&s)[KT], float from) {
+#pragma unroll
+        for (int kt = 0; kt < KT; ++kt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) sums[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.log2_scale, -from));
+      };
+      float ready[kTiles], most = 0.0f;
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        ready[i] = *reinterpret_cast<const float*>(queries_now + kQueries + (16 * i + col) * 4);
+        most = fmaxf(most, ready[i]);
+      }
+      if (all && (group + 1) * kTiles <= tiles && !__any(most == INFINITY)) {
+        // Every row sees every key: the exponentials of a tile beside the products of the next.
+        f32x4_t s[KT], next[KT];
+        multiply(0, s);
+#pragma unroll
+        for (int i = 0; i < kTiles; ++i) {
+          if (i + 1 < kTiles) multiply(i + 1, next);
+          add(s, ready[i]);
+#pragma unroll
+          for (int kt = 0; kt < KT; ++kt) s[kt] = next[kt];
+        }
+        continue;
+      }
+#pragma unroll
+      for (int i = 0; i < kTiles; ++i) {
+        const int tile = group * kTiles + i;
+        if (tile >= tiles) break;
+        f32x4_t s[KT];
+        multiply(i, s);
         if (!all || __any(ready[i] == INFINITY)) {
 #pragma unroll
           for (int kt = 0; kt < KT; ++kt) {
             const uint32_t seen = !(there >> kt & 1) || ready[i] == INFINITY
-                                      ? 0u : Ops::seen(a, c, b, min(r0 + col, a.rows - 1) / a.group, at + 16 * kt);
+                                      ? 0u : Ops::seen(a, c, b, min(16 * tile + col, a.rows - 1) / a.group, at + 16 * kt);
 #pragma unroll
             for (int e = 0; e < 4; ++e)
               if (!(seen >> (4 * quad + e) & 1)) s[kt][e] = -INFINITY;
           }
-          if (ready[i] == INFINITY) ready[i] = 0.0f;  // every score is -infinity
         }
-#pragma unroll
-        for (int kt = 0; kt < KT; ++kt)
-#pragma unroll
-          for (int e = 0; e < 4; ++e) sums[kt][e] += __builtin_amdgcn_exp2f(fmaf(s[kt][e], a.log2_scale, -ready[i]));
+        add(s, ready[i] == INFINITY ? 0.0f : ready[i]);  // every score is -infinity there
       }
     }
-    float* weights = a.weights + static_cast<int64_t>(unit) * p.batch.capacity;
 #pragma unroll
-    for (int kt = 0; kt < KT; ++kt)
+    for (int kt = 0; kt < KT; ++kt) {
+      float v = 0.0f;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        float v = sums[kt][i];
-#pragma unroll
-        for (int offset = 1; offset < 16; offset <<= 1) v += __shfl_xor(v, offset);
-        const uint32_t n = at + 16 * kt + 4 * quad + i;
-        if (col == i && n < c.n) weights[n] = n < c.length ? weights[n] + v : v;
+        const float sum = sum_of_16(sums[kt][i]);
+        if (col == i) v = sum;
       }
+      const uint32_t n = at + 16 * kt + 4 * quad + col;
+      if (col < 4 && n < c.n) weights[n] = n < c.length ? before[kt] + v : v;
+    }
   }
 }
 
@@ -695,7 +747,7 @@ hipError_t launch(const WeightArgs& a, int64_t units, hipStream_t stream) {
   if constexpr (most_tiles(KS) >= 4) {
     if (a.tiles == 4) launch_stats<T, KS, 4>(a, grid, stream);
   }
-  const int64_t packs = (units * ((a.rows + 15) / 16) + 3) / 4, ready_blocks = packs + units * ((a.rows + 255) / 256);
+  const int64_t packs = (units * ((a.rows + 15) / 16) + 3) / 4, ready_blocks = packs + units * ((a.row_slots + 255) / 256);
   if (ready_blocks > kMaxBlocks) return hipErrorInvalidValue;
   hipLaunchKernelGGL((ready_kernel<T, KS>), dim3(static_cast<unsigned>(ready_blocks)), dim3(256), 0, stream, a, packs);
   hipLaunchKernelGGL((gather_kernel<T, KS>), dim3(static_cast<unsigned>(gather_blocks)), dim3(256), 0, stream, a);
@@ -714,6 +766,7 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   const int64_t rows = static_cast<int64_t>(p.batch.rows) * a.group;
   if (rows > (int64_t(1) << 30)) return hipErrorInvalidValue;
   a.rows = static_cast<int>(rows);
+  a.row_slots = (a.rows + 63) / 64 * 64;
   const int pieces = (p.cache.head_dim * (half ? 2 : 4) + 63) / 64;
   int held = half ? 2 : 4;  // pieces of the instance that takes them
   while (held < pieces) held += held % 3 == 0 ? held / 3 : held > 2 ? held / 2 : 1;
@@ -743,7 +796,7 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   if (scratch != nullptr) {
     a.scores = reinterpret_cast<float*>(scratch + stats);
   } else {
-    const size_t ready = (static_cast<size_t>(units) * a.rows * sizeof(float) + 255) / 256 * 256;
+    const size_t ready = (static_cast<size_t>(units) * a.row_slots * sizeof(float) + 255) / 256 * 256;
     scratch = static_cast<uint8_t*>(l.scratch(stats + ready + static_cast<size_t>(units) * ((a.rows + 15) / 16) * 1024 * held));
     if (scratch == nullptr) return hipErrorOutOfMemory;
     a.ready = reinterpret_cast<float*>(scratch + stats);
