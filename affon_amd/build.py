@@ -40,12 +40,14 @@ EXACT_FLAGS = {"quantize.hip": ["-ffp-contract=off"], "generic.hip": ["-ffp-cont
 # (v_accvgpr_read) sits between each MFMA and its scaling. The attention
 # kernels' softmax reads every product's result the same way. With it no kernel
 # of gemv_mfma and vrow needs scratch memory; of the xgemm files 16 of 102 do,
-# 8 to 100 bytes a lane, and of the attention's 54 three, all of two row tiles a
-# wave and more than 64 rows: bf16 of width 128 (12 bytes), bf16 (52) and f32
-# (160) of widths 104 to 120.
+# 8 to 100 bytes a lane, and of the attention's 191 five, all of two row tiles a
+# wave and more than 64 rows: bf16 of width 128 (12 bytes), and of widths 104 to
+# 120 bf16 (52; over parts 40) and f32 (160; over parts 152).
 VGPR_MFMA = ["-mllvm", "-amdgpu-mfma-vgpr-form=1"]
-UNIT_FLAGS = {**EXACT_FLAGS, **{f: VGPR_MFMA for f in ("gemv_mfma.hip", "vrow_b2.hip", "vrow_b4.hip", "vrow_b8.hip",
-                                                     "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip", "attention_weights.hip", "attention_prefix_tiles.hip", *(f"attention_{part}{t}.hip" for part in ("", "parts_") for t in ("bf16", "f32")))}}
+UNIT_FLAGS = {**EXACT_FLAGS, **{f: VGPR_MFMA for f in (
+    "gemv_mfma.hip", "vrow_b2.hip", "vrow_b4.hip", "vrow_b8.hip", "xgemm_b2.hip", "xgemm_b4.hip", "xgemm_b8.hip",
+    "attention_bf16.hip", "attention_f32.hip", "attention_parts_bf16.hip", "attention_parts_f32.hip",
+    "attention_prefix_tiles.hip", "attention_weights.hip")}}
 
 
 def _sources() -> list[pathlib.Path]:

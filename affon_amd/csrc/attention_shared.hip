@@ -104,8 +104,14 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   parts.rows = parts.row_slots = p.batch.rows * parts.group;
   parts.prefix_rows = parts.prefix_slots = static_cast<int>(prefix_rows);
 
-  // Waves of the kernel for prefixes of many rows, or 0: the general one takes them.
-  const int tiles = !half || (D != 64 && D != 128) || prefix_rows <= 64 ? 0 : prefix_rows > 128 ? 8 : 4;
+  // Waves of the kernel for prefixes of many rows, one workgroup to a CU, or 0: the
+  // general one takes them, whose waves share 16 rows' keys. The whole call, 8 key
+  // heads of 128, general and 4 waves (us): 16 rows of a key head after 2048
+  // tokens 14.0 and 20.7, after 8192 26.2 and 25.6, after 32768 43.5 and 46.6; 32 rows
+  // 23.1 and 21.6, 31.0 and 26.2, 48.6 and 47.3; 128 rows 30.0 and 28.8, 37.6
+  // and 32.4, 58.3 and 52.5. 4 and 8 waves: 256 rows 29.1 and 37.8, 36.8 and
+  // 41.6, 73.0 and 70.0; 192 rows 31.1 and 33.8, 34.9 and 38.6, 70.4 and 61.0.
+  const int tiles = !half || (D != 64 && D != 128) || prefix_rows <= 16 ? 0 : prefix_rows > 128 ? 8 : 4;
   const Shape own_shape = shape_for(parts.rows, D), prefix_shape = shape_for(parts.prefix_rows, D);
   const int64_t at_once = tiles > 0 ? 32 * tiles : prefix_shape.rows();
   parts.row_groups = (parts.rows + own_shape.rows() - 1) / own_shape.rows();
@@ -115,7 +121,7 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   const int64_t most = std::max<int64_t>(1, p.batch.capacity / unit);
   parts.chunk = parts.prefix_chunk = static_cast<uint32_t>(unit);
   parts.splits = static_cast<int>(splits_for(kRound, units * parts.row_groups, most));
-  parts.prefix_splits = static_cast<int>(splits_for(tiles == 8 ? kRound / 2 : kRound, prefix_units * parts.prefix_row_groups, most));
+  parts.prefix_splits = static_cast<int>(splits_for(tiles > 0 ? kRound / 2 : kRound, prefix_units * parts.prefix_row_groups, most));
   const int64_t own_blocks = blocks_of(units, parts.splits, parts.row_groups);
   const int64_t prefix_blocks = blocks_of(prefix_units, parts.prefix_splits, parts.prefix_row_groups);
   if (own_blocks + prefix_blocks > kMaxBlocks) return hipErrorInvalidValue;
@@ -141,7 +147,7 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   };
   hipError_t e = hipSuccess;
   if (tiles == 0 && prefix_shape.tiles == own_shape.tiles && prefix_shape.waves == own_shape.waves) {
-    // One launch for both parts (four sequences of 40 tokens after 1008 @@ us, in two launches 19.8).
+    // One launch for both parts (four sequences of 40 tokens after 1008 12.7 us, in two launches 19.8).
     e = run(own_shape, prefix_blocks, own_blocks);
   } else {
     if (tiles > 0) {

@@ -6,7 +6,15 @@
 // first (stats_kernel). For up to 16 rows of a key head the scores are then kept
 // and summed over the rows by sum_kernel: the keys are read once. With more rows
 // the scores would be more to write and read than the keys, and are computed
-// again (gather_kernel). Products are S^T = K Q^T on the matrix cores: lane % 16
+// again (gather_kernel).
+//
+// What bounds it, bf16 heads of 128, 8 key heads: one token of 32 sequences over
+// up to 4096, memory (stats 41 us, 4.1 TB/s with the scores' writes; sum 7.3); 32
+// tokens of 8 query heads a key head, four sequences over up to 16384, the
+// exponentials (twice each, at a quarter of the vector rate) and what of the
+// products does not run beside them (stats 36 us, gathering 35, 6 between them; the
+// two sides' products are 30 us of the matrix rate); one token over 777,
+// two launches and their chains of loads (11 us). Products are S^T = K Q^T on the matrix cores: lane % 16
 // is a row, and a lane's four results are keys 4 (lane / 16) .. + 3 of a tile of
 // 16. stats_kernel holds queries in registers and walks over the keys,
 // gather_kernel holds keys and walks over the rows.
@@ -558,7 +566,10 @@ __device__ __forceinline__ float sum_of_16(float v) {
 }
 
 // Four waves side by side over the keys, KT tiles each, all rows one after the
-// other, kTiles tiles of them at a time through LDS.
+// other, kTiles tiles of them at a time through LDS, the next ones on their way
+// meanwhile, those of the next keys too. (Waited for at each step's start, with
+// pages looked up and weights loaded when they were needed, 43 us instead of 35;
+// four tiles of keys a wave 43: too few waves.)
 template <typename T, int KS>
 __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
   using Ops = Tiles<T, KS>;
@@ -713,19 +724,27 @@ __global__ __launch_bounds__(256) void gather_kernel(WeightArgs a) {
   }
 }
 
+// Tiles of 16 rows that a wave of stats_kernel holds beside its keys, at most.
+constexpr int most_tiles(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 2 : 1; }
+
 template <typename T, int KS, int RT>
 void launch_stats(const WeightArgs& a, dim3 grid, hipStream_t stream) {
-  if (a.over_rows)
-    hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, true>), grid, dim3(256), 0, stream, a);
-  else
-    hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, false>), grid, dim3(256), 0, stream, a);
+  if constexpr (RT > 1 || most_tiles(KS) < 4) {  // more than 64 rows take two tiles or more
+    if (a.over_rows) {
+      hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, true>), grid, dim3(256), 0, stream, a);
+      return;
+    }
+  }
+  hipLaunchKernelGGL((stats_kernel<T, KS, RT, false, false>), grid, dim3(256), 0, stream, a);
 }
 
 constexpr int64_t kMaxInt = 2147483647;
+// Workgroups of a round: what of each kernel runs at once, five, two and three to
+// a CU. Stats with kept scores, 32 sequences of one token over up to 4096: 512
+// 55.7 us, 1024 51.6, 1280 49.5, 2048 49.4, and 1280 leaves fewer pieces to join.
+// More rows, 32 tokens of four sequences over up to 16384: stats and gathering
+// in rounds of 512 and 768 80.8 us, 256 and 512 96.9, 1024 and 1536 93.8.
 constexpr int64_t kKeepRound = 1280, kStatsRound = 512, kGatherRound = 768;
-
-// Tiles of 16 rows that a wave of stats_kernel holds beside its keys, at most.
-constexpr int most_tiles(int pieces) { return pieces <= 4 ? 4 : pieces <= 8 ? 2 : 1; }
 
 template <typename T, int KS>
 hipError_t launch(const WeightArgs& a, int64_t units, hipStream_t stream) {
@@ -788,7 +807,10 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   a.pieces = pieces_for(a.rows <= 16 ? kKeepRound : kStatsRound, a.row_groups);
   a.gather_pieces = pieces_for(kGatherRound, 1);
   const size_t stats = (static_cast<size_t>(a.pieces + p.batch.sequences) * p.cache.kv_heads * a.rows * sizeof(float2) + 255) / 256 * 256;
-  // Up to 16 rows' scores are kept, where they find room.
+  // Up to 16 rows' scores are kept, where they find room: 32 sequences of up to
+  // 4096 tokens 49 us with 4 rows of a key head, 52 with 8 and 59 with 16, and
+  // 81 to 83 where they are computed again. More are more to write and read than
+  // the keys (bf16 heads of 128: 4 bytes a row each way, against 256).
   constexpr size_t kMostScores = size_t(1) << 30;
   const size_t scores = static_cast<size_t>(units) * a.rows * capacity * sizeof(float);
   uint8_t* scratch = nullptr;
