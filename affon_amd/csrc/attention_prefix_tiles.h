@@ -1,4 +1,4 @@
-// A prefix that many rows share, on the matrix cores: bf16, heads of 64 or 128.
+// A prefix that many rows share, on the matrix cores: bf16, heads of 64 or 128; f32 below.
 //
 // All its keys are committed and seen by every row, so nothing is masked: a
 // workgroup of W waves holds 32 W rows and walks over a piece of the keys 32 at
@@ -11,7 +11,11 @@
 // products, the vector unit about 400 of exponentials, sums and conversions,
 // and LDS 128 per CU and wave. They overlap within a wave: a step's exponentials run
 // between the scores of the step after it and the values' products of the one
-// before it, none of which waits for them.
+// before it, none of which waits for them. 64 rows of 8 query heads a key head
+// over 32768 tokens (8 key heads of 128): 80 us, 860 TFLOP/s, where a large library
+// product reaches 1192; 0.93 us a step of 8 waves, and 14 us for the start and the
+// results. Left out one at a time, on a copy (of 87 us then): the matrix products 13,
+// the exponentials 6, the LDS reads 6, the transfers 4.
 #pragma once
 
 #include "attention.h"
@@ -20,6 +24,65 @@ namespace affon {
 namespace attention {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
+
+// The keys of a workgroup: a piece of a group's prefix, of one key head; begin >= end: none.
+struct PrefixPiece {
+  int row_group, kv, group, split, holder;
+  uint32_t begin = 0, end = 0;
+  __device__ __forceinline__ explicit PrefixPiece(const Args& a) {
+    const AttentionProblem& p = a.p;
+    // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow each other there.
+    int id = blockIdx.x >> 3;
+    row_group = id % a.row_groups;
+    id = id / a.row_groups * 8 + (blockIdx.x & 7);
+    kv = id % p.cache.kv_heads;
+    id /= p.cache.kv_heads;
+    group = id % p.batch.sequences;
+    split = id / p.batch.sequences;
+    if (split >= a.splits) return;
+    const uint32_t n = prefix_tokens(a, p.batch, group);
+    if (n == 0) return;
+    holder = __builtin_amdgcn_readfirstlane(prefix_holder(a, group));
+    if (holder < 0) return;
+    const uint32_t chunk = piece_of(n, a.splits, a.chunk);
+    begin = split * chunk;
+    end = min(begin + chunk, n);
+  }
+};
+
+// Byte offsets of the tiles of 16 keys from `segment` on that lie somewhere, in
+// their order (others hold no keys), and how many; for whole workgroups of W waves.
+template <int W, int LIST>
+__device__ __forceinline__ int list_tiles(const Args& a, const PrefixPiece& piece, uint32_t segment, int row_bytes,
+                                          int64_t (&list)[LIST], int (&listed)[W]) {
+  const AttentionProblem& p = a.p;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int wanted = static_cast<int>(min(piece.end - segment, static_cast<uint32_t>(LIST * 16)) / 16);
+  int tiles = 0;
+  for (int i0 = 0; i0 < LIST && i0 < wanted; i0 += 64 * W) {
+    const int i = i0 + static_cast<int>(threadIdx.x);
+    int64_t offset = -1;
+    if (i < wanted) {
+      const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
+      const uint32_t page = page_of(p.cache, p.batch, piece.holder, index);
+      if (page != kNoPage)
+        offset = ((static_cast<int64_t>(page) * p.cache.kv_heads + piece.kv) * p.cache.page_size +
+                  (at - index * p.cache.page_size)) * row_bytes;
+    }
+    const uint64_t lies = __ballot(offset >= 0);
+    __syncthreads();  // the list, and `listed`, are free
+    if (lane == 0) listed[wave] = __popcll(lies);
+    __syncthreads();
+    int before = tiles;
+    for (int w = 0; w < W; ++w) {
+      if (w < wave) before += listed[w];
+      tiles += listed[w];
+    }
+    if (offset >= 0) list[before + __popcll(lies & ((uint64_t(1) << lane) - 1))] = offset;
+  }
+  __syncthreads();
+  return __builtin_amdgcn_readfirstlane(tiles);
+}
 
 // DT: 32-wide tiles of the head; W: waves, 32 rows each; STAGES: steps in LDS.
 template <int DT, int W, int STAGES>
@@ -45,24 +108,13 @@ struct PrefixKernel {
 
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const int col = lane & 31, side = lane >> 5;
-    // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow each other there.
-    int id = blockIdx.x >> 3;
-    const int rg = id % a.row_groups;
-    id = id / a.row_groups * 8 + (blockIdx.x & 7);
-    const int kv = id % p.cache.kv_heads;
-    id /= p.cache.kv_heads;
-    const int group = id % p.batch.sequences, split = id / p.batch.sequences;
-    if (split >= a.splits) return;
-    const uint32_t n = prefix_tokens(a, p.batch, group);
-    if (n == 0) return;
-    const int holder = prefix_holder(a, group);
-    if (holder < 0) return;
-    const uint32_t chunk = piece_of(n, a.splits, a.chunk), begin = split * chunk;
-    if (begin >= n) return;
-    const uint32_t end = min(begin + chunk, n);
+    const PrefixPiece piece(a);
+    if (piece.begin >= piece.end) return;
+    const int kv = piece.kv, group = piece.group, split = piece.split;
+    const uint32_t begin = piece.begin, end = piece.end;
 
     // This wave's rows.
-    const int row0 = (rg * W + wave) * 32;
+    const int row0 = (piece.row_group * W + wave) * 32;
     const bool active = row0 < a.rows;
     u32x4_t q[2 * DT];
     {
@@ -119,32 +171,7 @@ struct PrefixKernel {
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16_t{};
 
     for (uint32_t segment = begin; segment < end; segment += kList * 16) {
-      // The tiles that lie somewhere, in their order: others hold no keys.
-      const int wanted = static_cast<int>(min(end - segment, static_cast<uint32_t>(kList * 16)) / 16);
-      int tiles = 0;
-      for (int i0 = 0; i0 < kList && i0 < wanted; i0 += kThreads) {
-        const int i = i0 + static_cast<int>(threadIdx.x);
-        int64_t offset = -1;
-        if (i < wanted) {
-          const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
-          const uint32_t page = page_of(p.cache, p.batch, holder, index);
-          if (page != kNoPage)
-            offset = ((static_cast<int64_t>(page) * p.cache.kv_heads + kv) * p.cache.page_size + (at - index * p.cache.page_size)) *
-                     kRowBytes;
-        }
-        const uint64_t lies = __ballot(offset >= 0);
-        __syncthreads();  // the list, and `listed`, are free
-        if (lane == 0) listed[wave] = __popcll(lies);
-        __syncthreads();
-        int before = tiles;
-        for (int w = 0; w < W; ++w) {
-          if (w < wave) before += listed[w];
-          tiles += listed[w];
-        }
-        if (offset >= 0) tile_list[before + __popcll(lies & ((uint64_t(1) << lane) - 1))] = offset;
-      }
-      __syncthreads();
-      tiles = __builtin_amdgcn_readfirstlane(tiles);
+      const int tiles = list_tiles<W, kList>(a, piece, segment, kRowBytes, tile_list, listed);
       if (tiles == 0) continue;
       const int steps = (tiles + 1) / 2;
       const bool odd = tiles % 2 != 0;  // the last step's second tile holds no keys
@@ -303,6 +330,174 @@ struct PrefixKernel {
     wait_lds_reads();
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
+  }
+};
+
+// The same in f32, for heads of D = 64 to 128: S^T, and then O^T, by 32x32x2
+// products, of two dims or keys a time: the dims 8 j + 4 (lane / 32) + e and the
+// keys of a lane's score, so that both operands are read in their order and P^T
+// stays where it is. Bound by the matrix cores, whose f32 products take as many
+// cycles for a 16th of bf16's work: D + 32 ceil(D / 32) halves of 64 cycles
+// for 32 rows and keys, beside which all else is small (about 450 of exponentials and
+// sums), so a step's phases follow each other and the waves of a SIMD fill each other's gaps.
+template <int WIDTH, int W>
+struct PrefixF32 {
+  static constexpr int D = WIDTH, kRowBytes = 4 * D, kThreads = 64 * W, DT = (D + 31) / 32;
+  static constexpr int kTile = 16 * kRowBytes, kPieces = kTile / 1024;  // of 16 keys, or values
+  static constexpr int kStage = 4 * kTile;                              // keys, then values, of a step
+  static constexpr int kPer = (4 * kPieces + W - 1) / W;                // transfers of a wave and step
+  static constexpr int kList = 512;
+  static constexpr float kMostSum = 1024.0f;
+  static constexpr int kSwizzle = D == 64 || D == 128 ? 15 : 0;  // of a key's pieces, where its length is a power of two
+  static_assert(D % 16 == 0, "whole pieces");
+
+  static __device__ void run(const Args& a) {
+    const AttentionProblem& p = a.p;
+    // Reads of dims past the last value's end stay inside it.
+    __shared__ __attribute__((aligned(16))) uint8_t lds[2 * kStage + 128];
+    __shared__ int64_t tile_list[kList];
+    __shared__ int listed[W];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int col = lane & 31, side = lane >> 5;
+    const PrefixPiece piece(a);
+    if (piece.begin >= piece.end) return;
+    const int row0 = (piece.row_group * W + wave) * 32;
+    const bool active = row0 < a.rows;
+    f32x4_t q[D / 8];
+    {
+      const int r = min(row0 + col, a.rows - 1), t = r / a.group;
+      const auto* from = reinterpret_cast<const float*>(p.query) +
+                         (static_cast<int64_t>(piece.group) * p.batch.rows + t) * p.query_stride +
+                         static_cast<int64_t>(piece.kv * a.group + r - t * a.group) * D;
+      const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * 4)) % 16 == 0;
+#pragma unroll
+      for (int j = 0; j < D / 8; ++j) {
+        const float* four = from + 8 * j + 4 * side;
+        if (aligned) {
+          q[j] = *reinterpret_cast<const f32x4_t*>(four);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) q[j][e] = four[e];
+        }
+#pragma unroll
+        for (int e = 0; e < 4; ++e) q[j][e] = a.sign == 0.0f ? 0.0f : a.sign < 0.0f ? -q[j][e] : q[j][e];
+      }
+    }
+    // This wave's pieces of a step's four tiles; past the last the last again.
+    int which[kPer], into[kPer];
+    uint32_t from[kPer];
+#pragma unroll
+    for (int i = 0; i < kPer; ++i) {
+      const int number = min(wave + i * W, 4 * kPieces - 1), first = number % kPieces * 1024;
+      which[i] = number / kPieces;
+      into[i] = which[i] * kTile + first;
+      const int at = first + lane * 16, k = at / kRowBytes, c = at % kRowBytes / 16;
+      from[i] = k * kRowBytes + (which[i] < 2 ? c ^ (k & kSwizzle) : c) * 16;
+    }
+    const uint32_t base = lds_address(lds);
+
+    f32x16_t o[DT];
+    float m = kLowest, l = 0.0f;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16_t{};
+    for (uint32_t segment = piece.begin; segment < piece.end; segment += kList * 16) {
+      const int tiles = list_tiles<W, kList>(a, piece, segment, kRowBytes, tile_list, listed);
+      if (tiles == 0) continue;
+      const int steps = (tiles + 1) / 2;
+      const bool odd = tiles % 2 != 0;  // the last step's second tile holds no keys
+      auto issue = [&](int step) {
+        const uint32_t place = __builtin_amdgcn_readfirstlane(static_cast<int>(base + step % 2 * kStage));
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int64_t offset = tile_list[min(2 * step + which[i] % 2, tiles - 1)];
+          const uint32_t low = __builtin_amdgcn_readfirstlane(static_cast<int>(offset));
+          const uint32_t high = __builtin_amdgcn_readfirstlane(static_cast<int>(offset >> 32));
+          const uint8_t* source = which[i] < 2 ? p.cache.keys : p.cache.values;
+          dma16(uniform(source + (static_cast<int64_t>(high) << 32 | low)), from[i], place + into[i]);
+        }
+      };
+      issue(0);
+      for (int step = 0; step < steps; ++step) {
+        wait_lds_reads();
+        wait_vmcnt<0>();
+        __builtin_amdgcn_s_barrier();  // this step is there, and the place of the one before is free
+        asm volatile("" ::: "memory");
+        if (step + 1 < steps) issue(step + 1);
+        const uint8_t* keys = lds + step % 2 * kStage;
+        uint8_t* values = lds + step % 2 * kStage + 2 * kTile;
+        const bool half = odd && step == steps - 1;
+        if (half) {
+          for (int i = threadIdx.x; i < kTile / 16; i += kThreads)
+            reinterpret_cast<u32x4_t*>(values + kTile)[i] = u32x4_t{0, 0, 0, 0};
+          wait_lds_reads();
+          __builtin_amdgcn_s_barrier();
+          asm volatile("" ::: "memory");
+        }
+        if (!active) continue;
+        f32x16_t s{};
+        const uint8_t* row = keys + col * kRowBytes;
+#pragma unroll
+        for (int j = 0; j < D / 8; ++j) {
+          const f32x4_t k = *reinterpret_cast<const f32x4_t*>(row + ((2 * j + side) ^ (col & kSwizzle)) * 16);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) s = __builtin_amdgcn_mfma_f32_32x32x2f32(k[e], q[j][e], s, 0, 0, 0);
+        }
+        if (half) {
+#pragma unroll
+          for (int i = 8; i < 16; ++i) s[i] = -INFINITY;
+        }
+        auto largest = [&] {
+          float top = s[0];
+#pragma unroll
+          for (int i = 1; i < 16; ++i) top = fmaxf(top, s[i]);
+          top *= a.log2_scale;
+          return fmaxf(top, __shfl_xor(top, 32));
+        };
+        if (m == kLowest) m = fmaxf(m, largest());
+        f32x16_t probability;
+        float sum = 0.0f;
+        auto exponentials = [&] {
+          sum = 0.0f;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            probability[i] = __builtin_amdgcn_exp2f(fmaf(s[i], a.log2_scale, -m));
+            sum += probability[i];
+          }
+        };
+        exponentials();
+        if (__any(sum > kMostSum)) {  // a score far past the reference, which moves
+          const float top = fmaxf(m, largest()), keep = __builtin_amdgcn_exp2f(m - top);
+          m = top;
+          l *= keep;
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt) o[dt] *= keep;
+          exponentials();
+        }
+        l += sum;
+        const uint8_t* value = values + 4 * side * kRowBytes + col * 4;
+#pragma unroll
+        for (int i = 0; i < 16; ++i)
+#pragma unroll
+          for (int dt = 0; dt < DT; ++dt)
+            o[dt] = __builtin_amdgcn_mfma_f32_32x32x2f32(
+                *reinterpret_cast<const float*>(value + (8 * (i / 4) + i % 4) * kRowBytes + 128 * dt), probability[i], o[dt], 0, 0, 0);
+      }
+      wait_lds_reads();
+    }
+    if (!active) return;
+    l += __shfl_xor(l, 32);
+    const int r = row0 + col;
+    if (r >= a.rows) return;
+    const int64_t slot = ((static_cast<int64_t>(piece.group) * p.cache.kv_heads + piece.kv) * a.splits + piece.split) * a.row_slots + r;
+    float* to = a.sums + slot * D;
+#pragma unroll
+    for (int dt = 0; dt < DT; ++dt)
+#pragma unroll
+      for (int j = 0; j < 4; ++j)
+        if (32 * dt + 8 * j < D)
+          *reinterpret_cast<f32x4_t*>(to + 32 * dt + 8 * j + 4 * side) =
+              f32x4_t{o[dt][4 * j], o[dt][4 * j + 1], o[dt][4 * j + 2], o[dt][4 * j + 3]};
+    if (side == 0) *reinterpret_cast<float2*>(a.stats + 2 * slot) = float2{m, l};
   }
 };
 

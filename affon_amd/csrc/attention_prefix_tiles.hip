@@ -4,17 +4,33 @@
 namespace affon {
 namespace attention {
 
+template <typename K>
+void launch_prefix(const Args& a, dim3 grid, hipStream_t stream) {
+  hipLaunchKernelGGL(prefix_kernel<K>, grid, dim3(K::kThreads), 0, stream, a);
+}
+
+template <int D>
+void launch_f32(const Args& a, int waves, dim3 grid, hipStream_t stream) {
+  if (waves == 8)
+    launch_prefix<PrefixF32<D, 8>>(a, grid, stream);
+  else
+    launch_prefix<PrefixF32<D, 4>>(a, grid, stream);
+}
+
 void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream) {
-  if (a.p.cache.head_dim == 128) {
-    if (waves == 8)
-      hipLaunchKernelGGL((prefix_kernel<PrefixKernel<4, 8, 6>>), grid, dim3(512), 0, stream, a);
-    else
-      hipLaunchKernelGGL((prefix_kernel<PrefixKernel<4, 4, 4>>), grid, dim3(256), 0, stream, a);
-  } else {
-    if (waves == 8)
-      hipLaunchKernelGGL((prefix_kernel<PrefixKernel<2, 8, 6>>), grid, dim3(512), 0, stream, a);
-    else
-      hipLaunchKernelGGL((prefix_kernel<PrefixKernel<2, 4, 8>>), grid, dim3(256), 0, stream, a);
+  const int D = a.p.cache.head_dim;
+  if (a.p.cache.dtype == AFFON_ROCM_BF16) {
+    if (D == 128 && waves == 8) launch_prefix<PrefixKernel<4, 8, 6>>(a, grid, stream);
+    if (D == 128 && waves == 4) launch_prefix<PrefixKernel<4, 4, 4>>(a, grid, stream);
+    if (D == 64 && waves == 8) launch_prefix<PrefixKernel<2, 8, 6>>(a, grid, stream);
+    if (D == 64 && waves == 4) launch_prefix<PrefixKernel<2, 4, 8>>(a, grid, stream);
+    return;
+  }
+  switch (D) {
+    case 64: return launch_f32<64>(a, waves, grid, stream);
+    case 80: return launch_f32<80>(a, waves, grid, stream);
+    case 96: return launch_f32<96>(a, waves, grid, stream);
+    default: return launch_f32<128>(a, waves, grid, stream);
   }
 }
 

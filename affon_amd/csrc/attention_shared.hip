@@ -111,7 +111,8 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   // 23.1 and 21.6, 31.0 and 26.2, 48.6 and 47.3; 128 rows 30.0 and 28.8, 37.6
   // and 32.4, 58.3 and 52.5. 4 and 8 waves: 256 rows 29.1 and 37.8, 36.8 and
   // 41.6, 73.0 and 70.0; 192 rows 31.1 and 33.8, 34.9 and 38.6, 70.4 and 61.0.
-  const int tiles = !half || (D != 64 && D != 128) || prefix_rows <= 16 ? 0 : prefix_rows > 128 ? 8 : 4;
+  const bool takes = half ? D == 64 || D == 128 : D == 64 || D == 80 || D == 96 || D == 128;
+  const int tiles = !takes || prefix_rows <= 16 ? 0 : prefix_rows > 128 ? 8 : 4;
   const Shape own_shape = shape_for(parts.rows, D), prefix_shape = shape_for(parts.prefix_rows, D);
   const int64_t at_once = tiles > 0 ? 32 * tiles : prefix_shape.rows();
   parts.row_groups = (parts.rows + own_shape.rows() - 1) / own_shape.rows();
