@@ -77,6 +77,9 @@ struct Args {
   // shared[group] tokens of each in the same pages.
   const uint32_t* shared;
   int per;
+  // Its prefixes cut over all groups (by the tiles' kernels): of each group the
+  // number of its first piece and the pieces that each key head has, for the join.
+  uint2* plan;
 };
 
 // A call over shared prefixes: the part of its own keys, and what is another one's in
@@ -86,6 +89,7 @@ struct Parts : Args {
   int prefix_rows, prefix_row_groups, prefix_splits, prefix_slots;
   uint32_t prefix_chunk;   // the least keys of a piece: both parts are cut on the device
   float *prefix_sums, *prefix_stats;
+  uint2* prefix_plan;  // or null: each group is cut by itself
   unsigned prefix_blocks;  // workgroups of a launch that take prefixes, before the others
   __host__ __device__ Args prefix() const {
     Args a = *this;
@@ -99,6 +103,7 @@ struct Parts : Args {
     a.chunk = prefix_chunk;
     a.sums = prefix_sums;
     a.stats = prefix_stats;
+    a.plan = prefix_plan;
     return a;
   }
 };

@@ -25,35 +25,96 @@ namespace attention {
 
 typedef float f32x16_t __attribute__((ext_vector_type(16)));
 
-// The keys of a workgroup: a piece of a group's prefix, of one key head; begin >= end: none.
+// The keys of a workgroup: a piece of a group's prefix, of one key head; begin >=
+// end: none. All groups' prefixes are cut alike, into `splits` pieces a group on
+// average, so that a long one holds no workgroup longer than the others. (Four of
+// up to 6000 tokens, 8 sequences each, f32: 94 us, each cut into 16 101.) In the order
+// [group][key head][piece].
 struct PrefixPiece {
-  int row_group, kv, group, split, holder;
+  int row_group, kv, group;
+  int64_t number;
   uint32_t begin = 0, end = 0;
   __device__ __forceinline__ explicit PrefixPiece(const Args& a) {
-    const AttentionProblem& p = a.p;
+    const DraftBatch& batch = a.p.batch;
+    const int lane = threadIdx.x & 63, groups = batch.sequences, kv_heads = a.p.cache.kv_heads;
     // Workgroups b, b + 8, .. run on one XCD: those of the same keys follow each other there.
-    int id = blockIdx.x >> 3;
+    const int id = blockIdx.x >> 3;
     row_group = id % a.row_groups;
-    id = id / a.row_groups * 8 + (blockIdx.x & 7);
-    kv = id % p.cache.kv_heads;
-    id /= p.cache.kv_heads;
-    group = id % p.batch.sequences;
-    split = id / p.batch.sequences;
-    if (split >= a.splits) return;
-    const uint32_t n = prefix_tokens(a, p.batch, group);
-    if (n == 0) return;
-    holder = __builtin_amdgcn_readfirstlane(prefix_holder(a, group));
-    if (holder < 0) return;
-    const uint32_t chunk = piece_of(n, a.splits, a.chunk);
-    begin = split * chunk;
-    end = min(begin + chunk, n);
+    number = id / a.row_groups * 8 + (blockIdx.x & 7);
+    auto tokens = [&](int base) { return base + lane < groups ? prefix_tokens(a, batch, base + lane) : 0u; };
+    const uint32_t mine = tokens(0);
+    uint32_t chunk = batch.capacity + a.chunk;
+    if (a.splits > 1) {
+      uint64_t all = mine;
+      for (int base = 64; base < groups; base += 64) all += tokens(base);
+      all = wave_sum(all);
+      const uint32_t pieces = static_cast<uint32_t>(a.splits) * groups, high = static_cast<uint32_t>(all >> 32);
+      const uint32_t each = high != 0 ? static_cast<uint32_t>(all / pieces) : static_cast<uint32_t>(all) / pieces;
+      auto whole = [&](uint32_t n) { return (n + a.chunk) / a.chunk * a.chunk; };  // past n, where it is whole itself too
+      chunk = each == 0 ? a.chunk : whole(each - (all == static_cast<uint64_t>(each) * pieces ? 1 : 0));
+      // A few workgroups more than a round take as long as another: longer pieces, until they fit.
+      if (groups <= 64)
+        for (int i = 0; i < 16 && lane_of(scanned((mine + chunk - 1) / chunk), 63) > pieces; ++i) chunk += whole(chunk / 16);
+    }
+    chunk = __builtin_amdgcn_readfirstlane(static_cast<int>(chunk));
+    int64_t before = 0;
+    for (int base = 0; base < groups; base += 64) {
+      const uint32_t held = base == 0 ? mine : tokens(base), own = (held + chunk - 1) / chunk, sum = scanned(own);
+      const uint64_t past = __ballot((before + sum) * kv_heads > number);
+      if (past != 0) {
+        const int at = __builtin_ctzll(past);
+        const uint32_t count = lane_of(own, at), rest = static_cast<uint32_t>(number - (before + lane_of(sum, at) - count) * kv_heads);
+        group = base + at;
+        kv = static_cast<int>(rest / count);
+        const uint32_t piece = rest - static_cast<uint32_t>(kv) * count;
+        if (rest == 0 && row_group == 0 && threadIdx.x == 0) a.plan[group] = uint2{static_cast<uint32_t>(number), count};
+        begin = piece * chunk;
+        end = min(begin + chunk, lane_of(held, at));
+        return;
+      }
+      before += lane_of(sum, 63);
+    }
+  }
+};
+
+// The rows of a group that are in use, one after the other: of the sequences that
+// take the prefix, their drafted tokens in use. Lane by lane, row `at` of them as a row of the
+// group (-1: there are fewer), its token and its query head of the key head's; and the
+// first such sequence, whose pages are read for all (-1: none).
+struct UsedRow {
+  int row = -1, token = 0, head, holder = -1;
+  __device__ __forceinline__ UsedRow(const Args& a, int group, int at) {
+    const int lane = threadIdx.x & 63, wanted = at / a.group;
+    DraftBatch batch = a.p.batch;  // of the sequences themselves
+    batch.rows /= a.per;
+    head = at - wanted * a.group;
+    int before = 0;
+    for (int base = 0; base < a.per; base += 64) {
+      const int i = base + lane, b = group * a.per + min(i, a.per - 1), some = min(64, a.per - base);
+      const int own = i < a.per && takes_prefix(a, batch, b, group) ? static_cast<int>(drafted(batch, b)) : 0;
+      const uint64_t taken = __ballot(own > 0);
+      if (holder < 0 && taken != 0) holder = group * a.per + base + __builtin_ctzll(taken);
+      if (__all(own == batch.rows || i >= a.per)) {  // all in use
+        if (wanted >= before && wanted < before + some * batch.rows) token = base * batch.rows + wanted - before, row = 0;
+        before += some * batch.rows;
+      } else {
+        const int sum = static_cast<int>(scanned(static_cast<uint32_t>(own)));
+        int index = 0;  // sequences that end before the wanted row
+        for (int k = 0; k < some; ++k) index += before + static_cast<int>(lane_of(static_cast<uint32_t>(sum), k)) <= wanted ? 1 : 0;
+        const int start = before + __shfl(sum - own, min(index, 63));
+        if (wanted >= before && index < some) token = (base + index) * batch.rows + wanted - start, row = 0;
+        before += static_cast<int>(lane_of(static_cast<uint32_t>(sum), 63));
+      }
+      if (holder >= 0 && __all(row >= 0)) break;
+    }
+    if (row == 0) row = token * a.group + head;
   }
 };
 
 // Byte offsets of the tiles of 16 keys from `segment` on that lie somewhere, in
 // their order (others hold no keys), and how many; for whole workgroups of W waves.
 template <int W, int LIST>
-__device__ __forceinline__ int list_tiles(const Args& a, const PrefixPiece& piece, uint32_t segment, int row_bytes,
+__device__ __forceinline__ int list_tiles(const Args& a, const PrefixPiece& piece, int holder, uint32_t segment, int row_bytes,
                                           int64_t (&list)[LIST], int (&listed)[W]) {
   const AttentionProblem& p = a.p;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -64,7 +125,7 @@ __device__ __forceinline__ int list_tiles(const Args& a, const PrefixPiece& piec
     int64_t offset = -1;
     if (i < wanted) {
       const uint32_t at = segment + i * 16, index = at / p.cache.page_size;
-      const uint32_t page = page_of(p.cache, p.batch, piece.holder, index);
+      const uint32_t page = page_of(p.cache, p.batch, holder, index);
       if (page != kNoPage)
         offset = ((static_cast<int64_t>(page) * p.cache.kv_heads + piece.kv) * p.cache.page_size +
                   (at - index * p.cache.page_size)) * row_bytes;
@@ -110,17 +171,19 @@ struct PrefixKernel {
     const int col = lane & 31, side = lane >> 5;
     const PrefixPiece piece(a);
     if (piece.begin >= piece.end) return;
-    const int kv = piece.kv, group = piece.group, split = piece.split;
+    const int kv = piece.kv, group = piece.group;
     const uint32_t begin = piece.begin, end = piece.end;
 
     // This wave's rows.
     const int row0 = (piece.row_group * W + wave) * 32;
-    const bool active = row0 < a.rows;
+    const UsedRow used(a, group, row0 + col);
+    const int holder = __builtin_amdgcn_readfirstlane(used.holder);
+    if (holder < 0) return;
+    const bool active = __any(used.row >= 0);
     u32x4_t q[2 * DT];
     {
-      const int r = min(row0 + col, a.rows - 1), t = r / a.group;
-      const uint8_t* from = p.query + ((static_cast<int64_t>(group) * p.batch.rows + t) * p.query_stride +
-                                       static_cast<int64_t>(kv * a.group + r - t * a.group) * D) * 2;
+      const uint8_t* from = p.query + ((static_cast<int64_t>(group) * p.batch.rows + used.token) * p.query_stride +
+                                       static_cast<int64_t>(kv * a.group + used.head) * D) * 2;
       const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * 2)) % 16 == 0;
       const uint32_t flip = a.sign < 0.0f ? 0x80008000u : 0u, keep = a.sign == 0.0f ? 0u : ~0u;
 #pragma unroll
@@ -171,7 +234,7 @@ struct PrefixKernel {
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16_t{};
 
     for (uint32_t segment = begin; segment < end; segment += kList * 16) {
-      const int tiles = list_tiles<W, kList>(a, piece, segment, kRowBytes, tile_list, listed);
+      const int tiles = list_tiles<W, kList>(a, piece, holder, segment, kRowBytes, tile_list, listed);
       if (tiles == 0) continue;
       const int steps = (tiles + 1) / 2;
       const bool odd = tiles % 2 != 0;  // the last step's second tile holds no keys
@@ -311,9 +374,8 @@ struct PrefixKernel {
     }
     if (!active) return;
     l += __shfl_xor(l, 32);
-    const int r = row0 + col;
-    if (r >= a.rows) return;
-    const int64_t slot = ((static_cast<int64_t>(group) * p.cache.kv_heads + kv) * a.splits + split) * a.row_slots + r;
+    if (used.row < 0) return;
+    const int64_t slot = piece.number * a.row_slots + used.row;
     float* to = a.sums + slot * D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)
@@ -362,13 +424,15 @@ struct PrefixF32 {
     const PrefixPiece piece(a);
     if (piece.begin >= piece.end) return;
     const int row0 = (piece.row_group * W + wave) * 32;
-    const bool active = row0 < a.rows;
+    const UsedRow used(a, piece.group, row0 + col);
+    const int holder = __builtin_amdgcn_readfirstlane(used.holder);
+    if (holder < 0) return;
+    const bool active = __any(used.row >= 0);
     f32x4_t q[D / 8];
     {
-      const int r = min(row0 + col, a.rows - 1), t = r / a.group;
       const auto* from = reinterpret_cast<const float*>(p.query) +
-                         (static_cast<int64_t>(piece.group) * p.batch.rows + t) * p.query_stride +
-                         static_cast<int64_t>(piece.kv * a.group + r - t * a.group) * D;
+                         (static_cast<int64_t>(piece.group) * p.batch.rows + used.token) * p.query_stride +
+                         static_cast<int64_t>(piece.kv * a.group + used.head) * D;
       const bool aligned = (reinterpret_cast<uintptr_t>(p.query) | static_cast<uintptr_t>(p.query_stride * 4)) % 16 == 0;
 #pragma unroll
       for (int j = 0; j < D / 8; ++j) {
@@ -401,7 +465,7 @@ struct PrefixF32 {
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt) o[dt] = f32x16_t{};
     for (uint32_t segment = piece.begin; segment < piece.end; segment += kList * 16) {
-      const int tiles = list_tiles<W, kList>(a, piece, segment, kRowBytes, tile_list, listed);
+      const int tiles = list_tiles<W, kList>(a, piece, holder, segment, kRowBytes, tile_list, listed);
       if (tiles == 0) continue;
       const int steps = (tiles + 1) / 2;
       const bool odd = tiles % 2 != 0;  // the last step's second tile holds no keys
@@ -486,9 +550,8 @@ struct PrefixF32 {
     }
     if (!active) return;
     l += __shfl_xor(l, 32);
-    const int r = row0 + col;
-    if (r >= a.rows) return;
-    const int64_t slot = ((static_cast<int64_t>(piece.group) * p.cache.kv_heads + piece.kv) * a.splits + piece.split) * a.row_slots + r;
+    if (used.row < 0) return;
+    const int64_t slot = piece.number * a.row_slots + used.row;
     float* to = a.sums + slot * D;
 #pragma unroll
     for (int dt = 0; dt < DT; ++dt)

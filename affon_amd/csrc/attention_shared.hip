@@ -37,11 +37,16 @@ __global__ __launch_bounds__(256) void join_parts_kernel(Parts parts, int shares
     const uint32_t prefix = takes_prefix(parts, p.batch, b, group) ? prefix_tokens(parts, p.batch, group) : 0u;
     if (prefix > 0) {
       const Args a = parts.prefix();
-      const uint32_t chunk = piece_of(prefix, a.splits, a.chunk), used = (prefix + chunk - 1) / chunk;
+      const uint32_t chunk = piece_of(prefix, a.splits, a.chunk);
+      uint32_t used = (prefix + chunk - 1) / chunk;
+      int64_t first = (static_cast<int64_t>(group) * p.cache.kv_heads + kv) * a.splits;
+      if (a.plan != nullptr) {
+        const uint2 plan = a.plan[group];
+        used = plan.y;
+        first = plan.x + static_cast<int64_t>(kv) * used;
+      }
       const int64_t r = (row - static_cast<int64_t>(group) * parts.group_rows) * parts.group + g;
-      if (share < static_cast<int>(used))
-        v = joined_sums<false>(a, (static_cast<int64_t>(group) * p.cache.kv_heads + kv) * a.splits * a.row_slots + r, d, D, share,
-                               used, shares, &top, &sum);
+      if (share < static_cast<int>(used)) v = joined_sums<false>(a, first * a.row_slots + r, d, D, share, used, shares, &top, &sum);
     }
     const uint32_t chunk = piece_of(n - prefix, parts.splits, parts.chunk), used = max(1u, (n - prefix + chunk - 1) / chunk);
     const uint32_t own_share = static_cast<uint32_t>(shares - 1 - share);  // the prefix's last ones have fewer pieces
@@ -120,25 +125,30 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   const int64_t units = static_cast<int64_t>(p.batch.sequences) * p.cache.kv_heads;
   const int64_t prefix_units = static_cast<int64_t>(groups) * p.cache.kv_heads;
   const int64_t most = std::max<int64_t>(1, p.batch.capacity / unit);
-  parts.chunk = parts.prefix_chunk = static_cast<uint32_t>(unit);
+  parts.chunk = static_cast<uint32_t>(unit);
+  parts.prefix_chunk = static_cast<uint32_t>(tiles > 0 ? 32 : unit);  // a step of the tiles' kernels
   parts.splits = static_cast<int>(splits_for(kRound, units * parts.row_groups, most));
   parts.prefix_splits = static_cast<int>(splits_for(tiles > 0 ? kRound / 2 : kRound, prefix_units * parts.prefix_row_groups, most));
   const int64_t own_blocks = blocks_of(units, parts.splits, parts.row_groups);
-  const int64_t prefix_blocks = blocks_of(prefix_units, parts.prefix_splits, parts.prefix_row_groups);
+  // Cut over all groups, they may have a piece more each.
+  const int more = tiles > 0 && groups > 1 ? 1 : 0;
+  const int64_t prefix_blocks = blocks_of(prefix_units, parts.prefix_splits + more, parts.prefix_row_groups);
   if (own_blocks + prefix_blocks > kMaxBlocks) return hipErrorInvalidValue;
 
   auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   const size_t own_slots = static_cast<size_t>(units) * parts.splits * parts.row_slots;
-  const size_t prefix_slots = static_cast<size_t>(prefix_units) * parts.prefix_splits * parts.prefix_slots;
+  const size_t prefix_slots = static_cast<size_t>(prefix_units) * (parts.prefix_splits + more) * parts.prefix_slots;
   const size_t sums = whole(own_slots * D * sizeof(float)), stats = whole(own_slots * sizeof(float2));
-  const size_t prefix_sums = whole(prefix_slots * D * sizeof(float)), prefix_stats = prefix_slots * sizeof(float2);
-  auto* scratch = static_cast<uint8_t*>(l.scratch(sums + stats + prefix_sums + prefix_stats));
+  const size_t prefix_sums = whole(prefix_slots * D * sizeof(float)), prefix_stats = whole(prefix_slots * sizeof(float2));
+  const size_t plan = tiles > 0 ? groups * sizeof(uint2) : 0;
+  auto* scratch = static_cast<uint8_t*>(l.scratch(sums + stats + prefix_sums + prefix_stats + plan));
   // A captured stream whose workspace cannot grow: every sequence by itself.
   if (scratch == nullptr) return attention_launch(p, l);
   parts.sums = reinterpret_cast<float*>(scratch);
   parts.stats = reinterpret_cast<float*>(scratch + sums);
   parts.prefix_sums = reinterpret_cast<float*>(scratch + sums + stats);
   parts.prefix_stats = reinterpret_cast<float*>(scratch + sums + stats + prefix_sums);
+  if (tiles > 0) parts.prefix_plan = reinterpret_cast<uint2*>(scratch + sums + stats + prefix_sums + prefix_stats);
 
   auto launch = half ? launch_parts_bf16 : launch_parts_f32;
   auto run = [&](Shape shape, int64_t of_prefix, int64_t of_own) {

@@ -59,44 +59,51 @@ struct Context {
   }
 };
 
-// All contexts, cut into pieces of about the same number of keys by the lengths
-// that are there: workgroups that are numbered through them have equal work,
-// whatever the lengths and the table's width, and one round of them pays for its
-// start (lengths, table, queries: 5 us) once. For whole waves.
+// All contexts with rows in use, cut into pieces of about the same number of keys
+// by the lengths that are there: workgroups that are numbered through them have equal
+// work, whatever the lengths and the table's width, and one round of them pays for its
+// start (lengths, table, queries: 5 us) once. There are `pieces` of them for each key
+// head at most where sequences have two on average or more (and are no more than 64),
+// and never more than `pieces` + the sequences. For whole waves.
 constexpr uint32_t kPieceUnit = 128;
 struct Pieces {
   const DraftBatch& batch;
   uint32_t chunk;  // keys of a piece
-  // A whole wave's sum of numbers below 2^56.
-  static __device__ __forceinline__ uint64_t sum_of(uint64_t v) {
-    const uint32_t low = scanned(static_cast<uint32_t>(v) & 0xffffffu), high = scanned(static_cast<uint32_t>(v >> 24));
-    return (static_cast<uint64_t>(lane_of(high, 63)) << 24) + lane_of(low, 63);
-  }
+  uint32_t mine;   // keys of the sequence of this lane, among the first 64
   __device__ __forceinline__ uint32_t keys_of(int b) const {
     const uint32_t count = drafted(batch, b);
     return count == 0 ? 0u : min(committed(batch, b) + count, batch.capacity);
   }
+  __device__ __forceinline__ uint32_t keys_at(int base) const {
+    const int b = base + static_cast<int>(threadIdx.x & 63);
+    return base == 0 ? mine : b < batch.sequences ? keys_of(b) : 0u;
+  }
+  __device__ __forceinline__ uint32_t pieces_of(uint32_t keys) const { return (keys + chunk - 1) / chunk; }
   __device__ __forceinline__ Pieces(const DraftBatch& batch, int pieces) : batch(batch) {
-    uint64_t all = 0;
-    for (int b = threadIdx.x & 63; b < batch.sequences; b += 64) all += keys_of(b);
-    all = sum_of(all);
-    const uint64_t each = min(all / static_cast<uint32_t>(pieces) + 1, static_cast<uint64_t>(batch.capacity));
-    chunk = __builtin_amdgcn_readfirstlane(
-        static_cast<int>((static_cast<uint32_t>(each) + kPieceUnit - 1) / kPieceUnit * kPieceUnit));
+    const int lane = threadIdx.x & 63;
+    mine = lane < batch.sequences ? keys_of(lane) : 0u;
+    uint64_t all = mine;
+    for (int b = lane + 64; b < batch.sequences; b += 64) all += keys_of(b);
+    all = wave_sum(all) + (pieces - 1);
+    const uint32_t by = static_cast<uint32_t>(pieces);
+    const uint32_t each = all >> 32 != 0 ? static_cast<uint32_t>(min(all / by, static_cast<uint64_t>(batch.capacity)))
+                                         : min(static_cast<uint32_t>(all) / by, batch.capacity);
+    auto whole = [](uint32_t n) { return max(kPieceUnit, (n + kPieceUnit - 1) / kPieceUnit * kPieceUnit); };
+    chunk = __builtin_amdgcn_readfirstlane(static_cast<int>(whole(each)));
+    // A round of workgroups that a few more follow takes as long as two: longer pieces, until they fit.
+    if (batch.sequences <= 64 && pieces >= 2 * batch.sequences)
+      for (int i = 0; i < 16 && lane_of(scanned(pieces_of(mine)), 63) > by; ++i) chunk += whole(chunk / 16);
   }
   // Piece `id` of [sequence][key head][piece of the sequence]; false: there are fewer.
   __device__ __forceinline__ bool find(int64_t id, int kv_heads, int* b, int* kv, uint32_t* piece) const {
-    const int lane = threadIdx.x & 63;
     int64_t before = 0;
     for (int base = 0; base < batch.sequences; base += 64) {
-      const uint32_t own = base + lane < batch.sequences ? (keys_of(base + lane) + chunk - 1) / chunk : 0u;
-      const uint32_t sum = scanned(own);
+      const uint32_t own = pieces_of(keys_at(base)), sum = scanned(own);
       const uint64_t past = __ballot((before + sum) * kv_heads > id);
       if (past != 0) {
         const int at = __builtin_ctzll(past);
         const uint32_t pieces = lane_of(own, at);
-        const int64_t start = before + lane_of(sum, at) - pieces;
-        const uint32_t rest = static_cast<uint32_t>(id - start * kv_heads);
+        const uint32_t rest = static_cast<uint32_t>(id - (before + lane_of(sum, at) - pieces) * kv_heads);
         *b = base + at;
         *kv = static_cast<int>(rest / pieces);
         *piece = rest - static_cast<uint32_t>(*kv) * pieces;
@@ -106,12 +113,12 @@ struct Pieces {
     }
     return false;
   }
-  // Number of the first piece of a sequence's key head.
-  __device__ __forceinline__ int64_t first_of(int b, int kv, int kv_heads) const {
+  // Number of the first piece of a sequence's key head; `pieces`: of each of its key heads.
+  __device__ __forceinline__ int64_t first_of(int b, int kv, int kv_heads, uint32_t pieces) const {
     uint64_t before = 0;
-    for (int i = threadIdx.x & 63; i < b; i += 64) before += (keys_of(i) + chunk - 1) / chunk;
-    before = sum_of(before);
-    return static_cast<int64_t>(before) * kv_heads + static_cast<int64_t>(kv) * ((keys_of(b) + chunk - 1) / chunk);
+    for (int base = 0; base < b; base += 64)
+      before += base + static_cast<int>(threadIdx.x & 63) < b ? pieces_of(keys_at(base)) : 0u;
+    return static_cast<int64_t>(wave_sum(before)) * kv_heads + static_cast<int64_t>(kv) * pieces;
   }
 };
 
@@ -476,8 +483,8 @@ __global__ __launch_bounds__(256) void ready_kernel(WeightArgs a, int64_t packs)
   const Context c(a.p, b);
   if (c.n == 0 || c.count == 0) return;
   const Pieces pieces(a.p.batch, a.pieces);
-  const int64_t first = pieces.first_of(b, kv, a.p.cache.kv_heads);
-  const uint32_t used = (c.n + pieces.chunk - 1) / pieces.chunk;
+  const uint32_t used = pieces.pieces_of(c.n);
+  const int64_t first = pieces.first_of(b, kv, a.p.cache.kv_heads, used);
   if (r >= a.row_slots) return;
   if (r >= a.rows) {
     a.ready[static_cast<int64_t>(unit) * a.row_slots + r] = INFINITY;
@@ -509,8 +516,8 @@ __global__ __launch_bounds__(256) void sum_kernel(WeightArgs a) {
   const Context c(p, unit / p.cache.kv_heads);
   if (c.count == 0 || static_cast<uint32_t>(block) * 1024 >= c.n) return;
   const Pieces pieces(p.batch, a.pieces);
-  const int64_t first = pieces.first_of(unit / p.cache.kv_heads, unit % p.cache.kv_heads, p.cache.kv_heads);
-  const uint32_t used = (c.n + pieces.chunk - 1) / pieces.chunk;
+  const uint32_t used = pieces.pieces_of(c.n);
+  const int64_t first = pieces.first_of(unit / p.cache.kv_heads, unit % p.cache.kv_heads, p.cache.kv_heads, used);
   const int r = threadIdx.x / 16;
   float m = kLowest, l = 0.0f;
   if (r < a.rows) {
@@ -739,12 +746,12 @@ void launch_stats(const WeightArgs& a, dim3 grid, hipStream_t stream) {
 }
 
 constexpr int64_t kMaxInt = 2147483647;
-// Workgroups of a round: what of each kernel runs at once, five, two and three to
+// Workgroups of a round: what of each kernel runs at once, four, two and three to
 // a CU. Stats with kept scores, 32 sequences of one token over up to 4096: 512
-// 55.7 us, 1024 51.6, 1280 49.5, 2048 49.4, and 1280 leaves fewer pieces to join.
+// 55.7 us, 1024 47.6, 1280 49.5.
 // More rows, 32 tokens of four sequences over up to 16384: stats and gathering
 // in rounds of 512 and 768 80.8 us, 256 and 512 96.9, 1024 and 1536 93.8.
-constexpr int64_t kKeepRound = 1280, kStatsRound = 512, kGatherRound = 768;
+constexpr int64_t kKeepRound = 1024, kStatsRound = 512, kGatherRound = 768;
 
 template <typename T, int KS>
 hipError_t launch(const WeightArgs& a, int64_t units, hipStream_t stream) {
@@ -801,8 +808,8 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   const int64_t capacity = p.batch.capacity;
   // One round of workgroups, or two for every key head and sequence.
   auto pieces_for = [&](int64_t round, int64_t groups) {
-    const int64_t least = p.batch.sequences;
-    return static_cast<int>(std::min<int64_t>(std::max(round / (p.cache.kv_heads * groups) - least, least), kMaxInt / 2));
+    const int64_t least = 2 * static_cast<int64_t>(p.batch.sequences);
+    return static_cast<int>(std::min<int64_t>(std::max(round / (p.cache.kv_heads * groups), least), kMaxInt / 2));
   };
   a.pieces = pieces_for(a.rows <= 16 ? kKeepRound : kStatsRound, a.row_groups);
   a.gather_pieces = pieces_for(kGatherRound, 1);

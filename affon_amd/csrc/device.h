@@ -51,5 +51,10 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v) {
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
+// A whole wave's sum of numbers below 2^56.
+__device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
+  const uint32_t low = scanned(static_cast<uint32_t>(v) & 0xffffffu), high = scanned(static_cast<uint32_t>(v >> 24));
+  return (static_cast<uint64_t>(lane_of(high, 63)) << 24) + lane_of(low, 63);
+}
 
 }  // namespace affon
