@@ -6,8 +6,9 @@ tree: speculative decoding).
 * ``PagedCache`` holds the keys and values of one or several layers in pages;
 * ``DraftBatch`` says where a step's tokens lie: the page table, how many
   tokens of each sequence are committed, and how many drafted ones are in use;
-* ``cache_append`` rotates queries and keys by their positions and appends keys
-  and values to a layer;
+* ``cache_append`` norms the heads of queries and keys where a model does, rotates
+  them by their positions (of one axis, or ``rotary_axes``) and appends keys and
+  values to a layer;
 * ``tree_attention`` attends over the committed tokens and, by a mask, the drafted
   ones;
 * ``shared_attention`` does so where sequences share a prefix, read once for all;

@@ -1,6 +1,11 @@
 // The append with norms of the query and key heads, and with positions of
 // several axes: for each head, n = x / sqrt(mean(x^2) + epsilon) * w, and each
 // pair of n turned by the position of its axis, in one pass.
+//
+// Bound by memory where rows are many: 4096 rows of 80 heads of 128 (f32 to bf16
+// pages) 50.4 us, 5.0 TB/s of 5.2 that a large copy reaches; 2738 rows of 48 heads (bf16,
+// three axes) 15.6 us, 4.4 TB/s, where the instructions around 16 bytes a lane count too.
+// One row of 48 heads 3.7 us, a launch and a chain of three loads.
 
 #include <algorithm>
 
@@ -228,7 +233,8 @@ __global__ __launch_bounds__(320) void append_norm_kernel(AppendNormProblem q, i
   }
 }
 
-// As the plain append: eight values at a time for many rows.
+// As the plain append: eight values at a time for many rows (four: 4096 rows of 80
+// heads 58 us instead of 51; few rows then have too few lanes with loads on their way).
 constexpr int64_t kManyRows = 64;
 
 template <typename X, typename C, int V>

@@ -396,12 +396,15 @@ struct PrefixKernel {
 };
 
 // The same in f32, for heads of D = 64 to 128: S^T, and then O^T, by 32x32x2
-// products, of two dims or keys a time: the dims 8 j + 4 (lane / 32) + e and the
+// products, of two dims or keys at a time: the dims 8 j + 4 (lane / 32) + e and the
 // keys of a lane's score, so that both operands are read in their order and P^T
 // stays where it is. Bound by the matrix cores, whose f32 products take as many
 // cycles for a 16th of bf16's work: D + 32 ceil(D / 32) halves of 64 cycles
 // for 32 rows and keys, beside which all else is small (about 450 of exponentials and
-// sums), so a step's phases follow each other and the waves of a SIMD fill each other's gaps.
+// sums), so a step's phases follow each other and the waves of a SIMD fill each other's
+// gaps. 4 prompts of up to 6000 tokens, 4 key heads of 80, up to 200 rows of which some 120
+// are in use: 69 us, and 89 with the general kernel; rows fill whole tiles of 32, and
+// a SIMD with two of them holds up those with one.
 template <int WIDTH, int W>
 struct PrefixF32 {
   static constexpr int D = WIDTH, kRowBytes = 4 * D, kThreads = 64 * W, DT = (D + 31) / 32;

@@ -13,7 +13,8 @@ namespace {
 
 // Joins the pieces of the prefix and the own ones, in their order: head_dim / 4
 // threads for each of `shares` shares of the pieces of a row and head, which then
-// meet in LDS; several rows and heads to a workgroup.
+// meet in LDS; several rows and heads to a workgroup. Bound by the results it reads: 64
+// sequences of 64 heads of 128 in 17 pieces, 36 MB, 11 us.
 template <typename T>
 __global__ __launch_bounds__(256) void join_parts_kernel(Parts parts, int shares) {
   __shared__ __attribute__((aligned(16))) f32x4_t part[256];
