@@ -43,7 +43,8 @@ struct PrefixPiece {
     number = id / a.row_groups * 8 + (blockIdx.x & 7);
     auto tokens = [&](int base) { return base + lane < groups ? prefix_tokens(a, batch, base + lane) : 0u; };
     const uint32_t mine = tokens(0);
-    uint32_t chunk = batch.capacity + a.chunk;
+    uint32_t chunk = max(batch.capacity, 1u);
+    auto pieces_of = [&](uint32_t n) { return n == 0 ? 0u : (n - 1) / chunk + 1; };  // (n + chunk may pass 32 bits)
     if (a.splits > 1) {
       uint64_t all = mine;
       for (int base = 64; base < groups; base += 64) all += tokens(base);
@@ -54,12 +55,12 @@ struct PrefixPiece {
       chunk = each == 0 ? a.chunk : whole(each - (all == static_cast<uint64_t>(each) * pieces ? 1 : 0));
       // A few workgroups more than a round take as long as another: longer pieces, until they fit.
       if (groups <= 64)
-        for (int i = 0; i < 16 && lane_of(scanned((mine + chunk - 1) / chunk), 63) > pieces; ++i) chunk += whole(chunk / 16);
+        for (int i = 0; i < 16 && lane_of(scanned(pieces_of(mine)), 63) > pieces; ++i) chunk += whole(chunk / 16);
     }
     chunk = __builtin_amdgcn_readfirstlane(static_cast<int>(chunk));
     int64_t before = 0;
     for (int base = 0; base < groups; base += 64) {
-      const uint32_t held = base == 0 ? mine : tokens(base), own = (held + chunk - 1) / chunk, sum = scanned(own);
+      const uint32_t held = base == 0 ? mine : tokens(base), own = pieces_of(held), sum = scanned(own);
       const uint64_t past = __ballot((before + sum) * kv_heads > number);
       if (past != 0) {
         const int at = __builtin_ctzll(past);

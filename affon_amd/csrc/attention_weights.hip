@@ -78,7 +78,7 @@ struct Pieces {
     const int b = base + static_cast<int>(threadIdx.x & 63);
     return base == 0 ? mine : b < batch.sequences ? keys_of(b) : 0u;
   }
-  __device__ __forceinline__ uint32_t pieces_of(uint32_t keys) const { return (keys + chunk - 1) / chunk; }
+  __device__ __forceinline__ uint32_t pieces_of(uint32_t keys) const { return keys == 0 ? 0u : (keys - 1) / chunk + 1; }
   __device__ __forceinline__ Pieces(const DraftBatch& batch, int pieces) : batch(batch) {
     const int lane = threadIdx.x & 63;
     mine = lane < batch.sequences ? keys_of(lane) : 0u;

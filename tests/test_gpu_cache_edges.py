@@ -317,3 +317,28 @@ def test_refusals(session):
             A.cache_append(cache, batch, query, kv, kv, None, rotary, query_norm=other.empty("f32", (8,)))
         with pytest.raises(TypeError, match="same Session"):
             A.cache_evict(cache, batch, weights, two, other.empty("u32", (2,)))
+
+
+@pytest.mark.parametrize("B,groups,dtype", [(17, 1, "bf16"), (34, 2, "f32"), (3, 1, "bf16")])
+def test_tables_of_almost_2_to_the_31_tokens(session, rng, B, groups, dtype):
+    """Prefixes of as many tokens, of which the first page's alone lie anywhere: keys of 0, so
+    that the mean of their values is the result. The values are small integers, whose sums are exact
+    in f32 in any order; the quotient is rounded, and to bf16 again."""
+    page, columns = 65536, 32767
+    cache = A.PagedCache(session, pages=2, page_size=page, kv_heads=1, head_dim=64, dtype=dtype)
+    values = rng.integers(0, 5, (1, 2, 1, page, 64)).astype(np.float32)
+    values[..., :32] = 4
+    half = dtype == "bf16"
+    set_tensor(cache.keys, np.zeros(values.shape, np.uint16 if half else np.float32))
+    set_tensor(cache.values, (values.view(np.uint32) >> 16).astype(np.uint16) if half else values)
+    table = np.full((B, columns), 0xFFFFFFFF, np.uint32)
+    table[:, 0] = 1
+    tokens = page * columns
+    lengths = np.full(B, tokens - 5000, np.uint32)
+    shared = np.full(groups, tokens - 70000, np.uint32)
+    shared[1:] = 0
+    batch = A.DraftBatch(upload(session, table, "u32"), upload(session, lengths, "u32"), 1)
+    query = session.tensor(rng.standard_normal((B, 64)), dtype)
+    got = A.shared_attention(cache, batch, query, upload(session, shared, "u32")).numpy()
+    want = np.broadcast_to(values[0, 1, 0].mean(0, dtype=np.float64), got.shape)
+    np.testing.assert_allclose(got, want, rtol=2.0 ** -8 + 2.0 ** -20 if half else 2.0 ** -20)
