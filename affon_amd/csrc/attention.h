@@ -909,7 +909,7 @@ void launch_f32(const Args& a, Shape shape, dim3 grid, hipStream_t stream);
 void launch_parts_bf16(const Parts& parts, Shape shape, dim3 grid, hipStream_t stream);
 void launch_parts_f32(const Parts& parts, Shape shape, dim3 grid, hipStream_t stream);
 Shape shape_for(int rows, int head_dim);
-// Heads of 64 or 128 in bf16, workgroups of 4 or 8 waves of 32 rows.
+// Heads of 64 or 128 in bf16, workgroups of 4 or 8 waves of 32 rows; of 64, 80, 96 or 128 in f32, of 8.
 void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream);
 
 template <typename T, int DT, bool EXACT, int RT, int WR, int KEYS, typename Launched>

@@ -404,10 +404,11 @@ struct PrefixKernel {
 // for 32 rows and keys, beside which all else is small (about 450 of exponentials and
 // sums), so a step's phases follow each other and the waves of a SIMD fill each other's
 // gaps. 4 prompts of up to 6000 tokens, 4 key heads of 80, up to 200 rows of which some 120
-// are in use: 69 us, and 89 with the general kernel; rows fill whole tiles of 32, and
-// a SIMD with two of them holds up those with one.
-template <int WIDTH, int W>
+// are in use: 69 us (the call 92, and 110 with the general kernel, which takes them all);
+// rows fill whole tiles of 32, and a SIMD with two of them holds up those with one.
+template <int WIDTH>
 struct PrefixF32 {
+  static constexpr int W = 8;
   static constexpr int D = WIDTH, kRowBytes = 4 * D, kThreads = 64 * W, DT = (D + 31) / 32;
   static constexpr int kTile = 16 * kRowBytes, kPieces = kTile / 1024;  // of 16 keys, or values
   static constexpr int kStage = 4 * kTile;                              // keys, then values, of a step

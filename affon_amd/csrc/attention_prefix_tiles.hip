@@ -9,14 +9,6 @@ void launch_prefix(const Args& a, dim3 grid, hipStream_t stream) {
   hipLaunchKernelGGL(prefix_kernel<K>, grid, dim3(K::kThreads), 0, stream, a);
 }
 
-template <int D>
-void launch_f32(const Args& a, int waves, dim3 grid, hipStream_t stream) {
-  if (waves == 8)
-    launch_prefix<PrefixF32<D, 8>>(a, grid, stream);
-  else
-    launch_prefix<PrefixF32<D, 4>>(a, grid, stream);
-}
-
 void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream) {
   const int D = a.p.cache.head_dim;
   if (a.p.cache.dtype == AFFON_ROCM_BF16) {
@@ -27,10 +19,10 @@ void launch_prefix_tiles(const Args& a, int waves, dim3 grid, hipStream_t stream
     return;
   }
   switch (D) {
-    case 64: return launch_f32<64>(a, waves, grid, stream);
-    case 80: return launch_f32<80>(a, waves, grid, stream);
-    case 96: return launch_f32<96>(a, waves, grid, stream);
-    default: return launch_f32<128>(a, waves, grid, stream);
+    case 64: return launch_prefix<PrefixF32<64>>(a, grid, stream);
+    case 80: return launch_prefix<PrefixF32<80>>(a, grid, stream);
+    case 96: return launch_prefix<PrefixF32<96>>(a, grid, stream);
+    default: return launch_prefix<PrefixF32<128>>(a, grid, stream);
   }
 }
 

@@ -118,7 +118,11 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   // and 32.4, 58.3 and 52.5. 4 and 8 waves: 256 rows 29.1 and 37.8, 36.8 and
   // 41.6, 73.0 and 70.0; 192 rows 31.1 and 33.8, 34.9 and 38.6, 70.4 and 61.0.
   const bool takes = half ? D == 64 || D == 128 : D == 64 || D == 80 || D == 96 || D == 128;
-  const int tiles = !takes || prefix_rows <= 16 ? 0 : prefix_rows > 128 ? 8 : 4;
+  // f32, whose products bound both, from 129 rows on: one group's 128 rows of 80 after
+  // 2048 tokens 44.7 us by the general one and 47.4, 32 rows of 64 after 16000 36.6 and
+  // 41.7; 200 rows of 80 after 16000 151.3 and 144.5, of 64 114.3 and 111.3, and
+  // where a third of the rows is not in use 102 and 92.
+  const int tiles = !takes || prefix_rows <= (half ? 16 : 128) ? 0 : prefix_rows > 128 ? 8 : 4;
   const Shape own_shape = shape_for(parts.rows, D), prefix_shape = shape_for(parts.prefix_rows, D);
   const int64_t at_once = tiles > 0 ? 32 * tiles : prefix_shape.rows();
   parts.row_groups = (parts.rows + own_shape.rows() - 1) / own_shape.rows();
