@@ -171,16 +171,14 @@ def rotary_axes(sections, *, interleaved: bool = False) -> RotaryAxes:
     return RotaryAxes(a for turn in range(max(sections)) for a, n in enumerate(sections) if turn < n)
 
 
-_ONE_AXIS = (ctypes.c_uint8 * 128)()
-
-
 def _norm_weight(name: str, t: Tensor | None, heads: int, dim: int) -> tuple[int | None, int, int]:
     """Address, elements from head to head and type of a norm's weights."""
     if t is None:
         return None, 0, 0
-    if t.dtype not in ("f32", "bf16") or t.shape not in ((dim,), (heads * dim,)) or not t.is_contiguous():
+    stride = 0 if t.shape == (dim,) else dim if t.shape == (heads * dim,) else None
+    if stride is None or t.dtype not in ("f32", "bf16") or not t.is_contiguous():
         raise TypeError(f"cache_append {name} must be a contiguous f32/bf16 [{dim}] or [{heads * dim}] tensor")
-    return t.data_ptr, dim if t.shape[0] > dim else 0, _NATIVE_DTYPE[t.dtype]
+    return t.data_ptr, stride, _NATIVE_DTYPE[t.dtype]
 
 
 def _query_rows(op: str, cache: PagedCache, batch: DraftBatch, query: Tensor, dtypes: tuple[str, ...]) -> None:
@@ -252,7 +250,7 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
         q_data, q_stride, q_dtype = _norm_weight("query_norm", query_norm, query.shape[1] // cache.head_dim, cache.head_dim)
         k_data, k_stride, k_dtype = _norm_weight("key_norm", key_norm, cache.kv_heads, cache.head_dim)
         norm = _native.HeadNorm(q_data, k_data, q_stride, k_stride, q_dtype, k_dtype, epsilon,
-                                1 if axes is None else axes.count, _ONE_AXIS if axes is None else axes._packed)
+                                *((1,) if axes is None else (axes.count, axes._packed)))  # axis 0 of every pair
         status = native.affon_rocm_cache_append_normed(cache.session._handle, cache_struct, batch_struct, desc, norm)
     if status:
         def explain():

@@ -4,8 +4,8 @@ import numpy as np
 import pytest
 
 import affon_amd as A
-from tests.drafts import NO_PAGE, stored, upload
-from tests.test_gpu_shared_attention import copies, run
+from tests.drafts import NO_PAGE, Step, stored, upload
+from tests.test_gpu_shared_attention import copies, run, share
 
 pytestmark = pytest.mark.gpu
 
@@ -71,3 +71,39 @@ def test_odd_strides_in_f32(session, rng):
     wide[:, 1:-2] = step.query
     query = A.slice(upload(session, wide, "f32"), [{}, {"start": 1, "stop": 8 * 96 + 1}])
     step.check(A.shared_attention(step.cache, step.batch, query, upload(session, np.array([320], np.uint32), "u32")).storage())
+
+
+@pytest.mark.parametrize("dtype,dim", [("bf16", 64), ("bf16", 128), ("f32", 64), ("f32", 80)])
+@pytest.mark.parametrize("groups,per,T,heads,kv,shared", [
+    (1, 70, 3, 4, 2, (400,)), (2, 70, 2, 4, 1, (800, 96)), (3, 9, 5, 8, 1, (64, 1500, 640)), (1, 130, 2, 2, 1, (300,)),
+    (2, 40, 4, 2, 2, (0, 333))])
+def test_rows_in_use(session, rng, dtype, dim, groups, per, T, heads, kv, shared):
+    """Drafts of different lengths, none among them, and sequences that do not hold their group's prefix."""
+    B = groups * per
+    counts = rng.integers(0, T + 1, B)
+    counts[rng.integers(0, B, 3)] = T
+    if per > 64:
+        counts[:64] = T  # a whole wave of sequences with all their rows, and the rest without
+    lengths = np.array([shared[b // per] + (11 * b) % 37 for b in range(B)])
+    first = np.arange(groups) * per
+    for b in rng.permutation(B)[:B // 6]:
+        if b not in first and shared[b // per] > 16:
+            lengths[b] = int(rng.integers(0, shared[b // per]))
+    step = share(Step(rng, B=B, T=T, heads=heads, kv=kv, dim=dim, lengths=lengths, counts=counts, dtype=dtype, spread=2.0),
+                 groups, shared)
+    step.query.reshape(B, T, -1)[np.arange(T) >= counts[:, None]] = np.nan if dtype == "f32" else 0x7FC0
+    step.device(session)
+    got = run(session, step, shared)
+    unused = (np.arange(T) >= counts[:, None]).reshape(-1)
+    assert not got[unused].any()
+    step.check(got, rows=~unused)
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "f32"])
+def test_the_first_sequence_does_not_hold_it(session, rng, dtype):
+    """Pages are read from the first sequence that does; a group that none does is left to its sequences."""
+    step = share(Step(rng, B=60, T=5, heads=2, kv=1, lengths=[200 + b % 7 for b in range(60)], dtype=dtype), 2, [192, 192])
+    step.lengths[:5] = 3
+    step.lengths[30:] = 100
+    step.device(session)
+    step.check(run(session, step, [192, 192]))
