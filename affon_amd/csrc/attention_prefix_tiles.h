@@ -28,7 +28,7 @@ typedef float f32x16_t __attribute__((ext_vector_type(16)));
 // The keys of a workgroup: a piece of a group's prefix, of one key head; begin >=
 // end: none. All groups' prefixes are cut alike, into `splits` pieces a group on
 // average, so that a long one holds no workgroup longer than the others. (Four of
-// up to 6000 tokens, 8 sequences each, f32: 94 us, each cut into 16 101.) In the order
+// up to 6000 tokens, 8 sequences each, f32: 92 us, each cut into 16 101.) In the order
 // [group][key head][piece].
 struct PrefixPiece {
   int row_group, kv, group;
