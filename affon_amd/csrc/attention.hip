@@ -7,6 +7,7 @@
 #include <cmath>
 
 #include "attention.h"
+#include "join_thread.h"
 
 namespace affon {
 namespace attention {
@@ -16,16 +17,16 @@ namespace {
 // threads for each of `shares` shares of the splits of a row and head, which
 // then meet in LDS; several rows and heads to a workgroup.
 template <typename T>
-__global__ __launch_bounds__(256) void join_kernel(Args a, int shares) {
-  __shared__ __attribute__((aligned(16))) f32x4_t part[256];
-  __shared__ float2 stats[256];
+__global__ __launch_bounds__(kJoinThreads) void join_kernel(Args a, int shares) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[kJoinThreads];
+  __shared__ float2 stats[kJoinThreads];
   const AttentionProblem& p = a.p;
-  const int D = p.cache.head_dim, pieces = D / 4, own = pieces * shares, per = 256 / own;
-  const int local = threadIdx.x / own, share = (threadIdx.x - local * own) / pieces;
-  const int piece = threadIdx.x % pieces, d = 4 * piece;
-  const int64_t slot = static_cast<int64_t>(blockIdx.x) * per + local;  // of [row][head]
+  const int D = p.cache.head_dim, pieces = D / 4;
+  const JoinThread thread(threadIdx.x, pieces, shares);
+  const int share = thread.share, d = 4 * thread.piece;
+  const int64_t slot = static_cast<int64_t>(blockIdx.x) * thread.per + thread.local;  // of [row][head]
   const int64_t row = slot / p.heads;
-  const bool there = local < per && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
+  const bool there = thread.holds() && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   const int head = static_cast<int>(slot - row * p.heads), kv = head / a.group;
   const int b = there ? static_cast<int>(row / p.batch.rows) : 0;
   const int t = static_cast<int>(row - static_cast<int64_t>(b) * p.batch.rows);
@@ -44,7 +45,7 @@ __global__ __launch_bounds__(256) void join_kernel(Args a, int shares) {
     part[threadIdx.x] = v;
     stats[threadIdx.x] = float2{top, sum};
     __syncthreads();
-    if (share != 0 || local >= per) return;
+    if (!thread.adds_up()) return;
     for (int s = 1; s < shares; ++s) top = fmaxf(top, stats[threadIdx.x + s * pieces].x);
     v = f32x4_t{0, 0, 0, 0};
     sum = 0.0f;
@@ -159,15 +160,15 @@ hipError_t attention_launch(const AttentionProblem& p, const Launch& l) {
   if (e != hipSuccess || a.splits == 1 || a.tickets != nullptr) return e;
   // A share takes the eight splits that a thread has in flight.
   const int pieces = p.cache.head_dim / 4;
-  const int shares = few ? 1 : std::min((a.splits + 7) / 8, 256 / pieces);
-  const int64_t per = 256 / (pieces * shares);
+  const int shares = few ? 1 : std::min((a.splits + 7) / 8, kJoinThreads / pieces);
+  const int64_t per = kJoinThreads / (pieces * shares);
   const int64_t join_blocks = (static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads + per - 1) / per;
   if (join_blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 join_grid(static_cast<unsigned>(join_blocks));
   if (half)
-    hipLaunchKernelGGL(join_kernel<BF16>, join_grid, dim3(256), 0, l.stream, a, shares);
+    hipLaunchKernelGGL(join_kernel<BF16>, join_grid, dim3(kJoinThreads), 0, l.stream, a, shares);
   else
-    hipLaunchKernelGGL(join_kernel<F32>, join_grid, dim3(256), 0, l.stream, a, shares);
+    hipLaunchKernelGGL(join_kernel<F32>, join_grid, dim3(kJoinThreads), 0, l.stream, a, shares);
   return hipGetLastError();
 }
 

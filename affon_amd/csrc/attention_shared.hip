@@ -6,6 +6,7 @@
 #include <cmath>
 
 #include "attention.h"
+#include "join_thread.h"
 
 namespace affon {
 namespace attention {
@@ -16,16 +17,16 @@ namespace {
 // meet in LDS; several rows and heads to a workgroup. Bound by the results it reads: 64
 // sequences of 64 heads of 128 in 17 pieces, 36 MB, 11 us.
 template <typename T>
-__global__ __launch_bounds__(256) void join_parts_kernel(Parts parts, int shares) {
-  __shared__ __attribute__((aligned(16))) f32x4_t part[256];
-  __shared__ float2 stats[256];
+__global__ __launch_bounds__(kJoinThreads) void join_parts_kernel(Parts parts, int shares) {
+  __shared__ __attribute__((aligned(16))) f32x4_t part[kJoinThreads];
+  __shared__ float2 stats[kJoinThreads];
   const AttentionProblem& p = parts.p;
-  const int D = p.cache.head_dim, pieces = D / 4, each = pieces * shares, per = 256 / each;
-  const int local = threadIdx.x / each, share = (threadIdx.x - local * each) / pieces;
-  const int d = 4 * static_cast<int>(threadIdx.x % pieces);
-  const int64_t slot = static_cast<int64_t>(blockIdx.x) * per + local;  // of [row][head]
+  const int D = p.cache.head_dim, pieces = D / 4;
+  const JoinThread thread(threadIdx.x, pieces, shares);
+  const int share = thread.share, d = 4 * thread.piece;
+  const int64_t slot = static_cast<int64_t>(blockIdx.x) * thread.per + thread.local;  // of [row][head]
   const int64_t row = slot / p.heads;
-  const bool there = local < per && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
+  const bool there = thread.holds() && row < static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   const int head = static_cast<int>(slot - row * p.heads), kv = head / parts.group, g = head - kv * parts.group;
   const int b = there ? static_cast<int>(row / p.batch.rows) : 0;
   const int t = static_cast<int>(row - static_cast<int64_t>(b) * p.batch.rows);
@@ -66,7 +67,7 @@ __global__ __launch_bounds__(256) void join_parts_kernel(Parts parts, int shares
     part[threadIdx.x] = v;
     stats[threadIdx.x] = float2{top, sum};
     __syncthreads();
-    if (share != 0) return;
+    if (!thread.adds_up()) return;
     for (int s = 1; s < shares; ++s) top = fmaxf(top, stats[threadIdx.x + s * pieces].x);
     v = f32x4_t{0, 0, 0, 0};
     sum = 0.0f;
@@ -179,15 +180,15 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   // there are not enough workgroups.
   const int64_t results = static_cast<int64_t>(p.batch.sequences) * p.batch.rows * p.heads;
   const int threads = D / 4;
-  int shares = std::min((std::max(parts.prefix_splits, parts.splits) + 7) / 8, 256 / threads);
-  while (shares * 2 <= 256 / threads && shares * 2 <= parts.prefix_splits && results * threads * shares < 256 * 512) shares *= 2;
-  const int64_t per = 256 / (threads * shares), blocks = (results + per - 1) / per;
+  int shares = std::min((std::max(parts.prefix_splits, parts.splits) + 7) / 8, kJoinThreads / threads);
+  while (shares * 2 <= kJoinThreads / threads && shares * 2 <= parts.prefix_splits && results * threads * shares < 256 * 512) shares *= 2;
+  const int64_t per = kJoinThreads / (threads * shares), blocks = (results + per - 1) / per;
   if (blocks > kMaxBlocks) return hipErrorInvalidValue;
   const dim3 grid(static_cast<unsigned>(blocks));
   if (half)
-    hipLaunchKernelGGL(join_parts_kernel<BF16>, grid, dim3(256), 0, l.stream, parts, shares);
+    hipLaunchKernelGGL(join_parts_kernel<BF16>, grid, dim3(kJoinThreads), 0, l.stream, parts, shares);
   else
-    hipLaunchKernelGGL(join_parts_kernel<F32>, grid, dim3(256), 0, l.stream, parts, shares);
+    hipLaunchKernelGGL(join_parts_kernel<F32>, grid, dim3(kJoinThreads), 0, l.stream, parts, shares);
   return hipGetLastError();
 }
 
