@@ -19,6 +19,7 @@
 #pragma once
 
 #include "attention.h"
+#include "prefix_cut.h"
 
 namespace affon {
 namespace attention {
@@ -44,18 +45,16 @@ struct PrefixPiece {
     auto tokens = [&](int base) { return base + lane < groups ? prefix_tokens(a, batch, base + lane) : 0u; };
     const uint32_t mine = tokens(0);
     uint32_t chunk = max(batch.capacity, 1u);
-    auto pieces_of = [&](uint32_t n) { return n == 0 ? 0u : (n - 1) / chunk + 1; };  // (n + chunk may pass 32 bits)
+    auto pieces_of = [&](uint32_t n) { return cut_pieces(n, chunk); };
     if (a.splits > 1) {
       uint64_t all = mine;
       for (int base = 64; base < groups; base += 64) all += tokens(base);
       all = wave_sum(all);
-      const uint32_t pieces = static_cast<uint32_t>(a.splits) * groups, high = static_cast<uint32_t>(all >> 32);
-      const uint32_t each = high != 0 ? static_cast<uint32_t>(all / pieces) : static_cast<uint32_t>(all) / pieces;
-      auto whole = [&](uint32_t n) { return (n + a.chunk) / a.chunk * a.chunk; };  // past n, where it is whole itself too
-      chunk = each == 0 ? a.chunk : whole(each - (all == static_cast<uint64_t>(each) * pieces ? 1 : 0));
+      const uint32_t pieces = static_cast<uint32_t>(a.splits) * groups;
+      chunk = cut_chunk(all, pieces, a.chunk);
       // A few workgroups more than a round take as long as another: longer pieces, until they fit.
       if (groups <= 64)
-        for (int i = 0; i < 16 && lane_of(scanned(pieces_of(mine)), 63) > pieces; ++i) chunk += whole(chunk / 16);
+        for (int i = 0; i < 16 && lane_of(scanned(pieces_of(mine)), 63) > pieces; ++i) chunk = cut_longer(chunk, a.chunk);
     }
     chunk = __builtin_amdgcn_readfirstlane(static_cast<int>(chunk));
     int64_t before = 0;

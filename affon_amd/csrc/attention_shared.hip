@@ -7,6 +7,7 @@
 
 #include "attention.h"
 #include "join_thread.h"
+#include "prefix_cut.h"
 
 namespace affon {
 namespace attention {
@@ -136,14 +137,14 @@ hipError_t shared_attention_launch(const AttentionProblem& p, const uint32_t* sh
   parts.splits = static_cast<int>(splits_for(kRound, units * parts.row_groups, most));
   parts.prefix_splits = static_cast<int>(splits_for(tiles > 0 ? kRound / 2 : kRound, prefix_units * parts.prefix_row_groups, most));
   const int64_t own_blocks = blocks_of(units, parts.splits, parts.row_groups);
-  // Cut over all groups, they may have a piece more each.
-  const int more = tiles > 0 && groups > 1 ? 1 : 0;
-  const int64_t prefix_blocks = blocks_of(prefix_units, parts.prefix_splits + more, parts.prefix_row_groups);
+  // Pieces of all prefixes; cut over all groups, some have a few more.
+  const int64_t prefix_pieces = tiles > 0 ? cut_most(groups, parts.prefix_splits) * p.cache.kv_heads : prefix_units * parts.prefix_splits;
+  const int64_t prefix_blocks = blocks_of(prefix_pieces, 1, parts.prefix_row_groups);
   if (own_blocks + prefix_blocks > kMaxBlocks) return hipErrorInvalidValue;
 
   auto whole = [](size_t bytes) { return (bytes + 255) / 256 * 256; };
   const size_t own_slots = static_cast<size_t>(units) * parts.splits * parts.row_slots;
-  const size_t prefix_slots = static_cast<size_t>(prefix_units) * (parts.prefix_splits + more) * parts.prefix_slots;
+  const size_t prefix_slots = static_cast<size_t>(prefix_pieces) * parts.prefix_slots;
   const size_t sums = whole(own_slots * D * sizeof(float)), stats = whole(own_slots * sizeof(float2));
   const size_t prefix_sums = whole(prefix_slots * D * sizeof(float)), prefix_stats = whole(prefix_slots * sizeof(float2));
   const size_t plan = tiles > 0 ? groups * sizeof(uint2) : 0;
