@@ -140,14 +140,15 @@ class QuantizedDecoderBlock:
     @classmethod
     def from_checkpoint(cls, session: Session, path: str, index: int, shape: DecoderShape, *, bits: int,
                         group_size: int, prefix: str = "model.layers",
-                        head_norms: bool = False) -> "QuantizedDecoderBlock":
+                        head_norms: bool | None = None) -> "QuantizedDecoderBlock":
         """Binds block ``index`` of an MLX-affine checkpoint: ``<prefix>.<index>.
         <module>.weight`` (U32) with ``.scales`` / ``.biases`` per projection,
         and ``<module>.bias`` as the output bias where present. Norms' weights
         are read where they are f32/bf16 ``[width]``; without them the block runs
         its projections and refuses a ``step``. (A block that is made without
-        ``norms`` has norms of ones.) ``head_norms``: the model norms its query
-        and key heads, whose weights are read and needed likewise."""
+        ``norms`` has norms of ones.) Query and key heads are normed where the
+        checkpoint holds weights for it, which are read likewise; ``head_norms``
+        True: both are needed, False: neither is read."""
         base = f"{prefix}.{index}"
         modules = {field: f"{base}.{module}" for field, module, _, _ in PROJECTIONS}
         bound = ckpt.quantized_linears(session, path, bits=bits, group_size=group_size, prefixes=modules.values())
@@ -159,7 +160,8 @@ class QuantizedDecoderBlock:
         for name in [n for n in norm_names if header[norm_names[n]]["dtype"] not in ("F32", "BF16")
                      or header[norm_names[n]]["shape"] != [shape.width]]:
             del norm_names[name]
-        heads = {name: f"{base}.{module}.weight" for name, module in HEAD_NORMS.items()} if head_norms else {}
+        heads = {name: f"{base}.{module}.weight" for name, module in HEAD_NORMS.items()}
+        heads = {name: tensor for name, tensor in heads.items() if head_norms or head_norms is None and tensor in header}
         head_names = {name: tensor for name, tensor in heads.items() if tensor in header and
                       header[tensor]["dtype"] in ("F32", "BF16") and
                       tuple(header[tensor]["shape"]) in cls._head_norm_shapes(shape, name)}
