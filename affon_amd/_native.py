@@ -215,6 +215,7 @@ SIGNATURES = {
                                                ctypes.POINTER(AppendDesc), ctypes.POINTER(HeadNorm)]),
     "affon_rocm_shared_attention": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
                                             ctypes.POINTER(AttentionDesc), c_void_p, c_int64]),
+    "affon_rocm_token_weights": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch), c_void_p, c_size_t]),
     "affon_rocm_attention_weights": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch),
                                              ctypes.POINTER(WeightsDesc)]),
     "affon_rocm_cache_evict": (c_int, [c_void_p, ctypes.POINTER(KvCache), ctypes.POINTER(DraftBatch), c_void_p, c_void_p,

@@ -322,8 +322,15 @@ def shared_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, shared
 def token_weights(cache: PagedCache, batch: DraftBatch) -> Tensor:
     """Gathered weights of tokens that have gathered none: f32 zeros [layers, B,
     kv_heads, columns * page_size]. A row of them belongs to a row of the page table."""
-    batch._check("token_weights", cache, ())
-    return cache.session.tensor(np.zeros(_weights_shape(cache, batch), np.float32), "f32")
+    op = "token_weights"
+    cache_struct = cache._check(op)
+    batch_struct = batch._check(op, cache, ())
+    weights = cache.session.empty("f32", _weights_shape(cache, batch))
+    status = _native.load().affon_rocm_token_weights(cache.session._handle, cache_struct, batch_struct, weights.data_ptr,
+                                                     _space(weights))
+    if status:
+        _refused(status, op, lambda: None)
+    return weights
 
 
 def _weights_shape(cache: PagedCache, batch: DraftBatch) -> tuple[int, ...]:

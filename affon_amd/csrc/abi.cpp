@@ -1242,6 +1242,25 @@ int affon_rocm_shared_attention(affon_rocm_session* session, const affon_rocm_kv
   return AFFON_ROCM_OK;
 }
 
+int affon_rocm_token_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                             const affon_rocm_draft_batch* batch, float* weights, size_t weights_bytes) {
+  clear_error();
+  const char* op = "token_weights";
+  affon::PagedCache c{};
+  affon::DraftBatch b{};
+  int status = check_cache(cache, -1, op, &c);
+  if (status != AFFON_ROCM_OK || (status = check_batch(batch, c, op, &b)) != AFFON_ROCM_OK) return status;
+  affon::Rows to;
+  if ((status = check_weights(*cache, b, weights, weights_bytes, op, &to)) != AFFON_ROCM_OK ||
+      (status = check_session(session)) != AFFON_ROCM_OK)
+    return status;
+  if (meets(to, *cache, *batch, b, {})) return fail(AFFON_ROCM_INVALID_SHAPE, "%s weights overlap an operand", op);
+  const int64_t count = static_cast<int64_t>(c.layers) * b.sequences * c.kv_heads * static_cast<int64_t>(b.capacity);
+  const hipError_t e = affon::clear_weights_launch(weights, count, session->stream);
+  if (e != hipSuccess) return hip_fail(e, op);
+  return AFFON_ROCM_OK;
+}
+
 int affon_rocm_attention_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                                  const affon_rocm_draft_batch* batch, const affon_rocm_weights_desc* d) {
   clear_error();

@@ -346,4 +346,19 @@ hipError_t commit_weights_launch(const DraftBatch& batch, int layers, int kv_hea
   return hipGetLastError();
 }
 
+namespace {
+
+__global__ __launch_bounds__(256) void clear_weights_kernel(float* weights, int64_t count) {
+  for (int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x; i < count; i += static_cast<int64_t>(gridDim.x) * 256)
+    weights[i] = 0.0f;
+}
+
+}  // namespace
+
+hipError_t clear_weights_launch(float* weights, int64_t count, hipStream_t stream) {
+  const int64_t blocks = std::min<int64_t>((count + 255) / 256, 4096);
+  hipLaunchKernelGGL(clear_weights_kernel, dim3(static_cast<unsigned>(blocks)), dim3(256), 0, stream, weights, count);
+  return hipGetLastError();
+}
+
 }  // namespace affon

@@ -170,6 +170,7 @@ hipError_t commit_launch(const PagedCache& cache, const DraftBatch& batch, const
                          int path_columns, const uint32_t* accepted, hipStream_t stream);
 hipError_t commit_weights_launch(const DraftBatch& batch, int layers, int kv_heads, float* weights, const uint32_t* path,
                                  int64_t path_stride, int path_columns, const uint32_t* accepted, hipStream_t stream);
+hipError_t clear_weights_launch(float* weights, int64_t count, hipStream_t stream);
 hipError_t evict_launch(const PagedCache& cache, const DraftBatch& batch, const float* weights, float* out,
                         const uint32_t* keep, const uint32_t* recent, const Launch& l);
 

@@ -453,6 +453,10 @@ typedef struct {
 int affon_rocm_attention_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                                  const affon_rocm_draft_batch* batch, const affon_rocm_weights_desc* desc);
 
+/* Weights of tokens that have gathered none: zeros in all layers' (memory of no operand). */
+int affon_rocm_token_weights(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
+                             const affon_rocm_draft_batch* batch, float* weights, size_t weights_bytes);
+
 /* Evicts tokens, in every layer: of sequence b's lengths[b] tokens min(keep[b],
  * lengths[b]) stay for each layer and key head by itself: the recent[b] last
  * ones, and of those before the ones of the largest weights (equal ones: the
