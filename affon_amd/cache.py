@@ -302,7 +302,9 @@ def shared_attention(cache: PagedCache, batch: DraftBatch, query: Tensor, shared
     lengths[b] >= shared[g] holds the same first shared[g] tokens as its group's
     others, in the same pages or in copies of them. (Sequences with fewer
     tokens share nothing.) A prompt's samples are one group; answers to one
-    system prompt another."""
+    system prompt another. A page that holds tokens past the prefix is one
+    sequence's own. Sequences that ``cache_evict`` has cut down share nothing
+    any more: their shared[g] is 0 then, or more than every lengths[b]."""
     op = "shared_attention"
     cache_struct = cache._check(op, layer)
     batch_struct = batch._check(op, cache, (query, shared, mask))
@@ -372,7 +374,12 @@ def cache_evict(cache: PagedCache, batch: DraftBatch, weights: Tensor, keep: Ten
     behind them: the result, in ``out``, which may be ``weights`` itself. The caller then sets
     lengths[b] to min(keep[b], lengths[b]). Keys are turned by the positions
     that they were appended with, so later ones need ``positions`` of their own.
-    No page of a sequence may be another's."""
+    Drafted tokens that are not committed yet are lost, and so are their weights.
+
+    No page of a sequence may be another's: where a prefix is shared, each
+    sequence needs a copy of it. What is kept differs from sequence to sequence and from
+    key head to key head, so sequences of equal prefixes share nothing afterwards
+    (``shared_attention``)."""
     op = "cache_evict"
     cache_struct = cache._check(op)
     batch_struct = batch._check(op, cache, (weights, keep, recent))

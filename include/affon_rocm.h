@@ -428,8 +428,10 @@ int affon_rocm_tree_attention(affon_rocm_session* session, const affon_rocm_kv_c
  * multiplied once for all of them. The B sequences are `groups` groups of B /
  * groups one after the other; sequence b of group g with lengths[b] >=
  * shared[g] holds the same first shared[g] tokens as the others, in the same
- * pages or in copies of them. Sequences with fewer tokens share nothing. The
- * result is tree_attention's, up to the order of its sums. */
+ * pages or in copies of them. Sequences with fewer tokens share nothing, and
+ * neither do those that affon_rocm_cache_evict has cut down: their shared[g] is
+ * 0 from then on, or more than every lengths[b]. A page that holds tokens past the prefix
+ * is one sequence's own. The result is tree_attention's, up to the order of its sums. */
 int affon_rocm_shared_attention(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                                 const affon_rocm_draft_batch* batch, const affon_rocm_attention_desc* desc,
                                 const uint32_t* shared /* [groups] device words */, int64_t groups);
@@ -462,8 +464,10 @@ int affon_rocm_token_weights(affon_rocm_session* session, const affon_rocm_kv_ca
  * ones, and of those before the ones of the largest weights (equal ones: the
  * first; a NaN is below all). They become tokens 0, 1, .. in their order, keys and values in their
  * pages; out[layer, b, k, i] is the weight of the i-th of them, and 0 from
- * there on. The caller then sets lengths[b] = min(keep[b], lengths[b]). Every
- * token's pages have to be its sequence's own: nothing moves from or to a place that no page holds. */
+ * there on. The caller then sets lengths[b] = min(keep[b], lengths[b]). Drafted
+ * tokens that are not committed are lost. Every token's pages have to be its
+ * sequence's own (a shared prefix: a copy for each), or sequences overwrite each
+ * other's tokens: nothing detects it. Nothing moves from or to a place that no page holds. */
 int affon_rocm_cache_evict(affon_rocm_session* session, const affon_rocm_kv_cache* cache,
                            const affon_rocm_draft_batch* batch, const float* weights /* as affon_rocm_weights_desc's */,
                            float* out /* of the same shape: the weights themselves, or memory of no operand */,
