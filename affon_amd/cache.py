@@ -224,8 +224,9 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
     ``positions`` are then [axes, B*T], and each pair turns by those of its
     axis."""
     op = "cache_append"
+    plain = axes is None and query_norm is None and key_norm is None
     cache_struct = cache._check(op, layer)
-    batch_struct = batch._check(op, cache, (query, key, value, positions, rotary, query_norm, key_norm))
+    batch_struct = batch._check(op, cache, (query, key, value, positions, rotary))
     views = _rank_two(op, "query", query), _rank_two(op, "key", key), _rank_two(op, "value", value)
     if rotary.dtype != "f32" or len(rotary.shape) != 2 or not rotary.is_contiguous() or rotary.shape[1] % 2 or \
             not 2 <= rotary.shape[1] <= cache.head_dim:
@@ -244,9 +245,10 @@ def cache_append(cache: PagedCache, batch: DraftBatch, query: Tensor, key: Tenso
     desc = _native.AppendDesc(*views, place, rotary.data_ptr, *rotary.shape, 1 if interleaved else 0, layer, out.data_ptr,
                               _space(out))
     native = _native.load()
-    if axes is None and query_norm is None and key_norm is None:
+    if plain:
         status = native.affon_rocm_cache_append(cache.session._handle, cache_struct, batch_struct, desc)
     else:
+        batch._check(op, cache, (query_norm, key_norm))
         q_data, q_stride, q_dtype = _norm_weight("query_norm", query_norm, query.shape[1] // cache.head_dim, cache.head_dim)
         k_data, k_stride, k_dtype = _norm_weight("key_norm", key_norm, cache.kv_heads, cache.head_dim)
         norm = _native.HeadNorm(q_data, k_data, q_stride, k_stride, q_dtype, k_dtype, epsilon,
