@@ -243,11 +243,12 @@ hipError_t launch_wide(const AppendNormProblem& q, hipStream_t stream) {
   const int64_t rows = static_cast<int64_t>(p.batch.sequences) * p.batch.rows;
   int lanes_log = 0;
   while (lanes_log < 6 && (V << lanes_log) < p.cache.head_dim / 2) ++lanes_log;
-  // Few rows: a head to every group of lanes. Many: a workgroup to a row, of
-  // as few waves as take its heads in the same number of turns: bf16 operands,
-  // where the instructions bound it, in more turns, to set the row up less
-  // often (2738 rows of 48 heads 15.6 us in waves of three heads, 17.3 of two;
-  // f32, 4096 rows of 80 heads, 54.3 us in waves of five heads, 51.2 of two).
+  // Few rows: a head to every group of lanes. Many: a workgroup of at most `most`
+  // waves to a row, which take its heads in turns, and as few waves as need no more
+  // turns. bf16 operands, where the instructions bound it, in more turns, to set
+  // the row up less often: 2738 rows of 48 heads of 128 in two waves (three
+  // turns) 16.2 us, in three (two turns) 17.8 (whole calls). f32, 4096 rows of 80 heads, in
+  // two waves (five turns) 54.2, in five (two turns) 52.2.
   const int64_t waves = ((static_cast<int64_t>(p.heads + 2 * p.cache.kv_heads) << lanes_log) + 63) / 64;
   const int64_t most = X::bytes == 2 ? 2 : 5;
   const int64_t turns = rows < kManyRows ? 1 : (waves + most - 1) / most;
