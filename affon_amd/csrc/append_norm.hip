@@ -16,16 +16,12 @@
 namespace affon {
 namespace {
 
-template <int CTRL>
-__device__ __forceinline__ float plus_lane(float v) {
-  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), CTRL, 0xf, 0xf, true));
-}
 // The sum over each group of 2^lanes_log lanes, in all of them.
 __device__ __forceinline__ float group_sum(float v, int lanes_log) {
-  if (lanes_log > 0) v = plus_lane<0xB1>(v);   // lane ^ 1
-  if (lanes_log > 1) v = plus_lane<0x4E>(v);   // lane ^ 2
-  if (lanes_log > 2) v = plus_lane<0x141>(v);  // the other four of eight
-  if (lanes_log > 3) v = plus_lane<0x140>(v);  // the other eight of sixteen
+  if (lanes_log > 0) v = plus_lane<kNextLane>(v);
+  if (lanes_log > 1) v = plus_lane<kNextPair>(v);
+  if (lanes_log > 2) v = plus_lane<kOtherFour>(v);
+  if (lanes_log > 3) v = plus_lane<kOtherEight>(v);
   if (lanes_log > 4) v += __shfl_xor(v, 16);
   if (lanes_log > 5) v += __shfl_xor(v, 32);
   return v;

@@ -561,15 +561,8 @@ __global__ __launch_bounds__(256) void sum_kernel(WeightArgs a) {
 }
 
 // The sum over each 16 lanes, in all of them.
-template <int CTRL>
-__device__ __forceinline__ float plus_other(float v) {
-  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), CTRL, 0xf, 0xf, true));
-}
 __device__ __forceinline__ float sum_of_16(float v) {
-  v = plus_other<0xB1>(v);          // lane ^ 1
-  v = plus_other<0x4E>(v);          // lane ^ 2
-  v = plus_other<0x141>(v);         // the other four of eight
-  return plus_other<0x140>(v);      // the other eight of sixteen
+  return plus_lane<kOtherEight>(plus_lane<kOtherFour>(plus_lane<kNextPair>(plus_lane<kNextLane>(v))));
 }
 
 // Four waves side by side over the keys, KT tiles each, all rows one after the

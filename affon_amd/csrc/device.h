@@ -51,6 +51,12 @@ __device__ __forceinline__ uint32_t scanned(uint32_t v) {
 __device__ __forceinline__ uint32_t lane_of(uint32_t v, int lane) {
   return static_cast<uint32_t>(__builtin_amdgcn_readlane(static_cast<int>(v), lane));
 }
+// v plus another lane's, among 16, for sums over 2, 4, 8 and 16 lanes, in all of them.
+enum LaneStep { kNextLane = 0xB1, kNextPair = 0x4E, kOtherFour = 0x141, kOtherEight = 0x140 };
+template <LaneStep STEP>
+__device__ __forceinline__ float plus_lane(float v) {
+  return v + __uint_as_float(__builtin_amdgcn_update_dpp(0, static_cast<int>(__float_as_uint(v)), STEP, 0xf, 0xf, true));
+}
 // A whole wave's sum of numbers below 2^56.
 __device__ __forceinline__ uint64_t wave_sum(uint64_t v) {
   const uint32_t low = scanned(static_cast<uint32_t>(v) & 0xffffffu), high = scanned(static_cast<uint32_t>(v >> 24));
