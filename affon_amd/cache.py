@@ -377,6 +377,8 @@ def cache_evict(cache: PagedCache, batch: DraftBatch, weights: Tensor, keep: Ten
     lengths[b] to min(keep[b], lengths[b]). Keys are turned by the positions
     that they were appended with, so later ones need ``positions`` of their own.
     Drafted tokens that are not committed yet are lost, and so are their weights.
+    All that lies behind the first token to go moves, however few go: evict some tens
+    of them every so many steps rather than one at each.
 
     No page of a sequence may be another's: where a prefix is shared, each
     sequence needs a copy of it. What is kept differs from sequence to sequence and from

@@ -402,9 +402,9 @@ struct PrefixKernel {
 // cycles for a 16th of bf16's work: D + 32 ceil(D / 32) halves of 64 cycles
 // for 32 rows and keys, beside which all else is small (about 450 of exponentials and
 // sums), so a step's phases follow each other and the waves of a SIMD fill each other's
-// gaps. 4 prompts of up to 6000 tokens, 4 key heads of 80, up to 200 rows of which some 120
-// are in use: 69 us (the call 92, and 110 with the general kernel, which takes them all);
-// rows fill whole tiles of 32, and a SIMD with two of them holds up those with one.
+// gaps. 4 prompts of up to 6000 tokens, 4 key heads of 80, 200 rows of which 140 are in
+// use: 69 us (the call 92, and 110 with the general kernel, which takes them all); they
+// are five tiles of 32 on four SIMDs, and the one with two holds up the others.
 template <int WIDTH>
 struct PrefixF32 {
   static constexpr int W = 8;

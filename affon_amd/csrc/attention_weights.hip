@@ -810,7 +810,8 @@ hipError_t attention_weights_launch(const AttentionProblem& p, float* weights, c
   // Up to 16 rows' scores are kept, where they find room: 32 sequences of up to
   // 4096 tokens 49 us with 4 rows of a key head, 52 with 8 and 59 with 16, and
   // 81 to 83 where they are computed again. More are more to write and read than
-  // the keys (bf16 heads of 128: 4 bytes a row each way, against 256).
+  // the keys (bf16 heads of 128: 4 bytes a row each way, against 256). The lengths
+  // are on the device, so the room is for all tokens that the table could hold.
   constexpr size_t kMostScores = size_t(1) << 30;
   const size_t scores = static_cast<size_t>(units) * a.rows * capacity * sizeof(float);
   uint8_t* scratch = nullptr;

@@ -188,7 +188,9 @@ __global__ __launch_bounds__(kThreads) void select_kernel(EvictArgs a) {
 // line of its place or before has been read. Memory bounds it: 2048 rows of up to
 // 4096 tokens cut to 1024 (bf16, heads of 128) 445 us, 4.8 TB/s. (Accesses that
 // leave no lines in the caches took 15 us less there, but 3 more of 16 for 8 rows
-// of up to 2000.)
+// of up to 2000.) However few tokens go, all that lies behind the first of them moves: 32
+// layers of 8 sequences of 4096 cut by the one of least weight 536 us (the whole
+// call), by 16 of them 1118, by 256 1131.
 constexpr int kMoveThreads = 256, kDeep = 8;
 constexpr uint32_t kWindow = 4096;
 
@@ -307,7 +309,8 @@ namespace {
 
 // The weights of accepted tokens follow them: a thread for each layer,
 // sequence and key head, eight at a time as the path ascends. The other
-// drafted tokens' places have gathered nothing.
+// drafted tokens' places have gathered nothing. 8192 rows of 24 drafted tokens, 6
+// of them accepted: 8 us of the commit's 20 (a launch more: 8.5 against 5.2 for 8 rows).
 __global__ __launch_bounds__(256) void commit_weights_kernel(DraftBatch batch, int64_t total, int kv_heads, float* weights,
                                                              const uint32_t* path, int64_t path_stride, int path_columns,
                                                              const uint32_t* accepted) {
