@@ -147,8 +147,11 @@ class QuantizedDecoderBlock:
         are read where they are f32/bf16 ``[width]``; without them the block runs
         its projections and refuses a ``step``. (A block that is made without
         ``norms`` has norms of ones.) Query and key heads are normed where the
-        checkpoint holds weights for it, which are read likewise; ``head_norms``
-        True: both are needed, False: neither is read."""
+        checkpoint holds weights for it, which are read likewise: one
+        ``[head_dim]`` for all heads. (``[heads * head_dim]`` may be each head's own
+        or a norm's over the whole projection, which the block does not have, so a
+        ``step`` is refused.) ``head_norms`` True: both are needed, of all heads or
+        of each; False: neither is read."""
         base = f"{prefix}.{index}"
         modules = {field: f"{base}.{module}" for field, module, _, _ in PROJECTIONS}
         bound = ckpt.quantized_linears(session, path, bits=bits, group_size=group_size, prefixes=modules.values())
@@ -164,7 +167,7 @@ class QuantizedDecoderBlock:
         heads = {name: tensor for name, tensor in heads.items() if head_norms or head_norms is None and tensor in header}
         head_names = {name: tensor for name, tensor in heads.items() if tensor in header and
                       header[tensor]["dtype"] in ("F32", "BF16") and
-                      tuple(header[tensor]["shape"]) in cls._head_norm_shapes(shape, name)}
+                      tuple(header[tensor]["shape"]) in cls._head_norm_shapes(shape, name)[:2 if head_norms else 1]}
         wanted = bias_names + list(norm_names.values()) + list(head_names.values())
         loaded = ckpt.load(session, path, wanted) if wanted else {}
         layers = {field: bound[module] for field, module in modules.items()}
@@ -270,7 +273,8 @@ class QuantizedDecoderBlock:
         options."""
         if self.unread_norms:
             shape = f"[{self.shape.width}] " if set(self.unread_norms) <= set(NORMS) else ""
-            raise TypeError(f"the checkpoint holds no f32/bf16 {shape}tensor for {', '.join(self.unread_norms)}")
+            wider = "" if shape else f" (heads: [{self.shape.width // self.shape.heads}], or with head_norms=True each head's own)"
+            raise TypeError(f"the checkpoint holds no f32/bf16 {shape}tensor for {', '.join(self.unread_norms)}{wider}")
         stream, normalized = residual_norm(stream, update, weight=self.norms.get("attentionNorm"), epsilon=epsilon,
                                            dtype=cache.dtype)
         query, key, value = self.attention(normalized, **options)

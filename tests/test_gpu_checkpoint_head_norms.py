@@ -21,7 +21,7 @@ def run(session, blocks, arrays, rng, normed):
 
 
 def test_norms_that_are_there_are_read(session, rng, tmp_path):
-    arrays = checkpoint(tmp_path / "blocks.safetensors", rng, head_shapes={"queryNorm": 256})
+    arrays = checkpoint(tmp_path / "blocks.safetensors", rng)
     blocks = load(session, tmp_path / "blocks.safetensors")
     assert [sorted(b.head_norms) for b in blocks] == [["keyNorm", "queryNorm"]] * 2
     run(session, blocks, arrays, rng, True)
@@ -47,6 +47,16 @@ def test_a_norm_that_cannot_be_read(session, tmp_path):
     assert blocks[0].unread_norms == ("keyNorm",)
     with pytest.raises(TypeError, match="keyNorm"):
         Server(session, blocks, 1).run(np.zeros((1, 1, 256)), 1)
+
+
+def test_each_heads_own_weights_or_a_wider_norm(session, rng, tmp_path):
+    """The file does not tell them apart: taken for each head's own where the caller says so."""
+    arrays = checkpoint(tmp_path / "blocks.safetensors", rng, head_shapes={"queryNorm": 256, "keyNorm": 128})
+    blocks = load(session, tmp_path / "blocks.safetensors")
+    assert blocks[0].unread_norms == ("queryNorm", "keyNorm")
+    with pytest.raises(TypeError, match="queryNorm, keyNorm.*head_norms=True"):
+        Server(session, blocks, 1).run(np.zeros((1, 1, 256)), 1)
+    run(session, load(session, tmp_path / "blocks.safetensors", head_norms=True), arrays, rng, True)
 
 
 def test_norms_that_are_left_out(session, rng, tmp_path):
